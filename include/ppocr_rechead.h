@@ -38,6 +38,10 @@ extern "C" {
 #define PPOCR_ERR_NO_MEMORY 3   /* device allocation failed */
 #define PPOCR_ERR_MODEL 4       /* model file unreadable or malformed (ModelError / SafeTensorsError) */
 
+/* Types of the tensors that the training entry points name by `dtype`. */
+#define PPOCR_DTYPE_F32 0
+#define PPOCR_DTYPE_BF16 1
+
 /* How the projection's inner products are computed.  All modes accumulate in fp32 and
  * apply the per-class scale and bias in fp32 in the epilogue. */
 typedef enum {
@@ -345,6 +349,95 @@ int ppocr_rn_forward_marked_dev(const ppocr_rn_t* h, const float* d_x, const flo
                                 const int64_t* d_line_off, int64_t lines, int layout, float* d_out,
                                 void* d_workspace, size_t workspace_bytes, void* stream, void* const* events,
                                 int nevents, const char** names, int* recorded);
+
+/* ---------------------------------------------------------------- training the head
+ * No counterpart in the reference, which only infers: what a program needs to fine-tune the
+ * head or to calibrate a quantised one, the losses over the vocabulary with their gradients, a
+ * teacher's top logits, and the LayerNorm before the head in both directions.  The logits are
+ * never kept: each pass computes them again, tile by tile.
+ *
+ * Tensors whose type `dtype` names are passed to the `_dev` forms as void* (inputs are only
+ * read); the host forms take fp32.  Everything else (bias, losses, LayerNorm weights, statistics,
+ * the gradients of the bias and of the LayerNorm weights) is fp32 in both.  The `_dev` forms run
+ * on the current device, which must be the tensors'.  A `_dev` workspace is 16-byte aligned, needs
+ * no initial value and keeps none for a later call; its size is that of the shape (forward and
+ * backward alike), NULL allocates one on the stream; calls that share one must not overlap.
+ * Equal calls give equal bits. */
+
+/* Softmax cross entropy of the head's rows: with z = a w_t^T + bias (a [m][k], w_t [n][k], bias
+ * [n] or NULL), lse[r] = log sum_j exp(z[r][j]) and loss[r] = lse[r] - z[r][target[r]].  A row
+ * whose target is negative has no label: loss 0, no gradient, whatever the row holds (lse is
+ * still its own).  The host form refuses targets of n and above; the `_dev` form treats them as no
+ * label.  k is 1 to 256, m and n up to 2^24, n at least 1.  The products of fp32 tensors are
+ * taken as three products of fp16 halves (22 bits of each operand, scaled per 32 rows or classes
+ * by a power of two) summed in fp32, those of bf16 tensors exactly. */
+size_t ppocr_xent_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype);
+int ppocr_xent_forward(const float* a, const float* w_t, const float* bias, const int32_t* target, int64_t m, int64_t n,
+                       int64_t k, float* loss, float* lse);
+int ppocr_xent_forward_dev(void* d_a, void* d_w_t, const float* d_bias, const int32_t* d_target, int64_t m, int64_t n,
+                           int64_t k, int dtype, float* d_loss, float* d_lse, void* d_workspace, size_t workspace_bytes,
+                           void* stream);
+/* Its gradients: with lse of the forward call and grad[r] the loss's gradient by loss[r] (NULL: 1
+ * for every row), dz[r][j] = grad[r] (exp(z[r][j] - lse[r]) - (j == target[r])), da = dz w_t
+ * [m][k], dw_t = dz^T a [n][k] (both of the inputs' type) and dbias = sum_r dz[r] [n].  Each
+ * output is written whole and may be NULL (not computed); none may overlap an input.  A row whose grad is 0 adds nothing,
+ * whatever it holds.  m = 0 gives zeros. */
+int ppocr_xent_backward(const float* a, const float* w_t, const float* bias, const int32_t* target, const float* lse,
+                        const float* grad, int64_t m, int64_t n, int64_t k, float* da, float* dw_t, float* dbias);
+int ppocr_xent_backward_dev(void* d_a, void* d_w_t, const float* d_bias, const int32_t* d_target, const float* d_lse,
+                            const float* d_grad, int64_t m, int64_t n, int64_t k, int dtype, void* d_da, void* d_dw_t,
+                            float* d_dbias, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's top logits: row r of teacher_idx and teacher_logits [m][topk]
+ * (topk 1 to 64) holds classes and the teacher's logits for them, in any order (as
+ * ppocr_topk_rows writes them).  q = softmax of the row's entries over `temperature`, p = softmax of
+ * the head's logits z / temperature over all n classes, loss[r] = sum_i q_i (log q_i - log
+ * p[teacher_idx[i]]), the divergence of p from q, and lse[r] = log sum_j exp(z[r][j] /
+ * temperature).  An entry with a negative class is absent (also, in the `_dev` form, one of n or
+ * above, which the host form refuses); entries of one row may name the same class; an entry whose
+ * logit is -inf weighs nothing; a row without an entry of any weight has loss 0 and no gradient.
+ * Shapes and arithmetic as for the cross entropy. */
+size_t ppocr_distill_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t topk, int dtype);
+int ppocr_distill_forward(const float* a, const float* w_t, const float* bias, const int32_t* teacher_idx,
+                          const float* teacher_logits, int64_t topk, float temperature, int64_t m, int64_t n, int64_t k,
+                          float* loss, float* lse);
+int ppocr_distill_forward_dev(void* d_a, void* d_w_t, const float* d_bias, const int32_t* d_teacher_idx,
+                              const float* d_teacher_logits, int64_t topk, float temperature, int64_t m, int64_t n,
+                              int64_t k, int dtype, float* d_loss, float* d_lse, void* d_workspace,
+                              size_t workspace_bytes, void* stream);
+/* Its gradients for the head: dz[r][j] = grad[r] / temperature (p[r][j] - sum of q_i of the entries
+ * naming j); outputs as ppocr_xent_backward's.  (The usual weight of a distillation loss next to
+ * another, temperature squared, belongs into grad.) */
+int ppocr_distill_backward(const float* a, const float* w_t, const float* bias, const int32_t* teacher_idx,
+                           const float* teacher_logits, int64_t topk, float temperature, const float* lse,
+                           const float* grad, int64_t m, int64_t n, int64_t k, float* da, float* dw_t, float* dbias);
+int ppocr_distill_backward_dev(void* d_a, void* d_w_t, const float* d_bias, const int32_t* d_teacher_idx,
+                               const float* d_teacher_logits, int64_t topk, float temperature, const float* d_lse,
+                               const float* d_grad, int64_t m, int64_t n, int64_t k, int dtype, void* d_da,
+                               void* d_dw_t, float* d_dbias, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* The topk (1 to 64) largest values of each row of x [rows][cols] and their columns, largest first,
+ * equal values by column (-0 equals 0): idx and val [rows][topk].  NaN is never taken, as in
+ * ppocr_argmax_rows; places that a row has no value for hold -1 and -inf. */
+int ppocr_topk_rows(const float* x, int64_t rows, int64_t cols, int64_t topk, int32_t* idx, float* val);
+int ppocr_topk_rows_dev(const float* d_x, int64_t rows, int64_t cols, int64_t topk, int32_t* d_idx, float* d_val,
+                        void* stream);
+
+/* LayerNorm of rows x [m][d], d 1 to 16384: y = (x - mean) rstd w + b with rstd = 1 / sqrt(var +
+ * eps), var the mean of (x - mean)^2 (src/ops/layernorm.rs:5-244).  mean and rstd [m] may be NULL. y may be x. */
+int ppocr_layernorm_forward(const float* x, const float* w, const float* b, int64_t m, int64_t d, float eps, float* y,
+                            float* mean, float* rstd);
+int ppocr_layernorm_forward_dev(void* d_x, const float* d_w, const float* d_b, int64_t m, int64_t d, float eps,
+                                int dtype, void* d_y, float* d_mean, float* d_rstd, void* stream);
+/* Its gradients, from mean and rstd of the forward call: with h = (x - mean) rstd and t = dy w, dx =
+ * rstd (t - mean(t) - h mean(t h)), dw = sum over rows of dy h, db = sum over rows of dy.  Each
+ * output may be NULL (not computed); dx may be dy or x. m = 0 gives zeros. */
+size_t ppocr_layernorm_workspace_bytes(int64_t m, int64_t d);
+int ppocr_layernorm_backward(const float* dy, const float* x, const float* w, const float* mean, const float* rstd,
+                             int64_t m, int64_t d, float* dx, float* dw, float* db);
+int ppocr_layernorm_backward_dev(void* d_dy, void* d_x, const float* d_w, const float* d_mean, const float* d_rstd,
+                                 int64_t m, int64_t d, int dtype, void* d_dx, float* d_dw, float* d_db,
+                                 void* d_workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -12,9 +12,11 @@
 #include <vector>
 
 #include "kernels.hpp"
+#include "layernorm.hpp"
 #include "model_graph.hpp"
 #include "neck.hpp"
 #include "safetensors.hpp"
+#include "xent.hpp"
 
 namespace ppocr {
 
@@ -692,7 +694,8 @@ struct Workspace {
     ~Workspace() {
         if (owned && p) (void)hipFreeAsync(p, st);
     }
-    int get(void* user, size_t user_bytes, size_t need, hipStream_t s, const char* op) {
+    // guarded: the memory's first bytes are the precision guard's list header
+    int get(void* user, size_t user_bytes, size_t need, hipStream_t s, const char* op, bool guarded = true) {
         st = s;
         if (user) {
             if (user_bytes < need)
@@ -708,6 +711,7 @@ struct Workspace {
         }
         p = static_cast<uint8_t*>(q);
         owned = true;
+        if (!guarded) return PPOCR_OK;
         return launch_guard_clear(reinterpret_cast<unsigned long long*>(p), s);  // the header, at offset 0
     }
 };
@@ -1653,6 +1657,371 @@ int ppocr_rn_forward(const ppocr_rn_t* h, const float* x, const float* shortcut,
                            hc.out<float>(0), reinterpret_cast<float*>(hc.ws()), hc.stream()))
         return e;
     return hc.copy_out({out});
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- training the head
+namespace {
+
+constexpr const char* kXentOp = "SoftmaxCrossEntropy";
+constexpr const char* kDistillOp = "Distill";
+constexpr const char* kNormOp = "LayerNorm";
+constexpr const char* kTopkOp = "TopK";
+constexpr int64_t kLossMost = 1 << 24;  // rows and classes of a loss
+
+int bad_arg(const char* op, const std::string& msg) { return fail(PPOCR_ERR_INVALID_ARG, std::string(op) + ": " + msg); }
+
+int check_dtype(int dtype, const char* op) {
+    if (dtype != PPOCR_DTYPE_F32 && dtype != PPOCR_DTYPE_BF16) return bad_arg(op, "unknown type " + std::to_string(dtype));
+    return PPOCR_OK;
+}
+
+int check_loss_shape(const char* op, int64_t m, int64_t n, int64_t k, int dtype) {
+    if (m < 0 || n < 0 || k < 0) return bad_arg(op, "negative shape");
+    if (n == 0 || k == 0) return bad_arg(op, "weight must have positive shape");
+    if (k > kXentMaxK) return bad_arg(op, "inner dimension " + std::to_string(k) + " above " + std::to_string(kXentMaxK));
+    if (m > kLossMost) return bad_arg(op, "too many rows");
+    if (n > kLossMost) return bad_arg(op, "too many classes");
+    return check_dtype(dtype, op);
+}
+
+int check_teacher(int64_t topk, float temperature) {
+    if (topk < 1 || topk > kXentMaxTargets)
+        return bad_arg(kDistillOp, "topk must be 1 to " + std::to_string(kXentMaxTargets) + ", got " + std::to_string(topk));
+    if (!(temperature >= 1e-6f && temperature <= 1e6f)) return bad_arg(kDistillOp, "temperature must lie in [1e-6, 1e6]");
+    return PPOCR_OK;
+}
+
+// The workspace of a training call: the caller's, checked, or stream-ordered scratch.
+int train_workspace(Workspace* ws, void* user, size_t bytes, size_t need, hipStream_t st, const char* op) {
+    if (reinterpret_cast<uintptr_t>(user) % 16) return bad_arg(op, "workspace must be 16-byte aligned");
+    return ws->get(user, bytes, need, st, op, false);
+}
+
+XentProblem loss_problem(const void* a, const void* w, const float* bias, int64_t m, int64_t n, int64_t k, int dtype) {
+    XentProblem x{};
+    x.a = a;
+    x.w = w;
+    x.bias = bias;
+    x.tn = 1;
+    x.tau = 1.0f;
+    x.m = m;
+    x.n = n;
+    x.k = (int)k;
+    x.bf16 = dtype == PPOCR_DTYPE_BF16;
+    return x;
+}
+
+size_t loss_workspace(int64_t m, int64_t n, int64_t k, int tn, int dtype) {
+    return xent_layout(m, n, k, tn, dtype == PPOCR_DTYPE_BF16 ? 1 : 2).total();
+}
+
+int loss_forward_dev(const char* op, const XentProblem& x, float* loss, float* lse, void* workspace, size_t bytes,
+                     void* stream) {
+    if (!x.a || !x.w || !(x.target || (x.teacher_idx && x.teacher_z)) || !loss || !lse) return bad_arg(op, "null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    Workspace ws;
+    const size_t need = xent_layout(x.m, x.n, x.k, x.tn, x.planes()).total();
+    if (int e = train_workspace(&ws, workspace, bytes, need, st, op)) return e;
+    return launch_xent_forward(x, loss, lse, ws.p, st);
+}
+
+int loss_backward_dev(const char* op, const XentProblem& x, void* da, void* dw, float* db, void* workspace, size_t bytes,
+                      void* stream) {
+    hipStream_t st = (hipStream_t)stream;
+    if (!da && !dw && !db) return PPOCR_OK;
+    if (x.m == 0) return launch_xent_zero(x, dw, db, st);
+    if (!x.a || !x.w || !(x.target || (x.teacher_idx && x.teacher_z)) || !x.lse) return bad_arg(op, "null pointer");
+    Workspace ws;
+    const size_t need = xent_layout(x.m, x.n, x.k, x.tn, x.planes()).total();
+    if (int e = train_workspace(&ws, workspace, bytes, need, st, op)) return e;
+    return launch_xent_backward(x, da, dw, db, ws.p, st);
+}
+
+int check_classes(const char* op, const int32_t* c, int64_t count, int64_t n) {
+    for (int64_t i = 0; i < count; ++i)
+        if (c[i] >= n) return bad_arg(op, "class " + std::to_string(c[i]) + " of " + std::to_string(n));
+    return PPOCR_OK;
+}
+
+// The host forms: inputs in, the `_dev` form on the arena's memory, outputs back.  Targets are one
+// or two arrays of `entries` values (the second may be null).
+int loss_forward_host(const char* op, XentProblem x, float* loss, float* lse) {
+    const bool teach = x.teacher_idx != nullptr;
+    const int32_t* idx = teach ? x.teacher_idx : x.target;
+    if (!x.a || !x.w || !idx || (teach && !x.teacher_z) || !loss || !lse) return bad_arg(op, "null pointer");
+    const int64_t entries = x.m * x.tn;
+    if (int e = check_classes(op, idx, entries, x.n)) return e;
+    const size_t rb = (size_t)x.m * 4, eb = (size_t)entries * 4;
+    HostCall hc;
+    if (int e = hc.begin({(size_t)(x.m * x.k) * 4, (size_t)(x.n * x.k) * 4, x.bias ? (size_t)x.n * 4 : 0, eb, teach ? eb : 0},
+                         {rb, rb}, 256 + loss_workspace(x.m, x.n, x.k, x.tn, PPOCR_DTYPE_F32)))
+        return e;
+    if (int e = hc.copy_in({x.a, x.w, x.bias, idx, x.teacher_z})) return e;
+    x.a = hc.in<float>(0);
+    x.w = hc.in<float>(1);
+    if (x.bias) x.bias = hc.in<float>(2);
+    (teach ? x.teacher_idx : x.target) = hc.in<int32_t>(3);
+    if (teach) x.teacher_z = hc.in<float>(4);
+    if (int e = launch_xent_forward(x, hc.out<float>(0), hc.out<float>(1), hc.ws() + 256, hc.stream())) return e;
+    return hc.copy_out({loss, lse});
+}
+
+int loss_backward_host(const char* op, XentProblem x, float* da, float* dw, float* db) {
+    if (!da && !dw && !db) return PPOCR_OK;
+    if (x.m == 0) {
+        if (dw) std::memset(dw, 0, (size_t)(x.n * x.k) * 4);
+        if (db) std::memset(db, 0, (size_t)x.n * 4);
+        return PPOCR_OK;
+    }
+    const bool teach = x.teacher_idx != nullptr;
+    const int32_t* idx = teach ? x.teacher_idx : x.target;
+    if (!x.a || !x.w || !idx || (teach && !x.teacher_z) || !x.lse) return bad_arg(op, "null pointer");
+    const int64_t entries = x.m * x.tn;
+    if (int e = check_classes(op, idx, entries, x.n)) return e;
+    const size_t rb = (size_t)x.m * 4, eb = (size_t)entries * 4, ab = (size_t)(x.m * x.k) * 4, wb = (size_t)(x.n * x.k) * 4,
+                 nb = (size_t)x.n * 4;
+    HostCall hc;
+    if (int e = hc.begin({ab, wb, x.bias ? nb : 0, eb, teach ? eb : 0, rb, x.grad ? rb : 0},
+                         {da ? ab : 0, dw ? wb : 0, db ? nb : 0},
+                         256 + loss_workspace(x.m, x.n, x.k, x.tn, PPOCR_DTYPE_F32)))
+        return e;
+    if (int e = hc.copy_in({x.a, x.w, x.bias, idx, x.teacher_z, x.lse, x.grad})) return e;
+    x.a = hc.in<float>(0);
+    x.w = hc.in<float>(1);
+    if (x.bias) x.bias = hc.in<float>(2);
+    (teach ? x.teacher_idx : x.target) = hc.in<int32_t>(3);
+    if (teach) x.teacher_z = hc.in<float>(4);
+    x.lse = hc.in<float>(5);
+    if (x.grad) x.grad = hc.in<float>(6);
+    if (int e = launch_xent_backward(x, da ? hc.out<float>(0) : nullptr, dw ? hc.out<float>(1) : nullptr,
+                                     db ? hc.out<float>(2) : nullptr, hc.ws() + 256, hc.stream()))
+        return e;
+    return hc.copy_out({da, dw, db});
+}
+
+int check_norm_shape(int64_t m, int64_t d, int dtype) {
+    if (m < 0 || d < 0) return bad_arg(kNormOp, "negative shape");
+    if (d == 0 || d > kLayerNormMaxD) return bad_arg(kNormOp, "width must be 1 to " + std::to_string(kLayerNormMaxD));
+    if (m > (1LL << 31)) return bad_arg(kNormOp, "too many rows");
+    return check_dtype(dtype, kNormOp);
+}
+
+int check_topk(int64_t rows, int64_t cols, int64_t topk) {
+    if (rows < 0 || cols < 0) return bad_arg(kTopkOp, "negative shape");
+    if (topk < 1 || topk > kTopkMost)
+        return bad_arg(kTopkOp, "topk must be 1 to " + std::to_string(kTopkMost) + ", got " + std::to_string(topk));
+    if (cols > 0x7fffffffLL || rows > (1LL << 40)) return bad_arg(kTopkOp, "shape too large");
+    return PPOCR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ppocr_xent_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
+    if (m <= 0 || check_loss_shape(kXentOp, m, n, k, dtype)) return 0;
+    return loss_workspace(m, n, k, 1, dtype);
+}
+
+int ppocr_xent_forward_dev(void* d_a, void* d_w_t, const float* d_bias, const int32_t* d_target, int64_t m, int64_t n,
+                           int64_t k, int dtype, float* d_loss, float* d_lse, void* d_workspace, size_t workspace_bytes,
+                           void* stream) {
+    if (int e = check_loss_shape(kXentOp, m, n, k, dtype)) return e;
+    if (m == 0) return PPOCR_OK;
+    XentProblem x = loss_problem(d_a, d_w_t, d_bias, m, n, k, dtype);
+    x.target = d_target;
+    return loss_forward_dev(kXentOp, x, d_loss, d_lse, d_workspace, workspace_bytes, stream);
+}
+
+int ppocr_xent_forward(const float* a, const float* w_t, const float* bias, const int32_t* target, int64_t m, int64_t n,
+                       int64_t k, float* loss, float* lse) {
+    if (int e = check_loss_shape(kXentOp, m, n, k, PPOCR_DTYPE_F32)) return e;
+    if (m == 0) return PPOCR_OK;
+    XentProblem x = loss_problem(a, w_t, bias, m, n, k, PPOCR_DTYPE_F32);
+    x.target = target;
+    return loss_forward_host(kXentOp, x, loss, lse);
+}
+
+int ppocr_xent_backward_dev(void* d_a, void* d_w_t, const float* d_bias, const int32_t* d_target, const float* d_lse,
+                            const float* d_grad, int64_t m, int64_t n, int64_t k, int dtype, void* d_da, void* d_dw_t,
+                            float* d_dbias, void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (int e = check_loss_shape(kXentOp, m, n, k, dtype)) return e;
+    XentProblem x = loss_problem(d_a, d_w_t, d_bias, m, n, k, dtype);
+    x.target = d_target;
+    x.lse = d_lse;
+    x.grad = d_grad;
+    return loss_backward_dev(kXentOp, x, d_da, d_dw_t, d_dbias, d_workspace, workspace_bytes, stream);
+}
+
+int ppocr_xent_backward(const float* a, const float* w_t, const float* bias, const int32_t* target, const float* lse,
+                        const float* grad, int64_t m, int64_t n, int64_t k, float* da, float* dw_t, float* dbias) {
+    if (int e = check_loss_shape(kXentOp, m, n, k, PPOCR_DTYPE_F32)) return e;
+    XentProblem x = loss_problem(a, w_t, bias, m, n, k, PPOCR_DTYPE_F32);
+    x.target = target;
+    x.lse = lse;
+    x.grad = grad;
+    return loss_backward_host(kXentOp, x, da, dw_t, dbias);
+}
+
+size_t ppocr_distill_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t topk, int dtype) {
+    if (m <= 0 || check_loss_shape(kDistillOp, m, n, k, dtype) || check_teacher(topk, 1.0f)) return 0;
+    return loss_workspace(m, n, k, (int)topk, dtype);
+}
+
+int ppocr_distill_forward_dev(void* d_a, void* d_w_t, const float* d_bias, const int32_t* d_teacher_idx,
+                              const float* d_teacher_logits, int64_t topk, float temperature, int64_t m, int64_t n,
+                              int64_t k, int dtype, float* d_loss, float* d_lse, void* d_workspace,
+                              size_t workspace_bytes, void* stream) {
+    if (int e = check_loss_shape(kDistillOp, m, n, k, dtype)) return e;
+    if (int e = check_teacher(topk, temperature)) return e;
+    if (m == 0) return PPOCR_OK;
+    XentProblem x = loss_problem(d_a, d_w_t, d_bias, m, n, k, dtype);
+    x.teacher_idx = d_teacher_idx;
+    x.teacher_z = d_teacher_logits;
+    x.tn = (int)topk;
+    x.tau = temperature;
+    return loss_forward_dev(kDistillOp, x, d_loss, d_lse, d_workspace, workspace_bytes, stream);
+}
+
+int ppocr_distill_forward(const float* a, const float* w_t, const float* bias, const int32_t* teacher_idx,
+                          const float* teacher_logits, int64_t topk, float temperature, int64_t m, int64_t n, int64_t k,
+                          float* loss, float* lse) {
+    if (int e = check_loss_shape(kDistillOp, m, n, k, PPOCR_DTYPE_F32)) return e;
+    if (int e = check_teacher(topk, temperature)) return e;
+    if (m == 0) return PPOCR_OK;
+    if (!teacher_idx) return bad_arg(kDistillOp, "null pointer");
+    XentProblem x = loss_problem(a, w_t, bias, m, n, k, PPOCR_DTYPE_F32);
+    x.teacher_idx = teacher_idx;
+    x.teacher_z = teacher_logits;
+    x.tn = (int)topk;
+    x.tau = temperature;
+    return loss_forward_host(kDistillOp, x, loss, lse);
+}
+
+int ppocr_distill_backward_dev(void* d_a, void* d_w_t, const float* d_bias, const int32_t* d_teacher_idx,
+                               const float* d_teacher_logits, int64_t topk, float temperature, const float* d_lse,
+                               const float* d_grad, int64_t m, int64_t n, int64_t k, int dtype, void* d_da,
+                               void* d_dw_t, float* d_dbias, void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (int e = check_loss_shape(kDistillOp, m, n, k, dtype)) return e;
+    if (int e = check_teacher(topk, temperature)) return e;
+    XentProblem x = loss_problem(d_a, d_w_t, d_bias, m, n, k, dtype);
+    x.teacher_idx = d_teacher_idx;
+    x.teacher_z = d_teacher_logits;
+    x.tn = (int)topk;
+    x.tau = temperature;
+    x.lse = d_lse;
+    x.grad = d_grad;
+    return loss_backward_dev(kDistillOp, x, d_da, d_dw_t, d_dbias, d_workspace, workspace_bytes, stream);
+}
+
+int ppocr_distill_backward(const float* a, const float* w_t, const float* bias, const int32_t* teacher_idx,
+                           const float* teacher_logits, int64_t topk, float temperature, const float* lse,
+                           const float* grad, int64_t m, int64_t n, int64_t k, float* da, float* dw_t, float* dbias) {
+    if (int e = check_loss_shape(kDistillOp, m, n, k, PPOCR_DTYPE_F32)) return e;
+    if (int e = check_teacher(topk, temperature)) return e;
+    if (m > 0 && !teacher_idx) return bad_arg(kDistillOp, "null pointer");
+    XentProblem x = loss_problem(a, w_t, bias, m, n, k, PPOCR_DTYPE_F32);
+    x.teacher_idx = teacher_idx;
+    x.teacher_z = teacher_logits;
+    x.tn = (int)topk;
+    x.tau = temperature;
+    x.lse = lse;
+    x.grad = grad;
+    return loss_backward_host(kDistillOp, x, da, dw_t, dbias);
+}
+
+int ppocr_topk_rows_dev(const float* d_x, int64_t rows, int64_t cols, int64_t topk, int32_t* d_idx, float* d_val,
+                        void* stream) {
+    if (int e = check_topk(rows, cols, topk)) return e;
+    if (rows == 0) return PPOCR_OK;
+    if ((!d_x && cols) || !d_idx || !d_val) return bad_arg(kTopkOp, "null pointer");
+    return launch_topk_rows(d_x, rows, cols, (int)topk, d_idx, d_val, (hipStream_t)stream);
+}
+
+int ppocr_topk_rows(const float* x, int64_t rows, int64_t cols, int64_t topk, int32_t* idx, float* val) {
+    if (int e = check_topk(rows, cols, topk)) return e;
+    if (rows == 0) return PPOCR_OK;
+    if ((!x && cols) || !idx || !val) return bad_arg(kTopkOp, "null pointer");
+    const size_t xb = (size_t)rows * (size_t)cols * 4, ob = (size_t)(rows * topk) * 4;
+    HostCall hc;
+    if (int e = hc.begin({xb}, {ob, ob}, 0)) return e;
+    if (int e = hc.copy_in({x})) return e;
+    if (int e = launch_topk_rows(hc.in<float>(0), rows, cols, (int)topk, hc.out<int32_t>(0), hc.out<float>(1), hc.stream()))
+        return e;
+    return hc.copy_out({idx, val});
+}
+
+int ppocr_layernorm_forward_dev(void* d_x, const float* d_w, const float* d_b, int64_t m, int64_t d, float eps,
+                                int dtype, void* d_y, float* d_mean, float* d_rstd, void* stream) {
+    if (int e = check_norm_shape(m, d, dtype)) return e;
+    if (!(eps >= 0.0f && eps < INFINITY)) return bad_arg(kNormOp, "eps must be finite and not negative");
+    if (m == 0) return PPOCR_OK;
+    if (!d_x || !d_w || !d_b || !d_y) return bad_arg(kNormOp, "null pointer");
+    return launch_layernorm_forward(d_x, d_w, d_b, m, (int)d, eps, dtype == PPOCR_DTYPE_BF16, d_y, d_mean, d_rstd,
+                                    (hipStream_t)stream);
+}
+
+int ppocr_layernorm_forward(const float* x, const float* w, const float* b, int64_t m, int64_t d, float eps, float* y,
+                            float* mean, float* rstd) {
+    if (int e = check_norm_shape(m, d, PPOCR_DTYPE_F32)) return e;
+    if (!(eps >= 0.0f && eps < INFINITY)) return bad_arg(kNormOp, "eps must be finite and not negative");
+    if (m == 0) return PPOCR_OK;
+    if (!x || !w || !b || !y) return bad_arg(kNormOp, "null pointer");
+    const size_t xb = (size_t)m * (size_t)d * 4, wb = (size_t)d * 4, rb = (size_t)m * 4;
+    HostCall hc;
+    if (int e = hc.begin({xb, wb, wb}, {xb, rb, rb}, 0)) return e;
+    if (int e = hc.copy_in({x, w, b})) return e;
+    if (int e = launch_layernorm_forward(hc.in<float>(0), hc.in<float>(1), hc.in<float>(2), m, (int)d, eps, 0,
+                                         hc.out<float>(0), hc.out<float>(1), hc.out<float>(2), hc.stream()))
+        return e;
+    return hc.copy_out({y, mean, rstd});
+}
+
+size_t ppocr_layernorm_workspace_bytes(int64_t m, int64_t d) {
+    if (m <= 0 || check_norm_shape(m, d, PPOCR_DTYPE_F32)) return 0;
+    return 256 + (size_t)layernorm_parts(m, d) * 2 * (size_t)d * 4;
+}
+
+int ppocr_layernorm_backward_dev(void* d_dy, void* d_x, const float* d_w, const float* d_mean, const float* d_rstd,
+                                 int64_t m, int64_t d, int dtype, void* d_dx, float* d_dw, float* d_db,
+                                 void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (int e = check_norm_shape(m, d, dtype)) return e;
+    if (!d_dx && !d_dw && !d_db) return PPOCR_OK;
+    if (m > 0 && (!d_dy || !d_x || !d_w || !d_mean || !d_rstd)) return bad_arg(kNormOp, "null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    Workspace ws;
+    float* part = nullptr;
+    if (m > 0 && (d_dw || d_db)) {
+        // the first bytes are left to the head's calls, whose list header they hold
+        if (int e = train_workspace(&ws, d_workspace, workspace_bytes, ppocr_layernorm_workspace_bytes(m, d), st, kNormOp))
+            return e;
+        part = reinterpret_cast<float*>(ws.p + 256);
+    }
+    return launch_layernorm_backward(d_dy, d_x, d_w, d_mean, d_rstd, m, (int)d, dtype == PPOCR_DTYPE_BF16, d_dx, d_dw, d_db,
+                                     part, st);
+}
+
+int ppocr_layernorm_backward(const float* dy, const float* x, const float* w, const float* mean, const float* rstd,
+                             int64_t m, int64_t d, float* dx, float* dw, float* db) {
+    if (int e = check_norm_shape(m, d, PPOCR_DTYPE_F32)) return e;
+    if (!dx && !dw && !db) return PPOCR_OK;
+    if (m == 0) {
+        if (dw) std::memset(dw, 0, (size_t)d * 4);
+        if (db) std::memset(db, 0, (size_t)d * 4);
+        return PPOCR_OK;
+    }
+    if (!dy || !x || !w || !mean || !rstd) return bad_arg(kNormOp, "null pointer");
+    const size_t xb = (size_t)m * (size_t)d * 4, wb = (size_t)d * 4, rb = (size_t)m * 4;
+    HostCall hc;
+    if (int e = hc.begin({xb, xb, wb, rb, rb}, {xb, wb, wb}, ppocr_layernorm_workspace_bytes(m, d))) return e;
+    if (int e = hc.copy_in({dy, x, w, mean, rstd})) return e;
+    if (int e = launch_layernorm_backward(hc.in<float>(0), hc.in<float>(1), hc.in<float>(2), hc.in<float>(3), hc.in<float>(4), m,
+                                          (int)d, 0, dx ? hc.out<float>(0) : nullptr, hc.out<float>(1), hc.out<float>(2),
+                                          reinterpret_cast<float*>(hc.ws() + 256), hc.stream()))
+        return e;
+    return hc.copy_out({dx, dw, db});
 }
 
 }  // extern "C"

@@ -235,6 +235,8 @@ int launch_softmax_rows(float* x, int64_t rows, int64_t cols, int32_t* idx, floa
                         hipStream_t st);
 int launch_argmax_rows(const float* x, int64_t rows, int64_t cols, int32_t* idx, float* val,
                        hipStream_t st);
+constexpr int kTopkMost = 64;
+int launch_topk_rows(const float* x, int64_t rows, int64_t cols, int top, int32_t* idx, float* val, hipStream_t st);
 int launch_ctc_greedy(const int32_t* idx, const float* maxprob, const int64_t* line_off,
                       int64_t lines, int32_t blank, int32_t* seq, int64_t* seq_len, float* score,
                       hipStream_t st);

@@ -1,0 +1,320 @@
+// The matrix kernels of the vocabulary losses: the softmax statistics of the forward pass and
+// the two gradient products of the backward pass (xent.hpp for the records they read).
+#pragma once
+#include "xent.hpp"
+
+namespace ppocr {
+namespace xent {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// REC bytes of a record from global memory into LDS, 16 per lane, without registers.
+template <int REC>
+__device__ __forceinline__ void stage(const uint8_t* __restrict__ src, uint8_t* dst, int tid) {
+    constexpr int CH = REC / 16, PER = (CH + kThreads - 1) / kThreads;
+    static_assert(REC % 16 == 0, "record size");
+    const int wave_chunk = __builtin_amdgcn_readfirstlane(tid & ~63);
+#pragma unroll
+    for (int x = 0; x < PER; ++x) {
+        const int c0 = x * kThreads + wave_chunk;
+        if (CH % kThreads == 0 || c0 + (tid & 63) < CH)
+            __builtin_amdgcn_global_load_lds(
+                static_cast<const void*>(src + (size_t)(c0 + (tid & 63)) * 16),
+                reinterpret_cast<__attribute__((address_space(3))) void*>(
+                    reinterpret_cast<uintptr_t>(dst + (size_t)c0 * 16)),
+                16, 0, 0);
+    }
+}
+__device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_s_waitcnt(0x0 | (0x7 << 4) | (0xF << 8));  // vmcnt(0)
+}
+
+// One record's logits for this lane's owner entry: 16 entries of the stream record (8 (r / 4)
+// + 4 (lane / 32) + r % 4) against owner lane % 32.  With two planes the three products that
+// fp32 sums keep: high x high, high x low, low x high.
+template <int D, int P>
+__device__ __forceinline__ f32x16 scores(const uint8_t* rec, const f16x8 (&own)[P][2 * D], int lane) {
+    const f16x8* s0 = reinterpret_cast<const f16x8*>(rec) + lane;
+    f32x16 s = {};
+#pragma unroll
+    for (int ks = 0; ks < 2 * D; ++ks) {
+        const f16x8 hi = s0[ks * 64];
+        s = mma(hi, own[0][ks], s);
+        if constexpr (P == 2) {
+            const f16x8 lo = s0[(2 * D + ks) * 64];
+            s = mma(hi, own[1][ks], s);
+            s = mma(lo, own[0][ks], s);
+        }
+    }
+    return s;
+}
+
+template <int D, int P>
+__device__ __forceinline__ void load_owner(const uint8_t* rec, f16x8 (&own)[P][2 * D], int lane) {
+    const f16x8* s0 = reinterpret_cast<const f16x8*>(rec) + lane;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int ks = 0; ks < 2 * D; ++ks) own[p][ks] = s0[(p * 2 * D + ks) * 64];
+}
+
+// ---------------------------------------------------------------- forward: softmax statistics
+// Streams the class records of a chunk past 32 NB rows per wave.  t = z log2(e) / tau is kept
+// against a reference that moves only when a maximum beats it by 16 (so sums stay below 2^16 n
+// and lose nothing), and a lane needs no other lane until the chunk ends.
+template <int D, int P, int NB>
+__global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
+    constexpr int REC = P * D * 2048 + kXentAux;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int split = blockIdx.x % x.nsplit;
+    const int64_t rb = blockIdx.x / x.nsplit;
+    const int64_t t0 = (int64_t)split * x.per_split, t1 = min(t0 + x.per_split, x.tiles);
+    const int64_t row0 = rb * (32 * NB * kWaves) + wave * (32 * NB);
+
+    f16x8 own[NB][P][2 * D];
+    float c[NB], ref[NB], sum[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int64_t r = min(row0 + 32 * b, x.m - 1) / 32;  // a record that exists; unused rows are dropped at the end
+        const uint8_t* rec = x.own + r * REC;
+        load_owner<D, P>(rec, own[b], lane);
+        c[b] = x.c0 * reinterpret_cast<const float*>(rec + P * D * 2048)[64];
+        ref[b] = -INFINITY;
+        sum[b] = 0.0f;
+    }
+    stage<REC>(x.str + t0 * REC, lds, tid);
+    for (int64_t t = t0; t < t1; ++t) {
+        const uint8_t* cur = lds + ((t - t0) & 1) * REC;
+        wait_loads();
+        __syncthreads();
+        if (t + 1 < t1) stage<REC>(x.str + (t + 1) * REC, lds + ((t + 1 - t0) & 1) * REC, tid);
+        const float* aux = reinterpret_cast<const float*>(cur + P * D * 2048);
+        const float ce = aux[64];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            f32x16 s = scores<D, P>(cur, own[b], lane);
+            const float cc = c[b] * ce;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 bias = *reinterpret_cast<const f32x4*>(aux + 8 * q + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[4 * q + e] = fmaf(s[4 * q + e], cc, bias[e]);
+                    mx = fmaxf(mx, s[4 * q + e]);
+                }
+            }
+            if (__any(mx > ref[b] + 16.0f)) {
+                const float nr = mx > ref[b] + 16.0f ? mx : ref[b];
+                sum[b] = ref[b] == -INFINITY ? 0.0f : sum[b] * __builtin_amdgcn_exp2f(ref[b] - nr);
+                ref[b] = nr;
+            }
+            const float rf = ref[b] == -INFINITY ? 0.0f : ref[b];
+            float add = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) add += __builtin_amdgcn_exp2f(s[r] - rf);
+            sum[b] += add;
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        // the two halves of the wave hold the row's other classes
+        const float r2 = __shfl_xor(ref[b], 32, 64), s2 = __shfl_xor(sum[b], 32, 64);
+        const float nr = fmaxf(ref[b], r2);
+        float s = 0.0f;
+        s += ref[b] == -INFINITY ? sum[b] : sum[b] * __builtin_amdgcn_exp2f(ref[b] - nr);
+        s += r2 == -INFINITY ? s2 : s2 * __builtin_amdgcn_exp2f(r2 - nr);
+        const int64_t row = row0 + 32 * b + (lane & 31);
+        if (h == 0 && row < x.m) x.part[(int64_t)split * x.m + row] = make_float2(nr, s);
+    }
+}
+
+// ---------------------------------------------------------------- backward: one gradient
+// dX_o = sum_s P_os Y_s for the owners o of a workgroup (32 per wave), the stream records s of a
+// chunk in turn: the logits of 32 x 32 pairs, p = exp2(t - lse), the target entries' places
+// overwritten with p - q as the list holds it (exact in 32 bits, so that a nearly certain label
+// leaves its small difference), then P as the second product's operand without leaving the
+// registers: a result register's rows are the contraction's order, and the transposed part of
+// the record holds the entries in that order.
+//   ROWS: owners are activation rows, the stream is the classes (da).  P = p 2^(F - e).
+//   else: owners are classes, the stream is the rows (dW, db).  P = p g 2^(F - e), g the row's
+//   gradient factor.
+// e is the stream record's exponent and F one exponent for all records, so that P's largest
+// possible value is 2^14 and products of all records add up on one scale.
+__device__ __forceinline__ void set_entry(f32x16& p, int i, bool mine, float v) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if (r == i) p[r] = mine ? v : p[r];
+}
+
+template <int D, int P, bool ROWS>
+__global__ __launch_bounds__(kThreads, xent_grad_per_cu(D, P)) void grad_kernel(XentGradArgs x) {
+    constexpr int REC = 2 * P * D * 2048 + kXentAux, AUX = 2 * P * D * 2048;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int split = blockIdx.x % x.nsplit;
+    const int64_t ob = blockIdx.x / x.nsplit;
+    const int64_t t0 = (int64_t)split * x.per_split, t1 = min(t0 + x.per_split, x.str_tiles);
+    const int64_t og = ob * kWaves + wave;  // this wave's owner record
+    const int64_t owner = og * 32 + (lane & 31);
+
+    stage<REC>(x.str + t0 * REC, lds, tid);
+    // F from the largest exponent bound of the stream
+    int um = -200;
+    for (int64_t i = lane; i < x.str_tiles; i += 64) um = max(um, x.str_u[i]);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) um = max(um, __shfl_xor(um, o, 64));
+    const int F = 14 - um;
+
+    const bool have = og < x.own_tiles;
+    const uint8_t* orec = x.own + (have ? og : x.own_tiles - 1) * REC;
+    f16x8 own[P][2 * D];
+    load_owner<D, P>(orec, own, lane);
+    const float* oaux = reinterpret_cast<const float*>(orec + AUX);
+    const float c = x.c0 * oaux[64];
+    const float own0 = oaux[lane & 31];       // row: lse log2(e); class: bias log2(e) / tau
+    const float own1 = ROWS ? oaux[32 + (lane & 31)] : 0.0f;  // row: the gradient factor
+    f32x16 acc[D] = {};
+    float dbias = 0.0f;
+
+    // ROWS: the wave's row group is `og`, its list is walked along with the classes
+    const uint32_t* keys = x.keys + (ROWS && have ? og * x.list : 0);
+    const float* vals = x.vals + (ROWS && have ? og * x.list : 0);
+    int cur_hit = 0;
+    uint32_t next_key = 0xFFFFFFFFu;
+    if (ROWS && have && t0 < t1) {
+        cur_hit = __builtin_amdgcn_readfirstlane(x.offs[og * (x.blocks + 1) + t0 / 4]);
+        next_key = __builtin_amdgcn_readfirstlane(cur_hit < x.list ? keys[cur_hit] : 0xFFFFFFFFu);
+    }
+    for (int64_t t = t0; t < t1; ++t) {
+        const uint8_t* cur = lds + ((t - t0) & 1) * REC;
+        wait_loads();
+        __syncthreads();
+        if (t + 1 < t1) stage<REC>(x.str + (t + 1) * REC, lds + ((t + 1 - t0) & 1) * REC, tid);
+        f32x16 p = scores<D, P>(cur, own, lane);
+        const float* aux = reinterpret_cast<const float*>(cur + AUX);
+        const float cc = c * aux[64];
+        const int fe = min(F - (int)aux[65], 100);  // exponent of this record's factor
+        if constexpr (ROWS) {
+            const float shift = own0 - (float)fe;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 bias = *reinterpret_cast<const f32x4*>(aux + 8 * q + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    p[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(p[4 * q + e], cc, bias[e]) - shift);
+            }
+            const uint32_t end = (uint32_t)((t + 1) * 1024);  // keys below: classes of this record
+            while (next_key < end) {
+                const int cls = (int)(next_key >> 5) & 31, row = (int)next_key & 31;
+                const float v = ldexpf(vals[cur_hit], fe);
+                set_entry(p, (cls >> 3) * 4 + (cls & 3), lane == row + 32 * ((cls >> 2) & 1), v);
+                ++cur_hit;
+                next_key = __builtin_amdgcn_readfirstlane(cur_hit < x.list ? keys[cur_hit] : 0xFFFFFFFFu);
+            }
+        } else {
+            // (not below 2^-60, so that the bias's sum keeps the values of records of tiny activations)
+            const int fs = max(fe, -60);
+            const float shift = own0 + (float)fs;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 lse = *reinterpret_cast<const f32x4*>(aux + 8 * q + 4 * h);
+                const f32x4 g = *reinterpret_cast<const f32x4*>(aux + 32 + 8 * q + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    p[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(p[4 * q + e], cc, shift) - lse[e]) * g[e];
+            }
+            // the stream record is row group t; its entries in this workgroup's 128 classes
+            const uint16_t* of = x.offs + t * (x.blocks + 1) + ob;
+            const int i0 = __builtin_amdgcn_readfirstlane(of[0]), i1 = __builtin_amdgcn_readfirstlane(of[1]);
+            for (int i = i0; i < i1; ++i) {
+                const uint32_t key = __builtin_amdgcn_readfirstlane(x.keys[t * x.list + i]);
+                if ((int64_t)(key >> 10) != og) continue;
+                const int cls = (int)(key >> 5) & 31, row = (int)key & 31;
+                const float v = ldexpf(x.vals[t * x.list + i] * aux[32 + row], fs);
+                set_entry(p, (row >> 3) * 4 + (row & 3), lane == cls + 32 * ((row >> 2) & 1), v);
+            }
+            float add = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) add += p[r];
+            dbias += ldexpf(add, -fs);
+            if (fe != fs)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[r] = ldexpf(p[r], fe - fs);
+        }
+        const f16x8* tr = reinterpret_cast<const f16x8*>(cur + P * D * 2048) + lane;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            f16x8 ph, pl;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = p[8 * e + j];
+                ph[j] = (_Float16)v;
+                if constexpr (P == 2) pl[j] = (_Float16)(v - (float)ph[j]);
+            }
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                const f16x8 hi = tr[(d * 2 + e) * 64];
+                acc[d] = mma(hi, ph, acc[d]);
+                if constexpr (P == 2) {
+                    const f16x8 lo = tr[(D * 2 + d * 2 + e) * 64];
+                    acc[d] = mma(hi, pl, acc[d]);
+                    acc[d] = mma(lo, ph, acc[d]);
+                }
+            }
+        }
+    }
+    if (owner < x.owners) {
+        float* out = x.part + ((int64_t)split * x.owners + owner) * (32 * D);
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = ldexpf(acc[d][4 * q + e], -F);
+                    if (ROWS) v[e] *= own1;
+                }
+                *reinterpret_cast<f32x4*>(out + 32 * d + 8 * q + 4 * h) = v;
+            }
+    }
+    if constexpr (!ROWS) {
+        dbias += __shfl_xor(dbias, 32, 64);
+        if (x.part_db && h == 0 && owner < x.owners) x.part_db[(int64_t)split * x.owners + owner] = dbias;
+    }
+}
+
+}  // namespace xent
+
+template <int D, int P>
+int xent_stats_cfg(const XentStatsArgs& x, unsigned grid, hipStream_t st) {
+    constexpr int lds = 2 * (P * D * 2048 + kXentAux);
+    auto kernel = xent::stats_kernel<D, P, xent_stats_blocks(D, P)>;
+    kernel<<<grid, xent::kThreads, lds, st>>>(x);
+    PPOCR_HIP(hipGetLastError());
+    return PPOCR_OK;
+}
+
+template <int D, int P, bool ROWS>
+int xent_grad_cfg(const XentGradArgs& x, unsigned grid, hipStream_t st) {
+    constexpr int lds = 2 * (2 * P * D * 2048 + kXentAux);
+    auto kernel = xent::grad_kernel<D, P, ROWS>;
+    kernel<<<grid, xent::kThreads, lds, st>>>(x);
+    PPOCR_HIP(hipGetLastError());
+    return PPOCR_OK;
+}
+
+#define PPOCR_XENT_INSTANCES(D, P)                                                  \
+    template int xent_stats_cfg<D, P>(const XentStatsArgs&, unsigned, hipStream_t); \
+    template int xent_grad_cfg<D, P, true>(const XentGradArgs&, unsigned, hipStream_t); \
+    template int xent_grad_cfg<D, P, false>(const XentGradArgs&, unsigned, hipStream_t);
+
+}  // namespace ppocr

@@ -22,11 +22,17 @@ const SOURCES: &[&str] = &[
     "softmax_ctc.hip",
     "neck.hip",
     "neck_fused.hip",
+    "topk.hip",
+    "layernorm.hip",
+    "xent.hip",
+    "xent_cfg_1.hip",
+    "xent_cfg_2.hip",
     "safetensors.cpp",
     "model_graph.cpp",
 ];
 const HEADERS: &[&str] =
-    &["common.hpp", "kernels.hpp", "neck.hpp", "neck_device.hpp", "head_mfma.hpp", "safetensors.hpp", "json.hpp", "model_graph.hpp"];
+    &["common.hpp", "kernels.hpp", "neck.hpp", "neck_device.hpp", "head_mfma.hpp", "safetensors.hpp", "json.hpp", "model_graph.hpp",
+      "layernorm.hpp", "xent.hpp", "xent_kernels.hpp"];
 const FLAGS: &[&str] = &[
     "--offload-arch=gfx950",
     "-O3",

@@ -30,6 +30,9 @@ pub const PPOCR_MODE_BF16X3: c_int = 3;
 pub const PPOCR_MODE_F16X2: c_int = 4;
 pub const PPOCR_MODE_AUTO: c_int = 5;
 
+pub const PPOCR_DTYPE_F32: c_int = 0;
+pub const PPOCR_DTYPE_BF16: c_int = 1;
+
 pub const PPOCR_NECK_ROWS: c_int = 0;
 pub const PPOCR_NECK_CHANNELS_FIRST: c_int = 1;
 
@@ -178,4 +181,53 @@ extern "C" {
                                        d_workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
                                        events: *const *mut c_void, nevents: c_int, names: *mut *const c_char,
                                        recorded: *mut c_int) -> c_int;
+    // ---- training the head: losses over the vocabulary with their gradients, top logits, LayerNorm
+    pub fn ppocr_xent_workspace_bytes(m: i64, n: i64, k: i64, dtype: c_int) -> usize;
+    pub fn ppocr_xent_forward(a: *const f32, w_t: *const f32, bias: *const f32, target: *const i32, m: i64, n: i64,
+                              k: i64, loss: *mut f32, lse: *mut f32) -> c_int;
+    pub fn ppocr_xent_forward_dev(d_a: *mut c_void, d_w_t: *mut c_void, d_bias: *const f32, d_target: *const i32,
+                                  m: i64, n: i64, k: i64, dtype: c_int, d_loss: *mut f32, d_lse: *mut f32,
+                                  d_workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ppocr_xent_backward(a: *const f32, w_t: *const f32, bias: *const f32, target: *const i32,
+                               lse: *const f32, grad: *const f32, m: i64, n: i64, k: i64, da: *mut f32,
+                               dw_t: *mut f32, dbias: *mut f32) -> c_int;
+    pub fn ppocr_xent_backward_dev(d_a: *mut c_void, d_w_t: *mut c_void, d_bias: *const f32, d_target: *const i32,
+                                   d_lse: *const f32, d_grad: *const f32, m: i64, n: i64, k: i64, dtype: c_int,
+                                   d_da: *mut c_void, d_dw_t: *mut c_void, d_dbias: *mut f32,
+                                   d_workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ppocr_distill_workspace_bytes(m: i64, n: i64, k: i64, topk: i64, dtype: c_int) -> usize;
+    pub fn ppocr_distill_forward(a: *const f32, w_t: *const f32, bias: *const f32, teacher_idx: *const i32,
+                                 teacher_logits: *const f32, topk: i64, temperature: f32, m: i64, n: i64, k: i64,
+                                 loss: *mut f32, lse: *mut f32) -> c_int;
+    pub fn ppocr_distill_forward_dev(d_a: *mut c_void, d_w_t: *mut c_void, d_bias: *const f32,
+                                     d_teacher_idx: *const i32, d_teacher_logits: *const f32, topk: i64,
+                                     temperature: f32, m: i64, n: i64, k: i64, dtype: c_int, d_loss: *mut f32,
+                                     d_lse: *mut f32, d_workspace: *mut c_void, workspace_bytes: usize,
+                                     stream: *mut c_void) -> c_int;
+    pub fn ppocr_distill_backward(a: *const f32, w_t: *const f32, bias: *const f32, teacher_idx: *const i32,
+                                  teacher_logits: *const f32, topk: i64, temperature: f32, lse: *const f32,
+                                  grad: *const f32, m: i64, n: i64, k: i64, da: *mut f32, dw_t: *mut f32,
+                                  dbias: *mut f32) -> c_int;
+    pub fn ppocr_distill_backward_dev(d_a: *mut c_void, d_w_t: *mut c_void, d_bias: *const f32,
+                                      d_teacher_idx: *const i32, d_teacher_logits: *const f32, topk: i64,
+                                      temperature: f32, d_lse: *const f32, d_grad: *const f32, m: i64, n: i64,
+                                      k: i64, dtype: c_int, d_da: *mut c_void, d_dw_t: *mut c_void,
+                                      d_dbias: *mut f32, d_workspace: *mut c_void, workspace_bytes: usize,
+                                      stream: *mut c_void) -> c_int;
+    pub fn ppocr_topk_rows(x: *const f32, rows: i64, cols: i64, topk: i64, idx: *mut i32, val: *mut f32) -> c_int;
+    pub fn ppocr_topk_rows_dev(d_x: *const f32, rows: i64, cols: i64, topk: i64, d_idx: *mut i32, d_val: *mut f32,
+                               stream: *mut c_void) -> c_int;
+    pub fn ppocr_layernorm_forward(x: *const f32, w: *const f32, b: *const f32, m: i64, d: i64, eps: f32,
+                                   y: *mut f32, mean: *mut f32, rstd: *mut f32) -> c_int;
+    pub fn ppocr_layernorm_forward_dev(d_x: *mut c_void, d_w: *const f32, d_b: *const f32, m: i64, d: i64,
+                                       eps: f32, dtype: c_int, d_y: *mut c_void, d_mean: *mut f32,
+                                       d_rstd: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn ppocr_layernorm_workspace_bytes(m: i64, d: i64) -> usize;
+    pub fn ppocr_layernorm_backward(dy: *const f32, x: *const f32, w: *const f32, mean: *const f32,
+                                    rstd: *const f32, m: i64, d: i64, dx: *mut f32, dw: *mut f32,
+                                    db: *mut f32) -> c_int;
+    pub fn ppocr_layernorm_backward_dev(d_dy: *mut c_void, d_x: *mut c_void, d_w: *const f32, d_mean: *const f32,
+                                        d_rstd: *const f32, m: i64, d: i64, dtype: c_int, d_dx: *mut c_void,
+                                        d_dw: *mut f32, d_db: *mut f32, d_workspace: *mut c_void,
+                                        workspace_bytes: usize, stream: *mut c_void) -> c_int;
 }

@@ -19,12 +19,13 @@ import os
 import numpy as np
 
 from . import _lib
-from ._lib import (MODE_AUTO, MODE_BF16X1, MODE_BF16X2, MODE_BF16X3, MODE_F16X2, MODE_FP32_FMA, NECK_CHANNELS_FIRST,
+from ._lib import (DTYPE_BF16, DTYPE_F32, MODE_AUTO, MODE_BF16X1, MODE_BF16X2, MODE_BF16X3, MODE_F16X2, MODE_FP32_FMA, NECK_CHANNELS_FIRST,
                    NECK_ROWS, PPOCR_ERR_DEVICE, PPOCR_ERR_INVALID_ARG, PPOCR_ERR_MODEL, PPOCR_ERR_NO_MEMORY, PPOCR_OK)
 
 __all__ = [
     "OcrError", "QuantizedWeight", "RecHead", "RecNeck", "CtcDecoder", "find_rec_head", "matmul_quantized_b", "matmul_transposed_b",
-    "softmax", "softmax_inplace", "MODE_FP32_FMA", "MODE_BF16X1", "MODE_BF16X2", "MODE_BF16X3", "MODE_F16X2", "MODE_AUTO",
+    "softmax", "softmax_inplace", "cross_entropy", "cross_entropy_backward", "distill", "distill_backward", "topk",
+    "layer_norm", "layer_norm_backward", "DTYPE_F32", "DTYPE_BF16", "MODE_FP32_FMA", "MODE_BF16X1", "MODE_BF16X2", "MODE_BF16X3", "MODE_F16X2", "MODE_AUTO",
 ]
 
 
@@ -552,3 +553,135 @@ class CtcDecoder:
             _check(_lib.lib().ppocr_ctc_greedy(_ptr(idx), _ptr(maxprob), _ptr(line_off), lines, blank, _ptr(seq),
                                                _ptr(seq_len), _ptr(score)))
         return [seq[line_off[b]:line_off[b] + seq_len[b]].copy() for b in range(lines)], score[:max(lines, 0)].copy()
+
+
+# ---------------------------------------------------------------- training the head
+# The losses over the vocabulary with their gradients, a teacher's top logits and the LayerNorm in
+# front of the head, on host arrays (fp32).  Programs that keep their tensors on the GPU, or
+# train in bf16, call the `_dev` entry points (include/ppocr_rechead.h).
+
+
+def _head_args(op, a, w_t, bias):
+    a, w_t = _f32(a), _f32(w_t)
+    if a.ndim != 2 or w_t.ndim != 2:
+        raise OcrError(op, f"expected [m, k] rows and an [n, k] weight, got {list(a.shape)} and {list(w_t.shape)}")
+    if a.shape[1] != w_t.shape[1]:
+        raise OcrError(op, f"Inner dimensions must match: {a.shape[1]} != {w_t.shape[1]}")
+    b = None if bias is None else _f32(bias)
+    if b is not None and b.size != w_t.shape[0]:
+        raise OcrError(op, f"bias has {b.size} elements but n is {w_t.shape[0]}")
+    return a, w_t, b
+
+
+def _per_row(op, x, shape, dtype, what):
+    x = np.ascontiguousarray(x, dtype=dtype)
+    if x.shape != shape:
+        raise OcrError(op, f"expected {what} of shape {list(shape)}, got {list(x.shape)}")
+    return x
+
+
+def _teacher_args(m, teacher_idx, teacher_logits):
+    idx = np.ascontiguousarray(teacher_idx, dtype=np.int32)
+    if idx.ndim != 2 or idx.shape[0] != m:
+        raise OcrError("Distill", f"expected {m} rows of teacher classes, got shape {list(idx.shape)}")
+    return idx, _per_row("Distill", teacher_logits, idx.shape, np.float32, "teacher logits")
+
+
+def _loss_grads(a, w_t):
+    return np.empty_like(a), np.empty_like(w_t), np.empty(w_t.shape[0], np.float32)
+
+
+def cross_entropy(a, w_t, bias, target):
+    """(loss [m], lse [m]) of rows a [m, k] under the head w_t [n, k], bias [n] or None: the softmax
+    cross entropy of each row against its target class (negative: no label, loss 0)."""
+    op = "SoftmaxCrossEntropy"
+    a, w_t, b = _head_args(op, a, w_t, bias)
+    m, (n, k) = a.shape[0], w_t.shape
+    target = _per_row(op, target, (m,), np.int32, "targets")
+    loss, lse = np.empty(m, np.float32), np.empty(m, np.float32)
+    _check(_lib.lib().ppocr_xent_forward(_ptr(a), _ptr(w_t), _ptr(b), _ptr(target), m, n, k, _ptr(loss), _ptr(lse)))
+    return loss, lse
+
+
+def cross_entropy_backward(a, w_t, bias, target, lse, grad=None):
+    """(da [m, k], dw_t [n, k], dbias [n]) of cross_entropy, lse being its second result and grad
+    [m] the gradient by each row's loss (None: 1)."""
+    op = "SoftmaxCrossEntropy"
+    a, w_t, b = _head_args(op, a, w_t, bias)
+    m, (n, k) = a.shape[0], w_t.shape
+    target = _per_row(op, target, (m,), np.int32, "targets")
+    lse = _per_row(op, lse, (m,), np.float32, "lse")
+    grad = None if grad is None else _per_row(op, grad, (m,), np.float32, "grad")
+    da, dw, db = _loss_grads(a, w_t)
+    _check(_lib.lib().ppocr_xent_backward(_ptr(a), _ptr(w_t), _ptr(b), _ptr(target), _ptr(lse), _ptr(grad), m, n, k,
+                                          _ptr(da), _ptr(dw), _ptr(db)))
+    return da, dw, db
+
+
+def distill(a, w_t, bias, teacher_idx, teacher_logits, temperature=1.0):
+    """(loss [m], lse [m]): the divergence of the head's softmax from a teacher's, which is known by
+    the logits it gives to the classes teacher_idx [m, topk] (negative: absent), as topk returns
+    them."""
+    a, w_t, b = _head_args("Distill", a, w_t, bias)
+    m, (n, k) = a.shape[0], w_t.shape
+    idx, z = _teacher_args(m, teacher_idx, teacher_logits)
+    loss, lse = np.empty(m, np.float32), np.empty(m, np.float32)
+    _check(_lib.lib().ppocr_distill_forward(_ptr(a), _ptr(w_t), _ptr(b), _ptr(idx), _ptr(z), idx.shape[1],
+                                            float(temperature), m, n, k, _ptr(loss), _ptr(lse)))
+    return loss, lse
+
+
+def distill_backward(a, w_t, bias, teacher_idx, teacher_logits, temperature, lse, grad=None):
+    """(da [m, k], dw_t [n, k], dbias [n]) of distill, lse being its second result and grad [m] the
+    gradient by each row's loss (None: 1)."""
+    a, w_t, b = _head_args("Distill", a, w_t, bias)
+    m, (n, k) = a.shape[0], w_t.shape
+    idx, z = _teacher_args(m, teacher_idx, teacher_logits)
+    lse = _per_row("Distill", lse, (m,), np.float32, "lse")
+    grad = None if grad is None else _per_row("Distill", grad, (m,), np.float32, "grad")
+    da, dw, db = _loss_grads(a, w_t)
+    _check(_lib.lib().ppocr_distill_backward(_ptr(a), _ptr(w_t), _ptr(b), _ptr(idx), _ptr(z), idx.shape[1],
+                                             float(temperature), _ptr(lse), _ptr(grad), m, n, k, _ptr(da), _ptr(dw),
+                                             _ptr(db)))
+    return da, dw, db
+
+
+def topk(x, k):
+    """(columns, values), each [rows, k]: the k largest values of each row of x [rows, cols], largest
+    first, equal ones by column; NaN is never taken, missing places hold -1 and -inf."""
+    x = _f32(x)
+    if x.ndim != 2:
+        raise OcrError("TopK", f"expected [rows, cols], got {list(x.shape)}")
+    idx, val = np.empty((x.shape[0], max(int(k), 0)), np.int32), np.empty((x.shape[0], max(int(k), 0)), np.float32)
+    _check(_lib.lib().ppocr_topk_rows(_ptr(x), x.shape[0], x.shape[1], int(k), _ptr(idx), _ptr(val)))
+    return idx, val
+
+
+def _norm_rows(x, *vectors):
+    x = _f32(x)
+    if x.ndim != 2:
+        raise OcrError("LayerNorm", f"expected [m, d], got {list(x.shape)}")
+    return (x,) + tuple(_per_row("LayerNorm", v, (x.shape[1],), np.float32, "weights") for v in vectors)
+
+
+def layer_norm(x, w, b, eps):
+    """(y, mean, rstd) of rows x [m, d] (layer_norm, src/ops/layernorm.rs:5-244), with the statistics
+    that layer_norm_backward takes."""
+    x, w, b = _norm_rows(x, w, b)
+    m, d = x.shape
+    y, mean, rstd = np.empty_like(x), np.empty(m, np.float32), np.empty(m, np.float32)
+    _check(_lib.lib().ppocr_layernorm_forward(_ptr(x), _ptr(w), _ptr(b), m, d, float(eps), _ptr(y), _ptr(mean),
+                                              _ptr(rstd)))
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, w, mean, rstd):
+    """(dx [m, d], dw [d], db [d]) of layer_norm."""
+    x, w = _norm_rows(x, w)
+    m, d = x.shape
+    dy = _per_row("LayerNorm", dy, (m, d), np.float32, "dy")
+    mean, rstd = (_per_row("LayerNorm", v, (m,), np.float32, "statistics") for v in (mean, rstd))
+    dx, dw, db = np.empty_like(x), np.empty(d, np.float32), np.empty(d, np.float32)
+    _check(_lib.lib().ppocr_layernorm_backward(_ptr(dy), _ptr(x), _ptr(w), _ptr(mean), _ptr(rstd), m, d, _ptr(dx),
+                                               _ptr(dw), _ptr(db)))
+    return dx, dw, db

@@ -26,6 +26,9 @@ MODE_AUTO = 5
 NECK_ROWS = 0
 NECK_CHANNELS_FIRST = 1
 
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
@@ -90,6 +93,27 @@ SIGNATURES = {
     "ppocr_rn_forward_marked_dev": (_int, [_vp, _vp, _vp, _i64, _vp, _i64, _int, _vp, _vp, _sz, _vp,
                                            ctypes.POINTER(_vp), _int, ctypes.POINTER(ctypes.c_char_p),
                                            ctypes.POINTER(_int)]),
+    "ppocr_xent_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "ppocr_xent_forward": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "ppocr_xent_forward_dev": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp, _sz, _vp]),
+    "ppocr_xent_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "ppocr_xent_backward_dev": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _sz,
+                                     _vp]),
+    "ppocr_distill_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int]),
+    "ppocr_distill_forward": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, ctypes.c_float, _i64, _i64, _i64, _vp, _vp]),
+    "ppocr_distill_forward_dev": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, ctypes.c_float, _i64, _i64, _i64, _int, _vp,
+                                       _vp, _vp, _sz, _vp]),
+    "ppocr_distill_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, ctypes.c_float, _vp, _vp, _i64, _i64, _i64, _vp,
+                                    _vp, _vp]),
+    "ppocr_distill_backward_dev": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, ctypes.c_float, _vp, _vp, _i64, _i64, _i64,
+                                        _int, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ppocr_topk_rows": (_int, [_vp, _i64, _i64, _i64, _vp, _vp]),
+    "ppocr_topk_rows_dev": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "ppocr_layernorm_forward": (_int, [_vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp, _vp, _vp]),
+    "ppocr_layernorm_forward_dev": (_int, [_vp, _vp, _vp, _i64, _i64, ctypes.c_float, _int, _vp, _vp, _vp, _vp]),
+    "ppocr_layernorm_workspace_bytes": (_sz, [_i64, _i64]),
+    "ppocr_layernorm_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "ppocr_layernorm_backward_dev": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None
