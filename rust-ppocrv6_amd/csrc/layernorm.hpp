@@ -5,8 +5,7 @@
 namespace ppocr {
 
 constexpr int64_t kLayerNormMaxD = 16384;
-constexpr int kLayerNormParts = 512;  // workgroups of the backward pass, one partial sum of dw and db each
-
+// Workgroups of the backward pass, each with a sum of dw and db of its own.
 int layernorm_parts(int64_t m, int64_t d);
 int launch_layernorm_forward(const void* x, const float* w, const float* b, int64_t m, int d, float eps, int bf16, void* y,
                              float* mean, float* rstd, hipStream_t st);
