@@ -28,28 +28,6 @@ struct Targets {
     __device__ __forceinline__ float logit(int64_t r, int i) const { return target ? 0.0f : z[r * tn + i] * inv_tau; }
 };
 
-// The teacher's softmax over a row's entries, by 8 neighbouring lanes: the largest logit and the
-// sum of exp(logit - largest); a row without entries (or with only -inf) has sum 0.
-__device__ __forceinline__ void teacher_stats(const Targets& tg, int64_t r, bool live, int l8, float* top, float* sum) {
-    float m = -INFINITY;
-    bool bad = false;
-    for (int i = l8; i < tg.tn; i += 8)
-        if (live && tg.cls(r, i) >= 0) {
-            const float t = tg.logit(r, i);
-            bad |= !(t < INFINITY);
-            m = fmaxf(m, t);
-        }
-#pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    float s = bad ? NAN : 0.0f;
-    for (int i = l8; i < tg.tn; i += 8)
-        if (live && m > -INFINITY && tg.cls(r, i) >= 0) s += expf(tg.logit(r, i) - m);
-#pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-    *top = m;
-    *sum = s;
-}
-
 // a_r . w_c + b_c, by 8 neighbouring lanes (all of them call it); 0 for c < 0.
 template <typename T>
 __device__ __forceinline__ float logit_of(const T* __restrict__ a, const T* __restrict__ w, const float* bias, int64_t r,
@@ -58,11 +36,56 @@ __device__ __forceinline__ float logit_of(const T* __restrict__ a, const T* __re
     if (c >= 0) {
         const T* pa = a + r * k;
         const T* pw = w + (int64_t)c * k;
-        for (int j = l8; j < k; j += 8) s = fmaf(value(pa + j), value(pw + j), s);
+        int j = l8;
+        for (; j + 24 < k; j += 32) {
+            float x[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = value(pa + j + 8 * i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = value(pw + j + 8 * i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s = fmaf(x[i], y[i], s);
+        }
+        for (; j < k; j += 8) s = fmaf(value(pa + j), value(pw + j), s);
     }
 #pragma unroll
     for (int o = 4; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
     return c >= 0 && bias ? s + bias[c] : s;
+}
+
+// One row by a wave: lane i holds the row's entry i, its class (-1: none, or past the last), the log of
+// its weight and the weight (0 for none), and the head's logit for it.
+struct RowTargets {
+    int cls;
+    float logq, q, z;
+};
+template <typename T>
+__device__ __forceinline__ RowTargets row_targets(const Targets& tg, const T* a, const T* w, const float* bias, int64_t r,
+                                                  int k, int lane) {
+    RowTargets t;
+    t.cls = lane < tg.tn ? tg.cls(r, lane) : -1;
+    if (tg.target) {
+        t.logq = 0.0f;
+        t.q = t.cls >= 0 ? 1.0f : 0.0f;
+    } else {
+        const float x = t.cls >= 0 ? tg.logit(r, lane) : -INFINITY;
+        float top = x;  // NaN is left out here and returns with the sum
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        const float e = top == -INFINITY ? (x == x ? 0.0f : x) : expf(x - top);
+        const float sum = wave_sum(e);
+        t.logq = x - top - logf(sum);
+        t.q = sum == 0.0f ? 0.0f : e / sum;
+        if (!(t.q != 0.0f)) t.logq = 0.0f;
+    }
+    t.z = 0.0f;
+    for (int i = 0; i < tg.tn; i += 8) {
+        const int c = __shfl(t.cls, i + (lane >> 3), 64);
+        const float z = logit_of(a, w, bias, r, i + (lane >> 3) < tg.tn ? c : -1, k, lane & 7);
+        const float here = __shfl(z, (lane & 7) * 8, 64);
+        if ((lane & ~7) == i) t.z = here;
+    }
+    return t;
 }
 
 // A row's gradient factor: g / tau when it has a target, 0 otherwise.
@@ -83,54 +106,90 @@ struct RecordArgs {
     const float* lse;
     const float* grad;
     int64_t m, n, row_tiles;
-    int k, D;
+    int k, vec_a, vec_w;  // rows that can be read four values at a time
     uint8_t* row_rec;
     uint8_t* class_rec;
     int* row_u;
     int* class_u;
 };
 
-template <typename T, int P, bool BACK>
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+    T v[4];
+};
+
+template <typename T, int D, int P, bool BACK>
 __device__ void build_record(const RecordArgs<T>& x, int64_t t, bool rows, float* tile, float* red) {
-    const int tid = threadIdx.x, D = x.D, ld = 32 * D + 1;
+    constexpr int LD = 32 * D + 1;
+    const int tid = threadIdx.x, e = tid >> 3, l8 = tid & 7;  // 8 lanes an entry
     const int64_t first = t * 32, count = min((int64_t)32, (rows ? x.m : x.n) - first);
-    const T* src = (rows ? x.a : x.w) + first * x.k;
     float* gf = red + 8;  // 32 gradient factors
-    if (BACK && rows && tid < 32) gf[tid] = tid < count ? factor_of(x.tg, x.grad, first + tid) : 0.0f;
-    __syncthreads();
-    float top = 0.0f;
-    for (int i = tid; i < 32 * 32 * D; i += kThreads) {
-        const int e = i / (32 * D), j = i % (32 * D);
-        // a row without gradient reaches no sum, whatever it holds
-        const bool in = e < count && j < x.k && !(BACK && rows && gf[e] == 0.0f);
-        const float v = in ? value(src + (int64_t)e * x.k + j) : 0.0f;
-        tile[e * ld + j] = v;
-        if (fabsf(v) < INFINITY) top = fmaxf(top, fabsf(v));
+    float factor = 1.0f;
+    if (BACK && rows) {
+        factor = e < count ? factor_of(x.tg, x.grad, first + e) : 0.0f;
+        if (l8 == 0) gf[e] = factor;
     }
+    // a row without gradient reaches no sum, whatever it holds
+    const bool in = e < count && factor != 0.0f;
+    const T* src = (rows ? x.a : x.w) + (first + (e < count ? e : 0)) * x.k;
+    float v[4 * D];
+    if (rows ? x.vec_a : x.vec_w) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            const int j = 32 * i + 4 * l8;
+            Four<T> q{};
+            if (in && j < x.k) q = *reinterpret_cast<const Four<T>*>(src + j);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[4 * i + u] = value(q.v + u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4 * D; ++i) {
+            const int j = 32 * (i >> 2) + 4 * l8 + (i & 3);
+            v[i] = in && j < x.k ? value(src + j) : 0.0f;
+        }
+    }
+    float top = 0.0f, ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4 * D; ++i) {
+        tile[e * LD + 32 * (i >> 2) + 4 * l8 + (i & 3)] = v[i];
+        ss = fmaf(v[i], v[i], ss);
+        if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
+    }
+#pragma unroll
+    for (int o = 4; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
     top = wave_max(top);
-    if ((tid & 63) == 0) red[tid >> 6] = top;
+    const bool odd = __any(!(ss < INFINITY));
+    ss = wave_max(ss);
+    if ((tid & 63) == 0) {
+        red[tid >> 6] = top;
+        red[4 + (tid >> 6)] = odd ? INFINITY : ss;
+    }
     __syncthreads();
     top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     // largest magnitude to [2^14, 2^15); 2^100 at most, so that 2^-e and the factors stay in range
     const int ex = top > 0.0f ? min(14 - ilogbf(top), 100) : 100;
     uint8_t* rec = (rows ? x.row_rec : x.class_rec) + t * (int64_t)((size_t)P * D * 2048 * (BACK ? 2 : 1) + kXentAux);
-    const int form = 2 * D * 64;  // 16-byte pieces of one plane of one form
-    for (int i = tid; i < form * (BACK ? 2 : 1); i += kThreads) {
-        const bool tr = i >= form;
-        const int c = tr ? i - form : i, lane = c & 63, l = lane & 31, h = lane >> 5, step = c >> 6;
-        f16x8 hi, lo;
+    constexpr int FORM = 2 * D * 64;  // 16-byte pieces of one plane of one form
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            // transposed: step = 2 d + e, the entries of an MFMA result's rows
-            const int e = tr ? 16 * (step & 1) + 8 * (j >> 2) + 4 * h + (j & 3) : l;
-            const int kk = tr ? 32 * (step >> 1) + l : 16 * step + 8 * h + j;
-            const float v = ldexpf(tile[e * ld + kk], ex);
-            hi[j] = (_Float16)v;
-            if (P == 2) lo[j] = (_Float16)(v - (float)hi[j]);
-        }
+    for (int tr = 0; tr < (BACK ? 2 : 1); ++tr) {
         f16x8* dst = reinterpret_cast<f16x8*>(rec + (tr ? (size_t)P * D * 2048 : 0));
-        dst[c] = hi;
-        if (P == 2) dst[form + c] = lo;
+#pragma unroll
+        for (int c = tid; c < FORM; c += kThreads) {
+            const int lane = c & 63, l = lane & 31, h = lane >> 5, step = c >> 6;
+            f16x8 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // transposed: step = 2 d + e, the entries of an MFMA result's rows
+                const int en = tr ? 16 * (step & 1) + 8 * (j >> 2) + 4 * h + (j & 3) : l;
+                const int kk = tr ? 32 * (step >> 1) + l : 16 * step + 8 * h + j;
+                const float f = ldexpf(tile[en * LD + kk], ex);
+                hi[j] = (_Float16)f;
+                if (P == 2) lo[j] = (_Float16)(f - (float)hi[j]);
+            }
+            dst[c] = hi;
+            if (P == 2) dst[FORM + c] = lo;
+        }
     }
     float* aux = reinterpret_cast<float*>(rec + (size_t)P * D * 2048 * (BACK ? 2 : 1));
     if (tid < 32) {
@@ -145,7 +204,13 @@ __device__ void build_record(const RecordArgs<T>& x, int64_t t, bool rows, float
             aux[32 + tid] = 0.0f;
         }
     } else if (tid < 48) {
-        aux[32 + tid] = tid == 32 ? ldexpf(1.0f, -ex) : tid == 33 ? (float)ex : 0.0f;
+        const float norm = sqrtf(fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7])));
+        float most = 0.0f;
+        for (int i = 0; i < (int)count && !rows && x.bias; ++i) {
+            const float b = fabsf(x.bias[first + i] * (kLog2e * x.tg.inv_tau));
+            most = b < INFINITY ? fmaxf(most, b) : most;
+        }
+        aux[32 + tid] = tid == 32 ? ldexpf(1.0f, -ex) : tid == 33 ? (float)ex : tid == 34 ? norm : tid == 35 ? most : 0.0f;
     }
     if (BACK && tid == 0) {
         float s = 0.0f;
@@ -170,36 +235,49 @@ struct ListArgs {
     const float* lse;
     const float* grad;
     int64_t m;
-    int k, list, size, blocks;  // list = 32 tn entries, size = list rounded up to a power of two
+    int k, list, size, blocks;  // list = 32 tn entries, size = list rounded up to a power of two; blocks of 128 classes
     uint32_t* keys;
     float* vals;
     uint16_t* offs;
 };
 constexpr uint32_t kNoKey = 0xFFFFFFFFu;
 
-template <typename T>
+template <typename T, int NT>
 __device__ void build_list(const ListArgs<T>& x, int64_t g, unsigned long long* key, float* pv, float* qv) {
-    const int tid = threadIdx.x, l8 = tid & 7, row = tid >> 3, tn = x.tg.tn;
-    const int64_t r = g * 32 + row;
-    const bool live = r < x.m && factor_of(x.tg, x.grad, r) != 0.0f;
-    float top = 0.0f, sum = 1.0f;
-    if (!x.tg.target) teacher_stats(x.tg, r, live, l8, &top, &sum);
-    for (int i = 0; i < tn; ++i) {
-        const int c = live ? x.tg.cls(r, i) : -1;
-        const float z = logit_of(x.a, x.w, x.bias, r, c, x.k, l8);
-        if (l8 == 0) {
-            const int s = row * tn + i;
-            const float q = x.tg.target ? 1.0f : (c >= 0 ? expf(x.tg.logit(r, i) - top) / sum : 0.0f);
-            key[s] = c >= 0 ? ((unsigned long long)(((uint32_t)c << 5) | row) << 11) | s : ~0ull;
-            pv[s] = c >= 0 ? expf(z * x.tg.inv_tau - x.lse[r]) : 0.0f;
-            qv[s] = q;
+    const int tid = threadIdx.x, tn = x.tg.tn;
+    auto put = [&](int s, int row, int c, float z, float q, float lse) {
+        key[s] = c >= 0 ? ((unsigned long long)(((uint32_t)c << 5) | row) << 11) | s : ~0ull;
+        pv[s] = c >= 0 ? expf(z * x.tg.inv_tau - lse) : 0.0f;
+        qv[s] = q;
+    };
+    if (tn == 1 && x.tg.target) {
+        // 8 lanes a row
+        for (int row = tid >> 3; row < 32; row += NT / 8) {
+            const int64_t r = g * 32 + row;
+            const bool live = r < x.m && factor_of(x.tg, x.grad, r) != 0.0f;
+            const int c = live ? x.tg.cls(r, 0) : -1;
+            const float z = logit_of(x.a, x.w, x.bias, r, c, x.k, tid & 7);
+            if ((tid & 7) == 0) put(row, row, c, z, 1.0f, c >= 0 ? x.lse[r] : 0.0f);
+        }
+    } else {
+        // a wave a row
+        for (int row = tid >> 6; row < 32; row += NT / 64) {
+            const int64_t r = g * 32 + row;
+            const bool live = r < x.m && factor_of(x.tg, x.grad, r) != 0.0f;
+            const int lane = tid & 63;
+            if (live) {
+                const RowTargets t = row_targets(x.tg, x.a, x.w, x.bias, r, x.k, lane);
+                if (lane < tn) put(row * tn + lane, row, t.cls, t.z, t.q, x.lse[r]);
+            } else if (lane < tn) {
+                put(row * tn + lane, row, -1, 0.0f, 0.0f, 0.0f);
+            }
         }
     }
-    for (int s = x.list + tid; s < x.size; s += kThreads) key[s] = ~0ull;
+    for (int s = x.list + tid; s < x.size; s += NT) key[s] = ~0ull;
     __syncthreads();
     for (int w2 = 2; w2 <= x.size; w2 <<= 1)
         for (int d = w2 >> 1; d >= 1; d >>= 1) {
-            for (int p = tid; p < x.size / 2; p += kThreads) {
+            for (int p = tid; p < x.size / 2; p += NT) {
                 const int i = 2 * d * (p / d) + p % d, j = i + d;
                 const bool up = (i & w2) == 0;
                 const unsigned long long a = key[i], b = key[j];
@@ -210,7 +288,7 @@ __device__ void build_list(const ListArgs<T>& x, int64_t g, unsigned long long* 
             }
             __syncthreads();
         }
-    for (int s = tid; s < x.list; s += kThreads) {
+    for (int s = tid; s < x.list; s += NT) {
         const uint32_t kk = key[s] == ~0ull ? kNoKey : (uint32_t)(key[s] >> 11);
         float v = 0.0f;
         if (kk != kNoKey) {
@@ -225,7 +303,7 @@ __device__ void build_list(const ListArgs<T>& x, int64_t g, unsigned long long* 
         x.keys[g * x.list + s] = kk;
         x.vals[g * x.list + s] = v;
     }
-    for (int b = tid; b <= x.blocks; b += kThreads) {
+    for (int b = tid; b <= x.blocks; b += NT) {
         const unsigned long long lim = (unsigned long long)b << (7 + 5 + 11);
         int lo = 0, hi = x.list;
         while (lo < hi) {
@@ -237,65 +315,58 @@ __device__ void build_list(const ListArgs<T>& x, int64_t g, unsigned long long* 
     }
 }
 
-// LDS: a record's tile, or a list's keys and values.
-size_t prep_lds(int D, int size) {
-    return std::max((size_t)(32 * (32 * D + 1) + 8 + 32) * 4, (size_t)size * 16);
-}
-
-template <typename T, int P, bool BACK>
+// Records, and with one target a row (a label) the lists too.
+template <typename T, int D, int P, bool BACK>
 __global__ __launch_bounds__(kThreads) void prep_kernel(RecordArgs<T> x, ListArgs<T> y, unsigned class_tiles) {
-    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ __align__(16) float lds[32 * (32 * D + 1) + 8 + 32];
+    static_assert(sizeof(lds) >= 32 * 16, "a list of 32 entries");
     const unsigned b = blockIdx.x;
     if (b < x.row_tiles + class_tiles) {
-        float* tile = reinterpret_cast<float*>(lds);
         const bool rows = b < x.row_tiles;
-        build_record<T, P, BACK>(x, rows ? b : b - x.row_tiles, rows, tile, tile + 32 * (32 * x.D + 1));
+        build_record<T, D, P, BACK>(x, rows ? b : b - x.row_tiles, rows, lds, lds + 32 * (32 * D + 1));
     } else if constexpr (BACK) {
         unsigned long long* key = reinterpret_cast<unsigned long long*>(lds);
-        float* pv = reinterpret_cast<float*>(key + y.size);
-        build_list<T>(y, b - x.row_tiles - class_tiles, key, pv, pv + y.size);
+        float* pv = reinterpret_cast<float*>(key + 32);
+        build_list<T, kThreads>(y, b - x.row_tiles - class_tiles, key, pv, pv + 32);
     }
+}
+constexpr int kListThreads = 1024;
+template <typename T>
+__global__ __launch_bounds__(kListThreads) void list_kernel(ListArgs<T> y) {
+    extern __shared__ __align__(16) uint8_t list_lds[];
+    unsigned long long* key = reinterpret_cast<unsigned long long*>(list_lds);
+    float* pv = reinterpret_cast<float*>(key + y.size);
+    build_list<T, kListThreads>(y, blockIdx.x, key, pv, pv + y.size);
 }
 
 // ---------------------------------------------------------------- forward: merge and loss
-// Eight rows per wave, 8 lanes each: the chunks' statistics of a row, then its target's logits.
+// A wave per row: the chunks' statistics of the row, then its targets' logits.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void loss_kernel(const T* a, const T* w, const float* bias, Targets tg, int64_t m,
                                                         int k, int nsplit, const float2* __restrict__ part, float* loss,
                                                         float* lse) {
-    const int l8 = threadIdx.x & 7;
-    const int64_t row = (int64_t)blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3);
-    const bool live = row < m;
-    const int64_t r = live ? row : m - 1;
-    float ref = -INFINITY;
-    for (int s = l8; s < nsplit; s += 8) ref = fmaxf(ref, part[(int64_t)s * m + r].x);
-#pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) ref = fmaxf(ref, __shfl_xor(ref, o, 64));
-    float sum = 0.0f;
-    for (int s = l8; s < nsplit; s += 8) {
-        const float2 v = part[(int64_t)s * m + r];
-        sum += v.x == -INFINITY ? v.y : v.y * exp2f(v.x - ref);
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    if (row >= m) return;
+    const RowTargets t = row_targets(tg, a, w, bias, row, k, lane);
+    float ref = -INFINITY, sum = 0.0f;
+    for (int s = lane; s < nsplit; s += 64) {
+        const float2 v = part[(int64_t)s * m + row];
+        const float nr = fmaxf(ref, v.x);
+        sum = (ref == -INFINITY ? sum : sum * exp2f(ref - nr)) + (v.x == -INFINITY ? v.y : v.y * exp2f(v.x - nr));
+        ref = nr;
     }
 #pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    for (int o = 32; o >= 1; o >>= 1) {
+        const float r2 = __shfl_xor(ref, o, 64), s2 = __shfl_xor(sum, o, 64), nr = fmaxf(ref, r2);
+        sum = (ref == -INFINITY ? sum : sum * exp2f(ref - nr)) + (r2 == -INFINITY ? s2 : s2 * exp2f(r2 - nr));
+        ref = nr;
+    }
     // a row whose classes are all -inf keeps reference -inf and sum 0
     const float l = (ref == -INFINITY ? 0.0f : ref * (1.0f / kLog2e)) + logf(sum);
-    float top = 0.0f, qs = 1.0f, total = 0.0f;
-    if (!tg.target) teacher_stats(tg, r, true, l8, &top, &qs);
-    const float logqs = logf(qs);
-    for (int i = 0; i < tg.tn; ++i) {
-        const int c = tg.cls(r, i);
-        const float z = logit_of(a, w, bias, r, c, k, l8);
-        if (c < 0) continue;
-        if (tg.target) {
-            total = l - z * tg.inv_tau;
-        } else if (qs != 0.0f) {
-            const float lq = tg.logit(r, i) - top - logqs;
-            const float q = expf(lq);
-            if (q != 0.0f) total += q * (lq - z * tg.inv_tau + l);
-        }
-    }
-    if (live && l8 == 0) {
+    // entries without weight add nothing, whatever their class's logit
+    const float total = wave_sum(t.q != 0.0f ? t.q * (t.logq - t.z * tg.inv_tau + l) : 0.0f);
+    if (lane == 0) {
         loss[row] = total;
         lse[row] = l;
     }
@@ -303,6 +374,14 @@ __global__ __launch_bounds__(kThreads) void loss_kernel(const T* a, const T* w, 
 
 // ---------------------------------------------------------------- backward: sums of the chunks
 // out[o][j] = sum over chunks, for owners of k values held in rows of 32 D; then db.
+template <typename T>
+struct SumArgs {
+    const float* part;
+    int nsplit;
+    int64_t owners;
+    T* out;  // null: not asked for
+    int vec;  // out's rows can be written four values at a time
+};
 template <typename T>
 __device__ __forceinline__ void store(T* p, float v);
 template <>
@@ -314,94 +393,164 @@ __device__ __forceinline__ void store<uint16_t>(uint16_t* p, float v) {
     *p = __builtin_bit_cast(uint16_t, (__bf16)v);
 }
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sum_kernel(const float* __restrict__ part, int nsplit, int64_t owners, int k, int ld,
-                                                       T* out, const float* __restrict__ part_db, float* db) {
-    const int64_t stride = (int64_t)gridDim.x * kThreads, base = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (out) {
-        for (int64_t i = base; i < owners * k; i += stride) {
-            const int64_t at = i / k * ld + i % k;
-            float s = 0.0f;
-            for (int c = 0; c < nsplit; ++c) s += part[(int64_t)c * owners * ld + at];
-            store<T>(out + i, s);
+__device__ __forceinline__ void sum_chunks(const SumArgs<T>& x, int k, int ld, int64_t block, int64_t blocks) {
+    const unsigned quads = (unsigned)(ld / 4);
+    const int64_t all = x.owners * quads, plane = x.owners * ld;
+    for (int64_t i = block * kThreads + threadIdx.x; i < all; i += blocks * kThreads) {
+        const int64_t o = i / quads;
+        const int j = (int)(i - o * quads) * 4;
+        if (j >= k) continue;
+        f32x4 s = {};
+        for (int c = 0; c < x.nsplit; ++c) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(x.part + c * plane + i * 4);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s[u] += v[u];
+        }
+        T* out = x.out + o * k + j;
+        if (x.vec) {
+            Four<T> q;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) store<T>(q.v + u, s[u]);
+            *reinterpret_cast<Four<T>*>(out) = q;
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (j + u < k) store<T>(out + u, s[u]);
         }
     }
-    if (db) {
-        for (int64_t i = base; i < owners; i += stride) {
+}
+// da by the first `grid_a` workgroups, dW and db by the others.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs<T> a, SumArgs<T> w, int k, int ld, unsigned grid_a,
+                                                       const float* __restrict__ part_db, float* db) {
+    if (blockIdx.x < grid_a) {
+        sum_chunks<T>(a, k, ld, blockIdx.x, grid_a);
+        return;
+    }
+    const int64_t block = blockIdx.x - grid_a, blocks = gridDim.x - grid_a;
+    if (w.out) sum_chunks<T>(w, k, ld, block, blocks);
+    if (db)
+        for (int64_t i = block * kThreads + threadIdx.x; i < w.owners; i += blocks * kThreads) {
             float s = 0.0f;
-            for (int c = 0; c < nsplit; ++c) s += part_db[(int64_t)c * owners + i];
+            for (int c = 0; c < w.nsplit; ++c) s += part_db[c * w.owners + i];
             db[i] = s;
         }
-    }
 }
 
-// Chunks of the streamed records, so that the workgroups fill the GPU's places in whole rounds: the
-// fewest records in a row that any place works through, then the fewest chunks.
-int pick_split(int64_t blocks, int64_t tiles, int per_cu, int multiple, int most) {
-    const int64_t places = 256 * (int64_t)per_cu;
+// ---------------------------------------------------------------- shapes and launches
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+constexpr int kBlockTiles = 4;  // records of a block of 128 classes
+constexpr int kMostChunks = 64;
+
+// Chunks of the class records for the statistics: the fewest records that any place of the GPU works
+// through one after the other (a workgroup's start and end take about two records' time).
+void pick_stats(XentLayout* L, int64_t m, int planes) {
+    L->fblocks = m <= 128 ? 1 : xent_stats_most_blocks(L->D, planes);
+    const int64_t blocks = div_up(m, 128 * L->fblocks), places = 512;
     int64_t best = -1;
-    int pick = 1;
-    for (int s = 1; s <= most; ++s) {
-        int64_t per = (tiles + s - 1) / s;
-        per = (per + multiple - 1) / multiple * multiple;
-        if ((per * (s - 1)) >= tiles && s > 1) continue;  // an empty chunk
-        const int64_t rounds = (blocks * s + places - 1) / places;
-        const int64_t cost = rounds * (per + 2) + s / 16;  // a workgroup's start and end take about two records' time
+    for (int s = 1; s <= 256; ++s) {
+        const int64_t per = div_up(L->class_tiles, s);
+        if (div_up(L->class_tiles, per) != s) continue;
+        const int64_t cost = 8 * div_up(blocks * s, places) * (per + 2) + s / 4;
         if (best < 0 || cost < best) {
             best = cost;
-            pick = s;
+            L->fsplit = s;
+            L->fper = (int)per;
         }
     }
-    return pick;
 }
-int per_split(int64_t tiles, int split, int multiple) {
-    const int64_t per = (tiles + split - 1) / split;
-    return (int)((per + multiple - 1) / multiple * multiple);
-}
-constexpr int kBlockTiles = 4;  // records of a block of 128 classes
 
-template <typename T, int P, bool BACK>
-int prep(const XentProblem& x, const XentLayout& L, const Targets& tg, uint8_t* ws, hipStream_t st) {
-    RecordArgs<T> r{static_cast<const T*>(x.a), static_cast<const T*>(x.w), x.bias, tg, x.lse, x.grad, x.m, x.n,
-                    L.row_tiles, x.k, L.D, ws + (BACK ? L.b_row_rec : L.f_row_rec),
-                    ws + (BACK ? L.b_class_rec : L.f_class_rec), reinterpret_cast<int*>(ws + L.b_row_u),
-                    reinterpret_cast<int*>(ws + L.b_class_e)};
-    const int list = 32 * x.tn;
-    int size = 32;
-    while (size < list) size *= 2;
-    ListArgs<T> y{r.a, r.w, x.bias, tg, x.lse, x.grad, x.m, x.k, list, size, (int)((x.n + 127) / 128),
-                  reinterpret_cast<uint32_t*>(ws + L.b_keys), reinterpret_cast<float*>(ws + L.b_vals),
-                  reinterpret_cast<uint16_t*>(ws + L.b_offs)};
-    const int64_t grid = L.row_tiles * (BACK ? 2 : 1) + L.class_tiles;
-    prep_kernel<T, P, BACK><<<(unsigned)grid, kThreads, prep_lds(L.D, BACK ? size : 0), st>>>(r, y, (unsigned)L.class_tiles);
+// Chunks for the two gradients, whose workgroups share a launch: the same number of records for both,
+// the fewest that any place works through; a further chunk costs the time its sums take to be written
+// and read again (256 D bytes an owner at 5 TB/s, against 0.36 or 0.16 D us a record).
+void pick_grads(XentLayout* L, int64_t m, int64_t n, int planes) {
+    const int64_t places = 256 * xent_grad_per_cu(L->D, planes);
+    const int64_t ba = div_up(m, kXentGradOwners), bw = div_up(n, kXentGradOwners);
+    const double chunk_cost = 256.0 / 5e6 / (planes == 2 ? 0.36 : 0.16);
+    double best = -1.0;
+    for (int s = 1; s <= kMostChunks; ++s) {
+        // s chunks of the shorter side's stream; the other's of the same length
+        const bool by_a = L->class_tiles <= L->row_tiles;
+        const int64_t per = div_up(div_up(by_a ? L->class_tiles : L->row_tiles, s), kBlockTiles) * kBlockTiles;
+        const int64_t sa = div_up(L->class_tiles, per), sw = div_up(L->row_tiles, per);
+        if (sa > kMostChunks || sw > kMostChunks) break;
+        const double cost = (double)div_up(ba * sa + bw * sw, places) * (double)(per + 2) +
+                            chunk_cost * (double)(sa * m + sw * n);
+        if (best < 0 || cost < best) {
+            best = cost;
+            L->split_a = (int)sa;
+            L->split_w = (int)sw;
+            L->per_a = L->per_w = (int)per;
+        }
+    }
+    if (best < 0) {  // streams of very different lengths: whole, or in the most chunks
+        L->per_a = (int)(div_up(div_up(L->class_tiles, kMostChunks), kBlockTiles) * kBlockTiles);
+        L->per_w = (int)div_up(L->row_tiles, kMostChunks);
+        L->split_a = (int)div_up(L->class_tiles, L->per_a);
+        L->split_w = (int)div_up(L->row_tiles, L->per_w);
+    }
+}
+
+bool in_fours(const void* p, int k, bool bf16) { return k % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (bf16 ? 8 : 16) == 0; }
+
+Targets targets_of(const XentProblem& x) {
+    return Targets{x.target, x.teacher_idx, x.teacher_z, x.tn, 1.0f / x.tau, x.n};
+}
+
+template <typename T, int D, int P, bool BACK>
+int prep_cfg(const RecordArgs<T>& r, const ListArgs<T>& y, unsigned class_tiles, unsigned grid, hipStream_t st) {
+    prep_kernel<T, D, P, BACK><<<grid, kThreads, 0, st>>>(r, y, class_tiles);
     PPOCR_HIP(hipGetLastError());
     return PPOCR_OK;
 }
 
-template <int P>
-int stats_pass(int D, const XentStatsArgs& s, unsigned grid, hipStream_t st) {
+// f.template operator()<D>() for the layout's D.
+template <typename F>
+int by_pieces(int D, F&& f) {
     switch (D) {
-        case 1: return xent_stats_cfg<1, P>(s, grid, st);
-        case 2: return xent_stats_cfg<2, P>(s, grid, st);
-        case 3: return xent_stats_cfg<3, P>(s, grid, st);
-        case 4: return xent_stats_cfg<4, P>(s, grid, st);
-        case 6: return xent_stats_cfg<6, P>(s, grid, st);
-        default: return xent_stats_cfg<8, P>(s, grid, st);
-    }
-}
-template <int P, bool ROWS>
-int grad_pass(int D, const XentGradArgs& s, unsigned grid, hipStream_t st) {
-    switch (D) {
-        case 1: return xent_grad_cfg<1, P, ROWS>(s, grid, st);
-        case 2: return xent_grad_cfg<2, P, ROWS>(s, grid, st);
-        case 3: return xent_grad_cfg<3, P, ROWS>(s, grid, st);
-        case 4: return xent_grad_cfg<4, P, ROWS>(s, grid, st);
-        case 6: return xent_grad_cfg<6, P, ROWS>(s, grid, st);
-        default: return xent_grad_cfg<8, P, ROWS>(s, grid, st);
+        case 1: return f.template operator()<1>();
+        case 2: return f.template operator()<2>();
+        case 3: return f.template operator()<3>();
+        case 4: return f.template operator()<4>();
+        case 6: return f.template operator()<6>();
+        default: return f.template operator()<8>();
     }
 }
 
-Targets targets_of(const XentProblem& x) {
-    return Targets{x.target, x.teacher_idx, x.teacher_z, x.tn, 1.0f / x.tau, x.n};
+template <typename T, int P, bool BACK>
+int prep(const XentProblem& x, const XentLayout& L, uint8_t* ws, hipStream_t st) {
+    const Targets tg = targets_of(x);
+    const RecordArgs<T> r{static_cast<const T*>(x.a), static_cast<const T*>(x.w), x.bias, tg, x.lse, x.grad, x.m, x.n,
+                          L.row_tiles, x.k, in_fours(x.a, x.k, x.bf16), in_fours(x.w, x.k, x.bf16),
+                          ws + (BACK ? L.b_row_rec : L.f_row_rec), ws + (BACK ? L.b_class_rec : L.f_class_rec),
+                          reinterpret_cast<int*>(ws + L.b_row_u), reinterpret_cast<int*>(ws + L.b_class_e)};
+    const int list = 32 * x.tn;
+    int size = 32;
+    while (size < list) size *= 2;
+    const ListArgs<T> y{r.a, r.w, x.bias, tg, x.lse, x.grad, x.m, x.k, list, size, (int)div_up(x.n, 128),
+                        reinterpret_cast<uint32_t*>(ws + L.b_keys), reinterpret_cast<float*>(ws + L.b_vals),
+                        reinterpret_cast<uint16_t*>(ws + L.b_offs)};
+    const bool lists_here = BACK && x.target;
+    const unsigned grid = (unsigned)(L.row_tiles * (lists_here ? 2 : 1) + L.class_tiles);
+    if (int e = by_pieces(L.D, [&]<int D>() { return prep_cfg<T, D, P, BACK>(r, y, (unsigned)L.class_tiles, grid, st); }))
+        return e;
+    if (BACK && !x.target) {
+        list_kernel<T><<<(unsigned)L.row_tiles, kListThreads, (size_t)size * 16, st>>>(y);
+        PPOCR_HIP(hipGetLastError());
+    }
+    return PPOCR_OK;
+}
+
+template <typename T>
+int sums(const XentLayout& L, const float* pa, const float* pw, const float* pdb, int64_t m, int64_t n, int k, void* da,
+         void* dw, float* db, hipStream_t st) {
+    const bool bf16 = sizeof(T) == 2;
+    const SumArgs<T> a{pa, L.split_a, m, (T*)da, in_fours(da, k, bf16)}, w{pw, L.split_w, n, (T*)dw, in_fours(dw, k, bf16)};
+    auto blocks = [&](int64_t owners) { return (unsigned)std::min<int64_t>(div_up(owners * 8 * L.D, kThreads), 2048); };
+    const unsigned ga = da ? blocks(m) : 0, gw = dw || db ? blocks(n) : 0;
+    sum_kernel<T><<<ga + gw, kThreads, 0, st>>>(a, w, k, 32 * L.D, ga, pdb, db);
+    PPOCR_HIP(hipGetLastError());
+    return PPOCR_OK;
 }
 
 }  // namespace
@@ -412,13 +561,8 @@ XentLayout xent_layout(int64_t m, int64_t n, int64_t k, int tn, int planes) {
     L.planes = planes;
     L.row_tiles = xent_tiles(m);
     L.class_tiles = xent_tiles(n);
-    const int64_t frows = (m + xent_stats_rows(L.D, planes) - 1) / xent_stats_rows(L.D, planes),
-                  arows = (m + kXentGradOwners - 1) / kXentGradOwners,
-                  wrows = (n + kXentGradOwners - 1) / kXentGradOwners;
-    L.fsplit = pick_split(frows, L.class_tiles, 2, 1, 128);
-    const int occ = xent_grad_per_cu(L.D, planes);
-    L.gsplit_a = pick_split(arows, L.class_tiles, occ, kBlockTiles, 64);
-    L.gsplit_w = pick_split(wrows, L.row_tiles, occ, 1, 64);
+    pick_stats(&L, m, planes);
+    pick_grads(&L, m, n, planes);
     auto put = [](size_t* at, size_t bytes) {
         const size_t here = *at;
         *at += (bytes + 255) / 256 * 256;
@@ -437,10 +581,10 @@ XentLayout xent_layout(int64_t m, int64_t n, int64_t k, int tn, int planes) {
     L.b_class_e = put(&b, (size_t)L.class_tiles * 4);
     L.b_keys = put(&b, (size_t)L.row_tiles * 32 * tn * 4);
     L.b_vals = put(&b, (size_t)L.row_tiles * 32 * tn * 4);
-    L.b_offs = put(&b, (size_t)L.row_tiles * ((n + 127) / 128 + 1) * 2);
-    const size_t pa = (size_t)L.gsplit_a * m * 32 * L.D * 4, pw = (size_t)L.gsplit_w * n * 32 * L.D * 4;
-    L.b_part = put(&b, std::max(pa, pw));
-    L.b_part_db = put(&b, (size_t)L.gsplit_w * n * 4);
+    L.b_offs = put(&b, (size_t)L.row_tiles * (div_up(n, 128) + 1) * 2);
+    L.b_part_a = put(&b, (size_t)L.split_a * m * 32 * L.D * 4);
+    L.b_part_w = put(&b, (size_t)L.split_w * n * 32 * L.D * 4);
+    L.b_part_db = put(&b, (size_t)L.split_w * n * 4);
     L.b_total = b;
     return L;
 }
@@ -448,14 +592,15 @@ XentLayout xent_layout(int64_t m, int64_t n, int64_t k, int tn, int planes) {
 int launch_xent_forward(const XentProblem& x, float* loss, float* lse, uint8_t* ws, hipStream_t st) {
     const XentLayout L = xent_layout(x.m, x.n, x.k, x.tn, x.planes());
     const Targets tg = targets_of(x);
-    if (int e = x.bf16 ? prep<uint16_t, 1, false>(x, L, tg, ws, st) : prep<float, 2, false>(x, L, tg, ws, st)) return e;
+    if (int e = x.bf16 ? prep<uint16_t, 1, false>(x, L, ws, st) : prep<float, 2, false>(x, L, ws, st)) return e;
     float2* part = reinterpret_cast<float2*>(ws + L.f_part);
-    const int per = per_split(L.class_tiles, L.fsplit, 1);
-    XentStatsArgs s{ws + L.f_row_rec, ws + L.f_class_rec, x.m, L.class_tiles, L.fsplit, per, kLog2e / x.tau, part};
-    const int rows = xent_stats_rows(L.D, L.planes);
-    const unsigned grid = (unsigned)((x.m + rows - 1) / rows) * L.fsplit;
-    if (int e = x.bf16 ? stats_pass<1>(L.D, s, grid, st) : stats_pass<2>(L.D, s, grid, st)) return e;
-    const unsigned lg = (unsigned)((x.m + kThreads / 8 - 1) / (kThreads / 8));
+    const XentStatsArgs s{ws + L.f_row_rec, ws + L.f_class_rec, x.m, L.class_tiles, L.fsplit, L.fper, kLog2e / x.tau, part};
+    const unsigned grid = (unsigned)(div_up(x.m, 128 * L.fblocks) * L.fsplit);
+    if (int e = by_pieces(L.D, [&]<int D>() {
+            return x.bf16 ? xent_stats_cfg<D, 1>(s, L.fblocks, grid, st) : xent_stats_cfg<D, 2>(s, L.fblocks, grid, st);
+        }))
+        return e;
+    const unsigned lg = (unsigned)div_up(x.m, kThreads / 64);
     if (x.bf16)
         loss_kernel<uint16_t><<<lg, kThreads, 0, st>>>((const uint16_t*)x.a, (const uint16_t*)x.w, x.bias, tg, x.m, x.k,
                                                        L.fsplit, part, loss, lse);
@@ -466,51 +611,42 @@ int launch_xent_forward(const XentProblem& x, float* loss, float* lse, uint8_t* 
     return PPOCR_OK;
 }
 
-static int sum_pass(const XentProblem& x, const float* part, int split, int64_t owners, int ld, void* out, const float* part_db,
-                    float* db, hipStream_t st) {
-    const unsigned grid = (unsigned)std::min<int64_t>((owners * x.k + kThreads - 1) / kThreads, 2048);
-    if (x.bf16) sum_kernel<uint16_t><<<grid, kThreads, 0, st>>>(part, split, owners, x.k, ld, (uint16_t*)out, part_db, db);
-    else sum_kernel<float><<<grid, kThreads, 0, st>>>(part, split, owners, x.k, ld, (float*)out, part_db, db);
-    PPOCR_HIP(hipGetLastError());
-    return PPOCR_OK;
-}
-
 int launch_xent_zero(const XentProblem& x, void* dw, float* db, hipStream_t st) {
-    return dw || db ? sum_pass(x, nullptr, 0, x.n, 0, dw, nullptr, db, st) : PPOCR_OK;
+    if (!dw && !db) return PPOCR_OK;
+    XentLayout L{};
+    L.D = xent_pieces(x.k);
+    return x.bf16 ? sums<uint16_t>(L, nullptr, nullptr, nullptr, 0, x.n, x.k, nullptr, dw, db, st)
+                  : sums<float>(L, nullptr, nullptr, nullptr, 0, x.n, x.k, nullptr, dw, db, st);
 }
 
 int launch_xent_backward(const XentProblem& x, void* da, void* dw, float* db, uint8_t* ws, hipStream_t st) {
     const XentLayout L = xent_layout(x.m, x.n, x.k, x.tn, x.planes());
-    const Targets tg = targets_of(x);
-    if (int e = x.bf16 ? prep<uint16_t, 1, true>(x, L, tg, ws, st) : prep<float, 2, true>(x, L, tg, ws, st)) return e;
-    float* part = reinterpret_cast<float*>(ws + L.b_part);
-    float* part_db = reinterpret_cast<float*>(ws + L.b_part_db);
-    const int blocks = (int)((x.n + 127) / 128);
-    auto pass = [&](bool rows) -> int {
-        const int64_t owners = rows ? x.m : x.n, own_tiles = rows ? L.row_tiles : L.class_tiles,
-                      str_tiles = rows ? L.class_tiles : L.row_tiles;
-        const int split = rows ? L.gsplit_a : L.gsplit_w;
-        const uint8_t* rr = ws + L.b_row_rec;
-        const uint8_t* cr = ws + L.b_class_rec;
-        XentGradArgs s{rows ? rr : cr, rows ? cr : rr, owners, own_tiles, str_tiles,
-                       reinterpret_cast<const int*>(ws + (rows ? L.b_class_e : L.b_row_u)), split,
-                       per_split(str_tiles, split, rows ? kBlockTiles : 1), kLog2e / x.tau,
-                       reinterpret_cast<const uint32_t*>(ws + L.b_keys), reinterpret_cast<const float*>(ws + L.b_vals),
-                       reinterpret_cast<const uint16_t*>(ws + L.b_offs), 32 * x.tn, blocks, part,
-                       rows ? nullptr : part_db};
-        const unsigned grid = (unsigned)((owners + kXentGradOwners - 1) / kXentGradOwners) * split;
-        int e;
-        if (rows) e = x.bf16 ? grad_pass<1, true>(L.D, s, grid, st) : grad_pass<2, true>(L.D, s, grid, st);
-        else e = x.bf16 ? grad_pass<1, false>(L.D, s, grid, st) : grad_pass<2, false>(L.D, s, grid, st);
-        if (e) return e;
-        if (int e2 = sum_pass(x, part, split, owners, 32 * L.D, rows ? da : dw, part_db, rows ? nullptr : db, st)) return e2;
-        return PPOCR_OK;
-    };
-    if (da)
-        if (int e = pass(true)) return e;
-    if (dw || db)
-        if (int e = pass(false)) return e;
-    return PPOCR_OK;
+    if (int e = x.bf16 ? prep<uint16_t, 1, true>(x, L, ws, st) : prep<float, 2, true>(x, L, ws, st)) return e;
+    float* pa = reinterpret_cast<float*>(ws + L.b_part_a);
+    float* pw = reinterpret_cast<float*>(ws + L.b_part_w);
+    float* pdb = reinterpret_cast<float*>(ws + L.b_part_db);
+    const uint8_t* rr = ws + L.b_row_rec;
+    const uint8_t* cr = ws + L.b_class_rec;
+    const unsigned ga = da ? (unsigned)(div_up(x.m, kXentGradOwners) * L.split_a) : 0;
+    const unsigned gw = dw || db ? (unsigned)(div_up(x.n, kXentGradOwners) * L.split_w) : 0;
+    const XentGradArgs s{{rr, cr, x.m, L.row_tiles, L.class_tiles, reinterpret_cast<const int*>(ws + L.b_class_e), L.split_a,
+                          L.per_a, pa},
+                         {cr, rr, x.n, L.class_tiles, L.row_tiles, reinterpret_cast<const int*>(ws + L.b_row_u), L.split_w,
+                          L.per_w, pw},
+                         ga,
+                         kLog2e / x.tau,
+                         reinterpret_cast<const uint32_t*>(ws + L.b_keys),
+                         reinterpret_cast<const float*>(ws + L.b_vals),
+                         reinterpret_cast<const uint16_t*>(ws + L.b_offs),
+                         32 * x.tn,
+                         (int)div_up(x.n, 128),
+                         pdb};
+    if (int e = by_pieces(L.D, [&]<int D>() {
+            return x.bf16 ? xent_grad_cfg<D, 1>(s, ga + gw, st) : xent_grad_cfg<D, 2>(s, ga + gw, st);
+        }))
+        return e;
+    return x.bf16 ? sums<uint16_t>(L, pa, pw, pdb, x.m, x.n, x.k, da, dw, db, st)
+                  : sums<float>(L, pa, pw, pdb, x.m, x.n, x.k, da, dw, db, st);
 }
 
 }  // namespace ppocr

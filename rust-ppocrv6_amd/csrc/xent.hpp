@@ -28,7 +28,9 @@ constexpr int64_t kXentMaxN = 1 << 26;  // classes: a list key holds a class and
 //                                           in the order an MFMA result holds its rows
 //                                           (backward only)
 //   float[32], float[32], float[16]         per entry: class: bias log2(e) / tau; row: lse
-//                                           log2(e) and gradient factor; then 2^-e and e
+//                                           log2(e) and gradient factor; then 2^-e, e, the
+//                                           largest L2 norm of an entry and the largest finite
+//                                           magnitude among the first 32 values
 // D = the number of 32-wide pieces of k, one of 1, 2, 3, 4, 6, 8.
 constexpr int kXentAux = 320;
 inline int xent_pieces(int64_t k) {
@@ -62,11 +64,14 @@ struct XentProblem {
 struct XentLayout {
     int D, planes;
     int64_t row_tiles, class_tiles;
-    int fsplit, gsplit_a, gsplit_w;
+    int fblocks;             // blocks of 32 rows of a wave of the statistics pass
+    int fsplit, fper;        // its chunks of class records, records of a chunk
+    int split_a, per_a;      // chunks of class records for da
+    int split_w, per_w;      // chunks of row records for dW
     // forward
     size_t f_row_rec, f_class_rec, f_part, f_total;
     // backward
-    size_t b_row_rec, b_class_rec, b_row_e, b_row_u, b_class_e, b_keys, b_vals, b_offs, b_part, b_part_db, b_total;
+    size_t b_row_rec, b_class_rec, b_row_e, b_row_u, b_class_e, b_keys, b_vals, b_offs, b_part_a, b_part_w, b_part_db, b_total;
     size_t total() const { return f_total > b_total ? f_total : b_total; }
 };
 XentLayout xent_layout(int64_t m, int64_t n, int64_t k, int tn, int planes);
@@ -85,33 +90,38 @@ struct XentStatsArgs {
     float c0;     // log2(e) / tau
     float2* part;  // [nsplit][m]: reference and sum of exp2(t - reference)
 };
-struct XentGradArgs {
-    const uint8_t* own;
-    const uint8_t* str;
+struct XentGradSide {
+    const uint8_t* own;  // owner records
+    const uint8_t* str;  // stream records
     int64_t owners;     // rows or classes
     int64_t own_tiles;  // their records
     int64_t str_tiles;
     const int* str_u;  // per stream record: the exponent bound of what is summed over it
     int nsplit, per_split;
+    float* part;  // [nsplit][owners][32 D]
+};
+struct XentGradArgs {
+    XentGradSide rows, classes;  // da, dW
+    unsigned row_grid;           // workgroups of da, the others are dW's
     float c0;
     const uint32_t* keys;
     const float* vals;
     const uint16_t* offs;
     int list;     // entries of a row group's list
     int blocks;   // blocks of 128 classes; a group's offsets are blocks + 1
-    float* part;  // [nsplit][owners][32 D]
-    float* part_db;  // [nsplit][owners] (owner = class), may be null
+    float* part_db;  // [classes.nsplit][classes]
 };
 template <int D, int P>
-int xent_stats_cfg(const XentStatsArgs& x, unsigned grid, hipStream_t st);
-template <int D, int P, bool ROWS>
+int xent_stats_cfg(const XentStatsArgs& x, int blocks, unsigned grid, hipStream_t st);
+template <int D, int P>
 int xent_grad_cfg(const XentGradArgs& x, unsigned grid, hipStream_t st);
-// Blocks of 32 rows of a wave of the statistics pass (registers allow one only for wide records of
-// two planes), rows of its workgroups, owners of a gradient pass's workgroup, and how many of
-// those a CU's LDS holds.
-constexpr int xent_stats_blocks(int D, int planes) { return planes == 2 && D > 4 ? 1 : 2; }
-constexpr int xent_stats_rows(int D, int planes) { return 128 * xent_stats_blocks(D, planes); }
+// Blocks of 32 rows of a wave of the statistics pass (registers allow two but for wide records of
+// two planes), owners of a gradient workgroup, and how many workgroups of either a CU holds
+// (registers and LDS).
+constexpr int xent_stats_most_blocks(int D, int planes) { return planes == 2 && D > 4 ? 1 : 2; }
 constexpr int kXentGradOwners = 128;
-constexpr int xent_grad_per_cu(int D, int planes) { return planes == 2 && D > 4 ? 1 : 2; }
+constexpr int xent_grad_per_cu(int D, int planes) {
+    return planes == 1 ? (D <= 3 ? 4 : D == 4 ? 3 : 2) : (D <= 2 ? 4 : D == 3 ? 3 : D == 4 ? 2 : 1);
+}
 
 }  // namespace ppocr

@@ -36,21 +36,24 @@ __device__ __forceinline__ void wait_loads() {
 // One record's logits for this lane's owner entry: 16 entries of the stream record (8 (r / 4)
 // + 4 (lane / 32) + r % 4) against owner lane % 32.  With two planes the three products that
 // fp32 sums keep: high x high, high x low, low x high.
-template <int D, int P>
-__device__ __forceinline__ f32x16 scores(const uint8_t* rec, const f16x8 (&own)[P][2 * D], int lane) {
+template <int D, int P, int NB>
+__device__ __forceinline__ void scores(const uint8_t* rec, const f16x8 (&own)[NB][P][2 * D], f32x16 (&s)[NB], int lane) {
     const f16x8* s0 = reinterpret_cast<const f16x8*>(rec) + lane;
-    f32x16 s = {};
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s[b] = f32x16{};
 #pragma unroll
     for (int ks = 0; ks < 2 * D; ++ks) {
         const f16x8 hi = s0[ks * 64];
-        s = mma(hi, own[0][ks], s);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) s[b] = mma(hi, own[b][0][ks], s[b]);
         if constexpr (P == 2) {
             const f16x8 lo = s0[(2 * D + ks) * 64];
-            s = mma(hi, own[1][ks], s);
-            s = mma(lo, own[0][ks], s);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) s[b] = mma(hi, own[b][1][ks], s[b]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) s[b] = mma(lo, own[b][0][ks], s[b]);
         }
     }
-    return s;
 }
 
 template <int D, int P>
@@ -63,9 +66,11 @@ __device__ __forceinline__ void load_owner(const uint8_t* rec, f16x8 (&own)[P][2
 }
 
 // ---------------------------------------------------------------- forward: softmax statistics
-// Streams the class records of a chunk past 32 NB rows per wave.  t = z log2(e) / tau is kept
-// against a reference that moves only when a maximum beats it by 16 (so sums stay below 2^16 n
-// and lose nothing), and a lane needs no other lane until the chunk ends.
+// Streams the class records of a chunk past 32 NB rows per wave.  t = z log2(e) / tau, and a lane
+// needs no other lane until the chunk ends.  Where |a| |w| + |b| (the records' largest norms)
+// bounds |t| by 100, exp2(t) is summed as it is: no maximum and no reference, a third of the vector
+// work.  Other records keep a reference that moves only when a maximum beats it by 16 (so sums stay
+// below 2^16 n and lose nothing); a row that once needed one keeps it.
 template <int D, int P, int NB>
 __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
     constexpr int REC = P * D * 2048 + kXentAux;
@@ -77,29 +82,48 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
     const int64_t t0 = (int64_t)split * x.per_split, t1 = min(t0 + x.per_split, x.tiles);
     const int64_t row0 = rb * (32 * NB * kWaves) + wave * (32 * NB);
 
+    stage<REC>(x.str + t0 * REC, lds, tid);
     f16x8 own[NB][P][2 * D];
-    float c[NB], ref[NB], sum[NB];
+    float c[NB], norm[NB], ref[NB], sum[NB];
+    bool shifted[NB];  // some row has a reference other than 0
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int64_t r = min(row0 + 32 * b, x.m - 1) / 32;  // a record that exists; unused rows are dropped at the end
         const uint8_t* rec = x.own + r * REC;
+        const float* aux = reinterpret_cast<const float*>(rec + P * D * 2048);
         load_owner<D, P>(rec, own[b], lane);
-        c[b] = x.c0 * reinterpret_cast<const float*>(rec + P * D * 2048)[64];
+        c[b] = x.c0 * aux[64];
+        norm[b] = x.c0 * aux[66];
         ref[b] = -INFINITY;
         sum[b] = 0.0f;
+        shifted[b] = false;
     }
-    stage<REC>(x.str + t0 * REC, lds, tid);
     for (int64_t t = t0; t < t1; ++t) {
         const uint8_t* cur = lds + ((t - t0) & 1) * REC;
         wait_loads();
         __syncthreads();
         if (t + 1 < t1) stage<REC>(x.str + (t + 1) * REC, lds + ((t + 1 - t0) & 1) * REC, tid);
         const float* aux = reinterpret_cast<const float*>(cur + P * D * 2048);
-        const float ce = aux[64];
+        const float ce = aux[64], cn = aux[66], cb = aux[67];
+        f32x16 sc[NB];
+        scores<D, P, NB>(cur, own, sc, lane);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            f32x16 s = scores<D, P>(cur, own[b], lane);
+            f32x16& s = sc[b];
             const float cc = c[b] * ce;
+            const bool plain = !shifted[b] && __builtin_amdgcn_readfirstlane(norm[b] * cn + cb <= 100.0f);
+            if (plain) {
+                if (ref[b] == -INFINITY) ref[b] = 0.0f;
+                float add = 0.0f;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 bias = *reinterpret_cast<const f32x4*>(aux + 8 * q + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) add += __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], cc, bias[e]));
+                }
+                sum[b] += add;
+                continue;
+            }
             float mx = -INFINITY;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -114,6 +138,7 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
                 const float nr = mx > ref[b] + 16.0f ? mx : ref[b];
                 sum[b] = ref[b] == -INFINITY ? 0.0f : sum[b] * __builtin_amdgcn_exp2f(ref[b] - nr);
                 ref[b] = nr;
+                shifted[b] = true;
             }
             const float rf = ref[b] == -INFINITY ? 0.0f : ref[b];
             float add = 0.0f;
@@ -135,7 +160,7 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
     }
 }
 
-// ---------------------------------------------------------------- backward: one gradient
+// ---------------------------------------------------------------- backward: a gradient
 // dX_o = sum_s P_os Y_s for the owners o of a workgroup (32 per wave), the stream records s of a
 // chunk in turn: the logits of 32 x 32 pairs, p = exp2(t - lse), the target entries' places
 // overwritten with p - q as the list holds it (exact in 32 bits, so that a nearly certain label
@@ -147,61 +172,118 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
 //   gradient factor.
 // e is the stream record's exponent and F one exponent for all records, so that P's largest
 // possible value is 2^14 and products of all records add up on one scale.
+// The target lists are read 64 entries at a time, one a lane, and an entry's place is written by the
+// lane that holds it, in the register that its row (or class) of the tile is: a wave-uniform number.
 __device__ __forceinline__ void set_entry(f32x16& p, int i, bool mine, float v) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-        if (r == i) p[r] = mine ? v : p[r];
+    const float old = p[i];
+    p[i] = mine ? v : old;
 }
+__device__ __forceinline__ int lane_value(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+
+// A row group's list, walked along with the classes.
+struct ListWalk {
+    const uint32_t* keys;
+    const float* vals;
+    int at, end;        // the next entry, the list's length
+    int wkey, wval;     // this lane's entry of the window of 64 that holds `at`
+    uint32_t key;       // the next entry's
+    __device__ __forceinline__ void load(int lane) {
+        const int i = (at & ~63) + lane;
+        wkey = i < end ? (int)keys[i] : -1;
+        wval = i < end ? __float_as_int(vals[i]) : 0;
+    }
+    __device__ __forceinline__ void start(const XentGradArgs& x, bool have, int64_t group, int64_t tile, int lane) {
+        keys = x.keys + (have ? group * x.list : 0);
+        vals = x.vals + (have ? group * x.list : 0);
+        end = have ? x.list : 0;
+        at = have ? __builtin_amdgcn_readfirstlane(x.offs[group * (x.blocks + 1) + tile / 4]) : 0;
+        load(lane);
+        key = at < end ? (uint32_t)lane_value(wkey, at & 63) : 0xFFFFFFFFu;
+    }
+    __device__ __forceinline__ void step(int lane) {
+        ++at;
+        if ((at & 63) == 0) load(lane);
+        key = at < end ? (uint32_t)lane_value(wkey, at & 63) : 0xFFFFFFFFu;
+    }
+};
+
+// A row record's entries in a workgroup's 128 classes.
+struct ListSlice {
+    int from, to;  // where they are in the group's list
+    int key, val;  // this lane's entry of a window of 64
+    __device__ __forceinline__ void bounds(const XentGradArgs& x, int64_t t, int64_t ob) {
+        const uint16_t* of = x.offs + t * (x.blocks + 1) + ob;
+        from = of[0];
+        to = of[1];
+    }
+    __device__ __forceinline__ void read(const XentGradArgs& x, int64_t t, int first, int lane) {
+        const int i = first + lane;
+        key = i < to ? (int)x.keys[t * x.list + i] : -1;
+        val = i < to ? __float_as_int(x.vals[t * x.list + i]) : 0;
+    }
+};
 
 template <int D, int P, bool ROWS>
-__global__ __launch_bounds__(kThreads, xent_grad_per_cu(D, P)) void grad_kernel(XentGradArgs x) {
+__device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSide& y, unsigned block, uint8_t* lds) {
     constexpr int REC = 2 * P * D * 2048 + kXentAux, AUX = 2 * P * D * 2048;
-    extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int split = blockIdx.x % x.nsplit;
-    const int64_t ob = blockIdx.x / x.nsplit;
-    const int64_t t0 = (int64_t)split * x.per_split, t1 = min(t0 + x.per_split, x.str_tiles);
+    const int split = block % y.nsplit;
+    const int64_t ob = block / y.nsplit;
+    const int64_t t0 = (int64_t)split * y.per_split, t1 = min(t0 + y.per_split, y.str_tiles);
     const int64_t og = ob * kWaves + wave;  // this wave's owner record
     const int64_t owner = og * 32 + (lane & 31);
 
-    stage<REC>(x.str + t0 * REC, lds, tid);
+    stage<REC>(y.str + t0 * REC, lds, tid);
     // F from the largest exponent bound of the stream
     int um = -200;
-    for (int64_t i = lane; i < x.str_tiles; i += 64) um = max(um, x.str_u[i]);
+    for (int64_t i = lane; i < y.str_tiles; i += 64) um = max(um, y.str_u[i]);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) um = max(um, __shfl_xor(um, o, 64));
-    const int F = 14 - um;
+    const int F = 14 - __builtin_amdgcn_readfirstlane(um);
 
-    const bool have = og < x.own_tiles;
-    const uint8_t* orec = x.own + (have ? og : x.own_tiles - 1) * REC;
-    f16x8 own[P][2 * D];
-    load_owner<D, P>(orec, own, lane);
+    const bool have = og < y.own_tiles;
+    const uint8_t* orec = y.own + (have ? og : y.own_tiles - 1) * REC;
+    f16x8 own[1][P][2 * D];
+    load_owner<D, P>(orec, own[0], lane);
     const float* oaux = reinterpret_cast<const float*>(orec + AUX);
     const float c = x.c0 * oaux[64];
-    const float own0 = oaux[lane & 31];       // row: lse log2(e); class: bias log2(e) / tau
+    const float own0 = oaux[lane & 31];                      // row: lse log2(e); class: bias log2(e) / tau
     const float own1 = ROWS ? oaux[32 + (lane & 31)] : 0.0f;  // row: the gradient factor
     f32x16 acc[D] = {};
     float dbias = 0.0f;
 
-    // ROWS: the wave's row group is `og`, its list is walked along with the classes
-    const uint32_t* keys = x.keys + (ROWS && have ? og * x.list : 0);
-    const float* vals = x.vals + (ROWS && have ? og * x.list : 0);
-    int cur_hit = 0;
-    uint32_t next_key = 0xFFFFFFFFu;
-    if (ROWS && have && t0 < t1) {
-        cur_hit = __builtin_amdgcn_readfirstlane(x.offs[og * (x.blocks + 1) + t0 / 4]);
-        next_key = __builtin_amdgcn_readfirstlane(cur_hit < x.list ? keys[cur_hit] : 0xFFFFFFFFu);
+    // the slice of the next record is read while a record is worked on, its bounds one earlier
+    ListWalk walk;
+    ListSlice next, after;
+    if constexpr (ROWS) {
+        walk.start(x, have, og, t0, lane);
+    } else {
+        next.bounds(x, t0, ob);
+        next.read(x, t0, next.from, lane);
+        after.bounds(x, min(t0 + 1, y.str_tiles - 1), ob);
     }
     for (int64_t t = t0; t < t1; ++t) {
         const uint8_t* cur = lds + ((t - t0) & 1) * REC;
         wait_loads();
         __syncthreads();
-        if (t + 1 < t1) stage<REC>(x.str + (t + 1) * REC, lds + ((t + 1 - t0) & 1) * REC, tid);
-        f32x16 p = scores<D, P>(cur, own, lane);
+        if (t + 1 < t1) stage<REC>(y.str + (t + 1) * REC, lds + ((t + 1 - t0) & 1) * REC, tid);
+        ListSlice mine;
+        if constexpr (!ROWS) {
+            mine = next;
+            if (t + 1 < t1) {
+                next.from = after.from;
+                next.to = after.to;
+                next.read(x, t + 1, next.from, lane);
+                after.bounds(x, min(t + 2, y.str_tiles - 1), ob);
+            }
+        }
+        f32x16 s[1];
+        scores<D, P, 1>(cur, own, s, lane);
+        f32x16& p = s[0];
         const float* aux = reinterpret_cast<const float*>(cur + AUX);
         const float cc = c * aux[64];
-        const int fe = min(F - (int)aux[65], 100);  // exponent of this record's factor
+        const int fe = __builtin_amdgcn_readfirstlane(min(F - (int)aux[65], 100));  // exponent of this record's factor
         if constexpr (ROWS) {
             const float shift = own0 - (float)fe;
 #pragma unroll
@@ -212,12 +294,11 @@ __global__ __launch_bounds__(kThreads, xent_grad_per_cu(D, P)) void grad_kernel(
                     p[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(p[4 * q + e], cc, bias[e]) - shift);
             }
             const uint32_t end = (uint32_t)((t + 1) * 1024);  // keys below: classes of this record
-            while (next_key < end) {
-                const int cls = (int)(next_key >> 5) & 31, row = (int)next_key & 31;
-                const float v = ldexpf(vals[cur_hit], fe);
+            while (walk.key < end) {
+                const int cls = (int)(walk.key >> 5) & 31, row = (int)walk.key & 31;
+                const float v = ldexpf(__int_as_float(lane_value(walk.wval, walk.at & 63)), fe);
                 set_entry(p, (cls >> 3) * 4 + (cls & 3), lane == row + 32 * ((cls >> 2) & 1), v);
-                ++cur_hit;
-                next_key = __builtin_amdgcn_readfirstlane(cur_hit < x.list ? keys[cur_hit] : 0xFFFFFFFFu);
+                walk.step(lane);
             }
         } else {
             // (not below 2^-60, so that the bias's sum keeps the values of records of tiny activations)
@@ -231,15 +312,18 @@ __global__ __launch_bounds__(kThreads, xent_grad_per_cu(D, P)) void grad_kernel(
                 for (int e = 0; e < 4; ++e)
                     p[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(p[4 * q + e], cc, shift) - lse[e]) * g[e];
             }
-            // the stream record is row group t; its entries in this workgroup's 128 classes
-            const uint16_t* of = x.offs + t * (x.blocks + 1) + ob;
-            const int i0 = __builtin_amdgcn_readfirstlane(of[0]), i1 = __builtin_amdgcn_readfirstlane(of[1]);
-            for (int i = i0; i < i1; ++i) {
-                const uint32_t key = __builtin_amdgcn_readfirstlane(x.keys[t * x.list + i]);
-                if ((int64_t)(key >> 10) != og) continue;
-                const int cls = (int)(key >> 5) & 31, row = (int)key & 31;
-                const float v = ldexpf(x.vals[t * x.list + i] * aux[32 + row], fs);
-                set_entry(p, (row >> 3) * 4 + (row & 3), lane == cls + 32 * ((row >> 2) & 1), v);
+            const int from = __builtin_amdgcn_readfirstlane(mine.from), to = __builtin_amdgcn_readfirstlane(mine.to);
+            for (int first = from; first < to; first += 64) {
+                if (first != from) mine.read(x, t, first, lane);
+                unsigned long long todo = __ballot((int64_t)(uint32_t)mine.key >> 10 == og && first + lane < to);
+                while (todo) {
+                    const int l = __builtin_ctzll(todo);
+                    todo &= todo - 1;
+                    const int key = lane_value(mine.key, l);
+                    const int cls = (key >> 5) & 31, row = key & 31;
+                    const float v = ldexpf(__int_as_float(lane_value(mine.val, l)) * aux[32 + row], fs);
+                    set_entry(p, (row >> 3) * 4 + (row & 3), lane == cls + 32 * ((row >> 2) & 1), v);
+                }
             }
             float add = 0.0f;
 #pragma unroll
@@ -271,8 +355,8 @@ __global__ __launch_bounds__(kThreads, xent_grad_per_cu(D, P)) void grad_kernel(
             }
         }
     }
-    if (owner < x.owners) {
-        float* out = x.part + ((int64_t)split * x.owners + owner) * (32 * D);
+    if (owner < y.owners) {
+        float* out = y.part + ((int64_t)split * y.owners + owner) * (32 * D);
 #pragma unroll
         for (int d = 0; d < D; ++d)
 #pragma unroll
@@ -288,33 +372,45 @@ __global__ __launch_bounds__(kThreads, xent_grad_per_cu(D, P)) void grad_kernel(
     }
     if constexpr (!ROWS) {
         dbias += __shfl_xor(dbias, 32, 64);
-        if (x.part_db && h == 0 && owner < x.owners) x.part_db[(int64_t)split * x.owners + owner] = dbias;
+        if (h == 0 && owner < y.owners) x.part_db[(int64_t)split * y.owners + owner] = dbias;
     }
+}
+
+// Both gradients in one launch, so that the last workgroups of one fill up with the other's.
+template <int D, int P>
+__global__ __launch_bounds__(kThreads, xent_grad_per_cu(D, P)) void grad_kernel(XentGradArgs x) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    if (blockIdx.x < x.row_grid) gradient<D, P, true>(x, x.rows, blockIdx.x, lds);
+    else gradient<D, P, false>(x, x.classes, blockIdx.x - x.row_grid, lds);
 }
 
 }  // namespace xent
 
 template <int D, int P>
-int xent_stats_cfg(const XentStatsArgs& x, unsigned grid, hipStream_t st) {
+int xent_stats_cfg(const XentStatsArgs& x, int blocks, unsigned grid, hipStream_t st) {
     constexpr int lds = 2 * (P * D * 2048 + kXentAux);
-    auto kernel = xent::stats_kernel<D, P, xent_stats_blocks(D, P)>;
-    kernel<<<grid, xent::kThreads, lds, st>>>(x);
+    if constexpr (xent_stats_most_blocks(D, P) == 2) {
+        if (blocks == 2) {
+            xent::stats_kernel<D, P, 2><<<grid, xent::kThreads, lds, st>>>(x);
+            PPOCR_HIP(hipGetLastError());
+            return PPOCR_OK;
+        }
+    }
+    xent::stats_kernel<D, P, 1><<<grid, xent::kThreads, lds, st>>>(x);
     PPOCR_HIP(hipGetLastError());
     return PPOCR_OK;
 }
 
-template <int D, int P, bool ROWS>
+template <int D, int P>
 int xent_grad_cfg(const XentGradArgs& x, unsigned grid, hipStream_t st) {
     constexpr int lds = 2 * (2 * P * D * 2048 + kXentAux);
-    auto kernel = xent::grad_kernel<D, P, ROWS>;
-    kernel<<<grid, xent::kThreads, lds, st>>>(x);
+    xent::grad_kernel<D, P><<<grid, xent::kThreads, lds, st>>>(x);
     PPOCR_HIP(hipGetLastError());
     return PPOCR_OK;
 }
 
-#define PPOCR_XENT_INSTANCES(D, P)                                                  \
-    template int xent_stats_cfg<D, P>(const XentStatsArgs&, unsigned, hipStream_t); \
-    template int xent_grad_cfg<D, P, true>(const XentGradArgs&, unsigned, hipStream_t); \
-    template int xent_grad_cfg<D, P, false>(const XentGradArgs&, unsigned, hipStream_t);
+#define PPOCR_XENT_INSTANCES(D, P)                                                       \
+    template int xent_stats_cfg<D, P>(const XentStatsArgs&, int, unsigned, hipStream_t); \
+    template int xent_grad_cfg<D, P>(const XentGradArgs&, unsigned, hipStream_t);
 
 }  // namespace ppocr
