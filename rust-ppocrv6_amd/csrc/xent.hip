@@ -9,6 +9,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// log2(e) and ln 2 in two floats: a logarithm of 16 times log2(e) rounded to 32 bits would be off by
+// 2e-7, for every row in the same direction, and so would the sum of each row's probabilities.
+constexpr float kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147182f, kLn2Rest = -1.90465432e-9f;
+__device__ __forceinline__ float to_log2(float l) { return fmaf(l, kLog2e, l * kLog2eRest); }
+
 __device__ __forceinline__ float value(const float* p) { return *p; }
 __device__ __forceinline__ float value(const uint16_t* p) { return __uint_as_float((unsigned)*p << 16); }
 
@@ -88,11 +93,14 @@ __device__ __forceinline__ RowTargets row_targets(const Targets& tg, const T* a,
     return t;
 }
 
-// A row's gradient factor: g / tau when it has a target, 0 otherwise.
-__device__ __forceinline__ float factor_of(const Targets& tg, const float* grad, int64_t r) {
+// A row's gradient factor, by 8 neighbouring lanes: g / tau when it has a target, 0 otherwise.
+__device__ __forceinline__ float factor_of(const Targets& tg, const float* grad, int64_t r, int l8) {
     bool any = false;
-    for (int i = 0; i < tg.tn; ++i) any |= tg.cls(r, i) >= 0 && (tg.target || tg.logit(r, i) != -INFINITY);
-    return any ? (grad ? grad[r] : 1.0f) * tg.inv_tau : 0.0f;
+    for (int i = l8; i < tg.tn; i += 8) any |= tg.cls(r, i) >= 0 && (tg.target || tg.logit(r, i) != -INFINITY);
+    int n = any;
+#pragma unroll
+    for (int o = 4; o >= 1; o >>= 1) n |= __shfl_xor(n, o, 64);
+    return n ? (grad ? grad[r] : 1.0f) * tg.inv_tau : 0.0f;
 }
 
 // ---------------------------------------------------------------- operand records
@@ -126,7 +134,8 @@ __device__ void build_record(const RecordArgs<T>& x, int64_t t, bool rows, float
     float* gf = red + 8;  // 32 gradient factors
     float factor = 1.0f;
     if (BACK && rows) {
-        factor = e < count ? factor_of(x.tg, x.grad, first + e) : 0.0f;
+        factor = factor_of(x.tg, x.grad, first + min((int64_t)e, count - 1), l8);
+        if (e >= count) factor = 0.0f;
         if (l8 == 0) gf[e] = factor;
     }
     // a row without gradient reaches no sum, whatever it holds
@@ -197,7 +206,7 @@ __device__ void build_record(const RecordArgs<T>& x, int64_t t, bool rows, float
             aux[tid] = tid < count ? (x.bias ? x.bias[first + tid] * (kLog2e * x.tg.inv_tau) : 0.0f) : -INFINITY;
             aux[32 + tid] = 0.0f;
         } else if (BACK) {
-            aux[tid] = gf[tid] != 0.0f ? x.lse[first + tid] * kLog2e : INFINITY;
+            aux[tid] = gf[tid] != 0.0f ? to_log2(x.lse[first + tid]) : INFINITY;
             aux[32 + tid] = gf[tid];
         } else {
             aux[tid] = 0.0f;
@@ -242,6 +251,53 @@ struct ListArgs {
 };
 constexpr uint32_t kNoKey = 0xFFFFFFFFu;
 
+// Sorts `size` keys (a power of two from 32 to 2 NT; the last size - list count as largest): a bitonic
+// network whose elements tid and tid + NT each thread keeps, so that the steps within a wave are
+// exchanges of lanes and only the wider ones go through memory (2048 keys: 13 of 66).
+template <int NT>
+__device__ void sort_keys(unsigned long long* key, int list, int size) {
+    const int tid = threadIdx.x;
+    unsigned long long v[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) v[e] = e * NT + tid < list ? key[e * NT + tid] : ~0ull;
+    __syncthreads();
+    for (int w = 2; w <= size; w <<= 1)
+        for (int d = w >> 1; d >= 1; d >>= 1) {
+            if (d == NT) {
+                if (v[0] > v[1]) {
+                    const unsigned long long t = v[0];
+                    v[0] = v[1];
+                    v[1] = t;
+                }
+                continue;
+            }
+            unsigned long long other[2] = {~0ull, ~0ull};
+            if (d >= 64) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (e * NT + tid < size) key[e * NT + tid] = v[e];
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (e * NT + tid < size) other[e] = key[(e * NT + tid) ^ d];
+                __syncthreads();
+            } else {
+                other[0] = __shfl_xor(v[0], d, 64);
+                if (size > NT) other[1] = __shfl_xor(v[1], d, 64);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int i = e * NT + tid;
+                const bool low = ((i & d) == 0) == ((i & w) == 0);  // this place keeps the smaller one
+                v[e] = (other[e] < v[e]) == low ? other[e] : v[e];
+            }
+        }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (e * NT + tid < size) key[e * NT + tid] = v[e];
+    __syncthreads();
+}
+
 template <typename T, int NT>
 __device__ void build_list(const ListArgs<T>& x, int64_t g, unsigned long long* key, float* pv, float* qv) {
     const int tid = threadIdx.x, tn = x.tg.tn;
@@ -250,44 +306,31 @@ __device__ void build_list(const ListArgs<T>& x, int64_t g, unsigned long long* 
         pv[s] = c >= 0 ? expf(z * x.tg.inv_tau - lse) : 0.0f;
         qv[s] = q;
     };
-    if (tn == 1 && x.tg.target) {
+    if (x.tg.target) {
         // 8 lanes a row
         for (int row = tid >> 3; row < 32; row += NT / 8) {
             const int64_t r = g * 32 + row;
-            const bool live = r < x.m && factor_of(x.tg, x.grad, r) != 0.0f;
-            const int c = live ? x.tg.cls(r, 0) : -1;
+            const float f = factor_of(x.tg, x.grad, min(r, x.m - 1), tid & 7);
+            const int c = r < x.m && f != 0.0f ? x.tg.cls(r, 0) : -1;
             const float z = logit_of(x.a, x.w, x.bias, r, c, x.k, tid & 7);
             if ((tid & 7) == 0) put(row, row, c, z, 1.0f, c >= 0 ? x.lse[r] : 0.0f);
         }
     } else {
         // a wave a row
+        const int lane = tid & 63;
         for (int row = tid >> 6; row < 32; row += NT / 64) {
             const int64_t r = g * 32 + row;
-            const bool live = r < x.m && factor_of(x.tg, x.grad, r) != 0.0f;
-            const int lane = tid & 63;
+            RowTargets t{-1, 0.0f, 0.0f, 0.0f};
+            bool live = r < x.m && (!x.grad || x.grad[r] != 0.0f);
             if (live) {
-                const RowTargets t = row_targets(x.tg, x.a, x.w, x.bias, r, x.k, lane);
-                if (lane < tn) put(row * tn + lane, row, t.cls, t.z, t.q, x.lse[r]);
-            } else if (lane < tn) {
-                put(row * tn + lane, row, -1, 0.0f, 0.0f, 0.0f);
+                t = row_targets(x.tg, x.a, x.w, x.bias, r, x.k, lane);
+                live = __any(t.q != 0.0f);
             }
+            if (lane < tn) put(row * tn + lane, row, live ? t.cls : -1, t.z, t.q, live ? x.lse[r] : 0.0f);
         }
     }
-    for (int s = x.list + tid; s < x.size; s += NT) key[s] = ~0ull;
     __syncthreads();
-    for (int w2 = 2; w2 <= x.size; w2 <<= 1)
-        for (int d = w2 >> 1; d >= 1; d >>= 1) {
-            for (int p = tid; p < x.size / 2; p += NT) {
-                const int i = 2 * d * (p / d) + p % d, j = i + d;
-                const bool up = (i & w2) == 0;
-                const unsigned long long a = key[i], b = key[j];
-                if ((a > b) == up) {
-                    key[i] = b;
-                    key[j] = a;
-                }
-            }
-            __syncthreads();
-        }
+    sort_keys<NT>(key, x.list, x.size);
     for (int s = tid; s < x.list; s += NT) {
         const uint32_t kk = key[s] == ~0ull ? kNoKey : (uint32_t)(key[s] >> 11);
         float v = 0.0f;
@@ -340,6 +383,43 @@ __global__ __launch_bounds__(kListThreads) void list_kernel(ListArgs<T> y) {
 }
 
 // ---------------------------------------------------------------- forward: merge and loss
+// Joins two sums of exp2(t - reference).
+__device__ __forceinline__ void join(float* ref, float* sum, float2 v) {
+    const float nr = fmaxf(*ref, v.x);
+    const float s = *ref == -INFINITY ? *sum : *sum * exp2f(*ref - nr);
+    *sum = s + (v.x == -INFINITY ? v.y : v.y * exp2f(v.x - nr));
+    *ref = nr;
+}
+// Their natural logarithm; a row whose classes are all -inf keeps reference -inf and sum 0.  The sum's
+// exponent goes with the reference: logf of 18710 is off by half a step of 10 on average, one way.
+__device__ __forceinline__ float log_sum(float ref, float sum) {
+    if (!(sum > 0.0f && sum < INFINITY)) return ref == -INFINITY ? logf(sum) : ref + logf(sum);
+    int e;
+    const float m = frexpf(sum, &e);
+    const float two = (ref == -INFINITY ? 0.0f : ref) + (float)e;
+    return fmaf(two, kLn2, fmaf(two, kLn2Rest, logf(m)));
+}
+
+// Labels of many rows: 8 lanes a row (30720 rows: 9 us, 26 with a wave a row).
+template <typename T>
+__global__ __launch_bounds__(kThreads) void label_loss_kernel(const T* a, const T* w, const float* bias, Targets tg, int64_t m,
+                                                              int k, int nsplit, const float2* __restrict__ part, float* loss,
+                                                              float* lse) {
+    const int l8 = threadIdx.x & 7;
+    const int64_t row = (int64_t)blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3), r = min(row, m - 1);
+    const int c = tg.cls(r, 0);
+    float ref = -INFINITY, sum = 0.0f;
+    for (int s = l8; s < nsplit; s += 8) join(&ref, &sum, part[(int64_t)s * m + r]);
+#pragma unroll
+    for (int o = 4; o >= 1; o >>= 1) join(&ref, &sum, make_float2(__shfl_xor(ref, o, 64), __shfl_xor(sum, o, 64)));
+    const float z = logit_of(a, w, bias, r, c, k, l8);
+    if (row < m && l8 == 0) {
+        const float l = log_sum(ref, sum);
+        loss[row] = c >= 0 ? l - z : 0.0f;
+        lse[row] = l;
+    }
+}
+
 // A wave per row: the chunks' statistics of the row, then its targets' logits.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void loss_kernel(const T* a, const T* w, const float* bias, Targets tg, int64_t m,
@@ -350,20 +430,10 @@ __global__ __launch_bounds__(kThreads) void loss_kernel(const T* a, const T* w, 
     if (row >= m) return;
     const RowTargets t = row_targets(tg, a, w, bias, row, k, lane);
     float ref = -INFINITY, sum = 0.0f;
-    for (int s = lane; s < nsplit; s += 64) {
-        const float2 v = part[(int64_t)s * m + row];
-        const float nr = fmaxf(ref, v.x);
-        sum = (ref == -INFINITY ? sum : sum * exp2f(ref - nr)) + (v.x == -INFINITY ? v.y : v.y * exp2f(v.x - nr));
-        ref = nr;
-    }
+    for (int s = lane; s < nsplit; s += 64) join(&ref, &sum, part[(int64_t)s * m + row]);
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        const float r2 = __shfl_xor(ref, o, 64), s2 = __shfl_xor(sum, o, 64), nr = fmaxf(ref, r2);
-        sum = (ref == -INFINITY ? sum : sum * exp2f(ref - nr)) + (r2 == -INFINITY ? s2 : s2 * exp2f(r2 - nr));
-        ref = nr;
-    }
-    // a row whose classes are all -inf keeps reference -inf and sum 0
-    const float l = (ref == -INFINITY ? 0.0f : ref * (1.0f / kLog2e)) + logf(sum);
+    for (int o = 32; o >= 1; o >>= 1) join(&ref, &sum, make_float2(__shfl_xor(ref, o, 64), __shfl_xor(sum, o, 64)));
+    const float l = log_sum(ref, sum);
     // entries without weight add nothing, whatever their class's logit
     const float total = wave_sum(t.q != 0.0f ? t.q * (t.logq - t.z * tg.inv_tau + l) : 0.0f);
     if (lane == 0) {
@@ -542,6 +612,20 @@ int prep(const XentProblem& x, const XentLayout& L, uint8_t* ws, hipStream_t st)
 }
 
 template <typename T>
+int losses(const XentProblem& x, const Targets& tg, int nsplit, const float2* part, float* loss, float* lse, hipStream_t st) {
+    const T* a = static_cast<const T*>(x.a);
+    const T* w = static_cast<const T*>(x.w);
+    if (x.target && x.m > 4096)
+        label_loss_kernel<T><<<(unsigned)div_up(x.m, kThreads / 8), kThreads, 0, st>>>(a, w, x.bias, tg, x.m, x.k, nsplit, part,
+                                                                                     loss, lse);
+    else
+        loss_kernel<T><<<(unsigned)div_up(x.m, kThreads / 64), kThreads, 0, st>>>(a, w, x.bias, tg, x.m, x.k, nsplit, part,
+                                                                                loss, lse);
+    PPOCR_HIP(hipGetLastError());
+    return PPOCR_OK;
+}
+
+template <typename T>
 int sums(const XentLayout& L, const float* pa, const float* pw, const float* pdb, int64_t m, int64_t n, int k, void* da,
          void* dw, float* db, hipStream_t st) {
     const bool bf16 = sizeof(T) == 2;
@@ -600,15 +684,7 @@ int launch_xent_forward(const XentProblem& x, float* loss, float* lse, uint8_t* 
             return x.bf16 ? xent_stats_cfg<D, 1>(s, L.fblocks, grid, st) : xent_stats_cfg<D, 2>(s, L.fblocks, grid, st);
         }))
         return e;
-    const unsigned lg = (unsigned)div_up(x.m, kThreads / 64);
-    if (x.bf16)
-        loss_kernel<uint16_t><<<lg, kThreads, 0, st>>>((const uint16_t*)x.a, (const uint16_t*)x.w, x.bias, tg, x.m, x.k,
-                                                       L.fsplit, part, loss, lse);
-    else
-        loss_kernel<float><<<lg, kThreads, 0, st>>>((const float*)x.a, (const float*)x.w, x.bias, tg, x.m, x.k, L.fsplit,
-                                                    part, loss, lse);
-    PPOCR_HIP(hipGetLastError());
-    return PPOCR_OK;
+    return x.bf16 ? losses<uint16_t>(x, tg, L.fsplit, part, loss, lse, st) : losses<float>(x, tg, L.fsplit, part, loss, lse, st);
 }
 
 int launch_xent_zero(const XentProblem& x, void* dw, float* db, hipStream_t st) {

@@ -279,7 +279,10 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
             }
         }
         f32x16 s[1];
+        // the matrix instructions of one wave before the vector work of the CU's others
+        __builtin_amdgcn_s_setprio(1);
         scores<D, P, 1>(cur, own, s, lane);
+        __builtin_amdgcn_s_setprio(0);
         f32x16& p = s[0];
         const float* aux = reinterpret_cast<const float*>(cur + AUX);
         const float cc = c * aux[64];
@@ -303,14 +306,14 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
         } else {
             // (not below 2^-60, so that the bias's sum keeps the values of records of tiny activations)
             const int fs = max(fe, -60);
-            const float shift = own0 + (float)fs;
+            const float scale = ldexpf(1.0f, fs);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const f32x4 lse = *reinterpret_cast<const f32x4*>(aux + 8 * q + 4 * h);
                 const f32x4 g = *reinterpret_cast<const f32x4*>(aux + 32 + 8 * q + 4 * h);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    p[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(p[4 * q + e], cc, shift) - lse[e]) * g[e];
+                    p[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(p[4 * q + e], cc, own0) - lse[e]) * (g[e] * scale);
             }
             const int from = __builtin_amdgcn_readfirstlane(mine.from), to = __builtin_amdgcn_readfirstlane(mine.to);
             for (int first = from; first < to; first += 64) {
@@ -333,6 +336,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
 #pragma unroll
                 for (int r = 0; r < 16; ++r) p[r] = ldexpf(p[r], fe - fs);
         }
+        __builtin_amdgcn_s_setprio(1);
         const f16x8* tr = reinterpret_cast<const f16x8*>(cur + P * D * 2048) + lane;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -354,6 +358,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
                 }
             }
         }
+        __builtin_amdgcn_s_setprio(0);
     }
     if (owner < y.owners) {
         float* out = y.part + ((int64_t)split * y.owners + owner) * (32 * D);
