@@ -158,6 +158,11 @@ __device__ void build_record(const RecordArgs<T>& x, int64_t t, bool rows, float
             v[i] = in && j < x.k ? value(src + j) : 0.0f;
         }
     }
+    float first_aux = 0.0f;  // of entry `tid`
+    if (tid < 32 && tid < count) {
+        if (!rows) first_aux = x.bias ? x.bias[first + tid] * (kLog2e * x.tg.inv_tau) : 0.0f;
+        else if (BACK) first_aux = x.lse[first + tid];
+    }
     float top = 0.0f, ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4 * D; ++i) {
@@ -201,25 +206,24 @@ __device__ void build_record(const RecordArgs<T>& x, int64_t t, bool rows, float
         }
     }
     float* aux = reinterpret_cast<float*>(rec + (size_t)P * D * 2048 * (BACK ? 2 : 1));
-    if (tid < 32) {
-        if (!rows) {
-            aux[tid] = tid < count ? (x.bias ? x.bias[first + tid] * (kLog2e * x.tg.inv_tau) : 0.0f) : -INFINITY;
-            aux[32 + tid] = 0.0f;
-        } else if (BACK) {
-            aux[tid] = gf[tid] != 0.0f ? to_log2(x.lse[first + tid]) : INFINITY;
-            aux[32 + tid] = gf[tid];
-        } else {
-            aux[tid] = 0.0f;
-            aux[32 + tid] = 0.0f;
+    if (tid < 64) {
+        float most = !rows && fabsf(first_aux) < INFINITY ? fabsf(first_aux) : 0.0f;
+        most = wave_max(most);
+        if (tid < 32) {
+            if (!rows) {
+                aux[tid] = tid < count ? first_aux : -INFINITY;
+                aux[32 + tid] = 0.0f;
+            } else if (BACK) {
+                aux[tid] = gf[tid] != 0.0f ? to_log2(first_aux) : INFINITY;
+                aux[32 + tid] = gf[tid];
+            } else {
+                aux[tid] = 0.0f;
+                aux[32 + tid] = 0.0f;
+            }
+        } else if (tid < 48) {
+            const float norm = sqrtf(fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7])));
+            aux[32 + tid] = tid == 32 ? ldexpf(1.0f, -ex) : tid == 33 ? (float)ex : tid == 34 ? norm : tid == 35 ? most : 0.0f;
         }
-    } else if (tid < 48) {
-        const float norm = sqrtf(fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7])));
-        float most = 0.0f;
-        for (int i = 0; i < (int)count && !rows && x.bias; ++i) {
-            const float b = fabsf(x.bias[first + i] * (kLog2e * x.tg.inv_tau));
-            most = b < INFINITY ? fmaxf(most, b) : most;
-        }
-        aux[32 + tid] = tid == 32 ? ldexpf(1.0f, -ex) : tid == 33 ? (float)ex : tid == 34 ? norm : tid == 35 ? most : 0.0f;
     }
     if (BACK && tid == 0) {
         float s = 0.0f;

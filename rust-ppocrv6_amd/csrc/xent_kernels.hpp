@@ -179,6 +179,9 @@ __device__ __forceinline__ void set_entry(f32x16& p, int i, bool mine, float v) 
     p[i] = mine ? v : old;
 }
 __device__ __forceinline__ int lane_value(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+// Has a loaded value here, where nothing younger is on its way: left to itself the compiler waits
+// where the value is used, for everything loaded since.
+__device__ __forceinline__ void arrive(int& a, int& b) { asm volatile("" : "+v"(a), "+v"(b)); }
 
 // A row group's list, walked along with the classes.
 struct ListWalk {
@@ -191,6 +194,7 @@ struct ListWalk {
         const int i = (at & ~63) + lane;
         wkey = i < end ? (int)keys[i] : -1;
         wval = i < end ? __float_as_int(vals[i]) : 0;
+        arrive(wkey, wval);
     }
     __device__ __forceinline__ void start(const XentGradArgs& x, bool have, int64_t group, int64_t tile, int lane) {
         keys = x.keys + (have ? group * x.list : 0);
@@ -237,7 +241,13 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
     stage<REC>(y.str + t0 * REC, lds, tid);
     // F from the largest exponent bound of the stream
     int um = -200;
-    for (int64_t i = lane; i < y.str_tiles; i += 64) um = max(um, y.str_u[i]);
+    for (int64_t i = lane; i < y.str_tiles; i += 64 * 16) {
+        int u[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) u[j] = y.str_u[min(i + 64 * j, y.str_tiles - 1)];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) um = max(um, u[j]);
+    }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) um = max(um, __shfl_xor(um, o, 64));
     const int F = 14 - __builtin_amdgcn_readfirstlane(um);
@@ -253,31 +263,25 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
     f32x16 acc[D] = {};
     float dbias = 0.0f;
 
-    // the slice of the next record is read while a record is worked on, its bounds one earlier
+    // the slice of the next record is read while a record's second product runs, its bounds one earlier
     ListWalk walk;
-    ListSlice next, after;
+    ListSlice slice, after;
     if constexpr (ROWS) {
         walk.start(x, have, og, t0, lane);
     } else {
-        next.bounds(x, t0, ob);
-        next.read(x, t0, next.from, lane);
+        slice.bounds(x, t0, ob);
+        slice.read(x, t0, slice.from, lane);
         after.bounds(x, min(t0 + 1, y.str_tiles - 1), ob);
     }
     for (int64_t t = t0; t < t1; ++t) {
         const uint8_t* cur = lds + ((t - t0) & 1) * REC;
         wait_loads();
+        if constexpr (!ROWS) {
+            arrive(slice.key, slice.val);
+            arrive(after.from, after.to);
+        }
         __syncthreads();
         if (t + 1 < t1) stage<REC>(y.str + (t + 1) * REC, lds + ((t + 1 - t0) & 1) * REC, tid);
-        ListSlice mine;
-        if constexpr (!ROWS) {
-            mine = next;
-            if (t + 1 < t1) {
-                next.from = after.from;
-                next.to = after.to;
-                next.read(x, t + 1, next.from, lane);
-                after.bounds(x, min(t + 2, y.str_tiles - 1), ob);
-            }
-        }
         f32x16 s[1];
         // the matrix instructions of one wave before the vector work of the CU's others
         __builtin_amdgcn_s_setprio(1);
@@ -315,26 +319,32 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
                 for (int e = 0; e < 4; ++e)
                     p[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(p[4 * q + e], cc, own0) - lse[e]) * (g[e] * scale);
             }
-            const int from = __builtin_amdgcn_readfirstlane(mine.from), to = __builtin_amdgcn_readfirstlane(mine.to);
+            const int from = __builtin_amdgcn_readfirstlane(slice.from), to = __builtin_amdgcn_readfirstlane(slice.to);
             for (int first = from; first < to; first += 64) {
-                if (first != from) mine.read(x, t, first, lane);
-                unsigned long long todo = __ballot((int64_t)(uint32_t)mine.key >> 10 == og && first + lane < to);
+                if (first != from) {
+                    slice.read(x, t, first, lane);
+                    arrive(slice.key, slice.val);
+                }
+                unsigned long long todo = __ballot((int64_t)((uint32_t)slice.key >> 10) == og && first + lane < to);
                 while (todo) {
                     const int l = __builtin_ctzll(todo);
                     todo &= todo - 1;
-                    const int key = lane_value(mine.key, l);
+                    const int key = lane_value(slice.key, l);
                     const int cls = (key >> 5) & 31, row = key & 31;
-                    const float v = ldexpf(__int_as_float(lane_value(mine.val, l)) * aux[32 + row], fs);
+                    const float v = __int_as_float(lane_value(slice.val, l)) * aux[32 + row] * scale;
                     set_entry(p, (row >> 3) * 4 + (row & 3), lane == cls + 32 * ((row >> 2) & 1), v);
                 }
             }
+            slice.from = after.from;
+            slice.to = after.to;
+            slice.read(x, min(t + 1, y.str_tiles - 1), slice.from, lane);
+            after.bounds(x, min(t + 2, y.str_tiles - 1), ob);
             float add = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) add += p[r];
             dbias += ldexpf(add, -fs);
-            if (fe != fs)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) p[r] = ldexpf(p[r], fe - fs);
+            // a record whose values are 2^-60 of the largest: nothing of it reaches the sums
+            if (fe != fs) continue;
         }
         __builtin_amdgcn_s_setprio(1);
         const f16x8* tr = reinterpret_cast<const f16x8*>(cur + P * D * 2048) + lane;
