@@ -211,13 +211,15 @@ __global__ __launch_bounds__(threads_of(G)) void forward_kernel(const T* __restr
     }
 }
 
-template <typename T, int G, int R, bool VEC>
-__global__ __launch_bounds__(threads_of(G)) void backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+// A single workgroup (final: its sums are dw and db themselves) has no second kernel to wait for.
+template <typename T, int G, int R, bool VEC, int NT>
+__global__ __launch_bounds__(NT) void backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                                  const float* __restrict__ w,
                                                                  const float* __restrict__ mean,
                                                                  const float* __restrict__ rstd, int64_t m, int d,
-                                                                 T* __restrict__ dx, float* __restrict__ part) {
-    constexpr int TEAMS = threads_of(G) / G, V = kV<T>, E = V * R;
+                                                                 T* __restrict__ dx, float* __restrict__ part, float* final_dw,
+                                                                 float* final_db) {
+    constexpr int TEAMS = NT / G, V = kV<T>, E = V * R;
     constexpr bool AHEAD = G < 1024;  // its registers would not hold the next row beside this one
     __shared__ float2 red[2][G > 64 ? G / 64 : 1];
     __shared__ float cols[TEAMS > 1 ? TEAMS * E * G : 1];
@@ -269,27 +271,27 @@ __global__ __launch_bounds__(threads_of(G)) void backward_kernel(const T* __rest
         }
         if (!AHEAD && r0 + step < m) fetch(row + step);
     }
-    if (!part) return;
-    float* out = part + (int64_t)blockIdx.x * 2 * d;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
+        float* out = part ? part + ((int64_t)blockIdx.x * 2 + which) * d : which ? final_db : final_dw;
+        if (!out) continue;  // the same for the workgroup
         if constexpr (TEAMS > 1) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < E; ++i)
                 cols[team * (E * G) + column<V, G, VEC>(i / V, i % V, l)] = which ? db[i] : dw[i];
             __syncthreads();
-            for (int c = threadIdx.x; c < d; c += threads_of(G)) {
+            for (int c = threadIdx.x; c < d; c += NT) {
                 float s = 0.0f;
 #pragma unroll
                 for (int t = 0; t < TEAMS; ++t) s += cols[t * (E * G) + c];
-                out[which * d + c] = s;
+                out[c] = s;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 const int c = column<V, G, VEC>(i / V, i % V, l);
-                if (c < d) out[which * d + c] = which ? db[i] : dw[i];
+                if (c < d) out[c] = which ? db[i] : dw[i];
             }
         }
     }
@@ -332,15 +334,18 @@ int forward(const T* x, const float* w, const float* b, int64_t m, int d, float 
     PPOCR_HIP(hipGetLastError());
     return PPOCR_OK;
 }
-template <typename T, int G, int R>
+template <typename T, int G, int R, int NT = threads_of(G)>
 int backward(const T* dy, const T* x, const float* w, const float* mean, const float* rstd, int64_t m, int d, bool vec, T* dx,
-             float* part, int parts, hipStream_t st) {
-    constexpr int NT = threads_of(G);
-    if (vec) backward_kernel<T, G, R, true><<<parts, NT, 0, st>>>(dy, x, w, mean, rstd, m, d, dx, part);
-    else backward_kernel<T, G, R, false><<<parts, NT, 0, st>>>(dy, x, w, mean, rstd, m, d, dx, part);
+             float* part, int parts, float* dw, float* db, hipStream_t st) {
+    if (vec) backward_kernel<T, G, R, true, NT><<<parts, NT, 0, st>>>(dy, x, w, mean, rstd, m, d, dx, part, dw, db);
+    else backward_kernel<T, G, R, false, NT><<<parts, NT, 0, st>>>(dy, x, w, mean, rstd, m, d, dx, part, dw, db);
     PPOCR_HIP(hipGetLastError());
     return PPOCR_OK;
 }
+
+// Few narrow rows: one workgroup of 64 teams instead of a second kernel (120 rows of 120, with both
+// launches: 9.7 us of kernels so, see below).
+constexpr int kFewRows = 256;
 
 // Lanes of a row's team by its width.
 int team_of(int64_t d) { return d <= 128 ? 16 : d <= 1024 ? 64 : d <= 4096 ? 256 : d <= 8192 ? 512 : 1024; }
@@ -361,21 +366,24 @@ int forward_of(const T* x, const float* w, const float* b, int64_t m, int d, flo
 }
 template <typename T>
 int backward_of(const T* dy, const T* x, const float* w, const float* mean, const float* rstd, int64_t m, int d, T* dx,
-                float* part, int parts, hipStream_t st) {
+                float* part, int parts, float* dw, float* db, hipStream_t st) {
     const bool vec = d % kV<T> == 0 && aligned(x) && aligned(dy) && aligned(dx) && aligned(w);
-    if (d <= 128) return backward<T, 16, (sizeof(T) == 4 ? 2 : 1)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, st);
-    if (d <= 512) return backward<T, 64, (sizeof(T) == 4 ? 2 : 1)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, st);
-    if (d <= 1024) return backward<T, 64, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, st);
-    if (d <= 2048) return backward<T, 256, (sizeof(T) == 4 ? 2 : 1)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, st);
-    if (d <= 4096) return backward<T, 256, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, st);
-    if (d <= 8192) return backward<T, 512, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, st);
-    return backward<T, 1024, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, st);
+    if (d <= 128 && m <= kFewRows)
+        return backward<T, 16, (sizeof(T) == 4 ? 2 : 1), 1024>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
+    if (d <= 128) return backward<T, 16, (sizeof(T) == 4 ? 2 : 1)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
+    if (d <= 512) return backward<T, 64, (sizeof(T) == 4 ? 2 : 1)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
+    if (d <= 1024) return backward<T, 64, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
+    if (d <= 2048) return backward<T, 256, (sizeof(T) == 4 ? 2 : 1)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
+    if (d <= 4096) return backward<T, 256, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
+    if (d <= 8192) return backward<T, 512, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
+    return backward<T, 1024, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
 }
 
 }  // namespace
 
 int layernorm_parts(int64_t m, int64_t d) {
     const int g = team_of(d), teams = threads_of(g) / g;
+    if (m > 0 && d <= 128 && m <= kFewRows) return 1;
     return (int)std::min<int64_t>((m + teams - 1) / teams, parts_of(g));
 }
 
@@ -388,13 +396,17 @@ int launch_layernorm_forward(const void* x, const float* w, const float* b, int6
 int launch_layernorm_backward(const void* dy, const void* x, const float* w, const float* mean, const float* rstd, int64_t m,
                               int d, int bf16, void* dx, float* dw, float* db, float* part, hipStream_t st) {
     const int parts = layernorm_parts(m, d);
-    float* p = dw || db ? part : nullptr;
+    const bool sums = (dw || db) && parts != 1;
     if (parts) {
-        if (int e = bf16 ? backward_of((const uint16_t*)dy, (const uint16_t*)x, w, mean, rstd, m, d, (uint16_t*)dx, p, parts, st)
-                         : backward_of((const float*)dy, (const float*)x, w, mean, rstd, m, d, (float*)dx, p, parts, st))
+        float* p = sums ? part : nullptr;
+        float* fw = sums ? nullptr : dw;
+        float* fb = sums ? nullptr : db;
+        if (int e = bf16 ? backward_of((const uint16_t*)dy, (const uint16_t*)x, w, mean, rstd, m, d, (uint16_t*)dx, p, parts, fw,
+                                       fb, st)
+                         : backward_of((const float*)dy, (const float*)x, w, mean, rstd, m, d, (float*)dx, p, parts, fw, fb, st))
             return e;
     }
-    if (dw || db) {
+    if (sums) {
         // narrow rows: more workgroups (512 sums of 2 x 120 columns: 3.8 us, 4.4 with 16 columns each);
         // wide ones: whole lines (768 of 2 x 4096: 8.7 us, 16.5 with 8 columns each)
         if (d <= 512) columns_kernel<8><<<(unsigned)((2 * (int64_t)d + 7) / 8), 1024, 0, st>>>(part, parts, d, dw, db);

@@ -17,6 +17,18 @@ __device__ __forceinline__ float to_log2(float l) { return fmaf(l, kLog2e, l * k
 __device__ __forceinline__ float value(const float* p) { return *p; }
 __device__ __forceinline__ float value(const uint16_t* p) { return __uint_as_float((unsigned)*p << 16); }
 
+// The head and its rows: a [.][k], w [n][k].  VEC: k and both addresses are multiples of four values,
+// so that rows can be read four at a time.
+template <typename T, bool VEC>
+struct HeadRef {
+    typedef T type;
+    static constexpr bool vec = VEC;
+    const T* a;
+    const T* w;
+    const float* bias;
+    int k;
+};
+
 // ---------------------------------------------------------------- target entries
 // Entry i of row r: its class (-1: none) and, for distillation, the teacher's logit over tau.
 struct Targets {
@@ -33,29 +45,64 @@ struct Targets {
     __device__ __forceinline__ float logit(int64_t r, int i) const { return target ? 0.0f : z[r * tn + i] * inv_tau; }
 };
 
-// a_r . w_c + b_c, by 8 neighbouring lanes (all of them call it); 0 for c < 0.
 template <typename T>
-__device__ __forceinline__ float logit_of(const T* __restrict__ a, const T* __restrict__ w, const float* bias, int64_t r,
-                                          int c, int k, int l8) {
-    float s = 0.0f;
-    if (c >= 0) {
-        const T* pa = a + r * k;
-        const T* pw = w + (int64_t)c * k;
-        int j = l8;
-        for (; j + 24 < k; j += 32) {
-            float x[4], y[4];
+struct alignas(4 * sizeof(T)) Four {
+    T v[4];
+};
+// Values j .. j + 3 of a row of k, zeros past its end.
+template <bool VEC, typename T>
+__device__ __forceinline__ Four<T> read_four(const T* __restrict__ p, int j, int k) {
+    Four<T> q{};
+    if constexpr (VEC) {
+        if (j < k) q = *reinterpret_cast<const Four<T>*>(p + j);
+    } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = value(pa + j + 8 * i);
+        for (int u = 0; u < 4; ++u)
+            if (j + u < k) q.v[u] = p[j + u];
+    }
+    return q;
+}
+
+// a_r . w_c + b_c of N classes by 8 neighbouring lanes (all of them call it); 0 for c < 0, whose place
+// class 0 is read for, so that the reads of all N are on their way at once.
+template <int N, typename H>
+__device__ __forceinline__ void logits_of(const H& h, int64_t r, const int (&c)[N], int l8, float (&out)[N]) {
+    constexpr int PIECES = N == 1 ? 4 : 2;
+    const auto* pa = h.a + r * h.k;
+    float bias[N];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = value(pw + j + 8 * i);
+    for (int n = 0; n < N; ++n) {
+        bias[n] = h.bias ? h.bias[max(c[n], 0)] : 0.0f;
+        out[n] = 0.0f;
+    }
+    for (int j = 4 * l8; j < h.k; j += 32 * PIECES) {
+        Four<typename H::type> x[PIECES], y[N][PIECES];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s = fmaf(x[i], y[i], s);
-        }
-        for (; j < k; j += 8) s = fmaf(value(pa + j), value(pw + j), s);
+        for (int i = 0; i < PIECES; ++i) x[i] = read_four<H::vec>(pa, j + 32 * i, h.k);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) y[n][i] = read_four<H::vec>(h.w + (int64_t)max(c[n], 0) * h.k, j + 32 * i, h.k);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) out[n] = fmaf(value(x[i].v + u), value(y[n][i].v + u), out[n]);
     }
 #pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-    return c >= 0 && bias ? s + bias[c] : s;
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int o = 4; o >= 1; o >>= 1) out[n] += __shfl_xor(out[n], o, 64);
+        out[n] = c[n] >= 0 ? out[n] + bias[n] : 0.0f;
+    }
+}
+template <typename H>
+__device__ __forceinline__ float logit_of(const H& h, int64_t r, int c, int l8) {
+    const int cs[1] = {c};
+    float z[1];
+    logits_of(h, r, cs, l8, z);
+    return z[0];
 }
 
 // One row by a wave: lane i holds the row's entry i, its class (-1: none, or past the last), the log of
@@ -64,9 +111,9 @@ struct RowTargets {
     int cls;
     float logq, q, z;
 };
-template <typename T>
-__device__ __forceinline__ RowTargets row_targets(const Targets& tg, const T* a, const T* w, const float* bias, int64_t r,
-                                                  int k, int lane) {
+// MOST: entries of 8 lanes at a time (registers).
+template <int MOST, typename H>
+__device__ __forceinline__ RowTargets row_targets(const Targets& tg, const H& h, int64_t r, int lane) {
     RowTargets t;
     t.cls = lane < tg.tn ? tg.cls(r, lane) : -1;
     if (tg.target) {
@@ -84,12 +131,22 @@ __device__ __forceinline__ RowTargets row_targets(const Targets& tg, const T* a,
         if (!(t.q != 0.0f)) t.logq = 0.0f;
     }
     t.z = 0.0f;
-    for (int i = 0; i < tg.tn; i += 8) {
-        const int c = __shfl(t.cls, i + (lane >> 3), 64);
-        const float z = logit_of(a, w, bias, r, i + (lane >> 3) < tg.tn ? c : -1, k, lane & 7);
-        const float here = __shfl(z, (lane & 7) * 8, 64);
-        if ((lane & ~7) == i) t.z = here;
-    }
+    // 8 lanes an entry, N entries each at a time; lane i takes entry i's logit home
+    auto round = [&]<int N>(int first) {
+        int c[N];
+        float z[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) c[n] = __shfl(t.cls, first + 8 * n + (lane >> 3), 64);
+        logits_of(h, r, c, lane & 7, z);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const float here = __shfl(z[n], (lane & 7) * 8, 64);
+            if ((lane & ~7) == first + 8 * n) t.z = here;
+        }
+    };
+    if (tg.tn <= 8) round.template operator()<1>(0);
+    else
+        for (int i = 0; i < tg.tn; i += 8 * MOST) round.template operator()<MOST>(i);
     return t;
 }
 
@@ -105,29 +162,21 @@ __device__ __forceinline__ float factor_of(const Targets& tg, const float* grad,
 
 // ---------------------------------------------------------------- operand records
 // One workgroup per record of 32 entries, rows of `a` first and then classes of `w`.
-template <typename T>
+template <typename H>
 struct RecordArgs {
-    const T* a;
-    const T* w;
-    const float* bias;
+    H h;
     Targets tg;
     const float* lse;
     const float* grad;
     int64_t m, n, row_tiles;
-    int k, vec_a, vec_w;  // rows that can be read four values at a time
     uint8_t* row_rec;
     uint8_t* class_rec;
     int* row_u;
     int* class_u;
 };
 
-template <typename T>
-struct alignas(4 * sizeof(T)) Four {
-    T v[4];
-};
-
-template <typename T, int D, int P, bool BACK>
-__device__ void build_record(const RecordArgs<T>& x, int64_t t, bool rows, float* tile, float* red) {
+template <typename H, int D, int P, bool BACK>
+__device__ void build_record(const RecordArgs<H>& x, int64_t t, bool rows, float* tile, float* red) {
     constexpr int LD = 32 * D + 1;
     const int tid = threadIdx.x, e = tid >> 3, l8 = tid & 7;  // 8 lanes an entry
     const int64_t first = t * 32, count = min((int64_t)32, (rows ? x.m : x.n) - first);
@@ -140,36 +189,26 @@ __device__ void build_record(const RecordArgs<T>& x, int64_t t, bool rows, float
     }
     // a row without gradient reaches no sum, whatever it holds
     const bool in = e < count && factor != 0.0f;
-    const T* src = (rows ? x.a : x.w) + (first + (e < count ? e : 0)) * x.k;
-    float v[4 * D];
-    if (rows ? x.vec_a : x.vec_w) {
+    const int k = x.h.k;
+    const auto* src = (rows ? x.h.a : x.h.w) + (first + (e < count ? e : 0)) * k;
+    Four<typename H::type> v[D];
 #pragma unroll
-        for (int i = 0; i < D; ++i) {
-            const int j = 32 * i + 4 * l8;
-            Four<T> q{};
-            if (in && j < x.k) q = *reinterpret_cast<const Four<T>*>(src + j);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) v[4 * i + u] = value(q.v + u);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4 * D; ++i) {
-            const int j = 32 * (i >> 2) + 4 * l8 + (i & 3);
-            v[i] = in && j < x.k ? value(src + j) : 0.0f;
-        }
-    }
+    for (int i = 0; i < D; ++i) v[i] = read_four<H::vec>(src, 32 * i + 4 * l8, in ? k : 0);
     float first_aux = 0.0f;  // of entry `tid`
     if (tid < 32 && tid < count) {
-        if (!rows) first_aux = x.bias ? x.bias[first + tid] * (kLog2e * x.tg.inv_tau) : 0.0f;
+        if (!rows) first_aux = x.h.bias ? x.h.bias[first + tid] * (kLog2e * x.tg.inv_tau) : 0.0f;
         else if (BACK) first_aux = x.lse[first + tid];
     }
     float top = 0.0f, ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4 * D; ++i) {
-        tile[e * LD + 32 * (i >> 2) + 4 * l8 + (i & 3)] = v[i];
-        ss = fmaf(v[i], v[i], ss);
-        if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
-    }
+    for (int i = 0; i < D; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float f = value(v[i].v + u);
+            tile[e * LD + 32 * i + 4 * l8 + u] = f;
+            ss = fmaf(f, f, ss);
+            if (fabsf(f) < INFINITY) top = fmaxf(top, fabsf(f));
+        }
 #pragma unroll
     for (int o = 4; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
     top = wave_max(top);
@@ -239,16 +278,14 @@ __device__ void build_record(const RecordArgs<T>& x, int64_t t, bool rows, float
 // One workgroup per group of 32 rows: every target entry's p - q in 32 bits, sorted by class (then
 // row), entries of one row that name the same class joined, and where each block of 128 classes
 // starts in the list.
-template <typename T>
+template <typename H>
 struct ListArgs {
-    const T* a;
-    const T* w;
-    const float* bias;
+    H h;
     Targets tg;
     const float* lse;
     const float* grad;
     int64_t m;
-    int k, list, size, blocks;  // list = 32 tn entries, size = list rounded up to a power of two; blocks of 128 classes
+    int list, size, blocks;  // list = 32 tn entries, size = list rounded up to a power of two; blocks of 128 classes
     uint32_t* keys;
     float* vals;
     uint16_t* offs;
@@ -302,8 +339,8 @@ __device__ void sort_keys(unsigned long long* key, int list, int size) {
     __syncthreads();
 }
 
-template <typename T, int NT>
-__device__ void build_list(const ListArgs<T>& x, int64_t g, unsigned long long* key, float* pv, float* qv) {
+template <typename H, int NT>
+__device__ void build_list(const ListArgs<H>& x, int64_t g, unsigned long long* key, float* pv, float* qv) {
     const int tid = threadIdx.x, tn = x.tg.tn;
     auto put = [&](int s, int row, int c, float z, float q, float lse) {
         key[s] = c >= 0 ? ((unsigned long long)(((uint32_t)c << 5) | row) << 11) | s : ~0ull;
@@ -316,7 +353,7 @@ __device__ void build_list(const ListArgs<T>& x, int64_t g, unsigned long long* 
             const int64_t r = g * 32 + row;
             const float f = factor_of(x.tg, x.grad, min(r, x.m - 1), tid & 7);
             const int c = r < x.m && f != 0.0f ? x.tg.cls(r, 0) : -1;
-            const float z = logit_of(x.a, x.w, x.bias, r, c, x.k, tid & 7);
+            const float z = logit_of(x.h, min(r, x.m - 1), c, tid & 7);
             if ((tid & 7) == 0) put(row, row, c, z, 1.0f, c >= 0 ? x.lse[r] : 0.0f);
         }
     } else {
@@ -327,7 +364,7 @@ __device__ void build_list(const ListArgs<T>& x, int64_t g, unsigned long long* 
             RowTargets t{-1, 0.0f, 0.0f, 0.0f};
             bool live = r < x.m && (!x.grad || x.grad[r] != 0.0f);
             if (live) {
-                t = row_targets(x.tg, x.a, x.w, x.bias, r, x.k, lane);
+                t = row_targets<sizeof(typename H::type) == 2 ? 2 : 1>(x.tg, x.h, r, lane);
                 live = __any(t.q != 0.0f);
             }
             if (lane < tn) put(row * tn + lane, row, live ? t.cls : -1, t.z, t.q, live ? x.lse[r] : 0.0f);
@@ -363,27 +400,27 @@ __device__ void build_list(const ListArgs<T>& x, int64_t g, unsigned long long* 
 }
 
 // Records, and with one target a row (a label) the lists too.
-template <typename T, int D, int P, bool BACK>
-__global__ __launch_bounds__(kThreads) void prep_kernel(RecordArgs<T> x, ListArgs<T> y, unsigned class_tiles) {
+template <typename H, int D, int P, bool BACK>
+__global__ __launch_bounds__(kThreads) void prep_kernel(RecordArgs<H> x, ListArgs<H> y, unsigned class_tiles) {
     __shared__ __align__(16) float lds[32 * (32 * D + 1) + 8 + 32];
     static_assert(sizeof(lds) >= 32 * 16, "a list of 32 entries");
     const unsigned b = blockIdx.x;
     if (b < x.row_tiles + class_tiles) {
         const bool rows = b < x.row_tiles;
-        build_record<T, D, P, BACK>(x, rows ? b : b - x.row_tiles, rows, lds, lds + 32 * (32 * D + 1));
+        build_record<H, D, P, BACK>(x, rows ? b : b - x.row_tiles, rows, lds, lds + 32 * (32 * D + 1));
     } else if constexpr (BACK) {
         unsigned long long* key = reinterpret_cast<unsigned long long*>(lds);
         float* pv = reinterpret_cast<float*>(key + 32);
-        build_list<T, kThreads>(y, b - x.row_tiles - class_tiles, key, pv, pv + 32);
+        build_list<H, kThreads>(y, b - x.row_tiles - class_tiles, key, pv, pv + 32);
     }
 }
 constexpr int kListThreads = 1024;
-template <typename T>
-__global__ __launch_bounds__(kListThreads) void list_kernel(ListArgs<T> y) {
+template <typename H>
+__global__ __launch_bounds__(kListThreads, 8) void list_kernel(ListArgs<H> y) {
     extern __shared__ __align__(16) uint8_t list_lds[];
     unsigned long long* key = reinterpret_cast<unsigned long long*>(list_lds);
     float* pv = reinterpret_cast<float*>(key + y.size);
-    build_list<T, kListThreads>(y, blockIdx.x, key, pv, pv + y.size);
+    build_list<H, kListThreads>(y, blockIdx.x, key, pv, pv + y.size);
 }
 
 // ---------------------------------------------------------------- forward: merge and loss
@@ -405,9 +442,9 @@ __device__ __forceinline__ float log_sum(float ref, float sum) {
 }
 
 // Labels of many rows: 8 lanes a row (30720 rows: 9 us, 26 with a wave a row).
-template <typename T>
-__global__ __launch_bounds__(kThreads) void label_loss_kernel(const T* a, const T* w, const float* bias, Targets tg, int64_t m,
-                                                              int k, int nsplit, const float2* __restrict__ part, float* loss,
+template <typename H>
+__global__ __launch_bounds__(kThreads) void label_loss_kernel(H h, Targets tg, int64_t m, int nsplit,
+                                                              const float2* __restrict__ part, float* loss,
                                                               float* lse) {
     const int l8 = threadIdx.x & 7;
     const int64_t row = (int64_t)blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3), r = min(row, m - 1);
@@ -416,7 +453,7 @@ __global__ __launch_bounds__(kThreads) void label_loss_kernel(const T* a, const 
     for (int s = l8; s < nsplit; s += 8) join(&ref, &sum, part[(int64_t)s * m + r]);
 #pragma unroll
     for (int o = 4; o >= 1; o >>= 1) join(&ref, &sum, make_float2(__shfl_xor(ref, o, 64), __shfl_xor(sum, o, 64)));
-    const float z = logit_of(a, w, bias, r, c, k, l8);
+    const float z = logit_of(h, r, c, l8);
     if (row < m && l8 == 0) {
         const float l = log_sum(ref, sum);
         loss[row] = c >= 0 ? l - z : 0.0f;
@@ -425,14 +462,14 @@ __global__ __launch_bounds__(kThreads) void label_loss_kernel(const T* a, const 
 }
 
 // A wave per row: the chunks' statistics of the row, then its targets' logits.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void loss_kernel(const T* a, const T* w, const float* bias, Targets tg, int64_t m,
-                                                        int k, int nsplit, const float2* __restrict__ part, float* loss,
+template <typename H>
+__global__ __launch_bounds__(kThreads) void loss_kernel(H h, Targets tg, int64_t m, int nsplit,
+                                                        const float2* __restrict__ part, float* loss,
                                                         float* lse) {
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
     if (row >= m) return;
-    const RowTargets t = row_targets(tg, a, w, bias, row, k, lane);
+    const RowTargets t = row_targets<4>(tg, h, row, lane);
     float ref = -INFINITY, sum = 0.0f;
     for (int s = lane; s < nsplit; s += 64) join(&ref, &sum, part[(int64_t)s * m + row]);
 #pragma unroll
@@ -567,15 +604,17 @@ void pick_grads(XentLayout* L, int64_t m, int64_t n, int planes) {
 
 bool in_fours(const void* p, int k, bool bf16) { return k % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (bf16 ? 8 : 16) == 0; }
 
-Targets targets_of(const XentProblem& x) {
-    return Targets{x.target, x.teacher_idx, x.teacher_z, x.tn, 1.0f / x.tau, x.n};
+// f(head) with the problem's head as it can be read.
+template <typename T, typename F>
+int with_head(const XentProblem& x, F&& f) {
+    const T* a = static_cast<const T*>(x.a);
+    const T* w = static_cast<const T*>(x.w);
+    if (in_fours(x.a, x.k, x.bf16) && in_fours(x.w, x.k, x.bf16)) return f(HeadRef<T, true>{a, w, x.bias, x.k});
+    return f(HeadRef<T, false>{a, w, x.bias, x.k});
 }
 
-template <typename T, int D, int P, bool BACK>
-int prep_cfg(const RecordArgs<T>& r, const ListArgs<T>& y, unsigned class_tiles, unsigned grid, hipStream_t st) {
-    prep_kernel<T, D, P, BACK><<<grid, kThreads, 0, st>>>(r, y, class_tiles);
-    PPOCR_HIP(hipGetLastError());
-    return PPOCR_OK;
+Targets targets_of(const XentProblem& x) {
+    return Targets{x.target, x.teacher_idx, x.teacher_z, x.tn, 1.0f / x.tau, x.n};
 }
 
 // f.template operator()<D>() for the layout's D.
@@ -593,40 +632,42 @@ int by_pieces(int D, F&& f) {
 
 template <typename T, int P, bool BACK>
 int prep(const XentProblem& x, const XentLayout& L, uint8_t* ws, hipStream_t st) {
-    const Targets tg = targets_of(x);
-    const RecordArgs<T> r{static_cast<const T*>(x.a), static_cast<const T*>(x.w), x.bias, tg, x.lse, x.grad, x.m, x.n,
-                          L.row_tiles, x.k, in_fours(x.a, x.k, x.bf16), in_fours(x.w, x.k, x.bf16),
-                          ws + (BACK ? L.b_row_rec : L.f_row_rec), ws + (BACK ? L.b_class_rec : L.f_class_rec),
-                          reinterpret_cast<int*>(ws + L.b_row_u), reinterpret_cast<int*>(ws + L.b_class_e)};
-    const int list = 32 * x.tn;
-    int size = 32;
-    while (size < list) size *= 2;
-    const ListArgs<T> y{r.a, r.w, x.bias, tg, x.lse, x.grad, x.m, x.k, list, size, (int)div_up(x.n, 128),
-                        reinterpret_cast<uint32_t*>(ws + L.b_keys), reinterpret_cast<float*>(ws + L.b_vals),
-                        reinterpret_cast<uint16_t*>(ws + L.b_offs)};
-    const bool lists_here = BACK && x.target;
-    const unsigned grid = (unsigned)(L.row_tiles * (lists_here ? 2 : 1) + L.class_tiles);
-    if (int e = by_pieces(L.D, [&]<int D>() { return prep_cfg<T, D, P, BACK>(r, y, (unsigned)L.class_tiles, grid, st); }))
-        return e;
-    if (BACK && !x.target) {
-        list_kernel<T><<<(unsigned)L.row_tiles, kListThreads, (size_t)size * 16, st>>>(y);
+    return with_head<T>(x, [&]<typename H>(const H& h) -> int {
+        const Targets tg = targets_of(x);
+        const RecordArgs<H> r{h, tg, x.lse, x.grad, x.m, x.n, L.row_tiles, ws + (BACK ? L.b_row_rec : L.f_row_rec),
+                              ws + (BACK ? L.b_class_rec : L.f_class_rec), reinterpret_cast<int*>(ws + L.b_row_u),
+                              reinterpret_cast<int*>(ws + L.b_class_e)};
+        const int list = 32 * x.tn;
+        int size = 32;
+        while (size < list) size *= 2;
+        const ListArgs<H> y{h, tg, x.lse, x.grad, x.m, list, size, (int)div_up(x.n, 128),
+                            reinterpret_cast<uint32_t*>(ws + L.b_keys), reinterpret_cast<float*>(ws + L.b_vals),
+                            reinterpret_cast<uint16_t*>(ws + L.b_offs)};
+        const bool lists_here = BACK && x.target;
+        const unsigned grid = (unsigned)(L.row_tiles * (lists_here ? 2 : 1) + L.class_tiles);
+        by_pieces(L.D, [&]<int D>() {
+            prep_kernel<H, D, P, BACK><<<grid, kThreads, 0, st>>>(r, y, (unsigned)L.class_tiles);
+            return 0;
+        });
         PPOCR_HIP(hipGetLastError());
-    }
-    return PPOCR_OK;
+        if (BACK && !x.target) {
+            list_kernel<H><<<(unsigned)L.row_tiles, kListThreads, (size_t)size * 16, st>>>(y);
+            PPOCR_HIP(hipGetLastError());
+        }
+        return PPOCR_OK;
+    });
 }
 
 template <typename T>
 int losses(const XentProblem& x, const Targets& tg, int nsplit, const float2* part, float* loss, float* lse, hipStream_t st) {
-    const T* a = static_cast<const T*>(x.a);
-    const T* w = static_cast<const T*>(x.w);
-    if (x.target && x.m > 4096)
-        label_loss_kernel<T><<<(unsigned)div_up(x.m, kThreads / 8), kThreads, 0, st>>>(a, w, x.bias, tg, x.m, x.k, nsplit, part,
-                                                                                     loss, lse);
-    else
-        loss_kernel<T><<<(unsigned)div_up(x.m, kThreads / 64), kThreads, 0, st>>>(a, w, x.bias, tg, x.m, x.k, nsplit, part,
-                                                                                loss, lse);
-    PPOCR_HIP(hipGetLastError());
-    return PPOCR_OK;
+    return with_head<T>(x, [&]<typename H>(const H& h) -> int {
+        if (x.target && x.m > 4096)
+            label_loss_kernel<H><<<(unsigned)div_up(x.m, kThreads / 8), kThreads, 0, st>>>(h, tg, x.m, nsplit, part, loss, lse);
+        else
+            loss_kernel<H><<<(unsigned)div_up(x.m, kThreads / 64), kThreads, 0, st>>>(h, tg, x.m, nsplit, part, loss, lse);
+        PPOCR_HIP(hipGetLastError());
+        return PPOCR_OK;
+    });
 }
 
 template <typename T>
