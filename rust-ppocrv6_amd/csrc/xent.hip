@@ -259,18 +259,21 @@ __device__ void build_record(const RecordArgs<H>& x, int64_t t, bool rows, float
                 aux[tid] = 0.0f;
                 aux[32 + tid] = 0.0f;
             }
-        } else if (tid < 48) {
+        } else if (tid < 48 && tid != 36) {
             const float norm = sqrtf(fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7])));
             aux[32 + tid] = tid == 32 ? ldexpf(1.0f, -ex) : tid == 33 ? (float)ex : tid == 34 ? norm : tid == 35 ? most : 0.0f;
         }
     }
-    if (BACK && tid == 0) {
-        float s = 0.0f;
-        for (int i = 0; i < 32 && rows; ++i)
-            if (fabsf(gf[i]) < INFINITY) s = fmaxf(s, fabsf(gf[i]));
-        // the largest of what multiplies this record's values, as an exponent, against its own
-        if (rows) x.row_u[t] = s > 0.0f ? max(ilogbf(s) + 1 - ex, -200) : -200;
-        else x.class_u[t] = -ex;
+    if (BACK && tid < 64) {
+        // The largest of what multiplies this record's values, as an exponent, against its own.  Factors
+        // below 2^-112 are taken as that, so that the scale they get (up to 2^126) is a number.
+        float f = tid < 32 && rows ? fabsf(gf[tid]) : 0.0f;
+        f = wave_max(f < INFINITY ? f : 0.0f);
+        if (tid == 0) {
+            const int u = !rows ? -ex : f > 0.0f ? max(ilogbf(f) + 1, -112) - ex : -212;
+            (rows ? x.row_u : x.class_u)[t] = u;
+            aux[68] = (float)u;
+        }
     }
 }
 
@@ -552,6 +555,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs<T> a, SumArgs<T> 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int kBlockTiles = 4;  // records of a block of 128 classes
 constexpr int kMostChunks = 64;
+constexpr int64_t kMostGroups = 1 << 22;  // workgroups of a launch that is split further (grids count threads in 32 bits)
 
 // Chunks of the class records for the statistics: the fewest records that any place of the GPU works
 // through one after the other (a workgroup's start and end take about two records' time).
@@ -562,6 +566,7 @@ void pick_stats(XentLayout* L, int64_t m, int planes) {
     for (int s = 1; s <= 256; ++s) {
         const int64_t per = div_up(L->class_tiles, s);
         if (div_up(L->class_tiles, per) != s) continue;
+        if (s > 1 && blocks * s > kMostGroups) break;
         const int64_t cost = 8 * div_up(blocks * s, places) * (per + 2) + s / 4;
         if (best < 0 || cost < best) {
             best = cost;
@@ -584,7 +589,7 @@ void pick_grads(XentLayout* L, int64_t m, int64_t n, int planes) {
         const bool by_a = L->class_tiles <= L->row_tiles;
         const int64_t per = div_up(div_up(by_a ? L->class_tiles : L->row_tiles, s), kBlockTiles) * kBlockTiles;
         const int64_t sa = div_up(L->class_tiles, per), sw = div_up(L->row_tiles, per);
-        if (sa > kMostChunks || sw > kMostChunks) break;
+        if (sa > kMostChunks || sw > kMostChunks || (s > 1 && ba * sa + bw * sw > kMostGroups)) break;
         const double cost = (double)div_up(ba * sa + bw * sw, places) * (double)(per + 2) +
                             chunk_cost * (double)(sa * m + sw * n);
         if (best < 0 || cost < best) {

@@ -29,8 +29,9 @@ constexpr int64_t kXentMaxN = 1 << 26;  // classes: a list key holds a class and
 //                                           (backward only)
 //   float[32], float[32], float[16]         per entry: class: bias log2(e) / tau; row: lse
 //                                           log2(e) and gradient factor; then 2^-e, e, the
-//                                           largest L2 norm of an entry and the largest finite
-//                                           magnitude among the first 32 values
+//                                           largest L2 norm of an entry, the largest finite
+//                                           magnitude among the first 32 values and the exponent
+//                                           bound that XentGradSide::str_u holds
 // D = the number of 32-wide pieces of k, one of 1, 2, 3, 4, 6, 8.
 constexpr int kXentAux = 320;
 inline int xent_pieces(int64_t k) {

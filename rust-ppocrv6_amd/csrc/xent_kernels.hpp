@@ -240,7 +240,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
 
     stage<REC>(y.str + t0 * REC, lds, tid);
     // F from the largest exponent bound of the stream
-    int um = -200;
+    int um = -1000;
     for (int64_t i = lane; i < y.str_tiles; i += 64 * 16) {
         int u[16];
 #pragma unroll
@@ -290,7 +290,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
         f32x16& p = s[0];
         const float* aux = reinterpret_cast<const float*>(cur + AUX);
         const float cc = c * aux[64];
-        const int fe = __builtin_amdgcn_readfirstlane(min(F - (int)aux[65], 100));  // exponent of this record's factor
+        const int fe = __builtin_amdgcn_readfirstlane(F - (int)aux[65]);  // exponent of this record's factor
         if constexpr (ROWS) {
             const float shift = own0 - (float)fe;
 #pragma unroll
@@ -308,8 +308,10 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
                 walk.step(lane);
             }
         } else {
-            // (not below 2^-60, so that the bias's sum keeps the values of records of tiny activations)
-            const int fs = max(fe, -60);
+            // The bias's sum does not weigh a row by its activations: a record whose activations are 2^60
+            // smaller than others' keeps a scale of its own for it.
+            const int low = __builtin_amdgcn_readfirstlane(max(14 - F - (int)aux[68] - 60, 0));
+            const int fs = fe + low;
             const float scale = ldexpf(1.0f, fs);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -343,8 +345,8 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
 #pragma unroll
             for (int r = 0; r < 16; ++r) add += p[r];
             dbias += ldexpf(add, -fs);
-            // a record whose values are 2^-60 of the largest: nothing of it reaches the sums
-            if (fe != fs) continue;
+            // and nothing of it reaches the other sums
+            if (low > 0) continue;
         }
         __builtin_amdgcn_s_setprio(1);
         const f16x8* tr = reinterpret_cast<const f16x8*>(cur + P * D * 2048) + lane;
@@ -380,7 +382,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     v[e] = ldexpf(acc[d][4 * q + e], -F);
-                    if (ROWS) v[e] *= own1;
+                    if (ROWS) v[e] = own1 == 0.0f ? 0.0f : v[e] * own1;  // no gradient, whatever the head holds
                 }
                 *reinterpret_cast<f32x4*>(out + 32 * d + 8 * q + 4 * h) = v;
             }

@@ -132,6 +132,30 @@ def test_magnitudes(rh, dt):
     tc.check_step(rh, a * np.float32(1e18), w * np.float32(1e-18), b, dt, "large times small", target=to, grad=grad * np.float32(1e10))
 
 
+@pytest.mark.parametrize("size", [1e30, 1e-28, 1e-31])
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+def test_gradients_of_any_size(rh, dt, size):
+    """Loss scales far from 1, next to rows whose gradient is 2^-14 of theirs."""
+    rng = np.random.default_rng(17)
+    a, w, b, to = tc.head_inputs(rng, 100, 300, 64)
+    grad = (rng.standard_normal(100) * size).astype(np.float32)
+    grad[::5] *= np.float32(2.0 ** -14)
+    tc.check_step(rh, a, w, b, dt, f"grad {size}", target=to, grad=grad)
+    a[32:64] *= np.float32(1e-24)
+    tc.check_step(rh, a, w, b, dt, f"grad {size}, a group of tiny rows", target=to, grad=grad)
+
+
+def test_a_head_that_holds_nan(rh):
+    """NaN in a class's weights: every logit sum is NaN, but rows without label or gradient keep 0."""
+    rng = np.random.default_rng(18)
+    a, w, b, to = tc.head_inputs(rng, 64, 200, 32)
+    w[17, 3] = np.nan
+    target = np.where(np.arange(64) % 3 == 0, -1, to).astype(np.int32)
+    got = tc.Loss(rh, a, w, b, F32, target).step()
+    assert (got["loss"][::3] == 0).all() and (got["da"][::3] == 0).all()
+    assert np.isnan(got["loss"][1::3]).all() and np.isnan(got["da"][1::3]).all()
+
+
 @pytest.mark.parametrize("logit", [20.0, 9.0])
 @pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
 def test_nearly_certain_labels_keep_their_small_gradient(rh, dt, logit):
@@ -214,6 +238,39 @@ def test_equal_calls_give_equal_bits(rh, dt):
             for k, v in o.items():
                 assert np.array_equal(v.get().view(np.uint8), want[k].view(np.uint8)), (k, fill, ws)
             job.ws.d.fill_bytes(0xA5)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+def test_unaligned_tensors(rh, dt):
+    """Tensors that start one value past a vector boundary: the same bits."""
+    from ppocr_rechead.hip import synchronize
+    rng = np.random.default_rng(19)
+    a, w, b, to = tc.head_inputs(rng, 90, 300, 120)
+    idx, z = tc.teacher_inputs(rng, 90, 300, 5, to)
+    size = 4 if dt == F32 else 2
+    for kind in ({"target": to}, {"idx": idx, "z": z, "tau": 2.0}):
+        job = tc.Loss(rh, tc.typed(a, dt)[0], tc.typed(w, dt)[0], b, dt, **kind)
+        want = job.step()
+        o = job.outputs()
+        held = []
+
+        class At:
+            def __init__(self, d):
+                self.p = ctypes.c_void_p(d.p.value + size)
+
+        def past(x):
+            d = tc.up(np.concatenate([np.zeros(1, x.dtype), x.ravel()]))
+            held.append(d)
+            return At(d)
+
+        job.a, job.w = past(tc.typed(a, dt)[0]), past(tc.typed(w, dt)[0])
+        wide = {k: tc.Out((v.shape[0] * v.shape[1] + 1,), v.dtype) for k, v in o.items() if k in ("da", "dw")}
+        job.forward(o)
+        job.backward(dict(o, **{k: At(v) for k, v in wide.items()}))
+        synchronize()
+        for k, v in want.items():
+            got = wide[k].get()[1:].reshape(v.shape) if k in wide else o[k].get()
+            assert np.array_equal(got.view(np.uint8), v.view(np.uint8)), (kind.keys(), k)
 
 
 def test_replayed_graph(rh):

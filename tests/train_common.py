@@ -7,6 +7,7 @@ import numpy as np
 F32, BF16 = 0, 1
 U24 = 2.0 ** -24  # half a step of fp32, relative
 HALF = {F32: U24, BF16: 2.0 ** -8}  # largest rounding of a stored value, relative
+LEAST = {F32: 2.0 ** -150, BF16: 2.0 ** -134}  # and absolute: below 2^-126 the steps are 2^-149 and 2^-133
 
 
 def to_bf16(x):
@@ -180,8 +181,8 @@ def loss_tol(a, w, bias, z, p, dz, s, al, ref, dt, tau, q, logq):
     dw = prod(adz.T, e.T, aa, m, m * aa.max(initial=0.0) * tiny * smax)
     db = (np.where(p > 0, p * rel, 0.0) * np.abs(s)[:, None] + 8 * U24 * np.abs(dz)).sum(axis=0) \
         + adz.sum(axis=0) * 8 * np.sqrt(float(m)) * U24 + m * tiny * smax
-    return {"loss": loss, "lse": lse, "da": da + HALF[dt] * (np.abs(ref["da"]) + da),
-            "dw": dw + HALF[dt] * (np.abs(ref["dw"]) + dw), "db": db}
+    return {"loss": loss, "lse": lse, "da": da + HALF[dt] * (np.abs(ref["da"]) + da) + LEAST[dt],
+            "dw": dw + HALF[dt] * (np.abs(ref["dw"]) + dw) + LEAST[dt], "db": db + LEAST[F32]}
 
 
 def close(got, want, tol, label):
