@@ -7,27 +7,31 @@ namespace ppocr {
 namespace xent {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// REC bytes of a record from global memory into LDS, 16 per lane, without registers.
+// REC bytes of a record from global memory into LDS, 16 per lane, without registers: pieces of 1 KB, a
+// wave each in turn, and the rest by the first lanes of the next.  Addresses are the piece's (the
+// same for the wave) plus the lane's, so that a step of the stream costs no vector arithmetic.
 template <int REC>
-__device__ __forceinline__ void stage(const uint8_t* __restrict__ src, uint8_t* dst, int tid) {
-    constexpr int CH = REC / 16, PER = (CH + kThreads - 1) / kThreads;
+__device__ __forceinline__ void stage(const uint8_t* __restrict__ src, uint8_t* dst, int wave, unsigned lane16) {
+    constexpr int FULL = REC / 1024, REST = REC % 1024;
     static_assert(REC % 16 == 0, "record size");
-    const int wave_chunk = __builtin_amdgcn_readfirstlane(tid & ~63);
+    auto piece = [&](int p) {
+        const uint8_t* from = src + (size_t)p * 1024;
+        asm volatile("" : "+s"(from));  // a scalar address: the lane's part stays an offset
+        __builtin_amdgcn_global_load_lds(
+            static_cast<const void*>(from + lane16),
+            reinterpret_cast<__attribute__((address_space(3))) void*>(reinterpret_cast<uintptr_t>(dst + (size_t)p * 1024)), 16, 0,
+            0);
+    };
 #pragma unroll
-    for (int x = 0; x < PER; ++x) {
-        const int c0 = x * kThreads + wave_chunk;
-        if (CH % kThreads == 0 || c0 + (tid & 63) < CH)
-            __builtin_amdgcn_global_load_lds(
-                static_cast<const void*>(src + (size_t)(c0 + (tid & 63)) * 16),
-                reinterpret_cast<__attribute__((address_space(3))) void*>(
-                    reinterpret_cast<uintptr_t>(dst + (size_t)c0 * 16)),
-                16, 0, 0);
-    }
+    for (int x = 0; x < (FULL + kWaves - 1) / kWaves; ++x)
+        if (FULL % kWaves == 0 || x * kWaves + wave < FULL) piece(x * kWaves + wave);
+    if (REST > 0 && wave == FULL % kWaves && lane16 < REST) piece(FULL);
 }
 __device__ __forceinline__ void wait_loads() {
     __builtin_amdgcn_s_waitcnt(0x0 | (0x7 << 4) | (0xF << 8));  // vmcnt(0)
@@ -77,12 +81,13 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned lane16 = lane * 16;
     const int split = blockIdx.x % x.nsplit;
     const int64_t rb = blockIdx.x / x.nsplit;
     const int64_t t0 = (int64_t)split * x.per_split, t1 = min(t0 + x.per_split, x.tiles);
     const int64_t row0 = rb * (32 * NB * kWaves) + wave * (32 * NB);
 
-    stage<REC>(x.str + t0 * REC, lds, tid);
+    stage<REC>(x.str + t0 * REC, lds, wave, lane16);
     f16x8 own[NB][P][2 * D];
     float c[NB], norm[NB], ref[NB], sum[NB];
     bool shifted[NB];  // some row has a reference other than 0
@@ -102,11 +107,13 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
         const uint8_t* cur = lds + ((t - t0) & 1) * REC;
         wait_loads();
         __syncthreads();
-        if (t + 1 < t1) stage<REC>(x.str + (t + 1) * REC, lds + ((t + 1 - t0) & 1) * REC, tid);
+        if (t + 1 < t1) stage<REC>(x.str + (t + 1) * REC, lds + ((t + 1 - t0) & 1) * REC, wave, lane16);
         const float* aux = reinterpret_cast<const float*>(cur + P * D * 2048);
         const float ce = aux[64], cn = aux[66], cb = aux[67];
         f32x16 sc[NB];
+        __builtin_amdgcn_s_setprio(1);
         scores<D, P, NB>(cur, own, sc, lane);
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             f32x16& s = sc[b];
@@ -232,13 +239,14 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
     constexpr int REC = 2 * P * D * 2048 + kXentAux, AUX = 2 * P * D * 2048;
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned lane16 = lane * 16;
     const int split = block % y.nsplit;
     const int64_t ob = block / y.nsplit;
     const int64_t t0 = (int64_t)split * y.per_split, t1 = min(t0 + y.per_split, y.str_tiles);
     const int64_t og = ob * kWaves + wave;  // this wave's owner record
     const int64_t owner = og * 32 + (lane & 31);
 
-    stage<REC>(y.str + t0 * REC, lds, tid);
+    stage<REC>(y.str + t0 * REC, lds, wave, lane16);
     // F from the largest exponent bound of the stream
     int um = -1000;
     for (int64_t i = lane; i < y.str_tiles; i += 64 * 16) {
@@ -262,6 +270,8 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
     const float own1 = ROWS ? oaux[32 + (lane & 31)] : 0.0f;  // row: the gradient factor
     f32x16 acc[D] = {};
     float dbias = 0.0f;
+    float minus = -1.0f;  // a number the compiler does not know: it keeps the mixed-precision fma
+    asm volatile("" : "+s"(minus));
 
     // the slice of the next record is read while a record's second product runs, its bounds one earlier
     ListWalk walk;
@@ -281,7 +291,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
             arrive(after.from, after.to);
         }
         __syncthreads();
-        if (t + 1 < t1) stage<REC>(y.str + (t + 1) * REC, lds + ((t + 1 - t0) & 1) * REC, tid);
+        if (t + 1 < t1) stage<REC>(y.str + (t + 1) * REC, lds + ((t + 1 - t0) & 1) * REC, wave, lane16);
         f32x16 s[1];
         // the matrix instructions of one wave before the vector work of the CU's others
         __builtin_amdgcn_s_setprio(1);
@@ -354,10 +364,18 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
         for (int e = 0; e < 2; ++e) {
             f16x8 ph, pl;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v = p[8 * e + j];
-                ph[j] = (_Float16)v;
-                if constexpr (P == 2) pl[j] = (_Float16)(v - (float)ph[j]);
+            for (int j = 0; j < 8; j += 2) {
+                const f32x2 v = {p[8 * e + j], p[8 * e + j + 1]};
+                const f16x2 hv = __builtin_convertvector(v, f16x2);
+                ph[j] = hv[0];
+                ph[j + 1] = hv[1];
+                if constexpr (P == 2) {
+                    // what the high half leaves, in one instruction each (exact)
+                    const f32x2 r = {fmaf((float)hv[0], minus, v[0]), fmaf((float)hv[1], minus, v[1])};
+                    const f16x2 lv = __builtin_convertvector(r, f16x2);
+                    pl[j] = lv[0];
+                    pl[j + 1] = lv[1];
+                }
             }
 #pragma unroll
             for (int d = 0; d < D; ++d) {
