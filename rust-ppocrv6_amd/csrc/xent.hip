@@ -554,7 +554,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs<T> a, SumArgs<T> 
 // ---------------------------------------------------------------- shapes and launches
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int kBlockTiles = 4;  // records of a block of 128 classes
-constexpr int kMostChunks = 64;
+constexpr int kMostChunks = 128;
 constexpr int64_t kMostGroups = 1 << 22;  // workgroups of a launch that is split further (grids count threads in 32 bits)
 
 // Chunks of the class records for the statistics: the fewest records that any place of the GPU works

@@ -337,14 +337,16 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
                     slice.read(x, t, first, lane);
                     arrive(slice.key, slice.val);
                 }
+                // each lane its entry: the lane and the register it goes to, and what goes there
+                const int cls = (slice.key >> 5) & 31, row = slice.key & 31;
+                const int lane_reg = cls + 32 * ((row >> 2) & 1) + (((row >> 3) * 4 + (row & 3)) << 8);
+                const int v = __float_as_int(__int_as_float(slice.val) * aux[32 + row] * scale);
                 unsigned long long todo = __ballot((int64_t)((uint32_t)slice.key >> 10) == og && first + lane < to);
                 while (todo) {
                     const int l = __builtin_ctzll(todo);
                     todo &= todo - 1;
-                    const int key = lane_value(slice.key, l);
-                    const int cls = (key >> 5) & 31, row = key & 31;
-                    const float v = __int_as_float(lane_value(slice.val, l)) * aux[32 + row] * scale;
-                    set_entry(p, (row >> 3) * 4 + (row & 3), lane == cls + 32 * ((row >> 2) & 1), v);
+                    const int at = lane_value(lane_reg, l);
+                    set_entry(p, at >> 8, lane == (at & 63), __int_as_float(lane_value(v, l)));
                 }
             }
             slice.from = after.from;
