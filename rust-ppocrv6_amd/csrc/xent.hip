@@ -56,9 +56,14 @@ __device__ __forceinline__ Four<T> read_four(const T* __restrict__ p, int j, int
     if constexpr (VEC) {
         if (j < k) q = *reinterpret_cast<const Four<T>*>(p + j);
     } else {
+        // rows at any address: global memory is read in one piece from there too
+        if (j + 4 <= k) {
+            __builtin_memcpy(q.v, p + j, sizeof(q.v));
+        } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (j + u < k) q.v[u] = p[j + u];
+            for (int u = 0; u < 3; ++u)
+                if (j + u < k) q.v[u] = p[j + u];
+        }
     }
     return q;
 }
@@ -295,50 +300,83 @@ struct ListArgs {
 };
 constexpr uint32_t kNoKey = 0xFFFFFFFFu;
 
+// The value of lane ^ D, without memory: lane permutations within rows of 16, then swaps of halves.
+template <int D>
+__device__ __forceinline__ unsigned lane_xor(unsigned v) {
+    if constexpr (D == 1) return __builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false);        // quad 1 0 3 2
+    else if constexpr (D == 2) return __builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false);   // quad 2 3 0 1
+    else if constexpr (D == 4) {
+        const int t = __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false);                  // eight reversed: ^ 7
+        return __builtin_amdgcn_update_dpp(0, t, 0x1B, 0xF, 0xF, false);                               // quad reversed: ^ 3
+    } else if constexpr (D == 8) return __builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, false);  // row rotated by 8
+    else return (unsigned)__shfl_xor((int)v, D, 64);
+}
+template <int D>
+__device__ __forceinline__ unsigned long long lane_xor64(unsigned long long v) {
+    return ((unsigned long long)lane_xor<D>((unsigned)(v >> 32)) << 32) | lane_xor<D>((unsigned)v);
+}
+
 // Sorts `size` keys (a power of two from 32 to 2 NT; the last size - list count as largest): a bitonic
 // network whose elements tid and tid + NT each thread keeps, so that the steps within a wave are
 // exchanges of lanes and only the wider ones go through memory (2048 keys: 13 of 66).
 template <int NT>
-__device__ void sort_keys(unsigned long long* key, int list, int size) {
-    const int tid = threadIdx.x;
+struct Sorter {
     unsigned long long v[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) v[e] = e * NT + tid < list ? key[e * NT + tid] : ~0ull;
-    __syncthreads();
-    for (int w = 2; w <= size; w <<= 1)
-        for (int d = w >> 1; d >= 1; d >>= 1) {
-            if (d == NT) {
-                if (v[0] > v[1]) {
-                    const unsigned long long t = v[0];
-                    v[0] = v[1];
-                    v[1] = t;
-                }
-                continue;
+    unsigned long long* key;
+    int tid, size;
+
+    template <int W, int D>
+    __device__ __forceinline__ void step() {
+        if constexpr (D == NT) {
+            if (v[0] > v[1]) {
+                const unsigned long long t = v[0];
+                v[0] = v[1];
+                v[1] = t;
             }
+        } else {
             unsigned long long other[2] = {~0ull, ~0ull};
-            if (d >= 64) {
+            if constexpr (D >= 64) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                     if (e * NT + tid < size) key[e * NT + tid] = v[e];
                 __syncthreads();
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    if (e * NT + tid < size) other[e] = key[(e * NT + tid) ^ d];
+                    if (e * NT + tid < size) other[e] = key[(e * NT + tid) ^ D];
                 __syncthreads();
             } else {
-                other[0] = __shfl_xor(v[0], d, 64);
-                if (size > NT) other[1] = __shfl_xor(v[1], d, 64);
+                other[0] = lane_xor64<D>(v[0]);
+                if (size > NT) other[1] = lane_xor64<D>(v[1]);
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int i = e * NT + tid;
-                const bool low = ((i & d) == 0) == ((i & w) == 0);  // this place keeps the smaller one
+                const bool low = ((i & D) == 0) == ((i & W) == 0);  // this place keeps the smaller one
                 v[e] = (other[e] < v[e]) == low ? other[e] : v[e];
             }
         }
+        if constexpr (D > 1) step<W, D / 2>();
+    }
+    template <int W>
+    __device__ __forceinline__ void sort() {
+        step<W, W / 2>();
+        if constexpr (W < 2 * NT)
+            if (W < size) sort<2 * W>();
+    }
+};
+template <int NT>
+__device__ void sort_keys(unsigned long long* key, int list, int size) {
+    Sorter<NT> s;
+    s.tid = threadIdx.x;
+    s.key = key;
+    s.size = size;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) s.v[e] = e * NT + s.tid < list ? key[e * NT + s.tid] : ~0ull;
+    __syncthreads();
+    s.template sort<2>();
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-        if (e * NT + tid < size) key[e * NT + tid] = v[e];
+        if (e * NT + s.tid < size) key[e * NT + s.tid] = s.v[e];
     __syncthreads();
 }
 
@@ -515,10 +553,15 @@ __device__ __forceinline__ void sum_chunks(const SumArgs<T>& x, int k, int ld, i
         const int j = (int)(i - o * quads) * 4;
         if (j >= k) continue;
         f32x4 s = {};
-        for (int c = 0; c < x.nsplit; ++c) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(x.part + c * plane + i * 4);
+        for (int c0 = 0; c0 < x.nsplit; c0 += 8) {
+            // eight chunks on their way at once, added in their order
+            f32x4 v[8];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) s[u] += v[u];
+            for (int c = 0; c < 8; ++c) v[c] = *reinterpret_cast<const f32x4*>(x.part + min(c0 + c, x.nsplit - 1) * plane + i * 4);
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) s[u] += c0 + c < x.nsplit ? v[c][u] : 0.0f;
         }
         T* out = x.out + o * k + j;
         if (x.vec) {
@@ -554,7 +597,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs<T> a, SumArgs<T> 
 // ---------------------------------------------------------------- shapes and launches
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int kBlockTiles = 4;  // records of a block of 128 classes
-constexpr int kMostChunks = 128;
+constexpr int kMostChunks = 256;
 constexpr int64_t kMostGroups = 1 << 22;  // workgroups of a launch that is split further (grids count threads in 32 bits)
 
 // Chunks of the class records for the statistics: the fewest records that any place of the GPU works
