@@ -12,8 +12,8 @@
 // the workgroups' sums in a second kernel, in a fixed order.  A team reads its next row while it
 // sums the present one.
 //
-// 16384 bf16 rows of 4096: forward 50 us (5.4 TB/s), backward 95 + 9 us (4.2 TB/s; the last 9 the
-// workgroups' sums).  30720 fp32 rows of 120: 7.2 us (4.1 TB/s), 9.6 + 3.7 us.
+// 16384 bf16 rows of 4096: forward 50 us (5.4 TB/s), backward 94 + 8 us (4.3 TB/s; the last 8 the
+// workgroups' sums).  30720 fp32 rows of 120: 7.5 us (3.9 TB/s), 9.6 + 3.5 us.  120 rows: 3.3 + 5.2 us.
 #include <algorithm>
 
 #include "layernorm.hpp"
@@ -343,8 +343,8 @@ int backward(const T* dy, const T* x, const float* w, const float* mean, const f
     return PPOCR_OK;
 }
 
-// Few narrow rows: one workgroup of 64 teams instead of a second kernel (120 rows of 120, with both
-// launches: 9.7 us of kernels so, see below).
+// Few narrow rows: one workgroup of 64 teams instead of a second kernel (120 rows of 120: 5.2 us, with
+// the second kernel 3.6 + 2.5 and a launch more).
 constexpr int kFewRows = 256;
 
 // Lanes of a row's team by its width.

@@ -1,5 +1,13 @@
 // The matrix kernels of the vocabulary losses: the softmax statistics of the forward pass and
 // the two gradient products of the backward pass (xent.hpp for the records they read).
+//
+// Why tiles of 32 x 32 and owners in registers: an MFMA result of the logits then is, lane by lane, a
+// column of P, the operand of the second product, and a workgroup needs LDS only for the stream.
+// 30720 rows, 18710 classes, k = 120: statistics 363 us (fp32, 1220 TFLOP/s of fp16 products) and 176
+// (bf16, 840), both gradients 1700 (1040) and 742 (795).  The matrix pipe is busy 56% of the cycles in
+// the fp32 gradients and 43% in the bf16 ones, at 1.76 and 1.89 GHz.  fp32: 5% less time without the LDS
+// reads, none less for a fifth fewer vector instructions, so probably power (not measured).  bf16, an
+// earlier version: 9-10% less without the exponentials, 12-15% without the staging loads.
 #pragma once
 #include "xent.hpp"
 
@@ -413,7 +421,8 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
     }
 }
 
-// Both gradients in one launch, so that the last workgroups of one fill up with the other's.
+// Both gradients in one launch, so that the last workgroups of one fill up with the other's (and a
+// page's step has a launch less).
 template <int D, int P>
 __global__ __launch_bounds__(kThreads, xent_grad_per_cu(D, P)) void grad_kernel(XentGradArgs x) {
     extern __shared__ __align__(16) uint8_t lds[];

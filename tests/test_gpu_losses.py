@@ -369,3 +369,30 @@ def test_a_workspace_shared_with_the_head(rh):
         synchronize()
         assert np.array_equal(di.numpy(), want[0]) and np.array_equal(dm.numpy(), want[1])
     head.close()
+
+
+def test_allocation_failure(rh, monkeypatch):
+    """Without a workspace and without memory: PPOCR_ERR_NO_MEMORY from every entry point that
+    allocates, outputs untouched, and the next call works."""
+    from ppocr_rechead.hip import synchronize
+    rng = np.random.default_rng(20)
+    a, w, b, to = tc.head_inputs(rng, 50, 200, 40)
+    idx, z = tc.teacher_inputs(rng, 50, 200, 3, to)
+    for kind, op in (({"target": to}, "SoftmaxCrossEntropy"), ({"idx": idx, "z": z}, "Distill")):
+        job = tc.Loss(rh, a, w, b, F32, **kind)
+        o = job.outputs()
+        monkeypatch.setenv("PPOCR_RECHEAD_FAULT", "alloc")
+        for call in (job.forward, job.backward):
+            with pytest.raises(rh.OcrError) as e:
+                call(o, None, False)
+            assert e.value.code == rh.PPOCR_ERR_NO_MEMORY and e.value.op == op
+        monkeypatch.delenv("PPOCR_RECHEAD_FAULT")
+        synchronize()
+        for v in o.values():
+            assert (v.get().view(np.uint8) == 0xA5).all()
+        job.forward(o, None, False)
+        job.backward(o, None, False)
+        synchronize()
+        want = job.step()
+        for k, v in o.items():
+            assert np.array_equal(v.get(), want[k]), k
