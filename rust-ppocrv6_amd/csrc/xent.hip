@@ -263,25 +263,27 @@ __device__ void build_record(const RecordArgs<H>& x, int64_t t, bool rows, float
                 aux[32 + tid] = 0.0f;
             } else if (BACK) {
                 aux[tid] = gf[tid] != 0.0f ? to_log2(first_aux) : INFINITY;
-                aux[32 + tid] = gf[tid];
             } else {
                 aux[tid] = 0.0f;
                 aux[32 + tid] = 0.0f;
             }
-        } else if (tid < 48 && tid != 36) {
+        } else if (tid < 48 && tid != 36 && tid != 37) {
             const float norm = sqrtf(fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7])));
             aux[32 + tid] = tid == 32 ? ldexpf(1.0f, -ex) : tid == 33 ? (float)ex : tid == 34 ? norm : tid == 35 ? most : 0.0f;
         }
     }
     if (BACK && tid < 64) {
-        // The largest of what multiplies this record's values, as an exponent, against its own.  Factors
-        // below 2^-112 are taken as that, so that the scale they get (up to 2^126) is a number.
+        // The largest of what multiplies this record's values, as an exponent, against its own.
         float f = tid < 32 && rows ? fabsf(gf[tid]) : 0.0f;
         f = wave_max(f < INFINITY ? f : 0.0f);
+        const int ge = f > 0.0f ? ilogbf(f) + 1 : 0;
+        // an infinite one makes its sums NaN: P has a largest value
+        if (rows && tid < 32) aux[32 + tid] = fabsf(gf[tid]) == INFINITY ? NAN : ldexpf(gf[tid], -ge);
         if (tid == 0) {
-            const int u = !rows ? -ex : f > 0.0f ? max(ilogbf(f) + 1, -112) - ex : -212;
+            const int u = !rows ? -ex : f > 0.0f ? ge - ex : -1000;
             (rows ? x.row_u : x.class_u)[t] = u;
             aux[68] = (float)u;
+            aux[69] = (float)ge;
         }
     }
 }
@@ -389,7 +391,8 @@ __device__ void build_list(const ListArgs<H>& x, int64_t g, unsigned long long* 
     const int tid = threadIdx.x, tn = x.tg.tn;
     auto put = [&](int s, int row, int c, float z, float q, float lse) {
         key[s] = c >= 0 ? ((unsigned long long)(((uint32_t)c << 5) | row) << 11) | s : ~0ull;
-        pv[s] = c >= 0 ? expf(z * x.tg.inv_tau - lse) : 0.0f;
+        const float p = expf(z * x.tg.inv_tau - lse);
+        pv[s] = c >= 0 ? (p > 1.0f ? 1.0f : p) : 0.0f;  // more only by the roundings of large logits
         qv[s] = q;
     };
     if (x.tg.target) {

@@ -28,10 +28,10 @@ constexpr int64_t kXentMaxN = 1 << 26;  // classes: a list key holds a class and
 //                                           in the order an MFMA result holds its rows
 //                                           (backward only)
 //   float[32], float[32], float[16]         per entry: class: bias log2(e) / tau; row: lse
-//                                           log2(e) and gradient factor; then 2^-e, e, the
-//                                           largest L2 norm of an entry, the largest finite
-//                                           magnitude among the first 32 values and the exponent
-//                                           bound that XentGradSide::str_u holds
+//                                           log2(e) and gradient factor times 2^-ge; then 2^-e, e,
+//                                           the largest L2 norm of an entry, the largest finite
+//                                           magnitude among the first 32 values, the exponent
+//                                           bound that XentGradSide::str_u holds, and ge
 // D = the number of 32-wide pieces of k, one of 1, 2, 3, 4, 6, 8.
 constexpr int kXentAux = 320;
 inline int xent_pieces(int64_t k) {

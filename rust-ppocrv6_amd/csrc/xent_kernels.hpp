@@ -182,13 +182,19 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
 // leaves its small difference), then P as the second product's operand without leaving the
 // registers: a result register's rows are the contraction's order, and the transposed part of
 // the record holds the entries in that order.
-//   ROWS: owners are activation rows, the stream is the classes (da).  P = p 2^(F - e).
-//   else: owners are classes, the stream is the rows (dW, db).  P = p g 2^(F - e), g the row's
+//   ROWS: owners are activation rows, the stream is the classes (da).  P = p 2^(S - e).
+//   else: owners are classes, the stream is the rows (dW, db).  P = p g 2^(S - e), g the row's
 //   gradient factor.
-// e is the stream record's exponent and F one exponent for all records, so that P's largest
-// possible value is 2^14 and products of all records add up on one scale.
+// e is the stream record's exponent and S the owner's: P's fp16 halves end at 2^-25, so an owner whose
+// P are all small (a class that is improbable in every row) needs a larger S than others.  The first
+// record's P set it, so that the largest is 2^4 to 2^5, and where a later one comes above 2^15, the
+// owner's sums so far and its S go down with it: what a P loses is 2^-29 of the owner's largest.  S is
+// never below F, where no P is above 2^14 (u is the records' bound of what multiplies p, F = 14 - max u).
+// One S for all: 846 us a step of 30720 bf16 rows, 1981 fp32; so 892 and 2039 to 2058; the largest put to
+// 2^8, more owners come above 2^15 (tiny head under 32 teacher logits 271 us, 254 so), to 2^0: 871 and 2011.
 // The target lists are read 64 entries at a time, one a lane, and an entry's place is written by the
 // lane that holds it, in the register that its row (or class) of the tile is: a wave-uniform number.
+constexpr int kLargest = 4;
 __device__ __forceinline__ void set_entry(f32x16& p, int i, bool mine, float v) {
     const float old = p[i];
     p[i] = mine ? v : old;
@@ -266,7 +272,8 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) um = max(um, __shfl_xor(um, o, 64));
-    const int F = 14 - __builtin_amdgcn_readfirstlane(um);
+    const int F = 14 - __builtin_amdgcn_readfirstlane(um), most = F + 86;  // 2^(S + u) stays a number
+    int S = F;
 
     const bool have = og < y.own_tiles;
     const uint8_t* orec = y.own + (have ? og : y.own_tiles - 1) * REC;
@@ -274,8 +281,17 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
     load_owner<D, P>(orec, own[0], lane);
     const float* oaux = reinterpret_cast<const float*>(orec + AUX);
     const float c = x.c0 * oaux[64];
-    const float own0 = oaux[lane & 31];                      // row: lse log2(e); class: bias log2(e) / tau
-    const float own1 = ROWS ? oaux[32 + (lane & 31)] : 0.0f;  // row: the gradient factor
+    float own0 = oaux[lane & 31];                      // row: lse log2(e); class: bias log2(e) / tau
+    float own1 = ROWS ? oaux[32 + (lane & 31)] : 0.0f;  // row: the gradient factor, times 2^-own_ge
+    const int own_ge = ROWS ? __builtin_amdgcn_readfirstlane((int)oaux[69]) : 0;
+    // da's lse to 2^-14, so that whole exponents add to it exactly; the rest multiplies the sums
+    float rest = 1.0f;
+    if (ROWS && fabsf(own0) < 1024.0f) {
+        const float whole = rintf(own0 * 16384.0f) * (1.0f / 16384.0f);
+        rest = exp2f(own0 - whole);
+        own1 /= rest;
+        own0 = whole;
+    }
     f32x16 acc[D] = {};
     float dbias = 0.0f;
     float minus = -1.0f;  // a number the compiler does not know: it keeps the mixed-precision fma
@@ -308,9 +324,9 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
         f32x16& p = s[0];
         const float* aux = reinterpret_cast<const float*>(cur + AUX);
         const float cc = c * aux[64];
-        const int fe = __builtin_amdgcn_readfirstlane(F - (int)aux[65]);  // exponent of this record's factor
+        const int u = __builtin_amdgcn_readfirstlane((int)aux[68]);
         if constexpr (ROWS) {
-            const float shift = own0 - (float)fe;
+            const float shift = own0 - (float)(S + u);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const f32x4 bias = *reinterpret_cast<const f32x4*>(aux + 8 * q + 4 * h);
@@ -321,16 +337,15 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
             const uint32_t end = (uint32_t)((t + 1) * 1024);  // keys below: classes of this record
             while (walk.key < end) {
                 const int cls = (int)(walk.key >> 5) & 31, row = (int)walk.key & 31;
-                const float v = ldexpf(__int_as_float(lane_value(walk.wval, walk.at & 63)), fe);
-                set_entry(p, (cls >> 3) * 4 + (cls & 3), lane == row + 32 * ((cls >> 2) & 1), v);
+                const float v = __int_as_float(lane_value(walk.wval, walk.at & 63));
+                set_entry(p, (cls >> 3) * 4 + (cls & 3), lane == row + 32 * ((cls >> 2) & 1), ldexpf(v * rest, S + u));
                 walk.step(lane);
             }
         } else {
             // The bias's sum does not weigh a row by its activations: a record whose activations are 2^60
             // smaller than others' keeps a scale of its own for it.
-            const int low = __builtin_amdgcn_readfirstlane(max(14 - F - (int)aux[68] - 60, 0));
-            const int fs = fe + low;
-            const float scale = ldexpf(1.0f, fs);
+            const int at = max(S + u, -46);
+            const float scale = ldexpf(1.0f, at);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const f32x4 lse = *reinterpret_cast<const f32x4*>(aux + 8 * q + 4 * h);
@@ -348,13 +363,13 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
                 // each lane its entry: the lane and the register it goes to, and what goes there
                 const int cls = (slice.key >> 5) & 31, row = slice.key & 31;
                 const int lane_reg = cls + 32 * ((row >> 2) & 1) + (((row >> 3) * 4 + (row & 3)) << 8);
-                const int v = __float_as_int(__int_as_float(slice.val) * aux[32 + row] * scale);
+                const int v = __float_as_int(__int_as_float(slice.val) * aux[32 + row]);
                 unsigned long long todo = __ballot((int64_t)((uint32_t)slice.key >> 10) == og && first + lane < to);
                 while (todo) {
                     const int l = __builtin_ctzll(todo);
                     todo &= todo - 1;
-                    const int at = lane_value(lane_reg, l);
-                    set_entry(p, at >> 8, lane == (at & 63), __int_as_float(lane_value(v, l)));
+                    const int place = lane_value(lane_reg, l);
+                    set_entry(p, place >> 8, lane == (place & 63), __int_as_float(lane_value(v, l)) * scale);
                 }
             }
             slice.from = after.from;
@@ -364,9 +379,28 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
             float add = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) add += p[r];
-            dbias += ldexpf(add, -fs);
-            // and nothing of it reaches the other sums
-            if (low > 0) continue;
+            dbias += ldexpf(add, (int)aux[69] - at);
+        }
+        const bool low = !ROWS && 14 - F - u > 60;  // the same for all lanes
+        float mx = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fabsf(p[r]));
+        if (t == t0 || low || __any(mx > 32768.0f)) {
+            const int off = low ? min(S + u + 46, 0) : 0;
+            mx = ldexpf(fmaxf(mx, __shfl_xor(mx, 32, 64)), off);  // the owner's other half too
+            int to = S;
+            if (t == t0 || mx > 32768.0f) to = mx > 0.0f ? min(max(S + kLargest - ilogbf(mx), F), most) : most;
+            const float by = ldexpf(1.0f, to - S), byp = ldexpf(1.0f, to - S + off);
+            S = to;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r] *= byp;
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] *= by;
+            // still above at F: logits so large that their own roundings make p more than 1
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r] = fabsf(p[r]) > 32768.0f ? copysignf(16384.0f, p[r]) : p[r];
         }
         __builtin_amdgcn_s_setprio(1);
         const f16x8* tr = reinterpret_cast<const f16x8*>(cur + P * D * 2048) + lane;
@@ -409,7 +443,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
                 f32x4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    v[e] = ldexpf(acc[d][4 * q + e], -F);
+                    v[e] = ldexpf(acc[d][4 * q + e], own_ge - S);
                     if (ROWS) v[e] = own1 == 0.0f ? 0.0f : v[e] * own1;  // no gradient, whatever the head holds
                 }
                 *reinterpret_cast<f32x4*>(out + 32 * d + 8 * q + 4 * h) = v;
