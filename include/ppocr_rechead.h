@@ -369,8 +369,9 @@ int ppocr_rn_forward_marked_dev(const ppocr_rn_t* h, const float* d_x, const flo
  * whose target is negative has no label: loss 0, no gradient, whatever the row holds (lse is
  * still its own).  The host form refuses targets of n and above; the `_dev` form treats them as no
  * label.  k is 1 to 256, m and n up to 2^24, n at least 1.  The products of fp32 tensors are
- * taken as three products of fp16 halves (22 bits of each operand, scaled per 32 rows or classes
- * by a power of two) summed in fp32, those of bf16 tensors exactly. */
+ * taken as three products of fp16 halves (22 bits of each operand, at a power of two that its
+ * row's or class's largest value sets, whatever the others hold) summed in fp32, those of bf16
+ * tensors exactly. */
 size_t ppocr_xent_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype);
 int ppocr_xent_forward(const float* a, const float* w_t, const float* bias, const int32_t* target, int64_t m, int64_t n,
                        int64_t k, float* loss, float* lse);

@@ -189,7 +189,7 @@ __device__ void build_record(const RecordArgs<H>& x, int64_t t, bool rows, float
     constexpr int LD = 32 * D + 1;
     const int tid = threadIdx.x, e = tid >> 3, l8 = tid & 7;  // 8 lanes an entry
     const int64_t first = t * 32, count = min((int64_t)32, (rows ? x.m : x.n) - first);
-    float* gf = red + 8;  // 32 gradient factors
+    float* gf = red + 12;  // 32 gradient factors
     float factor = 1.0f;
     if (BACK && rows) {
         factor = factor_of(x.tg, x.grad, first + min((int64_t)e, count - 1), l8);
@@ -214,23 +214,34 @@ __device__ void build_record(const RecordArgs<H>& x, int64_t t, bool rows, float
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const float f = value(v[i].v + u);
-            tile[e * LD + 32 * i + 4 * l8 + u] = f;
             ss = fmaf(f, f, ss);
             if (fabsf(f) < INFINITY) top = fmaxf(top, fabsf(f));
         }
 #pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
-    top = wave_max(top);
+    for (int o = 4; o >= 1; o >>= 1) {
+        ss += __shfl_xor(ss, o, 64);
+        top = fmaxf(top, __shfl_xor(top, o, 64));
+    }
+    // the largest and the smallest of the entries' largest magnitudes (entries of zeros aside)
+    const float most = wave_max(top), least = -wave_max(top > 0.0f ? -top : -INFINITY);
     const bool odd = __any(!(ss < INFINITY));
     ss = wave_max(ss);
     if ((tid & 63) == 0) {
-        red[tid >> 6] = top;
+        red[tid >> 6] = most;
         red[4 + (tid >> 6)] = odd ? INFINITY : ss;
+        red[8 + (tid >> 6)] = least;
     }
     __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float largest = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const bool shared = largest <= 16.0f * fminf(fminf(red[8], red[9]), fminf(red[10], red[11]));
     // largest magnitude to [2^14, 2^15); 2^100 at most, so that 2^-e and the factors stay in range
-    const int ex = top > 0.0f ? min(14 - ilogbf(top), 100) : 100;
+    auto exponent = [](float t) { return t > 0.0f ? min(14 - ilogbf(t), 100) : 100; };
+    const int ex = exponent(largest), own = shared ? ex : exponent(top);
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) tile[e * LD + 32 * i + 4 * l8 + u] = ldexpf(value(v[i].v + u), own);
+    __syncthreads();
     uint8_t* rec = (rows ? x.row_rec : x.class_rec) + t * (int64_t)((size_t)P * D * 2048 * (BACK ? 2 : 1) + kXentAux);
     constexpr int FORM = 2 * D * 64;  // 16-byte pieces of one plane of one form
 #pragma unroll
@@ -245,7 +256,7 @@ __device__ void build_record(const RecordArgs<H>& x, int64_t t, bool rows, float
                 // transposed: step = 2 d + e, the entries of an MFMA result's rows
                 const int en = tr ? 16 * (step & 1) + 8 * (j >> 2) + 4 * h + (j & 3) : l;
                 const int kk = tr ? 32 * (step >> 1) + l : 16 * step + 8 * h + j;
-                const float f = ldexpf(tile[en * LD + kk], ex);
+                const float f = tile[en * LD + kk];
                 hi[j] = (_Float16)f;
                 if (P == 2) lo[j] = (_Float16)(f - (float)hi[j]);
             }
@@ -254,9 +265,9 @@ __device__ void build_record(const RecordArgs<H>& x, int64_t t, bool rows, float
         }
     }
     float* aux = reinterpret_cast<float*>(rec + (size_t)P * D * 2048 * (BACK ? 2 : 1));
+    if (l8 == 0) aux[80 + e] = ldexpf(1.0f, -own);
     if (tid < 64) {
-        float most = !rows && fabsf(first_aux) < INFINITY ? fabsf(first_aux) : 0.0f;
-        most = wave_max(most);
+        const float bound = wave_max(!rows && fabsf(first_aux) < INFINITY ? fabsf(first_aux) : 0.0f);
         if (tid < 32) {
             if (!rows) {
                 aux[tid] = tid < count ? first_aux : -INFINITY;
@@ -269,9 +280,10 @@ __device__ void build_record(const RecordArgs<H>& x, int64_t t, bool rows, float
             }
         } else if (tid < 48 && tid != 36 && tid != 37) {
             const float norm = sqrtf(fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7])));
-            aux[32 + tid] = tid == 32 ? ldexpf(1.0f, -ex) : tid == 33 ? (float)ex : tid == 34 ? norm : tid == 35 ? most : 0.0f;
+            aux[32 + tid] = tid == 32 ? ldexpf(1.0f, -ex) : tid == 33 ? (float)ex : tid == 34 ? norm : tid == 35 ? bound : tid == 38 && shared ? 1.0f : 0.0f;
         }
     }
+    if (!BACK && !rows && tid == 0) x.class_u[t] = !shared;
     if (BACK && tid < 64) {
         // The largest of what multiplies this record's values, as an exponent, against its own.
         float f = tid < 32 && rows ? fabsf(gf[tid]) : 0.0f;
@@ -280,8 +292,8 @@ __device__ void build_record(const RecordArgs<H>& x, int64_t t, bool rows, float
         // an infinite one makes its sums NaN: P has a largest value
         if (rows && tid < 32) aux[32 + tid] = fabsf(gf[tid]) == INFINITY ? NAN : ldexpf(gf[tid], -ge);
         if (tid == 0) {
-            const int u = !rows ? -ex : f > 0.0f ? ge - ex : -1000;
-            (rows ? x.row_u : x.class_u)[t] = u;
+            const int u = !rows ? -ex : f > 0.0f ? ge - ex : kXentNone;
+            (rows ? x.row_u : x.class_u)[t] = 2 * u + !shared;
             aux[68] = (float)u;
             aux[69] = (float)ge;
         }
@@ -450,7 +462,7 @@ __device__ void build_list(const ListArgs<H>& x, int64_t g, unsigned long long* 
 // Records, and with one target a row (a label) the lists too.
 template <typename H, int D, int P, bool BACK>
 __global__ __launch_bounds__(kThreads) void prep_kernel(RecordArgs<H> x, ListArgs<H> y, unsigned class_tiles) {
-    __shared__ __align__(16) float lds[32 * (32 * D + 1) + 8 + 32];
+    __shared__ __align__(16) float lds[32 * (32 * D + 1) + 12 + 32];
     static_assert(sizeof(lds) >= 32 * 16, "a list of 32 entries");
     const unsigned b = blockIdx.x;
     if (b < x.row_tiles + class_tiles) {
@@ -691,7 +703,7 @@ int prep(const XentProblem& x, const XentLayout& L, uint8_t* ws, hipStream_t st)
         const Targets tg = targets_of(x);
         const RecordArgs<H> r{h, tg, x.lse, x.grad, x.m, x.n, L.row_tiles, ws + (BACK ? L.b_row_rec : L.f_row_rec),
                               ws + (BACK ? L.b_class_rec : L.f_class_rec), reinterpret_cast<int*>(ws + L.b_row_u),
-                              reinterpret_cast<int*>(ws + L.b_class_e)};
+                              reinterpret_cast<int*>(ws + (BACK ? L.b_class_e : L.f_class_u))};
         const int list = 32 * x.tn;
         int size = 32;
         while (size < list) size *= 2;
@@ -756,6 +768,7 @@ XentLayout xent_layout(int64_t m, int64_t n, int64_t k, int tn, int planes) {
     size_t f = 256;
     L.f_row_rec = put(&f, (size_t)L.row_tiles * xent_rec_bytes(L.D, planes, false));
     L.f_class_rec = put(&f, (size_t)L.class_tiles * xent_rec_bytes(L.D, planes, false));
+    L.f_class_u = put(&f, (size_t)L.class_tiles * 4);
     L.f_part = put(&f, (size_t)L.fsplit * m * sizeof(float2));
     L.f_total = f;
     size_t b = 256;
@@ -778,7 +791,7 @@ int launch_xent_forward(const XentProblem& x, float* loss, float* lse, uint8_t* 
     const Targets tg = targets_of(x);
     if (int e = x.bf16 ? prep<uint16_t, 1, false>(x, L, ws, st) : prep<float, 2, false>(x, L, ws, st)) return e;
     float2* part = reinterpret_cast<float2*>(ws + L.f_part);
-    const XentStatsArgs s{ws + L.f_row_rec, ws + L.f_class_rec, x.m, L.class_tiles, L.fsplit, L.fper, kLog2e / x.tau, part};
+    const XentStatsArgs s{ws + L.f_row_rec, ws + L.f_class_rec, reinterpret_cast<const int*>(ws + L.f_class_u), x.m, L.class_tiles, L.fsplit, L.fper, kLog2e / x.tau, part};
     const unsigned grid = (unsigned)(div_up(x.m, 128 * L.fblocks) * L.fsplit);
     if (int e = by_pieces(L.D, [&]<int D>() {
             return x.bf16 ? xent_stats_cfg<D, 1>(s, L.fblocks, grid, st) : xent_stats_cfg<D, 2>(s, L.fblocks, grid, st);

@@ -20,20 +20,25 @@ constexpr int kXentMaxTargets = 64;  // target entries of a row
 constexpr int64_t kXentMaxN = 1 << 26;  // classes: a list key holds a class and 5 bits of row
 
 // Operand images.  A tensor of `rows` entries (activation rows or classes) of k values becomes
-// one record per 32 entries: every value times 2^e, e chosen per record so that its largest
-// magnitude lies in [2^14, 2^15), as one fp16 plane (bf16 tensors: exact) or two (32-bit
-// tensors: high and low halves, 22 bits), in the order the MFMA fragments are read:
+// one record per 32 entries: every value times 2^e, e chosen so that the largest magnitude lies in
+// [2^14, 2^15), as one fp16 plane (bf16 tensors: exact down to 2^-27 of an entry's largest value) or
+// two (32-bit tensors: high and low halves, 22 bits down to 2^-12 of it, and below that to within 2^-35
+// of it), in the order the MFMA fragments are read.  The entries share e where their own largest values are within 16 of each
+// other; otherwise each has its own, so that a row of huge values, padding perhaps, takes no bits from
+// its neighbours.
 //   [plane][2 D steps of 16 k][lane][8]     entry lane % 32, k = 16 step + 8 (lane / 32) + j
 //   [plane][D][2][lane][8]                  transposed: k = 32 d + lane % 32, and the entries
 //                                           in the order an MFMA result holds its rows
 //                                           (backward only)
-//   float[32], float[32], float[16]         per entry: class: bias log2(e) / tau; row: lse
-//                                           log2(e) and gradient factor times 2^-ge; then 2^-e, e,
-//                                           the largest L2 norm of an entry, the largest finite
-//                                           magnitude among the first 32 values, the exponent
-//                                           bound that XentGradSide::str_u holds, and ge
+//   float[32], float[32], float[16], float[32]   per entry: class: bias log2(e) / tau; row: lse
+//                                           log2(e) and gradient factor times 2^-ge; then 2^-e, e (of
+//                                           the largest entry), the largest L2 norm of an entry, the
+//                                           largest finite magnitude among the first 32 values, the
+//                                           exponent bound that XentGradSide::str_u holds, ge, and
+//                                           whether the entries share e; per entry 2^-e
 // D = the number of 32-wide pieces of k, one of 1, 2, 3, 4, 6, 8.
-constexpr int kXentAux = 320;
+constexpr int kXentAux = 448;
+constexpr int kXentNone = -1000;  // the exponent bound of a record without gradients
 inline int xent_pieces(int64_t k) {
     const int d = (int)((k + 31) / 32);
     return d <= 4 ? (d < 1 ? 1 : d) : (d <= 6 ? 6 : 8);
@@ -70,7 +75,7 @@ struct XentLayout {
     int split_a, per_a;      // chunks of class records for da
     int split_w, per_w;      // chunks of row records for dW
     // forward
-    size_t f_row_rec, f_class_rec, f_part, f_total;
+    size_t f_row_rec, f_class_rec, f_class_u, f_part, f_total;
     // backward
     size_t b_row_rec, b_class_rec, b_row_e, b_row_u, b_class_e, b_keys, b_vals, b_offs, b_part_a, b_part_w, b_part_db, b_total;
     size_t total() const { return f_total > b_total ? f_total : b_total; }
@@ -85,6 +90,7 @@ int launch_xent_zero(const XentProblem& x, void* dw, float* db, hipStream_t st);
 struct XentStatsArgs {
     const uint8_t* own;  // row records (forward form)
     const uint8_t* str;  // class records
+    const int* str_u;    // as XentGradSide's; only the last bit is used
     int64_t m;
     int64_t tiles;  // class records
     int nsplit, per_split;
@@ -97,7 +103,8 @@ struct XentGradSide {
     int64_t owners;     // rows or classes
     int64_t own_tiles;  // their records
     int64_t str_tiles;
-    const int* str_u;  // per stream record: the exponent bound of what is summed over it
+    const int* str_u;  // per stream record: twice the exponent bound of what is summed over it (kXentNone:
+                       // nothing), and 1 where its entries have scales of their own
     int nsplit, per_split;
     float* part;  // [nsplit][owners][32 D]
 };

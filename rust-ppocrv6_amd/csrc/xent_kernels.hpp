@@ -68,6 +68,33 @@ __device__ __forceinline__ void scores(const uint8_t* rec, const f16x8 (&own)[NB
     }
 }
 
+// Are there records from t0 to t1 whose entries have scales of their own?  Those take another form of
+// the loops: the branch in one form for all cost steps 4 to 13% of their time.  Steps whose rows or classes all do
+// take 2% (fp32) to 10% (bf16) longer for either, 20% at k = 256 for rows.
+__device__ __forceinline__ bool any_own(const int* __restrict__ u, int64_t t0, int64_t t1, int lane) {
+    int any = 0;
+    for (int64_t i = t0 + lane; i < t1; i += 64 * 8)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) any |= u[min(i + 64 * j, t1 - 1)];
+    return __any(any & 1);
+}
+// Where a stream record's entries have scales of their own (aux: its scalars and scales), the logits of
+// this lane's owner (c: its own) take them here, and the factor that is left is 1.
+__device__ __forceinline__ bool shared_scale(const float* aux) {
+    return __builtin_amdgcn_readfirstlane(__float_as_int(aux[70])) != 0;
+}
+__device__ __forceinline__ float own_scales(const float* aux, float c, f32x16& s, int h) {
+    if (shared_scale(aux)) return c * aux[64];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const f32x4 scale = *reinterpret_cast<const f32x4*>(aux + 80 + 8 * q + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * q + e] *= c * scale[e];
+        asm volatile("" ::: "memory");  // four scales at a time: this way is rare, its registers are not
+    }
+    return 1.0f;
+}
+
 template <int D, int P>
 __device__ __forceinline__ void load_owner(const uint8_t* rec, f16x8 (&own)[P][2 * D], int lane) {
     const f16x8* s0 = reinterpret_cast<const f16x8*>(rec) + lane;
@@ -83,10 +110,9 @@ __device__ __forceinline__ void load_owner(const uint8_t* rec, f16x8 (&own)[P][2
 // bounds |t| by 100, exp2(t) is summed as it is: no maximum and no reference, a third of the vector
 // work.  Other records keep a reference that moves only when a maximum beats it by 16 (so sums stay
 // below 2^16 n and lose nothing); a row that once needed one keeps it.
-template <int D, int P, int NB>
-__global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
+template <int D, int P, int NB, bool ODD>
+__device__ __forceinline__ void statistics(const XentStatsArgs& x, uint8_t* lds) {
     constexpr int REC = P * D * 2048 + kXentAux;
-    extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned lane16 = lane * 16;
@@ -105,7 +131,7 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
         const uint8_t* rec = x.own + r * REC;
         const float* aux = reinterpret_cast<const float*>(rec + P * D * 2048);
         load_owner<D, P>(rec, own[b], lane);
-        c[b] = x.c0 * aux[64];
+        c[b] = x.c0 * aux[80 + (lane & 31)];
         norm[b] = x.c0 * aux[66];
         ref[b] = -INFINITY;
         sum[b] = 0.0f;
@@ -125,7 +151,7 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             f32x16& s = sc[b];
-            const float cc = c[b] * ce;
+            const float cc = ODD ? own_scales(aux, c[b], s, h) : c[b] * ce;
             const bool plain = !shifted[b] && __builtin_amdgcn_readfirstlane(norm[b] * cn + cb <= 100.0f);
             if (plain) {
                 if (ref[b] == -INFINITY) ref[b] = 0.0f;
@@ -174,6 +200,13 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
         if (h == 0 && row < x.m) x.part[(int64_t)split * x.m + row] = make_float2(nr, s);
     }
 }
+template <int D, int P, int NB>
+__global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int64_t t0 = (int64_t)(blockIdx.x % x.nsplit) * x.per_split, t1 = min(t0 + x.per_split, x.tiles);
+    if (any_own(x.str_u, t0, t1, threadIdx.x & 63)) statistics<D, P, NB, true>(x, lds);
+    else statistics<D, P, NB, false>(x, lds);
+}
 
 // ---------------------------------------------------------------- backward: a gradient
 // dX_o = sum_s P_os Y_s for the owners o of a workgroup (32 per wave), the stream records s of a
@@ -185,7 +218,7 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
 //   ROWS: owners are activation rows, the stream is the classes (da).  P = p 2^(S - e).
 //   else: owners are classes, the stream is the rows (dW, db).  P = p g 2^(S - e), g the row's
 //   gradient factor.
-// e is the stream record's exponent and S the owner's: P's fp16 halves end at 2^-25, so an owner whose
+// e is the stream record's (or its entry's) exponent and S the owner's: P's fp16 halves end at 2^-25, so an owner whose
 // P are all small (a class that is improbable in every row) needs a larger S than others.  The first
 // record's P set it, so that the largest is 2^4 to 2^5, and where a later one comes above 2^15, the
 // owner's sums so far and its S go down with it: what a P loses is 2^-29 of the owner's largest.  S is
@@ -195,6 +228,7 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
 // The target lists are read 64 entries at a time, one a lane, and an entry's place is written by the
 // lane that holds it, in the register that its row (or class) of the tile is: a wave-uniform number.
 constexpr int kLargest = 4;
+constexpr int kLow = 60;
 __device__ __forceinline__ void set_entry(f32x16& p, int i, bool mine, float v) {
     const float old = p[i];
     p[i] = mine ? v : old;
@@ -248,8 +282,8 @@ struct ListSlice {
     }
 };
 
-template <int D, int P, bool ROWS>
-__device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSide& y, unsigned block, uint8_t* lds) {
+template <int D, int P, bool ROWS, bool ODD>
+__device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSide& y, unsigned block, int um, uint8_t* lds) {
     constexpr int REC = 2 * P * D * 2048 + kXentAux, AUX = 2 * P * D * 2048;
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -261,18 +295,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
     const int64_t owner = og * 32 + (lane & 31);
 
     stage<REC>(y.str + t0 * REC, lds, wave, lane16);
-    // F from the largest exponent bound of the stream
-    int um = -1000;
-    for (int64_t i = lane; i < y.str_tiles; i += 64 * 16) {
-        int u[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) u[j] = y.str_u[min(i + 64 * j, y.str_tiles - 1)];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) um = max(um, u[j]);
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) um = max(um, __shfl_xor(um, o, 64));
-    const int F = 14 - __builtin_amdgcn_readfirstlane(um), most = F + 86;  // 2^(S + u) stays a number
+    const int F = 14 - um, most = F + 86;  // 2^(S + u) stays a number
     int S = F;
 
     const bool have = og < y.own_tiles;
@@ -280,7 +303,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
     f16x8 own[1][P][2 * D];
     load_owner<D, P>(orec, own[0], lane);
     const float* oaux = reinterpret_cast<const float*>(orec + AUX);
-    const float c = x.c0 * oaux[64];
+    const float c = x.c0 * oaux[80 + (lane & 31)];
     float own0 = oaux[lane & 31];                      // row: lse log2(e); class: bias log2(e) / tau
     float own1 = ROWS ? oaux[32 + (lane & 31)] : 0.0f;  // row: the gradient factor, times 2^-own_ge
     const int own_ge = ROWS ? __builtin_amdgcn_readfirstlane((int)oaux[69]) : 0;
@@ -323,7 +346,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
         __builtin_amdgcn_s_setprio(0);
         f32x16& p = s[0];
         const float* aux = reinterpret_cast<const float*>(cur + AUX);
-        const float cc = c * aux[64];
+        const float cc = ODD ? own_scales(aux, c, p, h) : c * aux[64];
         const int u = __builtin_amdgcn_readfirstlane((int)aux[68]);
         if constexpr (ROWS) {
             const float shift = own0 - (float)(S + u);
@@ -344,7 +367,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
         } else {
             // The bias's sum does not weigh a row by its activations: a record whose activations are 2^60
             // smaller than others' keeps a scale of its own for it.
-            const int at = max(S + u, -46);
+            const int at = ODD ? max(S + u, -46) : S + u;
             const float scale = ldexpf(1.0f, at);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -380,8 +403,20 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
 #pragma unroll
             for (int r = 0; r < 16; ++r) add += p[r];
             dbias += ldexpf(add, (int)aux[69] - at);
+            if (u == kXentNone) continue;  // no row of the record has a gradient
         }
-        const bool low = !ROWS && 14 - F - u > 60;  // the same for all lanes
+        if (ODD && !shared_scale(aux)) {
+            // entries with scales of their own: what those are below the record's
+            const int e0 = __builtin_amdgcn_readfirstlane((int)aux[65]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 scale = *reinterpret_cast<const f32x4*>(aux + 80 + 8 * q + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[4 * q + e] *= ldexpf(scale[e], e0);
+                asm volatile("" ::: "memory");
+            }
+        }
+        const bool low = ODD && !ROWS && um - u > kLow;  // the same for all lanes
         float mx = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fabsf(p[r]));
@@ -453,6 +488,33 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
         dbias += __shfl_xor(dbias, 32, 64);
         if (h == 0 && owner < y.owners) x.part_db[(int64_t)split * y.owners + owner] = dbias;
     }
+}
+
+template <int D, int P, bool ROWS>
+__device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSide& y, unsigned block, uint8_t* lds) {
+    // the largest and the smallest exponent bound of the stream, and whether entries have scales of their own
+    int most = kXentNone, least = -kXentNone, own = 0;
+    for (int64_t i = threadIdx.x & 63; i < y.str_tiles; i += 64 * 16) {
+        int v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = y.str_u[min(i + 64 * j, y.str_tiles - 1)];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int u = v[j] >> 1;
+            most = max(most, u);
+            if (u != kXentNone) least = min(least, u);
+            own |= v[j] & 1;
+        }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        most = max(most, __shfl_xor(most, o, 64));
+        least = min(least, __shfl_xor(least, o, 64));
+    }
+    const int um = __builtin_amdgcn_readfirstlane(most);
+    const bool odd = __any(own) || (!ROWS && um - __builtin_amdgcn_readfirstlane(least) > kLow);
+    if (odd) gradient<D, P, ROWS, true>(x, y, block, um, lds);
+    else gradient<D, P, ROWS, false>(x, y, block, um, lds);
 }
 
 // Both gradients in one launch, so that the last workgroups of one fill up with the other's (and a
