@@ -60,8 +60,10 @@ struct Raw {
     Chunk c[R];
 };
 
+// The rows may be the output's own (y over x, dx over dy or x), each written after it was read: no
+// pointer to them is __restrict__.
 template <typename T, int G, int R, bool VEC>
-__device__ __forceinline__ void load_raw(const T* __restrict__ p, int d, int l, Raw<T, R>& x) {
+__device__ __forceinline__ void load_raw(const T* p, int d, int l, Raw<T, R>& x) {
     constexpr int V = kV<T>;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -84,7 +86,7 @@ __device__ __forceinline__ void widen(const Raw<T, R>& x, float (&f)[E]) {
     for (int i = 0; i < E; ++i) f[i] = up<T>(x.c[i / kV<T>].v[i % kV<T>]);
 }
 template <typename T, int G, int R, bool VEC, int E>
-__device__ __forceinline__ void store_row(T* __restrict__ p, int d, int l, const float (&x)[E]) {
+__device__ __forceinline__ void store_row(T* p, int d, int l, const float (&x)[E]) {
     constexpr int V = kV<T>;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -164,9 +166,9 @@ constexpr int parts_of(int G) { return G == 1024 ? 256 : G == 16 || G == 512 ? 5
 constexpr int threads_of(int G) { return G > 256 ? G : 256; }
 
 template <typename T, int G, int R, bool VEC>
-__global__ __launch_bounds__(threads_of(G)) void forward_kernel(const T* __restrict__ x, const float* __restrict__ w,
+__global__ __launch_bounds__(threads_of(G)) void forward_kernel(const T* x, const float* __restrict__ w,
                                                                 const float* __restrict__ b, int64_t m, int d, float eps,
-                                                                T* __restrict__ y, float* __restrict__ mean,
+                                                                T* y, float* __restrict__ mean,
                                                                 float* __restrict__ rstd) {
     constexpr int TEAMS = threads_of(G) / G, V = kV<T>, E = V * R;
     constexpr bool AHEAD = G < 1024;  // its registers would not hold the next row beside this one
@@ -213,11 +215,11 @@ __global__ __launch_bounds__(threads_of(G)) void forward_kernel(const T* __restr
 
 // A single workgroup (final: its sums are dw and db themselves) has no second kernel to wait for.
 template <typename T, int G, int R, bool VEC, int NT>
-__global__ __launch_bounds__(NT) void backward_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+__global__ __launch_bounds__(NT) void backward_kernel(const T* dy, const T* x,
                                                                  const float* __restrict__ w,
                                                                  const float* __restrict__ mean,
                                                                  const float* __restrict__ rstd, int64_t m, int d,
-                                                                 T* __restrict__ dx, float* __restrict__ part, float* final_dw,
+                                                                 T* dx, float* __restrict__ part, float* final_dw,
                                                                  float* final_db) {
     constexpr int TEAMS = NT / G, V = kV<T>, E = V * R;
     constexpr bool AHEAD = G < 1024;  // its registers would not hold the next row beside this one
