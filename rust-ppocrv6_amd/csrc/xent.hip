@@ -646,10 +646,12 @@ void pick_grads(XentLayout* L, int64_t m, int64_t n, int planes) {
     const int64_t ba = div_up(m, kXentGradOwners), bw = div_up(n, kXentGradOwners);
     const double chunk_cost = 256.0 / 5e6 / (planes == 2 ? 0.36 : 0.16);
     double best = -1.0;
+    // records of a chunk of a stream in `chunks`: da's walk the target lists from whole blocks of classes
+    auto whole = [](int64_t tiles, int64_t chunks) { return div_up(div_up(tiles, chunks), kBlockTiles) * kBlockTiles; };
     for (int s = 1; s <= kMostChunks; ++s) {
         // s chunks of the shorter side's stream; the other's of the same length
         const bool by_a = L->class_tiles <= L->row_tiles;
-        const int64_t per = div_up(div_up(by_a ? L->class_tiles : L->row_tiles, s), kBlockTiles) * kBlockTiles;
+        const int64_t per = whole(by_a ? L->class_tiles : L->row_tiles, s);
         const int64_t sa = div_up(L->class_tiles, per), sw = div_up(L->row_tiles, per);
         if (sa > kMostChunks || sw > kMostChunks || (s > 1 && ba * sa + bw * sw > kMostGroups)) break;
         const double cost = (double)div_up(ba * sa + bw * sw, places) * (double)(per + 2) +
@@ -661,9 +663,12 @@ void pick_grads(XentLayout* L, int64_t m, int64_t n, int planes) {
             L->per_a = L->per_w = (int)per;
         }
     }
-    if (best < 0) {  // streams of very different lengths: whole, or in the most chunks
-        L->per_a = (int)(div_up(div_up(L->class_tiles, kMostChunks), kBlockTiles) * kBlockTiles);
-        L->per_w = (int)div_up(L->row_tiles, kMostChunks);
+    if (best < 0) {
+        // Streams of very different lengths: each in the most chunks, but no more than keep the GPU busy
+        // (each has sums of its own: 63 of them for 2000 rows under 600000 classes would be 19 GB).
+        auto chunks = [&](int64_t blocks) { return std::clamp<int64_t>(8 * places / blocks, 1, kMostChunks); };
+        L->per_a = (int)whole(L->class_tiles, chunks(ba));
+        L->per_w = (int)div_up(L->row_tiles, chunks(bw));
         L->split_a = (int)div_up(L->class_tiles, L->per_a);
         L->split_w = (int)div_up(L->row_tiles, L->per_w);
     }
