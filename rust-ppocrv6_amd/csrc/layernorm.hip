@@ -349,8 +349,21 @@ int backward(const T* dy, const T* x, const float* w, const float* mean, const f
 // the second kernel 3.6 + 2.5 and a launch more).
 constexpr int kFewRows = 256;
 
-// Lanes of a row's team by its width.
-int team_of(int64_t d) { return d <= 128 ? 16 : d <= 1024 ? 64 : d <= 4096 ? 256 : d <= 8192 ? 512 : 1024; }
+// f.template operator()<G, C>(): the lanes of a row's team and the chunks of 8 values that each holds, by
+// the row's width.
+template <typename F>
+auto by_width(int64_t d, F&& f) {
+    if (d <= 128) return f.template operator()<16, 1>();
+    if (d <= 512) return f.template operator()<64, 1>();
+    if (d <= 1024) return f.template operator()<64, 2>();
+    if (d <= 2048) return f.template operator()<256, 1>();
+    if (d <= 4096) return f.template operator()<256, 2>();
+    if (d <= 8192) return f.template operator()<512, 2>();
+    return f.template operator()<1024, 2>();
+}
+int team_of(int64_t d) {
+    return by_width(d, []<int G, int C>() { return G; });
+}
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -358,13 +371,7 @@ template <typename T>
 int forward_of(const T* x, const float* w, const float* b, int64_t m, int d, float eps, T* y, float* mean, float* rstd,
                hipStream_t st) {
     const bool vec = d % kV<T> == 0 && aligned(x) && aligned(y) && aligned(w) && aligned(b);
-    if (d <= 128) return forward<T, 16, (sizeof(T) == 4 ? 2 : 1)>(x, w, b, m, d, eps, vec, y, mean, rstd, st);
-    if (d <= 512) return forward<T, 64, (sizeof(T) == 4 ? 2 : 1)>(x, w, b, m, d, eps, vec, y, mean, rstd, st);
-    if (d <= 1024) return forward<T, 64, (sizeof(T) == 4 ? 4 : 2)>(x, w, b, m, d, eps, vec, y, mean, rstd, st);
-    if (d <= 2048) return forward<T, 256, (sizeof(T) == 4 ? 2 : 1)>(x, w, b, m, d, eps, vec, y, mean, rstd, st);
-    if (d <= 4096) return forward<T, 256, (sizeof(T) == 4 ? 4 : 2)>(x, w, b, m, d, eps, vec, y, mean, rstd, st);
-    if (d <= 8192) return forward<T, 512, (sizeof(T) == 4 ? 4 : 2)>(x, w, b, m, d, eps, vec, y, mean, rstd, st);
-    return forward<T, 1024, (sizeof(T) == 4 ? 4 : 2)>(x, w, b, m, d, eps, vec, y, mean, rstd, st);
+    return by_width(d, [&]<int G, int C>() { return forward<T, G, C * 8 / kV<T>>(x, w, b, m, d, eps, vec, y, mean, rstd, st); });
 }
 template <typename T>
 int backward_of(const T* dy, const T* x, const float* w, const float* mean, const float* rstd, int64_t m, int d, T* dx,
@@ -372,13 +379,9 @@ int backward_of(const T* dy, const T* x, const float* w, const float* mean, cons
     const bool vec = d % kV<T> == 0 && aligned(x) && aligned(dy) && aligned(dx) && aligned(w);
     if (d <= 128 && m <= kFewRows)
         return backward<T, 16, (sizeof(T) == 4 ? 2 : 1), 1024>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
-    if (d <= 128) return backward<T, 16, (sizeof(T) == 4 ? 2 : 1)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
-    if (d <= 512) return backward<T, 64, (sizeof(T) == 4 ? 2 : 1)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
-    if (d <= 1024) return backward<T, 64, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
-    if (d <= 2048) return backward<T, 256, (sizeof(T) == 4 ? 2 : 1)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
-    if (d <= 4096) return backward<T, 256, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
-    if (d <= 8192) return backward<T, 512, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
-    return backward<T, 1024, (sizeof(T) == 4 ? 4 : 2)>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
+    return by_width(d, [&]<int G, int C>() {
+        return backward<T, G, C * 8 / kV<T>>(dy, x, w, mean, rstd, m, d, vec, dx, part, parts, dw, db, st);
+    });
 }
 
 }  // namespace
