@@ -1668,7 +1668,6 @@ constexpr const char* kXentOp = "SoftmaxCrossEntropy";
 constexpr const char* kDistillOp = "Distill";
 constexpr const char* kNormOp = "LayerNorm";
 constexpr const char* kTopkOp = "TopK";
-constexpr int64_t kLossMost = 1 << 24;  // rows and classes of a loss
 
 int bad_arg(const char* op, const std::string& msg) { return fail(PPOCR_ERR_INVALID_ARG, std::string(op) + ": " + msg); }
 
@@ -1681,8 +1680,8 @@ int check_loss_shape(const char* op, int64_t m, int64_t n, int64_t k, int dtype)
     if (m < 0 || n < 0 || k < 0) return bad_arg(op, "negative shape");
     if (n == 0 || k == 0) return bad_arg(op, "weight must have positive shape");
     if (k > kXentMaxK) return bad_arg(op, "inner dimension " + std::to_string(k) + " above " + std::to_string(kXentMaxK));
-    if (m > kLossMost) return bad_arg(op, "too many rows");
-    if (n > kLossMost) return bad_arg(op, "too many classes");
+    if (m > kXentMost) return bad_arg(op, "too many rows");
+    if (n > kXentMost) return bad_arg(op, "too many classes");
     return check_dtype(dtype, op);
 }
 

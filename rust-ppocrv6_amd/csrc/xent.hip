@@ -708,7 +708,7 @@ int prep(const XentProblem& x, const XentLayout& L, uint8_t* ws, hipStream_t st)
         const Targets tg = targets_of(x);
         const RecordArgs<H> r{h, tg, x.lse, x.grad, x.m, x.n, L.row_tiles, ws + (BACK ? L.b_row_rec : L.f_row_rec),
                               ws + (BACK ? L.b_class_rec : L.f_class_rec), reinterpret_cast<int*>(ws + L.b_row_u),
-                              reinterpret_cast<int*>(ws + (BACK ? L.b_class_e : L.f_class_u))};
+                              reinterpret_cast<int*>(ws + (BACK ? L.b_class_u : L.f_class_u))};
         const int list = 32 * x.tn;
         int size = 32;
         while (size < list) size *= 2;
@@ -759,7 +759,6 @@ int sums(const XentLayout& L, const float* pa, const float* pw, const float* pdb
 XentLayout xent_layout(int64_t m, int64_t n, int64_t k, int tn, int planes) {
     XentLayout L{};
     L.D = xent_pieces(k);
-    L.planes = planes;
     L.row_tiles = xent_tiles(m);
     L.class_tiles = xent_tiles(n);
     pick_stats(&L, m, planes);
@@ -780,7 +779,7 @@ XentLayout xent_layout(int64_t m, int64_t n, int64_t k, int tn, int planes) {
     L.b_row_rec = put(&b, (size_t)L.row_tiles * xent_rec_bytes(L.D, planes, true));
     L.b_class_rec = put(&b, (size_t)L.class_tiles * xent_rec_bytes(L.D, planes, true));
     L.b_row_u = put(&b, (size_t)L.row_tiles * 4);
-    L.b_class_e = put(&b, (size_t)L.class_tiles * 4);
+    L.b_class_u = put(&b, (size_t)L.class_tiles * 4);
     L.b_keys = put(&b, (size_t)L.row_tiles * 32 * tn * 4);
     L.b_vals = put(&b, (size_t)L.row_tiles * 32 * tn * 4);
     L.b_offs = put(&b, (size_t)L.row_tiles * (div_up(n, 128) + 1) * 2);
@@ -823,7 +822,7 @@ int launch_xent_backward(const XentProblem& x, void* da, void* dw, float* db, ui
     const uint8_t* cr = ws + L.b_class_rec;
     const unsigned ga = da ? (unsigned)(div_up(x.m, kXentGradOwners) * L.split_a) : 0;
     const unsigned gw = dw || db ? (unsigned)(div_up(x.n, kXentGradOwners) * L.split_w) : 0;
-    const XentGradArgs s{{rr, cr, x.m, L.row_tiles, L.class_tiles, reinterpret_cast<const int*>(ws + L.b_class_e), L.split_a,
+    const XentGradArgs s{{rr, cr, x.m, L.row_tiles, L.class_tiles, reinterpret_cast<const int*>(ws + L.b_class_u), L.split_a,
                           L.per_a, pa},
                          {cr, rr, x.n, L.class_tiles, L.row_tiles, reinterpret_cast<const int*>(ws + L.b_row_u), L.split_w,
                           L.per_w, pw},

@@ -17,7 +17,7 @@ namespace ppocr {
 
 constexpr int kXentMaxK = 256;       // inner dimension
 constexpr int kXentMaxTargets = 64;  // target entries of a row
-constexpr int64_t kXentMaxN = 1 << 26;  // classes: a list key holds a class and 5 bits of row
+constexpr int64_t kXentMost = 1 << 24;  // rows and classes (a list key holds a class and 5 bits of row in 32)
 
 // Operand images.  A tensor of `rows` entries (activation rows or classes) of k values becomes
 // one record per 32 entries: every value times 2^e, e chosen so that the largest magnitude lies in
@@ -68,7 +68,7 @@ struct XentProblem {
 
 // Sizes and offsets of a call's workspace.
 struct XentLayout {
-    int D, planes;
+    int D;
     int64_t row_tiles, class_tiles;
     int fblocks;             // blocks of 32 rows of a wave of the statistics pass
     int fsplit, fper;        // its chunks of class records, records of a chunk
@@ -77,7 +77,7 @@ struct XentLayout {
     // forward
     size_t f_row_rec, f_class_rec, f_class_u, f_part, f_total;
     // backward
-    size_t b_row_rec, b_class_rec, b_row_e, b_row_u, b_class_e, b_keys, b_vals, b_offs, b_part_a, b_part_w, b_part_db, b_total;
+    size_t b_row_rec, b_class_rec, b_row_u, b_class_u, b_keys, b_vals, b_offs, b_part_a, b_part_w, b_part_db, b_total;
     size_t total() const { return f_total > b_total ? f_total : b_total; }
 };
 XentLayout xent_layout(int64_t m, int64_t n, int64_t k, int tn, int planes);
