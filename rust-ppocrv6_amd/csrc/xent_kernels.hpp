@@ -434,8 +434,9 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[d][r] *= by;
             // still above at F: logits so large that their own roundings make p more than 1
+            if (__any(mx * by > 32768.0f))
 #pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] = fabsf(p[r]) > 32768.0f ? copysignf(16384.0f, p[r]) : p[r];
+                for (int r = 0; r < 16; ++r) p[r] = fabsf(p[r]) > 32768.0f ? copysignf(16384.0f, p[r]) : p[r];
         }
         __builtin_amdgcn_s_setprio(1);
         const f16x8* tr = reinterpret_cast<const f16x8*>(cur + P * D * 2048) + lane;
