@@ -371,7 +371,10 @@ int ppocr_rn_forward_marked_dev(const ppocr_rn_t* h, const float* d_x, const flo
  * label.  k is 1 to 256, m and n up to 2^24, n at least 1.  The products of fp32 tensors are
  * taken as three products of fp16 halves (22 bits of each operand, at a power of two that its
  * row's or class's largest value sets, whatever the others hold) summed in fp32, those of bf16
- * tensors exactly. */
+ * tensors exactly.  The gradients' products take exp(z - lse) - (j == target) from 32 bits to 22
+ * (fp32 tensors) or 11 (bf16 ones), at a power of two that the largest contributions to the same
+ * row of da or dw_t set, and are summed in fp32; dbias is summed from 32 bits.  exp(z - lse) is as
+ * exact as 32-bit logits of z's size let it be. */
 size_t ppocr_xent_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype);
 int ppocr_xent_forward(const float* a, const float* w_t, const float* bias, const int32_t* target, int64_t m, int64_t n,
                        int64_t k, float* loss, float* lse);
