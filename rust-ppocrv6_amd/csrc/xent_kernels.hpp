@@ -3,11 +3,11 @@
 //
 // Why tiles of 32 x 32 and owners in registers: an MFMA result of the logits then is, lane by lane, a
 // column of P, the operand of the second product, and a workgroup needs LDS only for the stream.
-// 30720 rows, 18710 classes, k = 120: statistics 363 us (fp32, 1220 TFLOP/s of fp16 products) and 176
-// (bf16, 840), both gradients 1700 (1040) and 742 (795).  The matrix pipe is busy 56% of the cycles in
-// the fp32 gradients and 43% in the bf16 ones, at 1.76 and 1.89 GHz.  fp32: 5% less time without the LDS
-// reads, none less for a fifth fewer vector instructions, so probably power (not measured).  bf16, an
-// earlier version: 9-10% less without the exponentials, 12-15% without the staging loads.
+// 30720 rows, 18710 classes, k = 120: statistics 354 us (fp32, 1250 TFLOP/s of fp16 products) and 173
+// (bf16, 850), both gradients 1672 (1055) and 750 (785).  The matrix pipe is busy 54% of the cycles in
+// the fp32 gradients and 39% in the bf16 ones, at 1.81 and 1.95 GHz.  Earlier versions: fp32 5% less time
+// without the LDS reads, none less for a fifth fewer vector instructions, which fits a limit by power
+// (not measured); bf16 9-10% less without the exponentials, 12-15% without the staging loads.
 #pragma once
 #include "xent.hpp"
 
@@ -223,6 +223,9 @@ __global__ __launch_bounds__(kThreads, 2) void stats_kernel(XentStatsArgs x) {
 // record's P set it, so that the largest is 2^4 to 2^5, and where a later one comes above 2^15, the
 // owner's sums so far and its S go down with it: what a P loses is 2^-29 of the owner's largest.  S is
 // never below F, where no P is above 2^14 (u is the records' bound of what multiplies p, F = 14 - max u).
+// With bf16 tensors P is one half, 11 bits (a bf16 product of its own would keep 8): da and dW are off
+// by 1.7e-3 of their norm as with P in 24 bits, that being the rounding of the bf16 outputs, while a second
+// half would be half as many matrix instructions again.
 // One S for all: 846 us a step of 30720 bf16 rows, 1981 fp32; so 892 and 2039 to 2058; the largest put to
 // 2^8, more owners come above 2^15 (tiny head under 32 teacher logits 271 us, 254 so), to 2^0: 871 and 2011.
 // The target lists are read 64 entries at a time, one a lane, and an entry's place is written by the
