@@ -300,6 +300,7 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
     stage<REC>(y.str + t0 * REC, lds, wave, lane16);
     const int F = 14 - um, most = F + 86;  // 2^(S + u) stays a number
     int S = F;
+    bool fresh = true;  // no record has set S
 
     const bool have = og < y.own_tiles;
     const uint8_t* orec = y.own + (have ? og : y.own_tiles - 1) * REC;
@@ -423,13 +424,14 @@ __device__ __forceinline__ void gradient(const XentGradArgs& x, const XentGradSi
         float mx = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fabsf(p[r]));
-        if (t == t0 || low || __any(mx > 32768.0f)) {
+        if (fresh || low || __any(mx > 32768.0f)) {
             const int off = low ? min(S + u + 46, 0) : 0;
             mx = ldexpf(fmaxf(mx, __shfl_xor(mx, 32, 64)), off);  // the owner's other half too
             int to = S;
-            if (t == t0 || mx > 32768.0f) to = mx > 0.0f ? min(max(S + kLargest - ilogbf(mx), F), most) : most;
+            if (fresh || mx > 32768.0f) to = mx > 0.0f ? min(max(S + kLargest - ilogbf(mx), F), most) : most;
             const float by = ldexpf(1.0f, to - S), byp = ldexpf(1.0f, to - S + off);
             S = to;
+            fresh = false;
 #pragma unroll
             for (int r = 0; r < 16; ++r) p[r] *= byp;
 #pragma unroll

@@ -119,3 +119,24 @@ def test_logits_beyond_what_32_bits_tell_apart(rh, dt):
     tol = tc.loss_tol(av, wv, b, z, p, dz, s, al, ref, dt, 1.0, q, logq)
     for key in ("loss", "lse", "da"):
         tc.close(got[key][rows], ref[key][rows], tol[key][rows], key)
+
+
+@pytest.mark.parametrize("kind", ["xent", "distill"])
+@DT
+def test_improbable_classes_behind_rows_without_target(rh, dt, kind):
+    """Every other group of 32 rows, the first among them, has no target: the groups that set the scales
+    are the others."""
+    rng = np.random.default_rng(46)
+    m, n, k = 700, 200, 64
+    a, w, b, to = tc.head_inputs(rng, m, n, k)
+    rare = np.arange(n) % 3 == 1
+    b[rare] -= (20 + 20 * rng.random(int(rare.sum()))).astype(np.float32)
+    to = np.where(rare[to], to - 1, to).astype(np.int32)
+    t = targets(kind, rng, m, n, to)
+    if kind == "distill":
+        t["idx"] = np.where(rare[t["idx"]], t["idx"] - 1, t["idx"]).astype(np.int32)
+    none = (np.arange(m) // 32) % 2 == 0
+    t["target" if kind == "xent" else "idx"][none] = -1
+    tau = np.float32(t.get("tau", 1.0))
+    got, _ = compare(rh, a, w * tau, b * tau, dt, t, None, np.arange(m), np.arange(n), f"{kind} rare classes, groups of padding")
+    assert (got["da"][none] == 0).all()
