@@ -99,3 +99,18 @@ def test_a_row_and_its_neighbours_do_not_meet(rh, dt):
         rows = np.arange(0, m, 2)
         for key in ("loss", "lse"):
             tc.close(got[key][rows], want[key][rows], 2 * tol[key][rows], f"{key} next to {size}")
+
+
+@pytest.mark.parametrize("kind", ["xent", "distill"])
+@pytest.mark.parametrize("m,n,k", [(300, 700, 40), (257, 300, 120), (150, 400, 180), (140, 130, 256), (1000, 2100, 64)])
+@DT
+def test_unlike_rows_and_classes(rh, dt, m, n, k, kind):
+    """Rows and classes of ordinary sizes and of a 64th and 64 times those in every group of both."""
+    rng = np.random.default_rng(m + k)
+    a, w, b, to = tc.head_inputs(rng, m, n, k)
+    a *= rng.choice([1 / 64, 1, 1, 1, 8], (m, 1)).astype(np.float32)
+    a[::17] *= np.float32(8)
+    w *= rng.choice([1 / 64, 1, 1, 4], (n, 1)).astype(np.float32)
+    t = targets(kind, rng, m, n, to)
+    grad = (rng.standard_normal(m) * 2.0 ** rng.integers(-12, 1, m)).astype(np.float32)
+    compare(rh, a, w, b, dt, t, grad, np.arange(m), np.arange(n), f"{kind} unlike")
