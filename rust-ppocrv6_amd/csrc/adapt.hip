@@ -1,0 +1,738 @@
+// Low-rank adapters of many text lines beside the shared vocabulary projection:
+//
+//   z[r][j] = scale[j] (sum_c a[r][c] q[j][c]) + bias[j] + s (down a[r])[.] . up[j][.]
+//
+// with the adapter (down [rank][k], up [n][rank], s) of the slot that row r's line names, or none.  The head's
+// weights are read once for rows of all adapters; only the rank products differ.
+//
+// Matrix bound at the head's own rate: 2 n k operations a row, of which an adapter of rank 16 adds 13%.
+// Rows are put in order by slot (plan_kernel) and padded to units of 32, so that a wave's rows have one
+// adapter; the four waves of a workgroup, each with a unit of its own, share the head's weight tiles through
+// LDS, and each wave reads its adapter's tile from L2.
+//
+// Arithmetic: fp16 halves of both operands (22 bits), as the head's F16X2 mode, all in one fp32
+// accumulator: up is held divided by the class's scale.  Each row is scaled by the power of two that its
+// largest value sets, so rows of any size keep their bits, whatever the rows beside them hold, and no row
+// has to be computed again.  u = down a is computed by each wave before its first tile, from the rows it
+// holds; the products' layout is that of the operand that the next product needs.
+#include <algorithm>
+
+#include "adapt.hpp"
+#include "head_mfma.hpp"
+
+namespace ppocr {
+
+size_t Adapters::down_bytes() const { return (size_t)((steps + 1) / 2) * (2 * (size_t)G * 512 + 1024); }
+size_t Adapters::up_bytes() const { return (size_t)tiles * 2 * steps * 1024; }
+
+namespace {
+
+constexpr int kUnit = 32;     // rows of a wave
+constexpr int kWaves = 4;
+constexpr int kDownShift = 10;  // down's halves are held 2^10 up: their low ones stay normal numbers
+constexpr int kTop = 15;        // rows, and u, stay below 2^15
+constexpr int kMostShift = 60;
+
+// ---------------------------------------------------------------- setting a slot
+__global__ __launch_bounds__(256) void clear_kernel(u32x4* p, int64_t count) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) p[i] = u32x4{0, 0, 0, 0};
+}
+__global__ void clear_meta_kernel(AdapterMeta* meta, int count) {
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < count; i += gridDim.x * blockDim.x) meta[i] = AdapterMeta{1.0f, kTop};
+}
+
+template <typename T>
+__device__ __forceinline__ float value(T v);
+template <>
+__device__ __forceinline__ float value<float>(float v) {
+    return v;
+}
+template <>
+__device__ __forceinline__ float value<uint16_t>(uint16_t v) {
+    return __uint_as_float((unsigned)v << 16);
+}
+
+// range[0][t]: the sum of |down[t]|; range[1][t]: cleared.
+template <typename T>
+__global__ __launch_bounds__(64) void down_range_kernel(const T* __restrict__ down, int rank, int k, unsigned* range) {
+    const int t = blockIdx.x;
+    float s = 0.0f;
+    if (t < rank)
+        for (int c = threadIdx.x; c < k; c += 64) s += __builtin_fabsf(value<T>(down[(int64_t)t * k + c]));
+    s = wave_sum(s);
+    if (threadIdx.x == 0) {
+        range[t] = __float_as_uint(s);
+        range[kAdaptMostRank + t] = 0u;
+    }
+}
+
+// The value that the up records hold before their power of two.
+__device__ __forceinline__ float up_value(float v, float scale, float class_scale) { return v * scale / class_scale; }
+
+// range[1][t]: the largest |up[.][t]| over its class's scale (maxima of non-negative bits: any order gives the
+// same).
+template <typename T>
+__global__ __launch_bounds__(256) void up_range_kernel(const T* __restrict__ up, int rank, float scale,
+                                                       const float* __restrict__ class_scale, int64_t n, unsigned* range) {
+    __shared__ unsigned top[kAdaptMostRank];
+    if (threadIdx.x < kAdaptMostRank) top[threadIdx.x] = 0u;
+    __syncthreads();
+    const int64_t count = n * rank;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < count; x += (int64_t)gridDim.x * 256) {
+        const int64_t j = x / rank;
+        const float v = __builtin_fabsf(up_value(value<T>(up[x]), scale, class_scale[j]));
+        if (v < INFINITY) atomicMax(&top[x - j * rank], __float_as_uint(v));
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < rank) atomicMax(&range[kAdaptMostRank + threadIdx.x], top[threadIdx.x]);
+}
+
+// Power of two above |down[t]|'s sum (1 where it is 0 or no finite number).
+__device__ __forceinline__ int down_exp(const unsigned* range, int t) {
+    const float s = __uint_as_float(range[t]);
+    return s > 0.0f && s < INFINITY ? ilogbf(s) + 1 : 0;
+}
+// How far the rows of this slot are scaled down so that the largest up value fits fp16.
+__device__ __forceinline__ int slot_shift(const unsigned* range, int rank) {
+    int s = 0;
+    for (int t = 0; t < rank; ++t) {
+        const float b = __uint_as_float(range[kAdaptMostRank + t]);
+        if (b > 0.0f) s = max(s, ilogbf(b) + 1 + down_exp(range, t) - (kTop - 1));
+    }
+    return min(s, kMostShift);
+}
+
+__device__ __forceinline__ unsigned short half_bits(float v) { return __builtin_bit_cast(unsigned short, (_Float16)v); }
+
+// down record: per 32 ranks, as an FP32 head's tile (Geo<CFG_HF3, G>): [half][group][rank][8].
+template <typename T>
+__global__ __launch_bounds__(256) void down_record_kernel(const T* __restrict__ down, int rank, int k, int G, int steps,
+                                                          const unsigned* __restrict__ range, uint8_t* rec, AdapterMeta* meta) {
+    const int blocks = (steps + 1) / 2;
+    const size_t stride = 2 * (size_t)G * 512 + 1024;
+    for (int x = blockIdx.x * 256 + threadIdx.x; x < blocks * 32 * G * 8; x += gridDim.x * 256) {
+        const int e = x % 8, i = x / 8 % 32, g = x / 256 % G, b = x / (256 * G);
+        const int t = 32 * b + i, c = 8 * g + e;
+        const float v = t < rank && c < k ? ldexpf(value<T>(down[(int64_t)t * k + c]), kDownShift - down_exp(range, t)) : 0.0f;
+        unsigned short* p = reinterpret_cast<unsigned short*>(rec + b * stride);
+        const unsigned short hi = half_bits(v);
+        p[(g * 32 + i) * 8 + e] = hi;
+        p[((G + g) * 32 + i) * 8 + e] = half_bits(v - (float)__builtin_bit_cast(_Float16, hi));
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        const int s = slot_shift(range, rank);
+        *meta = AdapterMeta{ldexpf(1.0f, s - kDownShift), kTop - s};
+    }
+}
+
+// The rank that element e of lane half h holds in 16-rank step s of an operand: the order in which
+// u = down a leaves the matrix unit (register r of a lane is row 8 (r / 4) + 4 h + r % 4).
+__device__ __forceinline__ int rank_of(int s, int h, int e) { return 32 * (s >> 1) + 8 * (2 * (s & 1) + (e >> 2)) + 4 * h + (e & 3); }
+
+// up record of a 32-class tile: [half][step][h][class][8].
+template <typename T>
+__global__ __launch_bounds__(256) void up_record_kernel(const T* __restrict__ up, int rank, float scale,
+                                                        const float* __restrict__ class_scale, int64_t n, int steps,
+                                                        const unsigned* __restrict__ range, uint8_t* rec) {
+    __shared__ int exps[kAdaptMostRank];
+    if (threadIdx.x < kAdaptMostRank) exps[threadIdx.x] = (int)threadIdx.x < rank ? down_exp(range, threadIdx.x) : 0;
+    __shared__ int shift;
+    if (threadIdx.x == 0) shift = slot_shift(range, rank);
+    __syncthreads();
+    const int per = steps * 512;  // values of a tile
+    unsigned short* p = reinterpret_cast<unsigned short*>(rec) + (size_t)blockIdx.x * 2 * per;
+    for (int x = threadIdx.x; x < per; x += 256) {
+        const int e = x % 8, i = x / 8 % 32, h = x / 256 % 2, s = x / 512;
+        const int t = rank_of(s, h, e);
+        const int64_t j = (int64_t)blockIdx.x * 32 + i;
+        float v = 0.0f;
+        if (t < rank && j < n) v = ldexpf(up_value(value<T>(up[j * rank + t]), scale, class_scale[j]), exps[t] - shift);
+        const unsigned short hi = half_bits(v);
+        p[x] = hi;
+        p[per + x] = half_bits(v - (float)__builtin_bit_cast(_Float16, hi));
+    }
+}
+
+template <typename T>
+int set_slot(const Adapters& ad, int slot, const T* down, const T* up, int rank, float scale, const float* class_scale, int64_t n,
+             int64_t k, hipStream_t st) {
+    unsigned* range = ad.range + (size_t)slot * 2 * kAdaptMostRank;
+    down_range_kernel<T><<<kAdaptMostRank, 64, 0, st>>>(down, rank, (int)k, range);
+    PPOCR_HIP(hipGetLastError());
+    if (rank) {
+        const unsigned grid = (unsigned)std::min<int64_t>((n * rank + 1023) / 1024, 1024);
+        up_range_kernel<T><<<grid, 256, 0, st>>>(up, rank, scale, class_scale, n, range);
+        PPOCR_HIP(hipGetLastError());
+    }
+    down_record_kernel<T><<<16, 256, 0, st>>>(down, rank, (int)k, ad.G, ad.steps, range, ad.down + slot * ad.down_bytes(),
+                                              ad.meta + slot);
+    PPOCR_HIP(hipGetLastError());
+    up_record_kernel<T><<<(unsigned)ad.tiles, 256, 0, st>>>(up, rank, scale, class_scale, n, ad.steps, range,
+                                                            ad.up + slot * ad.up_bytes());
+    PPOCR_HIP(hipGetLastError());
+    return PPOCR_OK;
+}
+
+// ---------------------------------------------------------------- rows in order of their slots
+// Plan of a call: rows[unit][32] (-1: none), the slot of each unit, the number of units.
+struct Plan {
+    int* units;
+    int* rows;
+    int* slot;
+};
+int64_t plan_units(int64_t m, int64_t groups) { return m / kUnit + groups; }
+
+// One workgroup.  A row's line is the last whose offset is not above it, so each row is placed once
+// whatever the offsets hold; rows of no line, and of lines that name no slot, form a group of their own.
+// Rows of a group are placed in any order: no row's result depends on its place.
+__global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int slots, int most_units, Plan plan) {
+    extern __shared__ int groups[];
+    int* count = groups;              // [slots + 1] rows of a group
+    int* first = groups + slots + 1;  // its first unit
+    const int tid = threadIdx.x, lane = tid & 63;
+    for (int g = tid; g <= slots; g += 1024) count[g] = 0;
+    __syncthreads();
+    auto group_of = [&](int r) -> int {
+        int64_t lo = 0, hi = lines.lines;  // off[lo] <= r < off[hi], if offsets rise
+        if (hi == 0 || lines.off[0] > r) return slots;
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) >> 1;
+            if (lines.off[mid] <= r) lo = mid;
+            else hi = mid;
+        }
+        if (lines.off[lo + 1] <= r) return slots;
+        const int s = lines.slot[lo];
+        return s >= 0 && s < slots ? s : slots;
+    };
+    // a slot for each lane's row in its group: lanes of one group together where the wave's rows all have it
+    auto take = [&](bool on, int g) -> int {
+        const unsigned long long mask = __ballot(on);
+        if (mask == 0ull) return 0;
+        const int leader = __ffsll((long long)mask) - 1;
+        const int g0 = __shfl(g, leader, 64);
+        if (__ballot(on && g != g0) == 0ull) {
+            int base = 0;
+            if (lane == leader) base = atomicAdd(&count[g0], __popcll(mask));
+            return __shfl(base, leader, 64) + __popcll(mask & ((1ull << lane) - 1ull));
+        }
+        return on ? atomicAdd(&count[g], 1) : 0;
+    };
+    for (int r0 = 0; r0 < m; r0 += 1024) {
+        const int r = r0 + tid;
+        (void)take(r < m, r < m ? group_of(r) : 0);
+    }
+    __syncthreads();
+    if (tid < 64) {
+        int before = 0;
+        for (int g0 = 0; g0 <= slots; g0 += 64) {
+            const int g = g0 + lane;
+            const int mine = g <= slots ? (count[g] + kUnit - 1) / kUnit : 0;
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(upto, o, 64);
+                if (lane >= o) upto += v;
+            }
+            if (g <= slots) first[g] = before + upto - mine;
+            before += __shfl(upto, 63, 64);
+        }
+        if (lane == 0) *plan.units = before;
+    }
+    __syncthreads();
+    // the units' slots, and the places that the last unit of a group has no row for
+    for (int g = tid; g <= slots; g += 1024) {
+        const int n = count[g], units = (n + kUnit - 1) / kUnit;
+        for (int u = 0; u < units; ++u) plan.slot[first[g] + u] = g;
+        for (int x = n; x < units * kUnit; ++x) plan.rows[first[g] * kUnit + x] = -1;
+        count[g] = 0;
+    }
+    __syncthreads();
+    for (int r0 = 0; r0 < m; r0 += 1024) {
+        const int r = r0 + tid;
+        const int g = r < m ? group_of(r) : 0;
+        const int at = take(r < m, g);
+        if (r < m) plan.rows[first[g] * kUnit + at] = r;
+    }
+}
+
+// ---------------------------------------------------------------- rows and their u in registers
+struct AdaptLaunch {
+    const float* a;
+    int64_t m;
+    int k, vec;
+    const uint8_t* rec;
+    int tiles, n, nsplit, tpc, mblocks;
+    Plan plan;
+    int slots;
+    const uint8_t* down;
+    size_t down_stride;
+    const uint8_t* up;
+    size_t up_stride;
+    const AdapterMeta* meta;
+    Partial* part;
+    float* out;
+};
+
+template <int C, int G, int NR>
+struct RowOperands {
+    u16x8 a[Geo<C, G>::S];
+    u16x8 uhi[NR], ulo[NR];
+    float inv;  // the row's power of two undone
+};
+
+// Row `row` (its lane's of 32) scaled, split, and multiplied with its adapter's down.
+template <int C, int G, int NR>
+__device__ __forceinline__ void load_rows(const AdaptLaunch& x, int64_t row, int slot, int i, int h, RowOperands<C, G, NR>& o) {
+    using A = ActPlan<C, G>;
+    using D = ActPlan<CFG_HF3, G>;
+    static_assert(A::NL == D::NL, "both products read the rows in the same pieces");
+    float raw[A::NL][8];
+    act_issue<C, G>(x.a, row, x.k, x.vec, h, raw);
+    const AdapterMeta meta = x.meta[slot];
+    float top = 0.0f;
+    bool odd = false;
+#pragma unroll
+    for (int l = 0; l < A::NL; ++l)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            top = fmaxf(top, __builtin_fabsf(raw[l][e]));
+            odd |= !(__builtin_fabsf(raw[l][e]) < INFINITY);
+        }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    odd |= (bool)__shfl_xor((int)odd, 32, 64);
+    int ex = 0;
+    if (top > 0.0f && !odd) ex = max(min(meta.top - 1 - ilogbf(top), 126), -126);
+    o.inv = ldexpf(1.0f, -ex);
+    const float to = ldexpf(1.0f, ex);
+#pragma unroll
+    for (int l = 0; l < A::NL; ++l)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[l][e] *= to;
+    float none = 0.0f, none2 = 0.0f;
+    {
+        u16x8 d[Geo<CFG_HF3, G>::S];
+        act_split_all<CFG_HF3, G>(raw, h, d, none, none2);
+        const uint8_t* rec = x.down + (size_t)slot * x.down_stride;
+#pragma unroll
+        for (int b = 0; b < (NR + 1) / 2; ++b) {
+            f32x16 u = {};
+#pragma unroll
+            for (int s = 0; s < Geo<CFG_HF3, G>::S; ++s)
+                u = mfma16<true>(weight_frag<CFG_HF3, G>(rec + b * (2 * G * 512 + 1024), s, i * 16 + h * 512, i * 16, h), d[s], u);
+#pragma unroll
+            for (int y = 0; y < 2 && 2 * b + y < NR; ++y)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float v = u[8 * y + e] * meta.ushift;
+                    o.uhi[2 * b + y][e] = split_term<true>(v, 0);
+                    o.ulo[2 * b + y][e] = split_term<true>(v, 1);
+                }
+        }
+    }
+    act_split_all<C, G>(raw, h, o.a, none, none2);
+}
+
+// The adapter's fragments of a class tile: NR steps, both halves.
+template <int NR>
+__device__ __forceinline__ void load_up(const uint8_t* up, int tile, int lane, u16x8 (&hi)[NR], u16x8 (&lo)[NR]) {
+    const u16x8* p = reinterpret_cast<const u16x8*>(up + (size_t)tile * (2 * NR * 1024)) + lane;
+#pragma unroll
+    for (int s = 0; s < NR; ++s) {
+        hi[s] = p[s * 64];
+        lo[s] = p[(NR + s) * 64];
+    }
+}
+
+// ---------------------------------------------------------------- statistics
+// One wave, 32 rows (columns of the matrix product), 32 classes a tile; the head's tiles through a ring in
+// LDS as in the head's statistics pass, the products of tile j + 1 interleaved with the epilogue of tile j.
+template <int P>
+__device__ __forceinline__ void adapt_piece(f32x16 (&t)[1], float inv, const float* __restrict__ ep, int h, int j, f32x4 (&cs)[2],
+                                            f32x4 (&cb)[2], const float (&ref)[1], float (&best)[1], int (&bt)[1], f32x4* save,
+                                            EpiState<1>& st) {
+    if constexpr (P < 12 && P % 3 == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[0][4 * (P / 3) + e] *= inv;
+    }
+    epi_piece<P, 1, false>(t, ep, h, j, cs, cb, ref, best, bt, save, st);
+}
+template <int H, int x>
+__device__ __forceinline__ void adapt_pieces(f32x16 (&t)[1], float inv, const float* __restrict__ ep, int h, int j, f32x4 (&cs)[2],
+                                             f32x4 (&cb)[2], const float (&ref)[1], float (&best)[1], int (&bt)[1], f32x4* save,
+                                             EpiState<1>& st) {
+    constexpr int NP = epi_pieces<1>();
+    constexpr int p0 = x * NP / H, p1 = (x + 1) * NP / H;
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+        (adapt_piece<p0 + I>(t, inv, ep, h, j, cs, cb, ref, best, bt, save, st), ...);
+    }(std::make_integer_sequence<int, p1 - p0>{});
+}
+
+template <int C, int G, int NR>
+__global__ __launch_bounds__(64 * kWaves, 2) void adapt_stats_kernel(AdaptLaunch x) {
+    using GE = Geo<C, G>;
+    constexpr int S = GE::S, NT = 64 * kWaves;
+    extern __shared__ __align__(16) uint8_t lds[];
+    int mbi, chunk;
+    map_block<true>(blockIdx.x, x.nsplit, &mbi, &chunk);
+    const int units = *x.plan.units;
+    if (mbi * kWaves >= units || chunk >= x.nsplit) return;
+    const int t0 = chunk * x.tpc, t1 = min(t0 + x.tpc, x.tiles);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 31, h = lane >> 5;
+    if (tid < 32 * kRing) reinterpret_cast<u32x4*>(lds + (tid >> 5) * GE::BUF + GE::REC)[tid & 31] = u32x4{0, 0, 0, 0};
+    const int lb = i * 16 + h * 512;
+    f32x4* save = reinterpret_cast<f32x4*>(lds + kRing * GE::BUF) + wave * (4 * 64) + lane;
+    constexpr int kOps = stage_direct_min_ops<GE::REC, NT>();
+    if (t0 < t1) {
+#pragma unroll
+        for (int y = 0; y < kRing - 1; ++y)
+            stage_direct<GE::REC, NT>(x.rec + (size_t)min(t0 + y, t1 - 1) * GE::REC, lds + y * GE::BUF, tid);
+    }
+    const int unit = mbi * kWaves + wave;
+    const bool live = unit < units;
+    const int row = live ? x.plan.rows[unit * kUnit + i] : -1;
+    const int slot = __builtin_amdgcn_readfirstlane(live ? x.plan.slot[unit] : x.slots);
+    const uint8_t* up = x.up + (size_t)slot * x.up_stride;
+    RowOperands<C, G, NR> o;
+    load_rows<C, G, NR>(x, max(row, 0), slot, i, h, o);
+
+    float best[1] = {-INFINITY}, ref[1] = {0.0f}, sum = 0.0f;
+    int bt[1] = {-1};
+    // the loads of the newest staged tile may still be in flight at a barrier
+    constexpr int kLead = (kRing - 3) * kOps;
+    if (t0 < t1) {
+        u16x8 whi[NR], wlo[NR];
+        load_up<NR>(up, t0, lane, whi, wlo);
+        ring_barrier<kLead>();  // tiles t0 and t0 + 1 are in LDS
+        f32x16 acc_a[1] = {f32x16{}}, acc_b[1];
+        auto adapter_products = [&](f32x16& acc) {
+#pragma unroll
+            for (int s = 0; s < NR; ++s) {
+                acc = mfma16<true>(whi[s], o.uhi[s], acc);
+                acc = mfma16<true>(whi[s], o.ulo[s], acc);
+                acc = mfma16<true>(wlo[s], o.uhi[s], acc);
+            }
+        };
+        adapter_products(acc_a[0]);
+        load_up<NR>(up, min(t0 + 1, t1 - 1), lane, whi, wlo);
+#pragma unroll
+        for (int s = 0; s < S; ++s) acc_a[0] = mfma16<true>(weight_frag<C, G>(lds, s, lb, i * 16, h), o.a[s], acc_a[0]);
+        auto step = [&]<int R>(int j, f32x16 (&accE)[1], f32x16 (&accM)[1]) {
+            constexpr unsigned rel = (unsigned)R;  // (j - t0) % kRing
+            const uint8_t* bufn = lds + ((rel + 1) & (kRing - 1)) * GE::BUF;
+            const float* ep = reinterpret_cast<const float*>(lds + (rel & (kRing - 1)) * GE::BUF + GE::FRAG);
+            f32x4 cs[2], cb[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                cs[q] = *reinterpret_cast<const f32x4*>(ep + 8 * q + 4 * h);
+                cb[q] = *reinterpret_cast<const f32x4*>(ep + 32 + 8 * q + 4 * h);
+            }
+            EpiState<1> st;
+            st.need = false;
+            accM[0] = f32x16{};
+            // the adapter's products first: their operands' registers then take the next tile's, which has
+            // the rest of the step to arrive.  Those loads are issued before the staged ones: the barrier's
+            // count of loads in flight stays that of the staged ones.
+            adapter_products(accM[0]);
+            load_up<NR>(up, min(j + 2, t1 - 1), lane, whi, wlo);
+            stage_direct<GE::REC, NT>(x.rec + (size_t)min(j + kRing - 1, t1 - 1) * GE::REC,
+                                      lds + ((rel + kRing - 1) & (kRing - 1)) * GE::BUF, tid);
+            u16x8 wq[kPrefetch];
+            frag_prefetch_first<C, G, kPrefetch>(wq, bufn, lb, i * 16, h);
+            [&]<int... s>(std::integer_sequence<int, s...>) {
+                ([&] {
+                    accM[0] = mfma16<true>(frag_of<C, G, kPrefetch, s>(wq), o.a[s], accM[0]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    adapt_pieces<2 * S, 2 * s>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
+                    frag_prefetch_after<C, G, kPrefetch, s>(wq, bufn, lb, i * 16, h);
+                    __builtin_amdgcn_sched_barrier(0);
+                    adapt_pieces<2 * S, 2 * s + 1>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
+                    __builtin_amdgcn_sched_barrier(0);
+                }(), ...);
+            }(std::make_integer_sequence<int, S>{});
+            if (__any(st.need)) {
+                if (best[0] != -INFINITY && __builtin_fabsf(best[0] - ref[0]) > 64.0f) {
+                    const float nr = best[0];
+                    sum = (sum == 0.0f) ? 0.0f : sum * __builtin_amdgcn_exp2f(ref[0] - nr);
+                    float v = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) v += __builtin_amdgcn_exp2f(accE[0][r] - nr);
+                    st.tsum[0] = v;
+                    ref[0] = nr;
+                }
+            }
+            sum += st.tsum[0];
+            ring_barrier<kLead>();
+        };
+        auto step_of = [&]<int R>(int jj) {
+            if constexpr (R % 2 == 0) step.template operator()<R>(jj, acc_a, acc_b);
+            else step.template operator()<R>(jj, acc_b, acc_a);
+        };
+        int j = t0;
+        for (; j + kRing - 1 < t1; j += kRing)
+            [&]<int... R>(std::integer_sequence<int, R...>) {
+                (step_of.template operator()<R>(j + R), ...);
+            }(std::make_integer_sequence<int, kRing>{});
+        [&]<int... R>(std::integer_sequence<int, R...>) {
+            ((j + R < t1 ? step_of.template operator()<R>(j + R) : void()), ...);
+        }(std::make_integer_sequence<int, kRing - 1>{});
+        // the ring's last loads (repeats of the last tile) land before the workgroup ends
+        vm_wait<0>();
+    }
+
+    int cls = 0;
+    if (bt[0] >= 0) {
+        int r0 = 16;
+#pragma unroll
+        for (int q = 3; q >= 0; --q) {
+            const f32x4 v = save[q * 64];
+#pragma unroll
+            for (int e = 3; e >= 0; --e) r0 = (v[e] == best[0]) ? 4 * q + e : r0;
+        }
+        cls = bt[0] * 32 + (r0 < 16 ? 8 * (r0 >> 2) + 4 * h + (r0 & 3) : 0);
+    }
+    const RowStat mine{best[0], sum, ref[0], cls};
+    const RowStat other{__shfl_xor(best[0], 32, 64), __shfl_xor(sum, 32, 64), __shfl_xor(ref[0], 32, 64), __shfl_xor(cls, 32, 64)};
+    const RowStat r = stat_merge(mine, other);
+    if (h == 0 && row >= 0) x.part[(int64_t)chunk * x.m + row] = Partial{r.best, r.sum, r.idx};
+}
+
+// ---------------------------------------------------------------- logits
+// Rows of the matrix product are the activation rows, columns the classes, so that a store writes 32
+// consecutive classes of two rows.  A producer wave keeps the ring of the head's tiles filled.
+template <int C, int G, int NR>
+__global__ __launch_bounds__(64 * (kWaves + 1), 1) void adapt_logits_kernel(AdaptLaunch x) {
+    using GE = Geo<C, G>;
+    constexpr int S = GE::S;
+    constexpr int R = writer_ring<GE::REC>();
+    extern __shared__ __align__(16) uint8_t lds[];  // [R tiles] x BUF
+    int mbi, chunk;
+    map_block<false>(blockIdx.x, x.nsplit, &mbi, &chunk);
+    const int units = *x.plan.units;
+    if (mbi * kWaves >= units) return;
+    const int t0 = chunk * x.tpc, t1 = min(t0 + x.tpc, x.tiles);
+    if (t0 >= t1) return;
+    const int ntiles = t1 - t0;
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // workgroups start at tiles of their own, as in the head's writer
+    const unsigned stride = x.nsplit == 1 ? kStartStepOne : kStartStepSeveral;
+    const int rot = (int)(((int64_t)((blockIdx.x * stride) & 0xffffu) * ntiles) >> 16);
+
+    if (wave == kWaves) {
+        constexpr int kOps = stage_wave_ops<GE::REC>();
+        int pt = t0 + rot, pslot = 0;
+        auto stage_next = [&] {
+            stage_wave<GE::REC>(x.rec + (size_t)pt * GE::REC, lds + pslot * GE::BUF, lane);
+            pt = pt + 1 == t1 ? t0 : pt + 1;
+            pslot = pslot + 1 == R ? 0 : pslot + 1;
+        };
+#pragma unroll
+        for (int g = 0; g < R - 1; ++g) stage_next();
+        vm_wait<kOps * (R - 2)>();  // tile 0 is in LDS
+        barrier_lds();
+        for (int g = 0; g < ntiles; ++g) {
+            stage_next();
+            vm_wait<kOps * (R - 2)>();  // tile g + 1 is in LDS
+            barrier_lds();
+        }
+        vm_wait<0>();  // the ring's last loads land before the workgroup ends
+        return;
+    }
+
+    for (int y = tid >> 5; y < R; y += 2 * kWaves)
+        reinterpret_cast<u32x4*>(lds + y * GE::BUF + GE::REC)[tid & 31] = u32x4{0, 0, 0, 0};
+    const int unit = mbi * kWaves + wave;
+    const bool live = unit < units;
+    const int row = live ? x.plan.rows[unit * kUnit + i] : -1;
+    const int slot = __builtin_amdgcn_readfirstlane(live ? x.plan.slot[unit] : x.slots);
+    const uint8_t* up = x.up + (size_t)slot * x.up_stride;
+    RowOperands<C, G, NR> o;
+    load_rows<C, G, NR>(x, max(row, 0), slot, i, h, o);
+    // rows of this lane's 16 accumulators
+    int orow[16];
+    float oinv[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int from = 8 * (r >> 2) + 4 * h + (r & 3);
+        orow[r] = __shfl(row, from, 64);
+        oinv[r] = __shfl(o.inv, from, 64);
+    }
+    const bool whole = __all(row >= 0);
+    int pt = t0 + rot, cslot = 0;
+    u16x8 whi[NR], wlo[NR];
+    load_up<NR>(up, pt, lane, whi, wlo);
+    barrier_lds();  // zero blocks written; tile 0 is in LDS
+    for (int g = 0; g < ntiles; ++g) {
+        const uint8_t* buf = lds + cslot * GE::BUF;
+        cslot = cslot + 1 == R ? 0 : cslot + 1;
+        const int next = pt + 1 == t1 ? t0 : pt + 1;
+        f32x16 acc = {};
+#pragma unroll
+        for (int s = 0; s < NR; ++s) {
+            acc = mfma16<true>(o.uhi[s], whi[s], acc);
+            acc = mfma16<true>(o.ulo[s], whi[s], acc);
+            acc = mfma16<true>(o.uhi[s], wlo[s], acc);
+        }
+        load_up<NR>(up, next, lane, whi, wlo);
+        constexpr int kAhead = S < 8 ? S : 8;
+        u16x8 wq[kAhead];
+        frag_prefetch_first<C, G, kAhead>(wq, buf, i * 16 + h * 512, i * 16, h);
+        [&]<int... st>(std::integer_sequence<int, st...>) {
+            ([&] {
+                acc = mfma16<true>(o.a[st], frag_of<C, G, kAhead, st>(wq), acc);
+                frag_prefetch_after<C, G, kAhead, st>(wq, buf, i * 16 + h * 512, i * 16, h);
+                __builtin_amdgcn_sched_barrier(0);
+            }(), ...);
+        }(std::make_integer_sequence<int, S>{});
+        const float* ep = reinterpret_cast<const float*>(buf + GE::FRAG);
+        const float c0 = ep[64 + i], c1 = ep[96 + i];
+        const int col = pt * 32 + i;
+        float v[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] = fmaf(acc[r] * oinv[r], c0, c1);
+        if (whole && pt * 32 + 32 <= x.n) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x.out[(int64_t)orow[r] * x.n + col] = v[r];
+        } else if (col < x.n) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (orow[r] >= 0) x.out[(int64_t)orow[r] * x.n + col] = v[r];
+        }
+        pt = next;
+        barrier_lds();  // this ring slot is read; the next tile is in LDS
+    }
+}
+
+// ---------------------------------------------------------------- launches
+int grid_of(int mblocks, int nsplit, bool rows_on_one_xcd) {
+    if (nsplit >= 8) return mblocks * 8 * ((nsplit + 7) / 8);
+    if (rows_on_one_xcd) return ((mblocks + 7) / 8) * nsplit * 8;
+    const int r8 = 8 / nsplit;
+    return ((mblocks + r8 - 1) / r8) * 8;
+}
+
+size_t align(size_t x) { return (x + 255) / 256 * 256; }
+
+struct AdaptLayout {
+    size_t units, rows, slot, part, total;
+};
+int chunks_of(const Adapters& ad, int64_t m) { return stats_nsplit(m, kUnit * kWaves, ad.tiles, 2); }
+AdaptLayout layout_of(const Adapters& ad, int64_t m) {
+    const int64_t units = plan_units(m, std::min<int64_t>(ad.slots, m) + 1);
+    AdaptLayout L;
+    L.units = 0;
+    L.rows = 256;
+    L.slot = L.rows + align((size_t)units * kUnit * 4);
+    L.part = L.slot + align((size_t)units * 4);
+    L.total = L.part + align((size_t)chunks_of(ad, m) * (size_t)m * sizeof(Partial));
+    return L;
+}
+
+int make_plan(const Adapters& ad, const AdaptLines& lines, int64_t m, const AdaptLayout& L, uint8_t* ws, Plan* plan, int64_t* units,
+              hipStream_t st) {
+    *plan = Plan{reinterpret_cast<int*>(ws + L.units), reinterpret_cast<int*>(ws + L.rows), reinterpret_cast<int*>(ws + L.slot)};
+    *units = plan_units(m, std::min<int64_t>(std::min<int64_t>(ad.slots, lines.lines) + 1, m));
+    plan_kernel<<<1, 1024, (size_t)(ad.slots + 1) * 8, st>>>(lines, (int)m, ad.slots, (int)*units, *plan);
+    PPOCR_HIP(hipGetLastError());
+    return PPOCR_OK;
+}
+
+AdaptLaunch launch_of(const TileGeom& tg, const uint8_t* rec, const Adapters& ad, const float* a, int64_t m, int64_t n, int64_t k,
+                      int64_t units, int nsplit, const Plan& plan) {
+    AdaptLaunch x{};
+    x.a = a;
+    x.m = m;
+    x.k = (int)k;
+    x.vec = k % 4 == 0 && reinterpret_cast<uintptr_t>(a) % 16 == 0 ? 1 : 0;
+    x.rec = rec;
+    x.tiles = tg.tiles;
+    x.n = (int)n;
+    x.nsplit = nsplit;
+    x.tpc = (tg.tiles + nsplit - 1) / nsplit;
+    x.mblocks = (int)((units + kWaves - 1) / kWaves);
+    x.plan = plan;
+    x.slots = ad.slots;
+    x.down = ad.down;
+    x.down_stride = ad.down_bytes();
+    x.up = ad.up;
+    x.up_stride = ad.up_bytes();
+    x.meta = ad.meta;
+    return x;
+}
+
+// f.template operator()<C, G, NR>() for the head's configuration and the adapters' steps.
+template <typename F>
+int by_config(int cfg, int G, int steps, F&& f) {
+    auto ranks = [&]<int C, int GG>() {
+        if (steps == 1) return f.template operator()<C, GG, 1>();
+        if (steps == 2) return f.template operator()<C, GG, 2>();
+        return f.template operator()<C, GG, 4>();
+    };
+    if (cfg == CFG_H2) return G == 15 ? ranks.template operator()<CFG_H2, 15>() : ranks.template operator()<CFG_H2, 10>();
+    return G == 15 ? ranks.template operator()<CFG_HF3, 15>() : ranks.template operator()<CFG_HF3, 10>();
+}
+
+}  // namespace
+
+int launch_adapters_clear(const Adapters& ad, hipStream_t st) {
+    const int64_t d = (int64_t)(ad.slots + 1) * ad.down_bytes() / 16, u = (int64_t)(ad.slots + 1) * ad.up_bytes() / 16;
+    clear_kernel<<<1024, 256, 0, st>>>(reinterpret_cast<u32x4*>(ad.down), d);
+    PPOCR_HIP(hipGetLastError());
+    clear_kernel<<<4096, 256, 0, st>>>(reinterpret_cast<u32x4*>(ad.up), u);
+    PPOCR_HIP(hipGetLastError());
+    clear_meta_kernel<<<16, 256, 0, st>>>(ad.meta, ad.slots + 1);
+    PPOCR_HIP(hipGetLastError());
+    return PPOCR_OK;
+}
+
+int launch_adapter_set(const Adapters& ad, int slot, const void* down, const void* up, int rank, float scale, int bf16,
+                       const float* class_scale, int64_t n, int64_t k, hipStream_t st) {
+    return bf16 ? set_slot(ad, slot, (const uint16_t*)down, (const uint16_t*)up, rank, scale, class_scale, n, k, st)
+                : set_slot(ad, slot, (const float*)down, (const float*)up, rank, scale, class_scale, n, k, st);
+}
+
+size_t adapt_workspace(const Adapters& ad, int64_t m) { return m > 0 ? layout_of(ad, m).total : 0; }
+
+int launch_adapt_decode(int cfg, const TileGeom& tg, const uint8_t* rec, const Adapters& ad, const AdaptLines& lines, const float* a,
+                        int64_t m, int64_t n, int64_t k, int32_t* idx, float* maxprob, const CtcOut& ctc, uint8_t* ws,
+                        hipStream_t st) {
+    const AdaptLayout L = layout_of(ad, m);
+    Plan plan;
+    int64_t units;
+    if (int e = make_plan(ad, lines, m, L, ws, &plan, &units, st)) return e;
+    const int nsplit = chunks_of(ad, m);
+    AdaptLaunch x = launch_of(tg, rec, ad, a, m, n, k, units, nsplit, plan);
+    x.part = reinterpret_cast<Partial*>(ws + L.part);
+    const unsigned grid = (unsigned)grid_of(x.mblocks, nsplit, true);
+    if (int e = by_config(cfg, tg.G, ad.steps, [&]<int C, int G, int NR>() {
+            constexpr int bytes = kRing * Geo<C, G>::BUF + kWaves * 16 * 64 * 4;
+            adapt_stats_kernel<C, G, NR><<<grid, 64 * kWaves, bytes, st>>>(x);
+            PPOCR_HIP(hipGetLastError());
+            return (int)PPOCR_OK;
+        }))
+        return e;
+    return launch_merge_ctc(x.part, m, nsplit, ctc, idx, maxprob, nullptr, st);
+}
+
+int launch_adapt_logits(int cfg, const TileGeom& tg, const uint8_t* rec, const Adapters& ad, const AdaptLines& lines, const float* a,
+                        int64_t m, int64_t n, int64_t k, float* out, uint8_t* ws, hipStream_t st) {
+    const AdaptLayout L = layout_of(ad, m);
+    Plan plan;
+    int64_t units;
+    if (int e = make_plan(ad, lines, m, L, ws, &plan, &units, st)) return e;
+    const int64_t mblocks = (units + kWaves - 1) / kWaves;
+    // enough workgroups for the CUs
+    int nsplit = 1;
+    while (nsplit < 64 && mblocks * nsplit < 256 && nsplit * 2 <= tg.tiles) nsplit *= 2;
+    AdaptLaunch x = launch_of(tg, rec, ad, a, m, n, k, units, nsplit, plan);
+    x.out = out;
+    const unsigned grid = (unsigned)grid_of(x.mblocks, nsplit, false);
+    return by_config(cfg, tg.G, ad.steps, [&]<int C, int G, int NR>() {
+        constexpr int bytes = writer_ring<Geo<C, G>::REC>() * Geo<C, G>::BUF;
+        adapt_logits_kernel<C, G, NR><<<grid, 64 * (kWaves + 1), bytes, st>>>(x);
+        PPOCR_HIP(hipGetLastError());
+        return (int)PPOCR_OK;
+    });
+}
+
+}  // namespace ppocr

@@ -11,11 +11,14 @@
 #include <string>
 #include <vector>
 
+#include "adapt.hpp"
+#include "grad_clip.hpp"
 #include "kernels.hpp"
 #include "layernorm.hpp"
 #include "model_graph.hpp"
 #include "neck.hpp"
 #include "safetensors.hpp"
+#include "sequence_loss.hpp"
 #include "xent.hpp"
 
 namespace ppocr {
@@ -59,6 +62,11 @@ struct ppocr_rh {
     // ... or rows with ||a||_2^2 at most range_ss: |logit| <= ||a||_2 * max_c ||w_c||_2 + max_c |b_c|
     float range_ss = 0.0f;
     bool range_ok = false;
+    // Handles that hold these weights: this one and the adapted heads made from it.
+    std::atomic<int> holders{1};
+    // An adapted head (ppocr_ra_create): the weights above are base's, the adapters its own.
+    ppocr_rh* base = nullptr;
+    Adapters adapters{};
 };
 
 namespace {
@@ -389,6 +397,16 @@ std::vector<uint8_t> build_records(const TileGeom& g, int64_t n, int64_t k, cons
 void free_handle(ppocr_rh* h) {
     if (!h) return;
     DeviceGuard dg(h->device);
+    if (h->base) {
+        if (h->adapters.down) (void)hipFree(h->adapters.down);
+        if (h->adapters.up) (void)hipFree(h->adapters.up);
+        if (h->adapters.meta) (void)hipFree(h->adapters.meta);
+        if (h->adapters.range) (void)hipFree(h->adapters.range);
+        free_handle(h->base);
+        delete h;
+        return;
+    }
+    if (h->holders.fetch_sub(1) != 1) return;
     if (h->d_q) (void)hipFree(h->d_q);
     if (h->d_w) (void)hipFree(h->d_w);
     if (h->d_scale) (void)hipFree(h->d_scale);
@@ -2021,6 +2039,505 @@ int ppocr_layernorm_backward(const float* dy, const float* x, const float* w, co
                                           reinterpret_cast<float*>(hc.ws() + 256), hc.stream()))
         return e;
     return hc.copy_out({dx, dw, db});
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- adapting the head
+namespace {
+
+constexpr const char* kAdaptOp = "LowRankAdapter";
+constexpr const char* kPolicyOp = "PolicyLoss";
+constexpr const char* kPreferenceOp = "PreferenceLoss";
+constexpr const char* kClipOp = "GradClip";
+constexpr int64_t kMostSteps = 1LL << 30;
+constexpr int64_t kClipMostTensors = 65536;
+
+int check_adapted(const ppocr_rh* h) {
+    if (int e = check_head(h, kAdaptOp)) return e;
+    if (!h->base) return bad_arg(kAdaptOp, "the head has no adapters (ppocr_ra_create)");
+    return PPOCR_OK;
+}
+int adapt_cfg(const ppocr_rh* h) { return h->quantized ? CFG_H2 : CFG_HF3; }
+
+// The workspace of an adapted call behind the first bytes, which are left to the head's calls.
+constexpr size_t kAdaptWs = 256;
+
+int check_adapter(const ppocr_rh* h, int64_t slot, const void* down, const void* up, int64_t rank, float scale) {
+    if (int e = check_adapted(h)) return e;
+    if (slot < 0 || slot >= h->adapters.slots)
+        return bad_arg(kAdaptOp, "slot " + std::to_string(slot) + " of " + std::to_string(h->adapters.slots));
+    if (rank < 0 || rank > h->adapters.max_rank)
+        return bad_arg(kAdaptOp, "rank must be 0 to " + std::to_string(h->adapters.max_rank) + ", got " + std::to_string(rank));
+    if (!std::isfinite(scale)) return bad_arg(kAdaptOp, "scale must be finite");
+    if (rank > 0 && (!down || !up)) return bad_arg(kAdaptOp, "null pointer");
+    return PPOCR_OK;
+}
+
+int check_adapt_rows(const ppocr_rh* h, int64_t m, int64_t lines) {
+    if (int e = check_adapted(h)) return e;
+    if (m < 0 || lines < 0) return bad_arg(kAdaptOp, "negative shape");
+    if (m > kMostSteps || lines > kMostSteps) return bad_arg(kAdaptOp, "too many rows");
+    return PPOCR_OK;
+}
+
+// Offsets and slots of the host forms.
+int check_host_lines(const ppocr_rh* h, const int64_t* line_off, int64_t lines, const int32_t* line_slot) {
+    if (!line_off || !line_slot) return bad_arg(kAdaptOp, "null pointer");
+    if (int e = check_offsets(line_off, lines)) return e;
+    for (int64_t i = 0; i < lines; ++i)
+        if (line_slot[i] >= h->adapters.slots)
+            return bad_arg(kAdaptOp, "slot " + std::to_string(line_slot[i]) + " of " + std::to_string(h->adapters.slots));
+    return PPOCR_OK;
+}
+
+int check_merge(int64_t n, int64_t k, int64_t rank, float scale, int dtype) {
+    if (n <= 0 || k <= 0) return bad_arg(kAdaptOp, "weight must have positive shape");
+    if (k > kXentMaxK) return bad_arg(kAdaptOp, "inner dimension " + std::to_string(k) + " above " + std::to_string(kXentMaxK));
+    if (n > kXentMost) return bad_arg(kAdaptOp, "too many classes");
+    if (rank < 1 || rank > kAdaptMostRank)
+        return bad_arg(kAdaptOp, "rank must be 1 to " + std::to_string(kAdaptMostRank) + ", got " + std::to_string(rank));
+    if (!std::isfinite(scale)) return bad_arg(kAdaptOp, "scale must be finite");
+    return check_dtype(dtype, kAdaptOp);
+}
+
+MergeArgs merge_args(const void* w, const void* dw, const void* down, const void* up, int64_t n, int64_t k, int64_t rank,
+                     float scale, int dtype, void* out) {
+    return MergeArgs{w, dw, down, up, n, (int)k, (int)rank, scale, dtype == PPOCR_DTYPE_BF16, out};
+}
+
+int check_lines(const char* op, int64_t lines, int64_t m) {
+    if (lines < 0 || m < 0) return bad_arg(op, "negative shape");
+    if (lines > kMostSteps || m > kMostSteps) return bad_arg(op, "too many steps");
+    return PPOCR_OK;
+}
+int check_host_steps(const char* op, const int64_t* line_off, int64_t lines, int64_t m) {
+    if (int e = check_offsets(line_off, lines)) return e;
+    if (line_off[lines] > m) return bad_arg(op, "line offsets pass the " + std::to_string(m) + " steps");
+    return PPOCR_OK;
+}
+
+int check_policy(int64_t lines, int64_t m, float low, float high, float beta) {
+    if (int e = check_lines(kPolicyOp, lines, m)) return e;
+    if (!(low >= 0.0f && low <= 1.0f)) return bad_arg(kPolicyOp, "clip_low must lie in [0, 1]");
+    if (!(high >= 0.0f)) return bad_arg(kPolicyOp, "clip_high must not be negative");
+    if (!std::isfinite(beta)) return bad_arg(kPolicyOp, "beta must be finite");
+    return PPOCR_OK;
+}
+int check_preference(int64_t pairs, int64_t m, float beta, float smoothing) {
+    if (pairs < 0 || pairs > kMostSteps / 2) return bad_arg(kPreferenceOp, pairs < 0 ? "negative shape" : "too many steps");
+    if (int e = check_lines(kPreferenceOp, 2 * pairs, m)) return e;
+    if (!std::isfinite(beta)) return bad_arg(kPreferenceOp, "beta must be finite");
+    if (!(smoothing >= 0.0f && smoothing <= 1.0f)) return bad_arg(kPreferenceOp, "smoothing must lie in [0, 1]");
+    return PPOCR_OK;
+}
+
+// The tensors of a clipping call.  An output that overlaps another, or a gradient other than its own in place,
+// is refused: the kernels take the tensors in any order.
+int clip_tensors(void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes, int64_t count,
+                 float max_norm, std::vector<GradTensor>* list) {
+    if (count < 0) return bad_arg(kClipOp, "negative count");
+    if (!(max_norm > 0.0f)) return bad_arg(kClipOp, "max_norm must be positive");
+    if (count > 0 && (!grads || !sizes)) return bad_arg(kClipOp, "null pointer");
+    if (count > kClipMostTensors) return bad_arg(kClipOp, "too many tensors");
+    struct Span {
+        uintptr_t at, end;
+        int64_t i;
+    };
+    std::vector<Span> in, to;
+    for (int64_t i = 0; i < count; ++i) {
+        if (sizes[i] < 0) return bad_arg(kClipOp, "negative size");
+        if (sizes[i] > (1LL << 40)) return bad_arg(kClipOp, "tensor too large");
+        const int dt = dtypes ? dtypes[i] : PPOCR_DTYPE_F32;
+        if (int e = check_dtype(dt, kClipOp)) return e;
+        if (sizes[i] == 0) continue;
+        void* const o = out ? out[i] : grads[i];
+        if (!grads[i] || !o) return bad_arg(kClipOp, "null pointer");
+        const uintptr_t width = dt == PPOCR_DTYPE_BF16 ? 2 : 4, bytes = (uintptr_t)sizes[i] * width;
+        const uintptr_t g = reinterpret_cast<uintptr_t>(grads[i]), w = reinterpret_cast<uintptr_t>(o);
+        if ((g | w) % width) return bad_arg(kClipOp, "tensor not aligned to its type");
+        in.push_back({g, g + bytes, i});
+        to.push_back({w, w + bytes, i});
+        list->push_back({grads[i], o, sizes[i], dt == PPOCR_DTYPE_BF16});
+    }
+    auto by_start = [](const Span& a, const Span& b) { return a.at < b.at; };
+    std::sort(in.begin(), in.end(), by_start);
+    std::sort(to.begin(), to.end(), by_start);
+    for (size_t i = 1; i < to.size(); ++i)
+        if (to[i].at < to[i - 1].end) return bad_arg(kClipOp, "outputs overlap");
+    // outputs do not overlap, so walking both lists by their starts, an output meets a gradient before it ends;
+    // gradients may overlap each other, so each one's reach is carried along
+    size_t g0 = 0;
+    for (const Span& w : to) {
+        while (g0 < in.size() && in[g0].end <= w.at) ++g0;
+        for (size_t j = g0; j < in.size() && in[j].at < w.end; ++j)
+            if (in[j].end > w.at && !(in[j].i == w.i && in[j].at == w.at))
+                return bad_arg(kClipOp, "an output overlaps a gradient other than its own");
+    }
+    return PPOCR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ppocr_ra_create(const ppocr_rh_t* head, int64_t slots, int64_t max_rank, ppocr_rh_t** out) {
+    if (!out) return bad_arg(kAdaptOp, "out handle pointer is null");
+    *out = nullptr;
+    if (int e = check_head(head, kAdaptOp)) return e;
+    if (slots < 1 || slots > kAdaptMostSlots)
+        return bad_arg(kAdaptOp, "slots must be 1 to " + std::to_string(kAdaptMostSlots) + ", got " + std::to_string(slots));
+    if (max_rank < 1 || max_rank > kAdaptMostRank)
+        return bad_arg(kAdaptOp, "max_rank must be 1 to " + std::to_string(kAdaptMostRank) + ", got " + std::to_string(max_rank));
+    if (!head->mfma_ok)
+        return bad_arg(kAdaptOp, "no kernel for k = " + std::to_string(head->k) + " (supported: 73..80, 113..120)");
+    if (!head->f16_ok) return bad_arg(kAdaptOp, "weights beyond the fp16 range (|w| >= 32768)");
+    DeviceGuard dg(head->device);
+    if (dg.err) return fail(PPOCR_ERR_DEVICE, std::string(kAdaptOp) + ": hipSetDevice failed");
+    std::unique_ptr<ppocr_rh, void (*)(ppocr_rh*)> h(new (std::nothrow) ppocr_rh, free_handle);
+    if (!h) return fail(PPOCR_ERR_NO_MEMORY, std::string(kAdaptOp) + ": host allocation failed");
+    ppocr_rh* base = head->base ? head->base : const_cast<ppocr_rh*>(head);
+    h->device = base->device;
+    h->n = base->n;
+    h->k = base->k;
+    h->quantized = base->quantized;
+    h->geom = base->geom;
+    h->mfma_ok = base->mfma_ok;
+    h->d_q = base->d_q;
+    h->d_w = base->d_w;
+    h->d_scale = base->d_scale;
+    h->d_bias = base->d_bias;
+    h->d_rec = base->d_rec;
+    h->d_rec_h = base->d_rec_h;
+    h->fma = base->fma;
+    h->amax_limit = base->amax_limit;
+    h->amax_limit_h = base->amax_limit_h;
+    h->f16_ok = base->f16_ok;
+    h->range_limit = base->range_limit;
+    h->range_ss = base->range_ss;
+    h->range_ok = base->range_ok;
+    base->holders.fetch_add(1);
+    h->base = base;
+    Adapters& ad = h->adapters;
+    ad.slots = (int)slots;
+    ad.max_rank = (int)max_rank;
+    ad.steps = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : 4;
+    ad.G = h->geom.G;
+    ad.tiles = h->geom.tiles;
+    const size_t sets = (size_t)slots + 1;
+    const size_t bytes[4] = {sets * ad.down_bytes(), sets * ad.up_bytes(), sets * sizeof(AdapterMeta),
+                             sets * 2 * kAdaptMostRank * sizeof(unsigned)};
+    void** to[4] = {(void**)&ad.down, (void**)&ad.up, (void**)&ad.meta, (void**)&ad.range};
+    for (int i = 0; i < 4; ++i) {
+        if (dev_malloc(to[i], bytes[i]) != hipSuccess) {
+            *to[i] = nullptr;
+            (void)hipGetLastError();
+            return fail(PPOCR_ERR_NO_MEMORY, std::string(kAdaptOp) + ": device allocation of " + std::to_string(bytes[i]) +
+                                                 " bytes failed");
+        }
+        h->device_bytes += bytes[i];
+    }
+    if (int e = launch_adapters_clear(ad, nullptr)) return e;
+    PPOCR_HIP(hipStreamSynchronize(nullptr));
+    *out = h.release();
+    return PPOCR_OK;
+}
+
+void ppocr_ra_destroy(ppocr_rh_t* h) { free_handle(h); }
+
+int ppocr_ra_shape(const ppocr_rh_t* h, int64_t* slots, int64_t* max_rank) {
+    if (int e = check_adapted(h)) return e;
+    if (slots) *slots = h->adapters.slots;
+    if (max_rank) *max_rank = h->adapters.max_rank;
+    return PPOCR_OK;
+}
+
+int ppocr_ra_set_dev(ppocr_rh_t* h, int64_t slot, void* d_down, void* d_up, int64_t rank, float scale, int dtype,
+                     void* stream) {
+    if (int e = check_adapter(h, slot, d_down, d_up, rank, scale)) return e;
+    if (int e = check_dtype(dtype, kAdaptOp)) return e;
+    DeviceGuard dg(h->device);
+    return launch_adapter_set(h->adapters, (int)slot, d_down, d_up, (int)rank, scale, dtype == PPOCR_DTYPE_BF16, h->d_scale, h->n,
+                              h->k, (hipStream_t)stream);
+}
+
+int ppocr_ra_set(ppocr_rh_t* h, int64_t slot, const float* down, const float* up, int64_t rank, float scale) {
+    if (int e = check_adapter(h, slot, down, up, rank, scale)) return e;
+    DeviceGuard dg(h->device);
+    HostCall hc;
+    if (int e = hc.begin({(size_t)(rank * h->k) * 4, (size_t)(rank * h->n) * 4}, {}, 0)) return e;
+    if (rank > 0)
+        if (int e = hc.copy_in({down, up})) return e;
+    if (int e = launch_adapter_set(h->adapters, (int)slot, hc.in<float>(0), hc.in<float>(1), (int)rank, scale, 0, h->d_scale,
+                                   h->n, h->k, hc.stream()))
+        return e;
+    return hc.copy_out({});
+}
+
+size_t ppocr_ra_workspace_bytes(const ppocr_rh_t* h, int64_t m) {
+    if (m <= 0 || check_adapt_rows(h, m, 0)) return 0;
+    return kAdaptWs + adapt_workspace(h->adapters, m);
+}
+
+int ppocr_ra_logits_dev(const ppocr_rh_t* h, const float* d_a, int64_t m, const int64_t* d_line_off, int64_t lines,
+                        const int32_t* d_line_slot, float* d_out, void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (int e = check_adapt_rows(h, m, lines)) return e;
+    if (m == 0) return PPOCR_OK;
+    if (!d_a || !d_out || (lines > 0 && (!d_line_off || !d_line_slot))) return bad_arg(kAdaptOp, "null pointer");
+    DeviceGuard dg(h->device);
+    hipStream_t st = (hipStream_t)stream;
+    Workspace ws;
+    if (int e = train_workspace(&ws, d_workspace, workspace_bytes, ppocr_ra_workspace_bytes(h, m), st, kAdaptOp)) return e;
+    return launch_adapt_logits(adapt_cfg(h), h->geom, h->d_rec_h, h->adapters, AdaptLines{d_line_off, lines, d_line_slot}, d_a,
+                               m, h->n, h->k, d_out, ws.p + kAdaptWs, st);
+}
+
+int ppocr_ra_logits(const ppocr_rh_t* h, const float* a, const int64_t* line_off, int64_t lines, const int32_t* line_slot,
+                    float* out) {
+    if (int e = check_adapt_rows(h, 0, lines)) return e;
+    if (lines == 0) return PPOCR_OK;
+    if (int e = check_host_lines(h, line_off, lines, line_slot)) return e;
+    const int64_t m = line_off[lines];
+    if (int e = check_adapt_rows(h, m, lines)) return e;
+    if (m == 0) return PPOCR_OK;
+    if (!a || !out) return bad_arg(kAdaptOp, "null pointer");
+    DeviceGuard dg(h->device);
+    HostCall hc;
+    if (int e = hc.begin({(size_t)(m * h->k) * 4, (size_t)(lines + 1) * 8, (size_t)lines * 4}, {(size_t)(m * h->n) * 4},
+                         ppocr_ra_workspace_bytes(h, m)))
+        return e;
+    if (int e = hc.copy_in({a, line_off, line_slot})) return e;
+    if (int e = ppocr_ra_logits_dev(h, hc.in<float>(0), m, hc.in<int64_t>(1), lines, hc.in<int32_t>(2), hc.out<float>(0),
+                                    hc.ws(), hc.ws_bytes(), hc.stream()))
+        return e;
+    return hc.copy_out({out});
+}
+
+int ppocr_ra_decode_dev(const ppocr_rh_t* h, const float* d_a, int64_t m, const int64_t* d_line_off, int64_t lines,
+                        const int32_t* d_line_slot, int32_t* d_idx, float* d_maxprob, int32_t* d_seq, int64_t* d_seq_len,
+                        float* d_score, void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (int e = check_adapt_rows(h, m, lines)) return e;
+    if (lines == 0) return PPOCR_OK;
+    if (!d_line_off || !d_line_slot || !d_seq_len || !d_score || (m > 0 && (!d_a || !d_seq)))
+        return bad_arg(kAdaptOp, "null pointer");
+    DeviceGuard dg(h->device);
+    hipStream_t st = (hipStream_t)stream;
+    const CtcOut ctc{d_line_off, lines, 0, d_seq, d_seq_len, d_score};
+    if (m == 0) return launch_merge_ctc(nullptr, 0, 1, ctc, nullptr, nullptr, nullptr, st);
+    Workspace ws;
+    if (int e = train_workspace(&ws, d_workspace, workspace_bytes, ppocr_ra_workspace_bytes(h, m), st, kAdaptOp)) return e;
+    return launch_adapt_decode(adapt_cfg(h), h->geom, h->d_rec_h, h->adapters, AdaptLines{d_line_off, lines, d_line_slot}, d_a,
+                               m, h->n, h->k, d_idx, d_maxprob, ctc, ws.p + kAdaptWs, st);
+}
+
+int ppocr_ra_decode(const ppocr_rh_t* h, const float* a, const int64_t* line_off, int64_t lines, const int32_t* line_slot,
+                    int32_t* idx, float* maxprob, int32_t* seq, int64_t* seq_len, float* score) {
+    if (int e = check_adapt_rows(h, 0, lines)) return e;
+    if (lines == 0) return PPOCR_OK;
+    if (int e = check_host_lines(h, line_off, lines, line_slot)) return e;
+    const int64_t m = line_off[lines];
+    if (int e = check_adapt_rows(h, m, lines)) return e;
+    if (!seq_len || !score || (m > 0 && (!a || !seq))) return bad_arg(kAdaptOp, "null pointer");
+    DeviceGuard dg(h->device);
+    const size_t rb = (size_t)m * 4;
+    HostCall hc;
+    if (int e = hc.begin({(size_t)(m * h->k) * 4, (size_t)(lines + 1) * 8, (size_t)lines * 4},
+                         {rb, (size_t)lines * 8, (size_t)lines * 4, idx ? rb : 0, maxprob ? rb : 0},
+                         ppocr_ra_workspace_bytes(h, m), true))
+        return e;
+    if (int e = hc.copy_in({a, line_off, line_slot})) return e;
+    if (int e = ppocr_ra_decode_dev(h, hc.in<float>(0), m, hc.in<int64_t>(1), lines, hc.in<int32_t>(2),
+                                    idx ? hc.out<int32_t>(3) : nullptr, maxprob ? hc.out<float>(4) : nullptr,
+                                    hc.out<int32_t>(0), hc.out<int64_t>(1), hc.out<float>(2), hc.ws(), hc.ws_bytes(),
+                                    hc.stream()))
+        return e;
+    return hc.copy_out({seq, seq_len, score, idx, maxprob});
+}
+
+int ppocr_ra_merge_dev(void* d_w_t, void* d_down, void* d_up, int64_t n, int64_t k, int64_t rank, float scale, int dtype,
+                       void* d_out, void* stream) {
+    if (int e = check_merge(n, k, rank, scale, dtype)) return e;
+    if (!d_w_t || !d_down || !d_up || !d_out) return bad_arg(kAdaptOp, "null pointer");
+    return launch_merge(merge_args(d_w_t, nullptr, d_down, d_up, n, k, rank, scale, dtype, d_out), (hipStream_t)stream);
+}
+
+int ppocr_ra_merge(const float* w_t, const float* down, const float* up, int64_t n, int64_t k, int64_t rank, float scale,
+                   float* out) {
+    if (int e = check_merge(n, k, rank, scale, PPOCR_DTYPE_F32)) return e;
+    if (!w_t || !down || !up || !out) return bad_arg(kAdaptOp, "null pointer");
+    const size_t wb = (size_t)(n * k) * 4;
+    HostCall hc;
+    if (int e = hc.begin({wb, (size_t)(rank * k) * 4, (size_t)(n * rank) * 4}, {wb}, 0)) return e;
+    if (int e = hc.copy_in({w_t, down, up})) return e;
+    if (int e = launch_merge(merge_args(hc.in<float>(0), nullptr, hc.in<float>(1), hc.in<float>(2), n, k, rank, scale,
+                                        PPOCR_DTYPE_F32, hc.out<float>(0)),
+                             hc.stream()))
+        return e;
+    return hc.copy_out({out});
+}
+
+size_t ppocr_ra_merge_workspace_bytes(int64_t n, int64_t k, int64_t rank) {
+    if (check_merge(n, k, rank, 1.0f, PPOCR_DTYPE_F32)) return 0;
+    return kAdaptWs + (size_t)merge_parts(n) * (size_t)(rank * k) * 4;
+}
+
+int ppocr_ra_merge_backward_dev(void* d_dw_t, void* d_down, void* d_up, int64_t n, int64_t k, int64_t rank, float scale,
+                                int dtype, void* d_ddown, void* d_dup, void* d_workspace, size_t workspace_bytes,
+                                void* stream) {
+    if (int e = check_merge(n, k, rank, scale, dtype)) return e;
+    if (!d_ddown && !d_dup) return PPOCR_OK;
+    if (!d_dw_t || !d_down || !d_up) return bad_arg(kAdaptOp, "null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    Workspace ws;
+    float* part = nullptr;
+    if (d_ddown) {
+        if (int e = train_workspace(&ws, d_workspace, workspace_bytes, ppocr_ra_merge_workspace_bytes(n, k, rank), st, kAdaptOp))
+            return e;
+        part = reinterpret_cast<float*>(ws.p + kAdaptWs);
+    }
+    return launch_merge_backward(merge_args(nullptr, d_dw_t, d_down, d_up, n, k, rank, scale, dtype, nullptr), d_ddown, d_dup,
+                                 part, st);
+}
+
+int ppocr_ra_merge_backward(const float* dw_t, const float* down, const float* up, int64_t n, int64_t k, int64_t rank,
+                            float scale, float* ddown, float* dup) {
+    if (int e = check_merge(n, k, rank, scale, PPOCR_DTYPE_F32)) return e;
+    if (!ddown && !dup) return PPOCR_OK;
+    if (!dw_t || !down || !up) return bad_arg(kAdaptOp, "null pointer");
+    const size_t db = (size_t)(rank * k) * 4, ub = (size_t)(n * rank) * 4;
+    HostCall hc;
+    if (int e = hc.begin({(size_t)(n * k) * 4, db, ub}, {ddown ? db : 0, dup ? ub : 0},
+                         ppocr_ra_merge_workspace_bytes(n, k, rank)))
+        return e;
+    if (int e = hc.copy_in({dw_t, down, up})) return e;
+    if (int e = launch_merge_backward(merge_args(nullptr, hc.in<float>(0), hc.in<float>(1), hc.in<float>(2), n, k, rank, scale,
+                                                 PPOCR_DTYPE_F32, nullptr),
+                                      ddown ? hc.out<float>(0) : nullptr, dup ? hc.out<float>(1) : nullptr,
+                                      reinterpret_cast<float*>(hc.ws() + kAdaptWs), hc.stream()))
+        return e;
+    return hc.copy_out({ddown, dup});
+}
+
+int ppocr_policy_loss_dev(const float* d_loss, const float* d_old_loss, const float* d_ref_loss, const int32_t* d_target,
+                          const float* d_adv, int adv_per_row, const int64_t* d_line_off, int64_t lines, int64_t m,
+                          float clip_low, float clip_high, float beta, const float* d_grad, float* d_line_loss,
+                          float* d_line_kl, float* d_line_clipped, float* d_row_grad, void* stream) {
+    if (int e = check_policy(lines, m, clip_low, clip_high, beta)) return e;
+    if (lines > 0 && (!d_line_off || (!d_adv && (m > 0 || !adv_per_row)))) return bad_arg(kPolicyOp, "null pointer");
+    if (lines > 0 && m > 0 && (!d_loss || !d_old_loss)) return bad_arg(kPolicyOp, "null pointer");
+    return launch_policy_loss(LineSteps{d_loss, d_target, d_line_off, lines, m},
+                              PolicyArgs{d_old_loss, d_ref_loss, d_adv, adv_per_row != 0, clip_low, clip_high, beta, d_grad,
+                                         d_line_loss, d_line_kl, d_line_clipped, d_row_grad},
+                              (hipStream_t)stream);
+}
+
+int ppocr_policy_loss(const float* loss, const float* old_loss, const float* ref_loss, const int32_t* target,
+                      const float* adv, int adv_per_row, const int64_t* line_off, int64_t lines, int64_t m, float clip_low,
+                      float clip_high, float beta, const float* grad, float* line_loss, float* line_kl,
+                      float* line_clipped, float* row_grad) {
+    if (int e = check_policy(lines, m, clip_low, clip_high, beta)) return e;
+    if (lines > 0 && (!line_off || (!adv && (m > 0 || !adv_per_row)))) return bad_arg(kPolicyOp, "null pointer");
+    if (lines > 0 && m > 0 && (!loss || !old_loss)) return bad_arg(kPolicyOp, "null pointer");
+    if (lines > 0)
+        if (int e = check_host_steps(kPolicyOp, line_off, lines, m)) return e;
+    const size_t rb = (size_t)m * 4, lb = (size_t)lines * 4, on = lines > 0 ? rb : 0;
+    HostCall hc;
+    if (int e = hc.begin({on, on, ref_loss ? on : 0, target ? on : 0, adv_per_row ? on : lb, lines > 0 ? (size_t)(lines + 1) * 8 : 0,
+                          grad ? lb : 0},
+                         {line_loss ? lb : 0, line_kl ? lb : 0, line_clipped ? lb : 0, row_grad ? rb : 0}, 0))
+        return e;
+    if (int e = hc.copy_in({loss, old_loss, ref_loss, target, adv, line_off, grad})) return e;
+    if (int e = ppocr_policy_loss_dev(hc.in<float>(0), hc.in<float>(1), ref_loss ? hc.in<float>(2) : nullptr,
+                                      target ? hc.in<int32_t>(3) : nullptr, hc.in<float>(4), adv_per_row, hc.in<int64_t>(5), lines,
+                                      m, clip_low, clip_high, beta, grad ? hc.in<float>(6) : nullptr,
+                                      line_loss ? hc.out<float>(0) : nullptr, line_kl ? hc.out<float>(1) : nullptr,
+                                      line_clipped ? hc.out<float>(2) : nullptr, row_grad ? hc.out<float>(3) : nullptr,
+                                      hc.stream()))
+        return e;
+    return hc.copy_out({line_loss, line_kl, line_clipped, row_grad});
+}
+
+int ppocr_preference_loss_dev(const float* d_loss, const float* d_ref_loss, const int32_t* d_target,
+                              const int64_t* d_line_off, int64_t pairs, int64_t m, float beta, float smoothing,
+                              int average, const float* d_grad, float* d_pair_loss, float* d_reward,
+                              float* d_row_grad, void* stream) {
+    if (int e = check_preference(pairs, m, beta, smoothing)) return e;
+    if (pairs > 0 && (!d_line_off || (m > 0 && !d_loss))) return bad_arg(kPreferenceOp, "null pointer");
+    return launch_preference_loss(LineSteps{d_loss, d_target, d_line_off, 2 * pairs, m},
+                                  PreferenceArgs{d_ref_loss, beta, smoothing, average != 0, d_grad, d_pair_loss, d_reward,
+                                                 d_row_grad},
+                                  (hipStream_t)stream);
+}
+
+int ppocr_preference_loss(const float* loss, const float* ref_loss, const int32_t* target, const int64_t* line_off,
+                          int64_t pairs, int64_t m, float beta, float smoothing, int average, const float* grad,
+                          float* pair_loss, float* reward, float* row_grad) {
+    if (int e = check_preference(pairs, m, beta, smoothing)) return e;
+    if (pairs > 0 && (!line_off || (m > 0 && !loss))) return bad_arg(kPreferenceOp, "null pointer");
+    if (pairs > 0)
+        if (int e = check_host_steps(kPreferenceOp, line_off, 2 * pairs, m)) return e;
+    const size_t rb = (size_t)m * 4, pb = (size_t)pairs * 4, on = pairs > 0 ? rb : 0;
+    HostCall hc;
+    if (int e = hc.begin({on, ref_loss ? on : 0, target ? on : 0, pairs > 0 ? (size_t)(2 * pairs + 1) * 8 : 0, grad ? pb : 0},
+                         {pair_loss ? pb : 0, reward ? 2 * pb : 0, row_grad ? rb : 0}, 0))
+        return e;
+    if (int e = hc.copy_in({loss, ref_loss, target, line_off, grad})) return e;
+    if (int e = ppocr_preference_loss_dev(hc.in<float>(0), ref_loss ? hc.in<float>(1) : nullptr,
+                                          target ? hc.in<int32_t>(2) : nullptr, hc.in<int64_t>(3), pairs, m, beta, smoothing,
+                                          average, grad ? hc.in<float>(4) : nullptr, pair_loss ? hc.out<float>(0) : nullptr,
+                                          reward ? hc.out<float>(1) : nullptr, row_grad ? hc.out<float>(2) : nullptr,
+                                          hc.stream()))
+        return e;
+    return hc.copy_out({pair_loss, reward, row_grad});
+}
+
+size_t ppocr_grad_clip_workspace_bytes(const int64_t* sizes, int64_t count) {
+    if (count < 0 || count > kClipMostTensors || (count > 0 && !sizes)) return 0;
+    for (int64_t i = 0; i < count; ++i)
+        if (sizes[i] < 0 || sizes[i] > (1LL << 40)) return 0;
+    return kAdaptWs + (size_t)grad_clip_most_parts(sizes, count) * sizeof(double);
+}
+
+int ppocr_grad_clip_dev(void* const* d_grads, void* const* d_out, const int64_t* sizes, const int32_t* dtypes,
+                        int64_t count, float max_norm, float* d_norm, void* d_workspace, size_t workspace_bytes,
+                        void* stream) try {
+    if (count > 0 && !dtypes) return bad_arg(kClipOp, "null pointer");
+    std::vector<GradTensor> list;
+    if (int e = clip_tensors(d_grads, d_out, sizes, dtypes, count, max_norm, &list)) return e;
+    hipStream_t st = (hipStream_t)stream;
+    Workspace ws;
+    if (int e = train_workspace(&ws, d_workspace, workspace_bytes, ppocr_grad_clip_workspace_bytes(sizes, count), st, kClipOp))
+        return e;
+    return launch_grad_clip(list, max_norm, d_norm, reinterpret_cast<double*>(ws.p + kAdaptWs), st);
+} catch (const std::bad_alloc&) {
+    return PPOCR_ERR_NO_MEMORY;
+}
+
+int ppocr_grad_clip(void* const* grads, void* const* out, const int64_t* sizes, int64_t count, float max_norm,
+                    float* norm) try {
+    std::vector<GradTensor> list;
+    if (int e = clip_tensors(grads, out, sizes, nullptr, count, max_norm, &list)) return e;
+    size_t total = 0;
+    for (const GradTensor& t : list) total += align256((size_t)t.count * 4);
+    HostCall hc;
+    if (int e = hc.begin({total}, {total, 4}, ppocr_grad_clip_workspace_bytes(sizes, count))) return e;
+    size_t at = 0;
+    std::vector<GradTensor> dev = list;
+    for (size_t i = 0; i < list.size(); ++i) {
+        const size_t bytes = (size_t)list[i].count * 4;
+        PPOCR_HIP(hipMemcpyAsync(hc.in<uint8_t>(0) + at, list[i].in, bytes, hipMemcpyHostToDevice, hc.stream()));
+        dev[i].in = hc.in<uint8_t>(0) + at;
+        dev[i].out = hc.out<uint8_t>(0) + at;
+        at += align256(bytes);
+    }
+    if (int e = launch_grad_clip(dev, max_norm, norm ? hc.out<float>(1) : nullptr,
+                                 reinterpret_cast<double*>(hc.ws() + kAdaptWs), hc.stream()))
+        return e;
+    for (size_t i = 0; i < list.size(); ++i)
+        PPOCR_HIP(hipMemcpyAsync(list[i].out, dev[i].out, (size_t)list[i].count * 4, hipMemcpyDeviceToHost, hc.stream()));
+    return hc.copy_out({nullptr, norm});
+} catch (const std::bad_alloc&) {
+    return PPOCR_ERR_NO_MEMORY;
 }
 
 }  // extern "C"

@@ -27,6 +27,10 @@ const SOURCES: &[&str] = &[
     "xent.hip",
     "xent_cfg_1.hip",
     "xent_cfg_2.hip",
+    "adapt.hip",
+    "merge.hip",
+    "sequence_loss.hip",
+    "grad_clip.hip",
     "safetensors.cpp",
     "model_graph.cpp",
 ];

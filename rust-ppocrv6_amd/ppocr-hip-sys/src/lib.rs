@@ -230,4 +230,61 @@ extern "C" {
                                         d_rstd: *const f32, m: i64, d: i64, dtype: c_int, d_dx: *mut c_void,
                                         d_dw: *mut f32, d_db: *mut f32, d_workspace: *mut c_void,
                                         workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    // ---- adapting the head: low-rank adapters of many lines, losses over lines, gradient clipping
+    pub fn ppocr_ra_create(head: *const ppocr_rh_t, slots: i64, max_rank: i64,
+                           out: *mut *mut ppocr_rh_t) -> c_int;
+    pub fn ppocr_ra_destroy(h: *mut ppocr_rh_t);
+    pub fn ppocr_ra_shape(h: *const ppocr_rh_t, slots: *mut i64, max_rank: *mut i64) -> c_int;
+    pub fn ppocr_ra_set(h: *mut ppocr_rh_t, slot: i64, down: *const f32, up: *const f32, rank: i64,
+                        scale: f32) -> c_int;
+    pub fn ppocr_ra_set_dev(h: *mut ppocr_rh_t, slot: i64, d_down: *mut c_void, d_up: *mut c_void, rank: i64,
+                            scale: f32, dtype: c_int, stream: *mut c_void) -> c_int;
+    pub fn ppocr_ra_workspace_bytes(h: *const ppocr_rh_t, m: i64) -> usize;
+    pub fn ppocr_ra_logits(h: *const ppocr_rh_t, a: *const f32, line_off: *const i64, lines: i64,
+                           line_slot: *const i32, out: *mut f32) -> c_int;
+    pub fn ppocr_ra_logits_dev(h: *const ppocr_rh_t, d_a: *const f32, m: i64, d_line_off: *const i64,
+                               lines: i64, d_line_slot: *const i32, d_out: *mut f32, d_workspace: *mut c_void,
+                               workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ppocr_ra_decode(h: *const ppocr_rh_t, a: *const f32, line_off: *const i64, lines: i64,
+                           line_slot: *const i32, idx: *mut i32, maxprob: *mut f32, seq: *mut i32,
+                           seq_len: *mut i64, score: *mut f32) -> c_int;
+    pub fn ppocr_ra_decode_dev(h: *const ppocr_rh_t, d_a: *const f32, m: i64, d_line_off: *const i64,
+                               lines: i64, d_line_slot: *const i32, d_idx: *mut i32, d_maxprob: *mut f32,
+                               d_seq: *mut i32, d_seq_len: *mut i64, d_score: *mut f32,
+                               d_workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ppocr_ra_merge(w_t: *const f32, down: *const f32, up: *const f32, n: i64, k: i64, rank: i64,
+                          scale: f32, out: *mut f32) -> c_int;
+    pub fn ppocr_ra_merge_dev(d_w_t: *mut c_void, d_down: *mut c_void, d_up: *mut c_void, n: i64, k: i64,
+                              rank: i64, scale: f32, dtype: c_int, d_out: *mut c_void,
+                              stream: *mut c_void) -> c_int;
+    pub fn ppocr_ra_merge_workspace_bytes(n: i64, k: i64, rank: i64) -> usize;
+    pub fn ppocr_ra_merge_backward(dw_t: *const f32, down: *const f32, up: *const f32, n: i64, k: i64,
+                                   rank: i64, scale: f32, ddown: *mut f32, dup: *mut f32) -> c_int;
+    pub fn ppocr_ra_merge_backward_dev(d_dw_t: *mut c_void, d_down: *mut c_void, d_up: *mut c_void, n: i64,
+                                       k: i64, rank: i64, scale: f32, dtype: c_int, d_ddown: *mut c_void,
+                                       d_dup: *mut c_void, d_workspace: *mut c_void, workspace_bytes: usize,
+                                       stream: *mut c_void) -> c_int;
+    pub fn ppocr_policy_loss(loss: *const f32, old_loss: *const f32, ref_loss: *const f32, target: *const i32,
+                             adv: *const f32, adv_per_row: c_int, line_off: *const i64, lines: i64, m: i64,
+                             clip_low: f32, clip_high: f32, beta: f32, grad: *const f32, line_loss: *mut f32,
+                             line_kl: *mut f32, line_clipped: *mut f32, row_grad: *mut f32) -> c_int;
+    pub fn ppocr_policy_loss_dev(d_loss: *const f32, d_old_loss: *const f32, d_ref_loss: *const f32,
+                                 d_target: *const i32, d_adv: *const f32, adv_per_row: c_int,
+                                 d_line_off: *const i64, lines: i64, m: i64, clip_low: f32, clip_high: f32,
+                                 beta: f32, d_grad: *const f32, d_line_loss: *mut f32, d_line_kl: *mut f32,
+                                 d_line_clipped: *mut f32, d_row_grad: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn ppocr_preference_loss(loss: *const f32, ref_loss: *const f32, target: *const i32,
+                                 line_off: *const i64, pairs: i64, m: i64, beta: f32, smoothing: f32,
+                                 average: c_int, grad: *const f32, pair_loss: *mut f32, reward: *mut f32,
+                                 row_grad: *mut f32) -> c_int;
+    pub fn ppocr_preference_loss_dev(d_loss: *const f32, d_ref_loss: *const f32, d_target: *const i32,
+                                     d_line_off: *const i64, pairs: i64, m: i64, beta: f32, smoothing: f32,
+                                     average: c_int, d_grad: *const f32, d_pair_loss: *mut f32,
+                                     d_reward: *mut f32, d_row_grad: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn ppocr_grad_clip_workspace_bytes(sizes: *const i64, count: i64) -> usize;
+    pub fn ppocr_grad_clip(grads: *const *mut c_void, out: *const *mut c_void, sizes: *const i64, count: i64,
+                           max_norm: f32, norm: *mut f32) -> c_int;
+    pub fn ppocr_grad_clip_dev(d_grads: *const *mut c_void, d_out: *const *mut c_void, sizes: *const i64,
+                               dtypes: *const i32, count: i64, max_norm: f32, d_norm: *mut f32,
+                               d_workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
 }

@@ -25,7 +25,8 @@ from ._lib import (DTYPE_BF16, DTYPE_F32, MODE_AUTO, MODE_BF16X1, MODE_BF16X2, M
 __all__ = [
     "OcrError", "QuantizedWeight", "RecHead", "RecNeck", "CtcDecoder", "find_rec_head", "matmul_quantized_b", "matmul_transposed_b",
     "softmax", "softmax_inplace", "cross_entropy", "cross_entropy_backward", "distill", "distill_backward", "topk",
-    "layer_norm", "layer_norm_backward", "DTYPE_F32", "DTYPE_BF16", "MODE_FP32_FMA", "MODE_BF16X1", "MODE_BF16X2", "MODE_BF16X3", "MODE_F16X2", "MODE_AUTO",
+    "layer_norm", "layer_norm_backward", "AdaptedHead", "merge_adapter", "merge_adapter_backward", "policy_loss",
+    "preference_loss", "clip_gradients", "DTYPE_F32", "DTYPE_BF16", "MODE_FP32_FMA", "MODE_BF16X1", "MODE_BF16X2", "MODE_BF16X3", "MODE_F16X2", "MODE_AUTO",
 ]
 
 
@@ -685,3 +686,146 @@ def layer_norm_backward(dy, x, w, mean, rstd):
     _check(_lib.lib().ppocr_layernorm_backward(_ptr(dy), _ptr(x), _ptr(w), _ptr(mean), _ptr(rstd), m, d, _ptr(dx),
                                                _ptr(dw), _ptr(db)))
     return dx, dw, db
+
+
+# ---------------------------------------------------------------- adapting the head
+
+
+class AdaptedHead(RecHead):
+    """A head with places for low-rank adapters, on the weights of `head`.
+
+    set_adapter puts one into a slot; logits_lines and decode_lines run each text line under the slot
+    that it names (negative: the head alone).  The other methods are the head's own, without adapters."""
+
+    def __init__(self, head, slots, max_rank):
+        self._h = ctypes.c_void_p()
+        self.quantized, self.n, self.k, self.default_mode = head.quantized, head.n, head.k, head.default_mode
+        _check(_lib.lib().ppocr_ra_create(head.handle, int(slots), int(max_rank), ctypes.byref(self._h)))
+        self.slots, self.max_rank = int(slots), int(max_rank)
+
+    def set_adapter(self, slot, down, up, scale=1.0):
+        """down [rank, k] and up [n, rank]: lines of this slot get scale * up (down a) added to their logits."""
+        down, up = _f32(down), _f32(up)
+        if down.ndim != 2 or up.ndim != 2 or down.shape[1] != self.k or up.shape != (self.n, down.shape[0]):
+            raise OcrError("LowRankAdapter", f"expected down [rank, {self.k}] and up [{self.n}, rank], got "
+                                             f"{list(down.shape)} and {list(up.shape)}")
+        _check(_lib.lib().ppocr_ra_set(self._h, int(slot), _ptr(down), _ptr(up), down.shape[0], float(scale)))
+
+    def clear_adapter(self, slot):
+        _check(_lib.lib().ppocr_ra_set(self._h, int(slot), None, None, 0, 1.0))
+
+    def _lines(self, a, line_off, line_slot):
+        a = _f32(a)
+        line_off = np.ascontiguousarray(line_off, dtype=np.int64)
+        line_slot = np.ascontiguousarray(line_slot, dtype=np.int32)
+        lines = line_off.size - 1
+        if a.ndim != 2 or a.shape[1] != self.k:
+            raise OcrError("LowRankAdapter", f"expected rows of {self.k} values, got shape {list(a.shape)}")
+        if lines < 0 or line_off[-1] != a.shape[0] or line_slot.shape != (lines,):
+            raise OcrError("LowRankAdapter", f"line offsets and slots of {line_slot.size} lines do not cover {a.shape[0]} rows")
+        return a, line_off, lines, line_slot
+
+    def logits_lines(self, a, line_off, line_slot):
+        """Logits [m, n] of the lines' rows, each line under its slot."""
+        a, line_off, lines, line_slot = self._lines(a, line_off, line_slot)
+        out = np.empty((a.shape[0], self.n), np.float32)
+        _check(_lib.lib().ppocr_ra_logits(self._h, _ptr(a), _ptr(line_off), lines, _ptr(line_slot), _ptr(out)))
+        return out
+
+    def decode_lines(self, a, line_off, line_slot):
+        """The lines decoded each under its slot; the result is RecHead.decode's."""
+        a, line_off, lines, line_slot = self._lines(a, line_off, line_slot)
+        m = a.shape[0]
+        idx, maxprob, seq = np.empty(m, np.int32), np.empty(m, np.float32), np.empty(m, np.int32)
+        seq_len, score = np.zeros(lines, np.int64), np.zeros(lines, np.float32)
+        _check(_lib.lib().ppocr_ra_decode(self._h, _ptr(a), _ptr(line_off), lines, _ptr(line_slot), _ptr(idx), _ptr(maxprob),
+                                          _ptr(seq), _ptr(seq_len), _ptr(score)))
+        return {"idx": idx, "maxprob": maxprob, "seq_len": seq_len, "score": score,
+                "seqs": [seq[line_off[i]:line_off[i] + seq_len[i]].copy() for i in range(lines)]}
+
+
+def _adapter_args(w, down, up):
+    w, down, up = _f32(w), _f32(down), _f32(up)
+    if w.ndim != 2 or down.ndim != 2 or down.shape[1] != w.shape[1] or up.shape != (w.shape[0], down.shape[0]):
+        raise OcrError("LowRankAdapter", f"expected a weight [n, k], down [rank, k] and up [n, rank], got "
+                                         f"{list(w.shape)}, {list(down.shape)} and {list(up.shape)}")
+    return w, down, up
+
+
+def merge_adapter(w_t, down, up, scale=1.0):
+    """w_t + scale up down [n, k]: the weight that an adapter is trained under."""
+    w_t, down, up = _adapter_args(w_t, down, up)
+    out = np.empty_like(w_t)
+    _check(_lib.lib().ppocr_ra_merge(_ptr(w_t), _ptr(down), _ptr(up), *w_t.shape, down.shape[0], float(scale), _ptr(out)))
+    return out
+
+
+def merge_adapter_backward(dw_t, down, up, scale=1.0):
+    """(ddown [rank, k], dup [n, rank]) of merge_adapter, from the merged weight's gradient."""
+    dw_t, down, up = _adapter_args(dw_t, down, up)
+    ddown, dup = np.empty_like(down), np.empty_like(up)
+    _check(_lib.lib().ppocr_ra_merge_backward(_ptr(dw_t), _ptr(down), _ptr(up), *dw_t.shape, down.shape[0], float(scale),
+                                              _ptr(ddown), _ptr(dup)))
+    return ddown, dup
+
+
+def _steps(op, loss, others, target, line_off):
+    loss = _f32(loss)
+    if loss.ndim != 1:
+        raise OcrError(op, f"expected the losses of [m] steps, got shape {list(loss.shape)}")
+    m = loss.shape[0]
+    others = [None if x is None else _per_row(op, x, (m,), np.float32, "losses") for x in others]
+    target = None if target is None else _per_row(op, target, (m,), np.int32, "targets")
+    line_off = np.ascontiguousarray(line_off, dtype=np.int64)
+    if line_off.ndim != 1 or line_off.size < 1:
+        raise OcrError(op, f"expected line offsets [lines + 1], got shape {list(line_off.shape)}")
+    return loss, others, target, line_off
+
+
+def policy_loss(loss, old_loss, adv, line_off, target=None, ref_loss=None, clip_low=0.2, clip_high=0.2, beta=0.0, grad=None):
+    """(line_loss, line_kl, line_clipped, row_grad) of the clipped policy loss over lines of steps, from the
+    steps' cross entropies now, when they were sampled and under a reference (None: no divergence term).
+    adv: the advantages of the lines, or of the steps.  row_grad is what cross_entropy_backward takes as
+    grad; grad [lines] is the gradient by line_loss (None: 1)."""
+    op = "PolicyLoss"
+    loss, (old, ref), target, line_off = _steps(op, loss, (old_loss, ref_loss), target, line_off)
+    m, lines = loss.shape[0], line_off.size - 1
+    adv = _f32(adv)
+    if adv.shape not in ((lines,), (m,)):
+        raise OcrError(op, f"expected advantages of {lines} lines or {m} steps, got shape {list(adv.shape)}")
+    per_row = adv.shape != (lines,)
+    grad = None if grad is None else _per_row(op, grad, (lines,), np.float32, "grad")
+    out = [np.empty(lines, np.float32) for _ in range(3)] + [np.empty(m, np.float32)]
+    _check(_lib.lib().ppocr_policy_loss(_ptr(loss), _ptr(old), _ptr(ref), _ptr(target), _ptr(adv), int(per_row), _ptr(line_off),
+                                        lines, m, float(clip_low), float(clip_high), float(beta), _ptr(grad),
+                                        *(_ptr(o) for o in out)))
+    return tuple(out)
+
+
+def preference_loss(loss, ref_loss, line_off, target=None, beta=0.1, smoothing=0.0, average=False, grad=None):
+    """(pair_loss [pairs], reward [pairs, 2], row_grad [m]) of the preference for line 2p over line 2p + 1,
+    from the steps' cross entropies and a reference's (None: no reference)."""
+    op = "PreferenceLoss"
+    loss, (ref,), target, line_off = _steps(op, loss, (ref_loss,), target, line_off)
+    m, lines = loss.shape[0], line_off.size - 1
+    if lines % 2:
+        raise OcrError(op, f"expected two lines a pair, got {lines} lines")
+    pairs = lines // 2
+    grad = None if grad is None else _per_row(op, grad, (pairs,), np.float32, "grad")
+    pair_loss, reward, row_grad = np.empty(pairs, np.float32), np.empty((pairs, 2), np.float32), np.empty(m, np.float32)
+    _check(_lib.lib().ppocr_preference_loss(_ptr(loss), _ptr(ref), _ptr(target), _ptr(line_off), pairs, m, float(beta),
+                                            float(smoothing), int(average), _ptr(grad), _ptr(pair_loss), _ptr(reward),
+                                            _ptr(row_grad)))
+    return pair_loss, reward, row_grad
+
+
+def clip_gradients(grads, max_norm):
+    """(clipped, norm): the tensors times min(1, max_norm / norm), norm being that of all of them together."""
+    grads = [_f32(g) for g in grads]
+    out = [np.empty_like(g) for g in grads]
+    count = len(grads)
+    norm = np.empty(1, np.float32)
+    _check(_lib.lib().ppocr_grad_clip((ctypes.c_void_p * count)(*[g.ctypes.data for g in grads]),
+                                      (ctypes.c_void_p * count)(*[o.ctypes.data for o in out]),
+                                      (ctypes.c_int64 * count)(*[g.size for g in grads]), count, float(max_norm), _ptr(norm)))
+    return out, float(norm[0])

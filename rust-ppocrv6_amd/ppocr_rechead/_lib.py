@@ -114,6 +114,33 @@ SIGNATURES = {
     "ppocr_layernorm_workspace_bytes": (_sz, [_i64, _i64]),
     "ppocr_layernorm_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp]),
     "ppocr_layernorm_backward_dev": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ppocr_ra_create": (_int, [_vp, _i64, _i64, ctypes.POINTER(_vp)]),
+    "ppocr_ra_destroy": (None, [_vp]),
+    "ppocr_ra_shape": (_int, [_vp, ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
+    "ppocr_ra_set": (_int, [_vp, _i64, _vp, _vp, _i64, ctypes.c_float]),
+    "ppocr_ra_set_dev": (_int, [_vp, _i64, _vp, _vp, _i64, ctypes.c_float, _int, _vp]),
+    "ppocr_ra_workspace_bytes": (_sz, [_vp, _i64]),
+    "ppocr_ra_logits": (_int, [_vp, _vp, _vp, _i64, _vp, _vp]),
+    "ppocr_ra_logits_dev": (_int, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _sz, _vp]),
+    "ppocr_ra_decode": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ppocr_ra_decode_dev": (_int, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ppocr_ra_merge": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, ctypes.c_float, _vp]),
+    "ppocr_ra_merge_dev": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, ctypes.c_float, _int, _vp, _vp]),
+    "ppocr_ra_merge_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "ppocr_ra_merge_backward": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, ctypes.c_float, _vp, _vp]),
+    "ppocr_ra_merge_backward_dev": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, ctypes.c_float, _int, _vp, _vp, _vp, _sz,
+                                           _vp]),
+    "ppocr_policy_loss": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, ctypes.c_float, ctypes.c_float,
+                                 ctypes.c_float, _vp, _vp, _vp, _vp, _vp]),
+    "ppocr_policy_loss_dev": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, ctypes.c_float, ctypes.c_float,
+                                     ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ppocr_preference_loss": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, ctypes.c_float, _int, _vp, _vp,
+                                     _vp, _vp]),
+    "ppocr_preference_loss_dev": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, ctypes.c_float, _int, _vp, _vp,
+                                         _vp, _vp, _vp]),
+    "ppocr_grad_clip_workspace_bytes": (_sz, [_vp, _i64]),
+    "ppocr_grad_clip": (_int, [_vp, _vp, _vp, _i64, ctypes.c_float, _vp]),
+    "ppocr_grad_clip_dev": (_int, [_vp, _vp, _vp, _vp, _i64, ctypes.c_float, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None
