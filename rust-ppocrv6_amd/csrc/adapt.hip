@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256) void clear_kernel(u32x4* p, int64_t count) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) p[i] = u32x4{0, 0, 0, 0};
 }
 __global__ void clear_meta_kernel(AdapterMeta* meta, int count) {
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < count; i += gridDim.x * blockDim.x) meta[i] = AdapterMeta{1.0f, kTop};
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < count; i += gridDim.x * blockDim.x) meta[i] = AdapterMeta{0};
 }
 
 template <typename T>
@@ -92,7 +92,8 @@ __device__ __forceinline__ int down_exp(const unsigned* range, int t) {
     const float s = __uint_as_float(range[t]);
     return s > 0.0f && s < INFINITY ? ilogbf(s) + 1 : 0;
 }
-// How far the rows of this slot are scaled down so that the largest up value fits fp16.
+// How far the head's products are scaled down beside the adapter's, so that the largest up value fits fp16: 0
+// unless the adapter's largest products are 2^7 above the head's.
 __device__ __forceinline__ int slot_shift(const unsigned* range, int rank) {
     int s = 0;
     for (int t = 0; t < rank; ++t) {
@@ -119,10 +120,7 @@ __global__ __launch_bounds__(256) void down_record_kernel(const T* __restrict__ 
         p[(g * 32 + i) * 8 + e] = hi;
         p[((G + g) * 32 + i) * 8 + e] = half_bits(v - (float)__builtin_bit_cast(_Float16, hi));
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        const int s = slot_shift(range, rank);
-        *meta = AdapterMeta{ldexpf(1.0f, s - kDownShift), kTop - s};
-    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *meta = AdapterMeta{slot_shift(range, rank)};
 }
 
 // The rank that element e of lane half h holds in 16-rank step s of an operand: the order in which
@@ -288,7 +286,7 @@ __device__ __forceinline__ void load_rows(const AdaptLaunch& x, int64_t row, int
     static_assert(A::NL == D::NL, "both products read the rows in the same pieces");
     float raw[A::NL][8];
     act_issue<C, G>(x.a, row, x.k, x.vec, h, raw);
-    const AdapterMeta meta = x.meta[slot];
+    const int shift = x.meta[slot].shift;
     float top = 0.0f;
     bool odd = false;
 #pragma unroll
@@ -300,10 +298,11 @@ __device__ __forceinline__ void load_rows(const AdaptLaunch& x, int64_t row, int
         }
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     odd |= (bool)__shfl_xor((int)odd, 32, 64);
+    // the row's largest value comes to below 2^kTop, in the head's products 2^-shift of it
     int ex = 0;
-    if (top > 0.0f && !odd) ex = max(min(meta.top - 1 - ilogbf(top), 126), -126);
-    o.inv = ldexpf(1.0f, -ex);
-    const float to = ldexpf(1.0f, ex);
+    if (top > 0.0f && !odd) ex = max(min(kTop - 1 - ilogbf(top), 126), shift - 126);
+    o.inv = ldexpf(1.0f, shift - ex);
+    const float to = ldexpf(1.0f, ex), lower = ldexpf(1.0f, -shift);
 #pragma unroll
     for (int l = 0; l < A::NL; ++l)
 #pragma unroll
@@ -323,12 +322,16 @@ __device__ __forceinline__ void load_rows(const AdaptLaunch& x, int64_t row, int
             for (int y = 0; y < 2 && 2 * b + y < NR; ++y)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float v = u[8 * y + e] * meta.ushift;
+                    const float v = u[8 * y + e] * (1.0f / (1 << kDownShift));
                     o.uhi[2 * b + y][e] = split_term<true>(v, 0);
                     o.ulo[2 * b + y][e] = split_term<true>(v, 1);
                 }
         }
     }
+#pragma unroll
+    for (int l = 0; l < A::NL; ++l)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[l][e] *= lower;
     act_split_all<C, G>(raw, h, o.a, none, none2);
 }
 

@@ -9,8 +9,7 @@ constexpr int kAdaptMostSlots = 4096;
 
 // What the kernels need of a slot's adapter (device memory, written when the slot is set).
 struct AdapterMeta {
-    float ushift;  // power of two between the products with the down record and the terms of u
-    int top;       // rows are scaled to below 2^top
+    int shift;  // the head's products are scaled by 2^-shift beside the adapter's
 };
 
 // The adapters of a head: records in device memory, one set a slot, and one of zeros behind the last slot
