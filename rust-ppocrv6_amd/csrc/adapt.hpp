@@ -60,8 +60,8 @@ struct MergeArgs {
     void* out;
 };
 int launch_merge(const MergeArgs& x, hipStream_t st);
-// Workgroups of the backward pass, each with a sum of ddown of its own: part [parts][rank][k].
-int merge_parts(int64_t n);
+// Groups of rows of the backward pass, each with a sum of ddown of its own: part [parts][rank][k].
+int merge_parts(int64_t n, int64_t k);
 int launch_merge_backward(const MergeArgs& x, void* ddown, void* dup, float* part, hipStream_t st);
 
 }  // namespace ppocr

@@ -2378,7 +2378,7 @@ int ppocr_ra_merge(const float* w_t, const float* down, const float* up, int64_t
 
 size_t ppocr_ra_merge_workspace_bytes(int64_t n, int64_t k, int64_t rank) {
     if (check_merge(n, k, rank, 1.0f, PPOCR_DTYPE_F32)) return 0;
-    return kAdaptWs + (size_t)merge_parts(n) * (size_t)(rank * k) * 4;
+    return kAdaptWs + (size_t)merge_parts(n, k) * (size_t)(rank * k) * 4;
 }
 
 int ppocr_ra_merge_backward_dev(void* d_dw_t, void* d_down, void* d_up, int64_t n, int64_t k, int64_t rank, float scale,
