@@ -180,16 +180,29 @@ struct Plan {
 };
 int64_t plan_units(int64_t m, int64_t groups) { return m / kUnit + groups; }
 
-// One workgroup.  A row's line is the last whose offset is not above it, so each row is placed once
-// whatever the offsets hold; rows of no line, and of lines that name no slot, form a group of their own.
-// Rows of a group are placed in any order: no row's result depends on its place.
-__global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int slots, int most_units, Plan plan) {
+// One workgroup.  Rows of a group are placed in any order: no row's result depends on its place.  Rows of no
+// line, and of lines that name no slot, form a group of their own.
+//
+// Where the offsets rise, whole lines are counted and placed (a wave a line, or a thread a line where they are
+// short; the rows before the first and behind the last line are two lines more).  Otherwise each row looks for
+// its line, the last whose offset is not above it, so that each is placed once whatever the offsets hold.
+// 256 lines of 120: PLANUS us, by rows 95.
+__global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int slots, Plan plan) {
     extern __shared__ int groups[];
     int* count = groups;              // [slots + 1] rows of a group
     int* first = groups + slots + 1;  // its first unit
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int g = tid; g <= slots; g += 1024) count[g] = 0;
-    __syncthreads();
+    bool rising = true;
+    for (int64_t i = tid; i <= lines.lines; i += 1024) {
+        const int64_t o = lines.off[i];
+        rising &= o >= 0 && o <= m && (i == 0 || lines.off[i - 1] <= o);
+    }
+    rising = __syncthreads_and(rising);
+    auto group_of_line = [&](int64_t i) -> int {
+        const int s = lines.slot[i];
+        return s >= 0 && s < slots ? s : slots;
+    };
     auto group_of = [&](int r) -> int {
         int64_t lo = 0, hi = lines.lines;  // off[lo] <= r < off[hi], if offsets rise
         if (hi == 0 || lines.off[0] > r) return slots;
@@ -199,10 +212,9 @@ __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int
             else hi = mid;
         }
         if (lines.off[lo + 1] <= r) return slots;
-        const int s = lines.slot[lo];
-        return s >= 0 && s < slots ? s : slots;
+        return group_of_line(lo);
     };
-    // a slot for each lane's row in its group: lanes of one group together where the wave's rows all have it
+    // a place in its group for each lane's row: lanes of one group together where the wave's rows all have it
     auto take = [&](bool on, int g) -> int {
         const unsigned long long mask = __ballot(on);
         if (mask == 0ull) return 0;
@@ -215,9 +227,25 @@ __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int
         }
         return on ? atomicAdd(&count[g], 1) : 0;
     };
-    for (int r0 = 0; r0 < m; r0 += 1024) {
-        const int r = r0 + tid;
-        (void)take(r < m, r < m ? group_of(r) : 0);
+    // Line i of lines.lines + 2: its rows and its group.
+    struct Span {
+        int lo, hi, g;
+    };
+    auto span = [&](int64_t i) {
+        if (i < lines.lines) return Span{(int)lines.off[i], (int)lines.off[i + 1], group_of_line(i)};
+        if (i == lines.lines) return Span{0, lines.lines ? (int)lines.off[0] : m, slots};
+        return Span{lines.lines ? (int)lines.off[lines.lines] : m, m, slots};
+    };
+    if (rising) {
+        for (int64_t i = tid; i < lines.lines + 2; i += 1024) {
+            const Span s = span(i);
+            if (s.hi > s.lo) atomicAdd(&count[s.g], s.hi - s.lo);
+        }
+    } else {
+        for (int r0 = 0; r0 < m; r0 += 1024) {
+            const int r = r0 + tid;
+            (void)take(r < m, r < m ? group_of(r) : 0);
+        }
     }
     __syncthreads();
     if (tid < 64) {
@@ -245,11 +273,39 @@ __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int
         count[g] = 0;
     }
     __syncthreads();
-    for (int r0 = 0; r0 < m; r0 += 1024) {
-        const int r = r0 + tid;
-        const int g = r < m ? group_of(r) : 0;
-        const int at = take(r < m, g);
-        if (r < m) plan.rows[first[g] * kUnit + at] = r;
+    if (rising) {
+        const bool brief = m / max(lines.lines, (int64_t)1) < 16;
+        for (int64_t i = brief ? tid : wave; i < lines.lines + 2; i += brief ? 1024 : 16) {
+            const Span s = span(i);
+            if (s.hi <= s.lo) continue;
+            if (brief && s.hi - s.lo < 1024) {
+                int* to = plan.rows + first[s.g] * kUnit + atomicAdd(&count[s.g], s.hi - s.lo);
+                for (int r = s.lo; r < s.hi; ++r) to[r - s.lo] = r;
+            } else if (!brief) {
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&count[s.g], s.hi - s.lo);
+                int* to = plan.rows + first[s.g] * kUnit + __shfl(at, 0, 64);
+                for (int r = s.lo + lane; r < s.hi; r += 64) to[r - s.lo] = r;
+            }
+        }
+        if (brief) {
+            // the few long lines among brief ones, by waves
+            for (int64_t i = wave; i < lines.lines + 2; i += 16) {
+                const Span s = span(i);
+                if (s.hi - s.lo < 1024) continue;
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&count[s.g], s.hi - s.lo);
+                int* to = plan.rows + first[s.g] * kUnit + __shfl(at, 0, 64);
+                for (int r = s.lo + lane; r < s.hi; r += 64) to[r - s.lo] = r;
+            }
+        }
+    } else {
+        for (int r0 = 0; r0 < m; r0 += 1024) {
+            const int r = r0 + tid;
+            const int g = r < m ? group_of(r) : 0;
+            const int at = take(r < m, g);
+            if (r < m) plan.rows[first[g] * kUnit + at] = r;
+        }
     }
 }
 
@@ -275,7 +331,8 @@ template <int C, int G, int NR>
 struct RowOperands {
     u16x8 a[Geo<C, G>::S];
     u16x8 uhi[NR], ulo[NR];
-    float inv;  // the row's power of two undone
+    float inv;    // the row's power of two undone
+    bool scaled;  // some row of the wave has one
 };
 
 // Row `row` (its lane's of 32) scaled, split, and multiplied with its adapter's down.
@@ -298,9 +355,12 @@ __device__ __forceinline__ void load_rows(const AdaptLaunch& x, int64_t row, int
         }
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     odd |= (bool)__shfl_xor((int)odd, 32, 64);
-    // the row's largest value comes to below 2^kTop, in the head's products 2^-shift of it
+    // The row's largest value comes to below 2^kTop, in the head's products 2^-shift of it.  A wave whose rows'
+    // largest values all lie in [0.5, 2^kTop) leaves them as they are: the low halves, whose smallest step is
+    // 2^-24, then still hold 24 bits of a row's largest value, and no logit needs the power undone.
+    o.scaled = shift != 0 || __any(!(top >= 0.5f && top < (float)(1 << kTop)));
     int ex = 0;
-    if (top > 0.0f && !odd) ex = max(min(kTop - 1 - ilogbf(top), 126), shift - 126);
+    if (o.scaled && top > 0.0f && !odd) ex = max(min(kTop - 1 - ilogbf(top), 126), shift - 126);
     o.inv = ldexpf(1.0f, shift - ex);
     const float to = ldexpf(1.0f, ex), lower = ldexpf(1.0f, -shift);
 #pragma unroll
@@ -349,24 +409,27 @@ __device__ __forceinline__ void load_up(const uint8_t* up, int tile, int lane, u
 // ---------------------------------------------------------------- statistics
 // One wave, 32 rows (columns of the matrix product), 32 classes a tile; the head's tiles through a ring in
 // LDS as in the head's statistics pass, the products of tile j + 1 interleaved with the epilogue of tile j.
-template <int P>
+// PLAIN: the rows have no powers of two, and the sums no reference (no logit beyond 2^64 so far): a multiplication and
+// a subtraction less for each of the wave's logits.
+template <int P, bool PLAIN>
 __device__ __forceinline__ void adapt_piece(f32x16 (&t)[1], float inv, const float* __restrict__ ep, int h, int j, f32x4 (&cs)[2],
                                             f32x4 (&cb)[2], const float (&ref)[1], float (&best)[1], int (&bt)[1], f32x4* save,
                                             EpiState<1>& st) {
-    if constexpr (P < 12 && P % 3 == 0) {
+    if constexpr (!PLAIN && P < 12 && P % 3 == 0) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[0][4 * (P / 3) + e] *= inv;
     }
-    epi_piece<P, 1, false>(t, ep, h, j, cs, cb, ref, best, bt, save, st);
+    epi_piece<P, 1, PLAIN>(t, ep, h, j, cs, cb, ref, best, bt, save, st);
+    if constexpr (PLAIN && P == epi_pieces<1>() - 1) st.need = (best[0] != -INFINITY) & (__builtin_fabsf(best[0]) > 64.0f);
 }
-template <int H, int x>
+template <int H, int x, bool PLAIN>
 __device__ __forceinline__ void adapt_pieces(f32x16 (&t)[1], float inv, const float* __restrict__ ep, int h, int j, f32x4 (&cs)[2],
                                              f32x4 (&cb)[2], const float (&ref)[1], float (&best)[1], int (&bt)[1], f32x4* save,
                                              EpiState<1>& st) {
     constexpr int NP = epi_pieces<1>();
     constexpr int p0 = x * NP / H, p1 = (x + 1) * NP / H;
     [&]<int... I>(std::integer_sequence<int, I...>) {
-        (adapt_piece<p0 + I>(t, inv, ep, h, j, cs, cb, ref, best, bt, save, st), ...);
+        (adapt_piece<p0 + I, PLAIN>(t, inv, ep, h, j, cs, cb, ref, best, bt, save, st), ...);
     }(std::make_integer_sequence<int, p1 - p0>{});
 }
 
@@ -419,7 +482,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void adapt_stats_kernel(AdaptLaunch
         load_up<NR>(up, min(t0 + 1, t1 - 1), lane, whi, wlo);
 #pragma unroll
         for (int s = 0; s < S; ++s) acc_a[0] = mfma16<true>(weight_frag<C, G>(lds, s, lb, i * 16, h), o.a[s], acc_a[0]);
-        auto step = [&]<int R>(int j, f32x16 (&accE)[1], f32x16 (&accM)[1]) {
+        bool plain = !o.scaled;  // the same for the wave
+        auto step_as = [&]<int R, bool PLAIN>(int j, f32x16 (&accE)[1], f32x16 (&accM)[1]) __attribute__((always_inline)) {
             constexpr unsigned rel = (unsigned)R;  // (j - t0) % kRing
             const uint8_t* bufn = lds + ((rel + 1) & (kRing - 1)) * GE::BUF;
             const float* ep = reinterpret_cast<const float*>(lds + (rel & (kRing - 1)) * GE::BUF + GE::FRAG);
@@ -432,10 +496,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void adapt_stats_kernel(AdaptLaunch
             EpiState<1> st;
             st.need = false;
             accM[0] = f32x16{};
-            // the adapter's products first: their operands' registers then take the next tile's, which has
-            // the rest of the step to arrive.  Those loads are issued before the staged ones: the barrier's
-            // count of loads in flight stays that of the staged ones.
-            adapter_products(accM[0]);
+            // products 0 .. 3 NR - 1: the adapter's, the rest the head's; the epilogue's pieces between them all
+            constexpr int STEPS = S + 3 * NR;
+            [&]<int... s>(std::integer_sequence<int, s...>) {
+                ([&] {
+                    constexpr int r = s / 3, y = s % 3;
+                    accM[0] = mfma16<true>(y == 2 ? wlo[r] : whi[r], y == 1 ? o.ulo[r] : o.uhi[r], accM[0]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    adapt_pieces<2 * STEPS, 2 * s, PLAIN>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
+                    adapt_pieces<2 * STEPS, 2 * s + 1, PLAIN>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
+                    __builtin_amdgcn_sched_barrier(0);
+                }(), ...);
+            }(std::make_integer_sequence<int, 3 * NR>{});
+            // The adapter's operands' registers take the next tile's, which has the rest of the step to arrive.  Those
+            // loads are issued before the staged ones: the barrier's count of loads in flight stays that of the staged.
             load_up<NR>(up, min(j + 2, t1 - 1), lane, whi, wlo);
             stage_direct<GE::REC, NT>(x.rec + (size_t)min(j + kRing - 1, t1 - 1) * GE::REC,
                                       lds + ((rel + kRing - 1) & (kRing - 1)) * GE::BUF, tid);
@@ -443,16 +517,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void adapt_stats_kernel(AdaptLaunch
             frag_prefetch_first<C, G, kPrefetch>(wq, bufn, lb, i * 16, h);
             [&]<int... s>(std::integer_sequence<int, s...>) {
                 ([&] {
+                    constexpr int g = s + 3 * NR;
                     accM[0] = mfma16<true>(frag_of<C, G, kPrefetch, s>(wq), o.a[s], accM[0]);
                     __builtin_amdgcn_sched_barrier(0);
-                    adapt_pieces<2 * S, 2 * s>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
+                    adapt_pieces<2 * STEPS, 2 * g, PLAIN>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
                     frag_prefetch_after<C, G, kPrefetch, s>(wq, bufn, lb, i * 16, h);
                     __builtin_amdgcn_sched_barrier(0);
-                    adapt_pieces<2 * S, 2 * s + 1>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
+                    adapt_pieces<2 * STEPS, 2 * g + 1, PLAIN>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
                     __builtin_amdgcn_sched_barrier(0);
                 }(), ...);
             }(std::make_integer_sequence<int, S>{});
             if (__any(st.need)) {
+                plain = false;
                 if (best[0] != -INFINITY && __builtin_fabsf(best[0] - ref[0]) > 64.0f) {
                     const float nr = best[0];
                     sum = (sum == 0.0f) ? 0.0f : sum * __builtin_amdgcn_exp2f(ref[0] - nr);
@@ -466,9 +542,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void adapt_stats_kernel(AdaptLaunch
             sum += st.tsum[0];
             ring_barrier<kLead>();
         };
-        auto step_of = [&]<int R>(int jj) {
-            if constexpr (R % 2 == 0) step.template operator()<R>(jj, acc_a, acc_b);
-            else step.template operator()<R>(jj, acc_b, acc_a);
+        auto step_of = [&]<int R>(int jj) __attribute__((always_inline)) {
+            auto both = [&](f32x16 (&accE)[1], f32x16 (&accM)[1]) __attribute__((always_inline)) {
+                if (plain) step_as.template operator()<R, true>(jj, accE, accM);
+                else step_as.template operator()<R, false>(jj, accE, accM);
+            };
+            if constexpr (R % 2 == 0) both(acc_a, acc_b);
+            else both(acc_b, acc_a);
         };
         int j = t0;
         for (; j + kRing - 1 < t1; j += kRing)
@@ -635,7 +715,7 @@ int make_plan(const Adapters& ad, const AdaptLines& lines, int64_t m, const Adap
               hipStream_t st) {
     *plan = Plan{reinterpret_cast<int*>(ws + L.units), reinterpret_cast<int*>(ws + L.rows), reinterpret_cast<int*>(ws + L.slot)};
     *units = plan_units(m, std::min<int64_t>(std::min<int64_t>(ad.slots, lines.lines) + 1, m));
-    plan_kernel<<<1, 1024, (size_t)(ad.slots + 1) * 8, st>>>(lines, (int)m, ad.slots, (int)*units, *plan);
+    plan_kernel<<<1, 1024, (size_t)(ad.slots + 1) * 8, st>>>(lines, (int)m, ad.slots, *plan);
     PPOCR_HIP(hipGetLastError());
     return PPOCR_OK;
 }
