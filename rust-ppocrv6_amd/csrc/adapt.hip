@@ -27,7 +27,6 @@ size_t Adapters::up_bytes() const { return (size_t)tiles * 2 * steps * 1024; }
 
 namespace {
 
-constexpr int kUnit = 32;     // rows of a wave
 constexpr int kWaves = 4;
 constexpr int kDownShift = 10;  // down's halves are held 2^10 up: their low ones stay normal numbers
 constexpr int kTop = 15;        // rows, and u, stay below 2^15
@@ -172,13 +171,18 @@ int set_slot(const Adapters& ad, int slot, const T* down, const T* up, int rank,
 }
 
 // ---------------------------------------------------------------- rows in order of their slots
-// Plan of a call: rows[unit][32] (-1: none), the slot of each unit, the number of units.
+// Plan of a call: rows[units][unit], unit = 32 or 64 rows of a wave, the slot of each unit, the number of units.  Places
+// that the last unit of a slot has no row for repeat the slot's first row: it is computed, and its results written,
+// again, which are the same bits.
+// A single line needs no lists: its rows are one run, the rows of no line before and behind it another.
 struct Plan {
     int* units;
     int* rows;
     int* slot;
+    const int64_t* one_off;  // a single line: its offsets and slot, the lists unused
+    const int32_t* one_slot;
 };
-int64_t plan_units(int64_t m, int64_t groups) { return m / kUnit + groups; }
+int64_t plan_units(int64_t m, int64_t groups, int unit) { return m / unit + groups; }
 
 // One workgroup.  Rows of a group are placed in any order: no row's result depends on its place.  Rows of no
 // line, and of lines that name no slot, form a group of their own.
@@ -187,14 +191,14 @@ int64_t plan_units(int64_t m, int64_t groups) { return m / kUnit + groups; }
 // short; the rows before the first and behind the last line are two lines more).  Otherwise each row looks for
 // its line, the last whose offset is not above it, so that each is placed once whatever the offsets hold.
 // 256 lines of 120: PLANUS us, by rows 95.
-__global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int slots, Plan plan) {
+__global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int slots, int unit, Plan plan) {
     extern __shared__ int groups[];
     int* count = groups;              // [slots + 1] rows of a group
     int* first = groups + slots + 1;  // its first unit
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int g = tid; g <= slots; g += 1024) count[g] = 0;
     bool rising = true;
-    for (int64_t i = tid; i <= lines.lines; i += 1024) {
+    for (int64_t i = tid; i <= lines.lines && lines.lines > 0; i += 1024) {
         const int64_t o = lines.off[i];
         rising &= o >= 0 && o <= m && (i == 0 || lines.off[i - 1] <= o);
     }
@@ -252,7 +256,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int
         int before = 0;
         for (int g0 = 0; g0 <= slots; g0 += 64) {
             const int g = g0 + lane;
-            const int mine = g <= slots ? (count[g] + kUnit - 1) / kUnit : 0;
+            const int mine = g <= slots ? (count[g] + unit - 1) / unit : 0;
             int upto = mine;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -265,11 +269,10 @@ __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int
         if (lane == 0) *plan.units = before;
     }
     __syncthreads();
-    // the units' slots, and the places that the last unit of a group has no row for
+    // the units' slots
     for (int g = tid; g <= slots; g += 1024) {
-        const int n = count[g], units = (n + kUnit - 1) / kUnit;
+        const int n = count[g], units = (n + unit - 1) / unit;
         for (int u = 0; u < units; ++u) plan.slot[first[g] + u] = g;
-        for (int x = n; x < units * kUnit; ++x) plan.rows[first[g] * kUnit + x] = -1;
         count[g] = 0;
     }
     __syncthreads();
@@ -279,12 +282,12 @@ __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int
             const Span s = span(i);
             if (s.hi <= s.lo) continue;
             if (brief && s.hi - s.lo < 1024) {
-                int* to = plan.rows + first[s.g] * kUnit + atomicAdd(&count[s.g], s.hi - s.lo);
+                int* to = plan.rows + first[s.g] * unit + atomicAdd(&count[s.g], s.hi - s.lo);
                 for (int r = s.lo; r < s.hi; ++r) to[r - s.lo] = r;
             } else if (!brief) {
                 int at = 0;
                 if (lane == 0) at = atomicAdd(&count[s.g], s.hi - s.lo);
-                int* to = plan.rows + first[s.g] * kUnit + __shfl(at, 0, 64);
+                int* to = plan.rows + first[s.g] * unit + __shfl(at, 0, 64);
                 for (int r = s.lo + lane; r < s.hi; r += 64) to[r - s.lo] = r;
             }
         }
@@ -295,7 +298,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int
                 if (s.hi - s.lo < 1024) continue;
                 int at = 0;
                 if (lane == 0) at = atomicAdd(&count[s.g], s.hi - s.lo);
-                int* to = plan.rows + first[s.g] * kUnit + __shfl(at, 0, 64);
+                int* to = plan.rows + first[s.g] * unit + __shfl(at, 0, 64);
                 for (int r = s.lo + lane; r < s.hi; r += 64) to[r - s.lo] = r;
             }
         }
@@ -304,10 +307,47 @@ __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int
             const int r = r0 + tid;
             const int g = r < m ? group_of(r) : 0;
             const int at = take(r < m, g);
-            if (r < m) plan.rows[first[g] * kUnit + at] = r;
+            if (r < m) plan.rows[first[g] * unit + at] = r;
         }
     }
+    __syncthreads();  // the rows are placed, count is the groups' again
+    for (int g = tid; g <= slots; g += 1024) {
+        const int n = count[g];
+        int* rows = plan.rows + first[g] * unit;
+        for (int x = n; x % unit; ++x) rows[x] = rows[0];
+    }
 }
+
+// The plan as the kernels read it, for units of U rows.
+template <int U>
+struct PlanView {
+    const Plan& plan;
+    int m, slots, units;
+    int lo = 0, len = 0, first = 0;  // a single line: its rows, and the units they take
+    __device__ __forceinline__ PlanView(const Plan& p, int64_t rows, int slot_count) : plan(p), m((int)rows), slots(slot_count) {
+        if (p.one_off) {
+            const int64_t b = p.one_off[0], e = p.one_off[1];
+            lo = (int)min(max(b, (int64_t)0), rows);
+            len = (int)max(min(max(e, (int64_t)0), rows) - lo, (int64_t)0);
+            first = (len + U - 1) / U;
+            units = first + (m - len + U - 1) / U;
+        } else {
+            units = *p.units;
+        }
+    }
+    __device__ __forceinline__ int slot_of(int unit) const {
+        if (!plan.one_off) return plan.slot[unit];
+        const int s = *plan.one_slot;
+        return unit < first && s >= 0 && s < slots ? s : slots;
+    }
+    // row `i` of a unit; places past the rows repeat one of them
+    __device__ __forceinline__ int row_of(int unit, int i) const {
+        if (!plan.one_off) return plan.rows[unit * U + i];
+        if (unit < first) return lo + min(unit * U + i, len - 1);
+        const int k = min((unit - first) * U + i, m - len - 1);
+        return k < lo ? k : k + len;
+    }
+};
 
 // ---------------------------------------------------------------- rows and their u in registers
 struct AdaptLaunch {
@@ -407,46 +447,53 @@ __device__ __forceinline__ void load_up(const uint8_t* up, int tile, int lane, u
 }
 
 // ---------------------------------------------------------------- statistics
-// One wave, 32 rows (columns of the matrix product), 32 classes a tile; the head's tiles through a ring in
-// LDS as in the head's statistics pass, the products of tile j + 1 interleaved with the epilogue of tile j.
-// PLAIN: the rows have no powers of two, and the sums no reference (no logit beyond 2^64 so far): a multiplication and
-// a subtraction less for each of the wave's logits.
-template <int P, bool PLAIN>
-__device__ __forceinline__ void adapt_piece(f32x16 (&t)[1], float inv, const float* __restrict__ ep, int h, int j, f32x4 (&cs)[2],
-                                            f32x4 (&cb)[2], const float (&ref)[1], float (&best)[1], int (&bt)[1], f32x4* save,
-                                            EpiState<1>& st) {
-    if constexpr (!PLAIN && P < 12 && P % 3 == 0) {
+// A wave takes MB blocks of 32 rows (columns of the matrix product) of one slot, 32 classes a tile; the head's
+// tiles go through a ring in LDS as in the head's statistics pass, the products of tile j + 1 interleaved with the
+// epilogue of tile j.  PLAIN: the rows have no powers of two, and the sums no reference (no logit beyond 2^64 so far): a
+// multiplication and a subtraction less for each logit.
+template <int P, int MB, bool PLAIN>
+__device__ __forceinline__ void adapt_piece(f32x16 (&t)[MB], const float (&inv)[MB], const float* __restrict__ ep, int h, int j,
+                                            f32x4 (&cs)[2], f32x4 (&cb)[2], const float (&ref)[MB], float (&best)[MB],
+                                            int (&bt)[MB], f32x4* save, EpiState<MB>& st) {
+    if constexpr (!PLAIN && P < 12 * MB && P % (3 * MB) < MB) {
+        constexpr int b = P % (3 * MB), q = P / (3 * MB);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t[0][4 * (P / 3) + e] *= inv;
+        for (int e = 0; e < 4; ++e) t[b][4 * q + e] *= inv[b];
     }
-    epi_piece<P, 1, PLAIN>(t, ep, h, j, cs, cb, ref, best, bt, save, st);
-    if constexpr (PLAIN && P == epi_pieces<1>() - 1) st.need = (best[0] != -INFINITY) & (__builtin_fabsf(best[0]) > 64.0f);
+    epi_piece<P, MB, PLAIN>(t, ep, h, j, cs, cb, ref, best, bt, save, st);
+    if constexpr (PLAIN && P == epi_pieces<MB>() - 1) {
+#pragma unroll
+        for (int b = 0; b < MB; ++b) st.need = st.need | ((best[b] != -INFINITY) & (__builtin_fabsf(best[b]) > 64.0f));
+    }
 }
-template <int H, int x, bool PLAIN>
-__device__ __forceinline__ void adapt_pieces(f32x16 (&t)[1], float inv, const float* __restrict__ ep, int h, int j, f32x4 (&cs)[2],
-                                             f32x4 (&cb)[2], const float (&ref)[1], float (&best)[1], int (&bt)[1], f32x4* save,
-                                             EpiState<1>& st) {
-    constexpr int NP = epi_pieces<1>();
+template <int H, int x, int MB, bool PLAIN>
+__device__ __forceinline__ void adapt_pieces(f32x16 (&t)[MB], const float (&inv)[MB], const float* __restrict__ ep, int h, int j,
+                                             f32x4 (&cs)[2], f32x4 (&cb)[2], const float (&ref)[MB], float (&best)[MB],
+                                             int (&bt)[MB], f32x4* save, EpiState<MB>& st) {
+    constexpr int NP = epi_pieces<MB>();
     constexpr int p0 = x * NP / H, p1 = (x + 1) * NP / H;
     [&]<int... I>(std::integer_sequence<int, I...>) {
-        (adapt_piece<p0 + I, PLAIN>(t, inv, ep, h, j, cs, cb, ref, best, bt, save, st), ...);
+        (adapt_piece<p0 + I, MB, PLAIN>(t, inv, ep, h, j, cs, cb, ref, best, bt, save, st), ...);
     }(std::make_integer_sequence<int, p1 - p0>{});
 }
 
-template <int C, int G, int NR>
-__global__ __launch_bounds__(64 * kWaves, 2) void adapt_stats_kernel(AdaptLaunch x) {
+constexpr int kAhead = 4;  // MFMA steps that a weight fragment is read ahead of its use
+
+template <int C, int G, int NR, int MB, int OCC>
+__global__ __launch_bounds__(64 * kWaves, OCC) void adapt_stats_kernel(AdaptLaunch x) {
     using GE = Geo<C, G>;
-    constexpr int S = GE::S, NT = 64 * kWaves;
+    constexpr int S = GE::S, NT = 64 * kWaves, UNIT = 32 * MB;
+    constexpr int AHEAD = OCC == 1 ? kAhead : kPrefetch;
     extern __shared__ __align__(16) uint8_t lds[];
     int mbi, chunk;
     map_block<true>(blockIdx.x, x.nsplit, &mbi, &chunk);
-    const int units = *x.plan.units;
-    if (mbi * kWaves >= units || chunk >= x.nsplit) return;
+    const PlanView<UNIT> plan(x.plan, x.m, x.slots);
+    if (mbi * kWaves >= plan.units || chunk >= x.nsplit) return;
     const int t0 = chunk * x.tpc, t1 = min(t0 + x.tpc, x.tiles);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 31, h = lane >> 5;
     if (tid < 32 * kRing) reinterpret_cast<u32x4*>(lds + (tid >> 5) * GE::BUF + GE::REC)[tid & 31] = u32x4{0, 0, 0, 0};
     const int lb = i * 16 + h * 512;
-    f32x4* save = reinterpret_cast<f32x4*>(lds + kRing * GE::BUF) + wave * (4 * 64) + lane;
+    f32x4* save = reinterpret_cast<f32x4*>(lds + kRing * GE::BUF) + wave * (MB * 4 * 64) + lane;
     constexpr int kOps = stage_direct_min_ops<GE::REC, NT>();
     if (t0 < t1) {
 #pragma unroll
@@ -454,36 +501,54 @@ __global__ __launch_bounds__(64 * kWaves, 2) void adapt_stats_kernel(AdaptLaunch
             stage_direct<GE::REC, NT>(x.rec + (size_t)min(t0 + y, t1 - 1) * GE::REC, lds + y * GE::BUF, tid);
     }
     const int unit = mbi * kWaves + wave;
-    const bool live = unit < units;
-    const int row = live ? x.plan.rows[unit * kUnit + i] : -1;
-    const int slot = __builtin_amdgcn_readfirstlane(live ? x.plan.slot[unit] : x.slots);
+    const bool live = unit < plan.units;
+    const int slot = __builtin_amdgcn_readfirstlane(live ? plan.slot_of(unit) : x.slots);
     const uint8_t* up = x.up + (size_t)slot * x.up_stride;
-    RowOperands<C, G, NR> o;
-    load_rows<C, G, NR>(x, max(row, 0), slot, i, h, o);
+    int row[MB];
+    RowOperands<C, G, NR> o[MB];
+    float inv[MB];
+    bool plain = true;  // the same for the wave
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+        row[b] = live ? plan.row_of(unit, 32 * b + i) : 0;
+        load_rows<C, G, NR>(x, row[b], slot, i, h, o[b]);
+        inv[b] = o[b].inv;
+        plain = plain && !o[b].scaled;
+    }
 
-    float best[1] = {-INFINITY}, ref[1] = {0.0f}, sum = 0.0f;
-    int bt[1] = {-1};
+    float best[MB], ref[MB], sum[MB];
+    int bt[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+        best[b] = -INFINITY;
+        ref[b] = sum[b] = 0.0f;
+        bt[b] = -1;
+    }
     // the loads of the newest staged tile may still be in flight at a barrier
     constexpr int kLead = (kRing - 3) * kOps;
     if (t0 < t1) {
         u16x8 whi[NR], wlo[NR];
         load_up<NR>(up, t0, lane, whi, wlo);
         ring_barrier<kLead>();  // tiles t0 and t0 + 1 are in LDS
-        f32x16 acc_a[1] = {f32x16{}}, acc_b[1];
-        auto adapter_products = [&](f32x16& acc) {
+        f32x16 acc_a[MB], acc_b[MB];
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+            acc_a[b] = f32x16{};
 #pragma unroll
             for (int s = 0; s < NR; ++s) {
-                acc = mfma16<true>(whi[s], o.uhi[s], acc);
-                acc = mfma16<true>(whi[s], o.ulo[s], acc);
-                acc = mfma16<true>(wlo[s], o.uhi[s], acc);
+                acc_a[b] = mfma16<true>(whi[s], o[b].uhi[s], acc_a[b]);
+                acc_a[b] = mfma16<true>(whi[s], o[b].ulo[s], acc_a[b]);
+                acc_a[b] = mfma16<true>(wlo[s], o[b].uhi[s], acc_a[b]);
             }
-        };
-        adapter_products(acc_a[0]);
+        }
         load_up<NR>(up, min(t0 + 1, t1 - 1), lane, whi, wlo);
 #pragma unroll
-        for (int s = 0; s < S; ++s) acc_a[0] = mfma16<true>(weight_frag<C, G>(lds, s, lb, i * 16, h), o.a[s], acc_a[0]);
-        bool plain = !o.scaled;  // the same for the wave
-        auto step_as = [&]<int R, bool PLAIN>(int j, f32x16 (&accE)[1], f32x16 (&accM)[1]) __attribute__((always_inline)) {
+        for (int s = 0; s < S; ++s) {
+            const u16x8 wf = weight_frag<C, G>(lds, s, lb, i * 16, h);
+#pragma unroll
+            for (int b = 0; b < MB; ++b) acc_a[b] = mfma16<true>(wf, o[b].a[s], acc_a[b]);
+        }
+        auto step_as = [&]<int R, bool PLAIN>(int j, f32x16 (&accE)[MB], f32x16 (&accM)[MB]) __attribute__((always_inline)) {
             constexpr unsigned rel = (unsigned)R;  // (j - t0) % kRing
             const uint8_t* bufn = lds + ((rel + 1) & (kRing - 1)) * GE::BUF;
             const float* ep = reinterpret_cast<const float*>(lds + (rel & (kRing - 1)) * GE::BUF + GE::FRAG);
@@ -493,18 +558,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void adapt_stats_kernel(AdaptLaunch
                 cs[q] = *reinterpret_cast<const f32x4*>(ep + 8 * q + 4 * h);
                 cb[q] = *reinterpret_cast<const f32x4*>(ep + 32 + 8 * q + 4 * h);
             }
-            EpiState<1> st;
+            EpiState<MB> st;
             st.need = false;
-            accM[0] = f32x16{};
+#pragma unroll
+            for (int b = 0; b < MB; ++b) accM[b] = f32x16{};
             // products 0 .. 3 NR - 1: the adapter's, the rest the head's; the epilogue's pieces between them all
             constexpr int STEPS = S + 3 * NR;
+            u16x8 wq[AHEAD];
+            frag_prefetch_first<C, G, AHEAD>(wq, bufn, lb, i * 16, h);
             [&]<int... s>(std::integer_sequence<int, s...>) {
                 ([&] {
                     constexpr int r = s / 3, y = s % 3;
-                    accM[0] = mfma16<true>(y == 2 ? wlo[r] : whi[r], y == 1 ? o.ulo[r] : o.uhi[r], accM[0]);
+                    const u16x8& wf = y == 2 ? wlo[r] : whi[r];
+                    accM[0] = mfma16<true>(wf, y == 1 ? o[0].ulo[r] : o[0].uhi[r], accM[0]);
                     __builtin_amdgcn_sched_barrier(0);
-                    adapt_pieces<2 * STEPS, 2 * s, PLAIN>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
-                    adapt_pieces<2 * STEPS, 2 * s + 1, PLAIN>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
+                    adapt_pieces<2 * STEPS, 2 * s, MB, PLAIN>(accE, inv, ep, h, j, cs, cb, ref, best, bt, save, st);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int b = 1; b < MB; ++b) accM[b] = mfma16<true>(wf, y == 1 ? o[b].ulo[r] : o[b].uhi[r], accM[b]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    adapt_pieces<2 * STEPS, 2 * s + 1, MB, PLAIN>(accE, inv, ep, h, j, cs, cb, ref, best, bt, save, st);
                     __builtin_amdgcn_sched_barrier(0);
                 }(), ...);
             }(std::make_integer_sequence<int, 3 * NR>{});
@@ -513,37 +586,42 @@ __global__ __launch_bounds__(64 * kWaves, 2) void adapt_stats_kernel(AdaptLaunch
             load_up<NR>(up, min(j + 2, t1 - 1), lane, whi, wlo);
             stage_direct<GE::REC, NT>(x.rec + (size_t)min(j + kRing - 1, t1 - 1) * GE::REC,
                                       lds + ((rel + kRing - 1) & (kRing - 1)) * GE::BUF, tid);
-            u16x8 wq[kPrefetch];
-            frag_prefetch_first<C, G, kPrefetch>(wq, bufn, lb, i * 16, h);
             [&]<int... s>(std::integer_sequence<int, s...>) {
                 ([&] {
                     constexpr int g = s + 3 * NR;
-                    accM[0] = mfma16<true>(frag_of<C, G, kPrefetch, s>(wq), o.a[s], accM[0]);
+                    const u16x8& wf = frag_of<C, G, AHEAD, s>(wq);
+                    accM[0] = mfma16<true>(wf, o[0].a[s], accM[0]);
                     __builtin_amdgcn_sched_barrier(0);
-                    adapt_pieces<2 * STEPS, 2 * g, PLAIN>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
-                    frag_prefetch_after<C, G, kPrefetch, s>(wq, bufn, lb, i * 16, h);
+                    adapt_pieces<2 * STEPS, 2 * g, MB, PLAIN>(accE, inv, ep, h, j, cs, cb, ref, best, bt, save, st);
                     __builtin_amdgcn_sched_barrier(0);
-                    adapt_pieces<2 * STEPS, 2 * g + 1, PLAIN>(accE, o.inv, ep, h, j, cs, cb, ref, best, bt, save, st);
+#pragma unroll
+                    for (int b = 1; b < MB; ++b) accM[b] = mfma16<true>(wf, o[b].a[s], accM[b]);
+                    frag_prefetch_after<C, G, AHEAD, s>(wq, bufn, lb, i * 16, h);
+                    __builtin_amdgcn_sched_barrier(0);
+                    adapt_pieces<2 * STEPS, 2 * g + 1, MB, PLAIN>(accE, inv, ep, h, j, cs, cb, ref, best, bt, save, st);
                     __builtin_amdgcn_sched_barrier(0);
                 }(), ...);
             }(std::make_integer_sequence<int, S>{});
             if (__any(st.need)) {
                 plain = false;
-                if (best[0] != -INFINITY && __builtin_fabsf(best[0] - ref[0]) > 64.0f) {
-                    const float nr = best[0];
-                    sum = (sum == 0.0f) ? 0.0f : sum * __builtin_amdgcn_exp2f(ref[0] - nr);
-                    float v = 0.0f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) v += __builtin_amdgcn_exp2f(accE[0][r] - nr);
-                    st.tsum[0] = v;
-                    ref[0] = nr;
-                }
+                for (int b = 0; b < MB; ++b)
+                    if (best[b] != -INFINITY && __builtin_fabsf(best[b] - ref[b]) > 64.0f) {
+                        const float nr = best[b];
+                        sum[b] = (sum[b] == 0.0f) ? 0.0f : sum[b] * __builtin_amdgcn_exp2f(ref[b] - nr);
+                        float v = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) v += __builtin_amdgcn_exp2f(accE[b][r] - nr);
+                        st.tsum[b] = v;
+                        ref[b] = nr;
+                    }
             }
-            sum += st.tsum[0];
+#pragma unroll
+            for (int b = 0; b < MB; ++b) sum[b] += st.tsum[b];
             ring_barrier<kLead>();
         };
         auto step_of = [&]<int R>(int jj) __attribute__((always_inline)) {
-            auto both = [&](f32x16 (&accE)[1], f32x16 (&accM)[1]) __attribute__((always_inline)) {
+            auto both = [&](f32x16 (&accE)[MB], f32x16 (&accM)[MB]) __attribute__((always_inline)) {
                 if (plain) step_as.template operator()<R, true>(jj, accE, accM);
                 else step_as.template operator()<R, false>(jj, accE, accM);
             };
@@ -562,36 +640,62 @@ __global__ __launch_bounds__(64 * kWaves, 2) void adapt_stats_kernel(AdaptLaunch
         vm_wait<0>();
     }
 
-    int cls = 0;
-    if (bt[0] >= 0) {
-        int r0 = 16;
 #pragma unroll
-        for (int q = 3; q >= 0; --q) {
-            const f32x4 v = save[q * 64];
+    for (int b = 0; b < MB; ++b) {
+        int cls = 0;
+        if (bt[b] >= 0) {
+            int r0 = 16;
 #pragma unroll
-            for (int e = 3; e >= 0; --e) r0 = (v[e] == best[0]) ? 4 * q + e : r0;
+            for (int q = 3; q >= 0; --q) {
+                const f32x4 v = save[(b * 4 + q) * 64];
+#pragma unroll
+                for (int e = 3; e >= 0; --e) r0 = (v[e] == best[b]) ? 4 * q + e : r0;
+            }
+            cls = bt[b] * 32 + (r0 < 16 ? 8 * (r0 >> 2) + 4 * h + (r0 & 3) : 0);
         }
-        cls = bt[0] * 32 + (r0 < 16 ? 8 * (r0 >> 2) + 4 * h + (r0 & 3) : 0);
+        const RowStat mine{best[b], sum[b], ref[b], cls};
+        const RowStat other{__shfl_xor(best[b], 32, 64), __shfl_xor(sum[b], 32, 64), __shfl_xor(ref[b], 32, 64),
+                            __shfl_xor(cls, 32, 64)};
+        const RowStat r = stat_merge(mine, other);
+        if (h == 0 && live) x.part[(int64_t)chunk * x.m + row[b]] = Partial{r.best, r.sum, r.idx};
     }
-    const RowStat mine{best[0], sum, ref[0], cls};
-    const RowStat other{__shfl_xor(best[0], 32, 64), __shfl_xor(sum, 32, 64), __shfl_xor(ref[0], 32, 64), __shfl_xor(cls, 32, 64)};
-    const RowStat r = stat_merge(mine, other);
-    if (h == 0 && row >= 0) x.part[(int64_t)chunk * x.m + row] = Partial{r.best, r.sum, r.idx};
 }
 
 // ---------------------------------------------------------------- logits
 // Rows of the matrix product are the activation rows, columns the classes, so that a store writes 32
-// consecutive classes of two rows.  A producer wave keeps the ring of the head's tiles filled.
+// consecutive classes of two rows.  Four waves multiply and store, one on a SIMD; a producer wave keeps a ring of
+// tiles in LDS filled, the head's and those of the adapters of the workgroup's units.  The four load nothing: a
+// wave's memory operations end in order, so that one which loaded its adapter's tiles itself waited for its own
+// stores with them.  More waves on a CU write more pieces of rows at once and slower: rank 16 of 7680 rows of an INT8
+// head 235 us, 258 with seven waves, 270 in two workgroups a CU (2.4 TB/s; the head's own logits 172).
+//
+// Units of a slot follow each other, so that a workgroup's units have few slots.  The ring holds those of kSets<NR>; a
+// workgroup whose units have more (ranks above 32 only, where LDS holds no more) goes over its tiles again for the
+// units behind.
+constexpr int kLogitWaves = 4;
+template <int NR>
+constexpr int kSets = NR == 4 ? 3 : kLogitWaves;
+constexpr int kLdsBytes = 160 * 1024;
 template <int C, int G, int NR>
-__global__ __launch_bounds__(64 * (kWaves + 1), 1) void adapt_logits_kernel(AdaptLaunch x) {
+struct LogitRing {
+    static constexpr int SET = 2 * NR * 1024;  // an adapter's tile
+    static constexpr int SLOT = Geo<C, G>::BUF + kSets<NR> * SET;
+    static constexpr int HEAD_OPS = stage_wave_ops<Geo<C, G>::REC>();
+    // tiles held: LDS, and the loads that the producer's wait can count (those of all but two tiles)
+    static constexpr int BY_LDS = kLdsBytes / SLOT, BY_WAIT = 2 + 63 / (HEAD_OPS + 2 * NR * kSets<NR>);
+    static constexpr int R = BY_LDS < BY_WAIT ? BY_LDS : BY_WAIT;
+    static_assert(R >= 3, "a tile in use, one behind it and one on its way");
+};
+
+template <int C, int G, int NR>
+__global__ __launch_bounds__(64 * (kLogitWaves + 1), 1) void adapt_logits_kernel(AdaptLaunch x) {
     using GE = Geo<C, G>;
-    constexpr int S = GE::S;
-    constexpr int R = writer_ring<GE::REC>();
-    extern __shared__ __align__(16) uint8_t lds[];  // [R tiles] x BUF
-    int mbi, chunk;
-    map_block<false>(blockIdx.x, x.nsplit, &mbi, &chunk);
-    const int units = *x.plan.units;
-    if (mbi * kWaves >= units) return;
+    using RING = LogitRing<C, G, NR>;
+    constexpr int S = GE::S, R = RING::R, D = kSets<NR>;
+    extern __shared__ __align__(16) uint8_t lds[];  // [R] x SLOT
+    const int mbi = blockIdx.x / x.nsplit, chunk = blockIdx.x % x.nsplit;
+    const PlanView<32> plan(x.plan, x.m, x.slots);
+    if (mbi * kLogitWaves >= plan.units) return;
     const int t0 = chunk * x.tpc, t1 = min(t0 + x.tpc, x.tiles);
     if (t0 >= t1) return;
     const int ntiles = t1 - t0;
@@ -600,89 +704,127 @@ __global__ __launch_bounds__(64 * (kWaves + 1), 1) void adapt_logits_kernel(Adap
     // workgroups start at tiles of their own, as in the head's writer
     const unsigned stride = x.nsplit == 1 ? kStartStepOne : kStartStepSeveral;
     const int rot = (int)(((int64_t)((blockIdx.x * stride) & 0xffffu) * ntiles) >> 16);
-
-    if (wave == kWaves) {
-        constexpr int kOps = stage_wave_ops<GE::REC>();
-        int pt = t0 + rot, pslot = 0;
-        auto stage_next = [&] {
-            stage_wave<GE::REC>(x.rec + (size_t)pt * GE::REC, lds + pslot * GE::BUF, lane);
-            pt = pt + 1 == t1 ? t0 : pt + 1;
-            pslot = pslot + 1 == R ? 0 : pslot + 1;
-        };
+    // the slots of the workgroup's units, each run of units with one counted once
+    int slot_of[kLogitWaves], set_of[kLogitWaves];
 #pragma unroll
-        for (int g = 0; g < R - 1; ++g) stage_next();
-        vm_wait<kOps * (R - 2)>();  // tile 0 is in LDS
-        barrier_lds();
-        for (int g = 0; g < ntiles; ++g) {
-            stage_next();
-            vm_wait<kOps * (R - 2)>();  // tile g + 1 is in LDS
+    for (int u = 0; u < kLogitWaves; ++u) {
+        const int unit = mbi * kLogitWaves + u;
+        slot_of[u] = unit < plan.units ? plan.slot_of(unit) : (u ? slot_of[u - 1] : x.slots);
+        set_of[u] = u == 0 ? 0 : set_of[u - 1] + (slot_of[u] != slot_of[u - 1] ? 1 : 0);
+    }
+    const int sets = set_of[kLogitWaves - 1] + 1;
+    const int passes = (sets + D - 1) / D;
+
+    if (wave == kLogitWaves) {
+        int pslot = 0;
+        // N sets of adapters beside the head's tiles, from the first-th set on
+        auto produce = [&]<int N>(int first) {
+            constexpr int kOps = RING::HEAD_OPS + N * 2 * NR;
+            const uint8_t* up[N];
+#pragma unroll
+            for (int d = 0; d < N; ++d) {
+                int s = x.slots;
+#pragma unroll
+                for (int u = 0; u < kLogitWaves; ++u) s = set_of[u] == first + d ? slot_of[u] : s;
+                up[d] = x.up + (size_t)s * x.up_stride;
+            }
+            int pt = t0 + rot;
+            auto stage_next = [&] {
+                uint8_t* to = lds + pslot * RING::SLOT;
+                stage_wave<GE::REC>(x.rec + (size_t)pt * GE::REC, to, lane);
+#pragma unroll
+                for (int d = 0; d < N; ++d)
+                    stage_wave<RING::SET>(up[d] + (size_t)pt * RING::SET, to + GE::BUF + d * RING::SET, lane);
+                pt = pt + 1 == t1 ? t0 : pt + 1;
+                pslot = pslot + 1 == R ? 0 : pslot + 1;
+            };
+#pragma unroll
+            for (int g = 0; g < R - 1; ++g) stage_next();
+            vm_wait<kOps*(R - 2)>();  // the first tile is in LDS
             barrier_lds();
+            for (int g = 0; g < ntiles; ++g) {
+                stage_next();
+                vm_wait<kOps*(R - 2)>();  // tile g + 1 is in LDS
+                barrier_lds();
+            }
+            vm_wait<0>();  // the ring's last loads land before the next pass, and before the workgroup ends
+            barrier_lds();
+        };
+        for (int p = 0; p < passes; ++p) {
+            const int n = min(sets - p * D, D);
+            [&]<int... k>(std::integer_sequence<int, k...>) {
+                ((n == k + 1 ? produce.template operator()<k + 1>(p * D) : void()), ...);
+            }(std::make_integer_sequence<int, D>{});
+            pslot = 0;
         }
-        vm_wait<0>();  // the ring's last loads land before the workgroup ends
         return;
     }
 
-    for (int y = tid >> 5; y < R; y += 2 * kWaves)
-        reinterpret_cast<u32x4*>(lds + y * GE::BUF + GE::REC)[tid & 31] = u32x4{0, 0, 0, 0};
-    const int unit = mbi * kWaves + wave;
-    const bool live = unit < units;
-    const int row = live ? x.plan.rows[unit * kUnit + i] : -1;
-    const int slot = __builtin_amdgcn_readfirstlane(live ? x.plan.slot[unit] : x.slots);
-    const uint8_t* up = x.up + (size_t)slot * x.up_stride;
-    RowOperands<C, G, NR> o;
-    load_rows<C, G, NR>(x, max(row, 0), slot, i, h, o);
-    // rows of this lane's 16 accumulators
-    int orow[16];
-    float oinv[16];
+    for (int y = tid >> 5; y < R; y += 2 * kLogitWaves)
+        reinterpret_cast<u32x4*>(lds + y * RING::SLOT + GE::REC)[tid & 31] = u32x4{0, 0, 0, 0};
+    const int unit = mbi * kLogitWaves + wave;
+    int slot = 0, set = 0;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int from = 8 * (r >> 2) + 4 * h + (r & 3);
-        orow[r] = __shfl(row, from, 64);
-        oinv[r] = __shfl(o.inv, from, 64);
+    for (int u = 0; u < kLogitWaves; ++u) {
+        slot = u == wave ? slot_of[u] : slot;
+        set = u == wave ? set_of[u] : set;
     }
-    const bool whole = __all(row >= 0);
-    int pt = t0 + rot, cslot = 0;
-    u16x8 whi[NR], wlo[NR];
-    load_up<NR>(up, pt, lane, whi, wlo);
-    barrier_lds();  // zero blocks written; tile 0 is in LDS
-    for (int g = 0; g < ntiles; ++g) {
-        const uint8_t* buf = lds + cslot * GE::BUF;
-        cslot = cslot + 1 == R ? 0 : cslot + 1;
-        const int next = pt + 1 == t1 ? t0 : pt + 1;
-        f32x16 acc = {};
+    const bool live = unit < plan.units;
+    const int row = live ? plan.row_of(unit, i) : 0;
+    RowOperands<C, G, NR> o;
+    load_rows<C, G, NR>(x, row, slot, i, h, o);
+    // where the rows of this lane's 16 accumulators begin in the output
+    float* to[16];
 #pragma unroll
-        for (int s = 0; s < NR; ++s) {
-            acc = mfma16<true>(o.uhi[s], whi[s], acc);
-            acc = mfma16<true>(o.ulo[s], whi[s], acc);
-            acc = mfma16<true>(o.uhi[s], wlo[s], acc);
+    for (int r = 0; r < 16; ++r) to[r] = x.out + (int64_t)__shfl(row, 8 * (r >> 2) + 4 * h + (r & 3), 64) * x.n;
+    for (int p = 0; p < passes; ++p) {
+        const bool mine = live && set / D == p;
+        int pt = t0 + rot, cslot = 0;
+        barrier_lds();  // zero blocks written; the first tile is in LDS
+        for (int g = 0; g < ntiles; ++g) {
+            const uint8_t* buf = lds + cslot * RING::SLOT;
+            cslot = cslot + 1 == R ? 0 : cslot + 1;
+            if (mine) {
+                constexpr int AHEAD = S < kAhead ? S : kAhead;
+                const u16x8* up = reinterpret_cast<const u16x8*>(buf + GE::BUF + (set % D) * RING::SET) + lane;
+                u16x8 wq[AHEAD];
+                f32x16 acc = {};
+#pragma unroll
+                for (int s = 0; s < NR; ++s) {
+                    const u16x8 hi = up[s * 64], lo = up[(NR + s) * 64];
+                    acc = mfma16<true>(o.uhi[s], hi, acc);
+                    acc = mfma16<true>(o.ulo[s], hi, acc);
+                    acc = mfma16<true>(o.uhi[s], lo, acc);
+                }
+                frag_prefetch_first<C, G, AHEAD>(wq, buf, i * 16 + h * 512, i * 16, h);
+                [&]<int... st>(std::integer_sequence<int, st...>) {
+                    ([&] {
+                        acc = mfma16<true>(o.a[st], frag_of<C, G, AHEAD, st>(wq), acc);
+                        frag_prefetch_after<C, G, AHEAD, st>(wq, buf, i * 16 + h * 512, i * 16, h);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }(), ...);
+                }(std::make_integer_sequence<int, S>{});
+                const float* ep = reinterpret_cast<const float*>(buf + GE::FRAG);
+                const float c0 = ep[64 + i], c1 = ep[96 + i];
+                const int col = pt * 32 + i;
+                float v[16];
+                if (o.scaled) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        v[r] = fmaf(acc[r] * __shfl(o.inv, 8 * (r >> 2) + 4 * h + (r & 3), 64), c0, c1);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) v[r] = fmaf(acc[r], c0, c1);
+                }
+                if (col < x.n) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) to[r][col] = v[r];
+                }
+            }
+            pt = pt + 1 == t1 ? t0 : pt + 1;
+            barrier_lds();  // this ring slot is read; the next tile is in LDS
         }
-        load_up<NR>(up, next, lane, whi, wlo);
-        constexpr int kAhead = S < 8 ? S : 8;
-        u16x8 wq[kAhead];
-        frag_prefetch_first<C, G, kAhead>(wq, buf, i * 16 + h * 512, i * 16, h);
-        [&]<int... st>(std::integer_sequence<int, st...>) {
-            ([&] {
-                acc = mfma16<true>(o.a[st], frag_of<C, G, kAhead, st>(wq), acc);
-                frag_prefetch_after<C, G, kAhead, st>(wq, buf, i * 16 + h * 512, i * 16, h);
-                __builtin_amdgcn_sched_barrier(0);
-            }(), ...);
-        }(std::make_integer_sequence<int, S>{});
-        const float* ep = reinterpret_cast<const float*>(buf + GE::FRAG);
-        const float c0 = ep[64 + i], c1 = ep[96 + i];
-        const int col = pt * 32 + i;
-        float v[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) v[r] = fmaf(acc[r] * oinv[r], c0, c1);
-        if (whole && pt * 32 + 32 <= x.n) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x.out[(int64_t)orow[r] * x.n + col] = v[r];
-        } else if (col < x.n) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (orow[r] >= 0) x.out[(int64_t)orow[r] * x.n + col] = v[r];
-        }
-        pt = next;
-        barrier_lds();  // this ring slot is read; the next tile is in LDS
+        barrier_lds();  // the ring is empty
     }
 }
 
@@ -699,23 +841,52 @@ size_t align(size_t x) { return (x + 255) / 256 * 256; }
 struct AdaptLayout {
     size_t units, rows, slot, part, total;
 };
-int chunks_of(const Adapters& ad, int64_t m) { return stats_nsplit(m, kUnit * kWaves, ad.tiles, 2); }
+// Blocks of 32 rows of a wave of the statistics pass, and workgroups that a CU holds of it.  Ranks above 32 keep
+// too many operands for two waves a SIMD: one wave then, with two blocks where there are rows enough (rank 64,
+// 30720 rows in us: 539 so, 581 with one block, 728 in two spilling waves; 1200 rows: 60 and 56).  Up to rank 32 two
+// waves with a block each are ahead of one with two (rank 16: 368 and 390, rank 32: 424 and 445).
+int blocks_of(int64_t m, int steps) { return steps == 4 && m > 2048 ? 2 : 1; }
+int per_cu_of(int steps) { return steps == 4 ? 1 : 2; }
+// Vocabulary chunks of the statistics pass: the count with the fewest tile times, as the head's (stats_nsplit), of
+// the row blocks that the plan is likely to make, half a unit lost a slot.
+int chunks_of(const Adapters& ad, int64_t m) {
+    const int64_t unit = 32 * blocks_of(m, ad.steps), slots = 32 * (int64_t)per_cu_of(ad.steps), fixed = 8;
+    const int64_t whole = (m + unit - 1) / unit, units = whole + std::min<int64_t>(ad.slots, whole) / 2;
+    const int64_t mblocks = (units + kWaves - 1) / kWaves;
+    int best = 1;
+    int64_t best_cost = -1;
+    for (int cand = 1; cand <= 128; cand += cand < 2 ? 1 : cand < 8 ? cand : 8) {
+        // the chunks that hold tiles; below 8 a count that divides 8
+        int ns = (ad.tiles + (ad.tiles + cand - 1) / cand - 1) / ((ad.tiles + cand - 1) / cand);
+        if (ns < 8) ns = ns <= 1 ? 1 : ns <= 2 ? 2 : ns <= 4 ? 4 : 8;
+        const int64_t per_xcd = ns >= 8 ? mblocks * ((ns + 7) / 8) : (mblocks + 7) / 8 * ns;
+        const int64_t rounds = (per_xcd + slots - 1) / slots;
+        const int64_t cost = rounds * (fixed + (ad.tiles + ns - 1) / ns);
+        if ((cand & (cand - 1)) != 0 && rounds > 1) continue;
+        if (ns > 64 && per_xcd > 32) continue;
+        if (best_cost < 0 || cost < best_cost) best = ns, best_cost = cost;
+    }
+    return best;
+}
 AdaptLayout layout_of(const Adapters& ad, int64_t m) {
-    const int64_t units = plan_units(m, std::min<int64_t>(ad.slots, m) + 1);
+    const int64_t units = plan_units(m, std::min<int64_t>(ad.slots, m) + 1, 32);  // of the smaller size: places of the larger one fit
     AdaptLayout L;
     L.units = 0;
     L.rows = 256;
-    L.slot = L.rows + align((size_t)units * kUnit * 4);
+    L.slot = L.rows + align((size_t)(units + std::min<int64_t>(ad.slots, m) + 1) * 32 * 4);
     L.part = L.slot + align((size_t)units * 4);
     L.total = L.part + align((size_t)chunks_of(ad, m) * (size_t)m * sizeof(Partial));
     return L;
 }
 
-int make_plan(const Adapters& ad, const AdaptLines& lines, int64_t m, const AdaptLayout& L, uint8_t* ws, Plan* plan, int64_t* units,
+int make_plan(const Adapters& ad, const AdaptLines& lines, int64_t m, int unit, const AdaptLayout& L, uint8_t* ws, Plan* plan, int64_t* units,
               hipStream_t st) {
-    *plan = Plan{reinterpret_cast<int*>(ws + L.units), reinterpret_cast<int*>(ws + L.rows), reinterpret_cast<int*>(ws + L.slot)};
-    *units = plan_units(m, std::min<int64_t>(std::min<int64_t>(ad.slots, lines.lines) + 1, m));
-    plan_kernel<<<1, 1024, (size_t)(ad.slots + 1) * 8, st>>>(lines, (int)m, ad.slots, *plan);
+    const bool one = lines.lines == 1;
+    *plan = Plan{reinterpret_cast<int*>(ws + L.units), reinterpret_cast<int*>(ws + L.rows), reinterpret_cast<int*>(ws + L.slot),
+                 one ? lines.off : nullptr, one ? lines.slot : nullptr};
+    *units = plan_units(m, std::min<int64_t>(std::min<int64_t>(ad.slots, lines.lines) + 1, m), unit);
+    if (one) return PPOCR_OK;
+    plan_kernel<<<1, 1024, (size_t)(ad.slots + 1) * 8, st>>>(lines, (int)m, ad.slots, unit, *plan);
     PPOCR_HIP(hipGetLastError());
     return PPOCR_OK;
 }
@@ -782,14 +953,19 @@ int launch_adapt_decode(int cfg, const TileGeom& tg, const uint8_t* rec, const A
     const AdaptLayout L = layout_of(ad, m);
     Plan plan;
     int64_t units;
-    if (int e = make_plan(ad, lines, m, L, ws, &plan, &units, st)) return e;
+    if (int e = make_plan(ad, lines, m, 32 * blocks_of(m, ad.steps), L, ws, &plan, &units, st)) return e;
     const int nsplit = chunks_of(ad, m);
     AdaptLaunch x = launch_of(tg, rec, ad, a, m, n, k, units, nsplit, plan);
     x.part = reinterpret_cast<Partial*>(ws + L.part);
     const unsigned grid = (unsigned)grid_of(x.mblocks, nsplit, true);
     if (int e = by_config(cfg, tg.G, ad.steps, [&]<int C, int G, int NR>() {
-            constexpr int bytes = kRing * Geo<C, G>::BUF + kWaves * 16 * 64 * 4;
-            adapt_stats_kernel<C, G, NR><<<grid, 64 * kWaves, bytes, st>>>(x);
+            auto go = [&]<int MB, int OCC>() {
+                constexpr int bytes = kRing * Geo<C, G>::BUF + kWaves * MB * 16 * 64 * 4;
+                adapt_stats_kernel<C, G, NR, MB, OCC><<<grid, 64 * kWaves, bytes, st>>>(x);
+            };
+            if constexpr (NR < 4) go.template operator()<1, 2>();
+            else if (blocks_of(m, ad.steps) == 2) go.template operator()<2, 1>();
+            else go.template operator()<1, 1>();
             PPOCR_HIP(hipGetLastError());
             return (int)PPOCR_OK;
         }))
@@ -802,17 +978,25 @@ int launch_adapt_logits(int cfg, const TileGeom& tg, const uint8_t* rec, const A
     const AdaptLayout L = layout_of(ad, m);
     Plan plan;
     int64_t units;
-    if (int e = make_plan(ad, lines, m, L, ws, &plan, &units, st)) return e;
-    const int64_t mblocks = (units + kWaves - 1) / kWaves;
-    // enough workgroups for the CUs
+    if (int e = make_plan(ad, lines, m, 32, L, ws, &plan, &units, st)) return e;
+    const int64_t mblocks = (units + kLogitWaves - 1) / kLogitWaves;
+    // The chunk count with the fewest tile times, a workgroup a CU at once and its start worth 8 tiles, of the row
+    // blocks that the plan is likely to make; counts that keep an XCD at its own chunks (7680 rows in 8 and 16 chunks
+    // 236 us, in 6 and 12 260 and 255).
+    const int64_t whole = (m + 31) / 32;
+    const int64_t likely = (whole + std::min<int64_t>(ad.slots, whole) / 2 + kLogitWaves - 1) / kLogitWaves;
     int nsplit = 1;
-    while (nsplit < 64 && mblocks * nsplit < 256 && nsplit * 2 <= tg.tiles) nsplit *= 2;
+    int64_t best = -1;
+    for (int ns = 1; ns <= 128 && ns <= tg.tiles; ns += ns < 8 ? ns : 8) {
+        const int64_t cost = (likely * ns + 255) / 256 * (8 + (tg.tiles + ns - 1) / ns);
+        if (best < 0 || cost < best) nsplit = ns, best = cost;
+    }
     AdaptLaunch x = launch_of(tg, rec, ad, a, m, n, k, units, nsplit, plan);
     x.out = out;
-    const unsigned grid = (unsigned)grid_of(x.mblocks, nsplit, false);
+    const unsigned grid = (unsigned)(mblocks * nsplit);
     return by_config(cfg, tg.G, ad.steps, [&]<int C, int G, int NR>() {
-        constexpr int bytes = writer_ring<Geo<C, G>::REC>() * Geo<C, G>::BUF;
-        adapt_logits_kernel<C, G, NR><<<grid, 64 * (kWaves + 1), bytes, st>>>(x);
+        constexpr int bytes = LogitRing<C, G, NR>::R * LogitRing<C, G, NR>::SLOT;
+        adapt_logits_kernel<C, G, NR><<<grid, 64 * (kLogitWaves + 1), bytes, st>>>(x);
         PPOCR_HIP(hipGetLastError());
         return (int)PPOCR_OK;
     });

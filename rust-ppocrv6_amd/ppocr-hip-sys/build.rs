@@ -48,12 +48,14 @@ const FLAGS: &[&str] = &[
     "-packed-fp32-ops",
 ];
 
-// Per-file flags: the tail's kernels keep MFMA results in ordinary vector registers (no
+// Per-file flags: the tail's and the adapters' kernels keep MFMA results in ordinary vector registers (no
 // accumulator-register copies before their vector work).
 fn file_flags(src: &str) -> &'static [&'static str] {
     if src == "neck.hip" {
         &["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
     } else if src == "neck_fused.hip" {
+        &["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+    } else if src == "adapt.hip" {
         &["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
     } else {
         &[]

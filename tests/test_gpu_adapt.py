@@ -213,6 +213,39 @@ def test_rows_of_no_line_and_offsets_that_go_backwards(rh):
     tc.close(none.logits().get(), *each[0], "no lines")
 
 
+def test_single_lines(rh):
+    """One line, wherever it begins and ends and whatever slot it names; rows before and behind it are the head's."""
+    rng = np.random.default_rng(17)
+    h = ac.Head(rh, rng, 333, 120, True, 2, 16)
+    big = ac.Head(rh, rng, 333, 120, False, 2, 64)
+    for m in (1, 31, 32, 33, 100, 2100):
+        for head in (h, big):
+            a = rows(rng, head, m)
+            each = [head.exact(a, np.full(m, s)) for s in (-1, 0, 1)]
+            for off, slot in (([0, m], 1), ([0, m], -1), ([0, m], 2), ([m // 3, m], 0), ([0, m - m // 3], 1), ([m // 3, m // 2], 0),
+                              ([-9, 1 << 40], 1), ([m, 0], 1), ([m, m], 0)):
+                lo, hi = (min(max(x, 0), m) for x in off)
+                used = slot if 0 <= slot < 2 else -1
+                at = np.zeros((m, 1), bool)
+                at[lo:hi] = True
+                z, e = (np.where(at, each[used + 1][x], each[0][x]) for x in (0, 1))
+                call = ac.Call(head, a, off, [slot])
+                tc.close(call.logits().get(), z, e, f"{m} {off} {slot}")
+                o = {k: v.get() for k, v in call.decode().items()}
+                if off == [0, m]:
+                    check_decode(head, a, np.array(off), [slot], o, f"{m} {slot}")
+
+
+def test_no_lines(rh):
+    """Without lines every row is the head's, and no table is read."""
+    rng = np.random.default_rng(18)
+    h = ac.Head(rh, rng, 100, 80, True, 2, 4)
+    a = rows(rng, h, 50)
+    d, out = tc.up(a), tc.Out((50, 100), np.float32)
+    h.rh._check(h.rh._lib.lib().ppocr_ra_logits_dev(h.head.handle, d.p, 50, None, 0, None, out.p, None, 0, None))
+    tc.close(out.get(), *h.exact(a, np.full(50, -1)), "no lines")
+
+
 def test_slots_beyond_the_first_thousand(rh):
     rng = np.random.default_rng(11)
     h = ac.Head(rh, rng, 64, 80, True, 4096, 1, ranks=[0] * 4096)
