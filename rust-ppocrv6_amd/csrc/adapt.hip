@@ -188,24 +188,47 @@ int64_t plan_units(int64_t m, int64_t groups, int unit) { return m / unit + grou
 // line, and of lines that name no slot, form a group of their own.
 //
 // Where the offsets rise, whole lines are counted and placed (a wave a line, or a thread a line where they are
-// short; the rows before the first and behind the last line are two lines more).  Otherwise each row looks for
-// its line, the last whose offset is not above it, so that each is placed once whatever the offsets hold.
-// 256 lines of 120: PLANUS us, by rows 95.
+// short; the rows before the first and behind the last line are two lines more); the first kSpans are kept in LDS
+// between the two.  Otherwise each row looks for its line, the last whose offset is not above it, so that each is
+// placed once whatever the offsets hold.  Latency bound: 256 lines of 120 PLANUS us (by rows 95), of which most is three
+// memory round trips.
+constexpr int kSpans = 1024;
+struct Span {
+    int lo, hi, g;
+};
 __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int slots, int unit, Plan plan) {
     extern __shared__ int groups[];
-    int* count = groups;              // [slots + 1] rows of a group
-    int* first = groups + slots + 1;  // its first unit
+    __shared__ Span kept[kSpans];
+    int* count = groups;                // [slots + 1] rows of a group
+    int* some = groups + slots + 1;     // a row of it
+    int* start = some + slots + 1;      // its first place
+    int* cursor = start + slots + 1;    // its next place
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int g = tid; g <= slots; g += 1024) count[g] = 0;
-    bool rising = true;
-    for (int64_t i = tid; i <= lines.lines && lines.lines > 0; i += 1024) {
-        const int64_t o = lines.off[i];
-        rising &= o >= 0 && o <= m && (i == 0 || lines.off[i - 1] <= o);
-    }
-    rising = __syncthreads_and(rising);
     auto group_of_line = [&](int64_t i) -> int {
         const int s = lines.slot[i];
         return s >= 0 && s < slots ? s : slots;
+    };
+    // Line i of lines.lines + 2; no rows where its offsets do not rise within [0, m].
+    auto span = [&](int64_t i, bool& ok) {
+        if (lines.lines == 0) return Span{0, i == 0 ? m : 0, slots};
+        const bool inner = i < lines.lines;
+        const int64_t a = i == lines.lines ? 0 : lines.off[inner ? i : lines.lines];
+        const int64_t b = inner ? lines.off[i + 1] : i == lines.lines ? lines.off[0] : m;
+        const bool good = a >= 0 && a <= b && b <= m;
+        ok &= good;
+        return Span{good ? (int)a : 0, good ? (int)b : 0, inner ? group_of_line(i) : slots};
+    };
+    const int64_t spans = lines.lines + 2;
+    bool rising = true;
+    for (int64_t i = tid; i < spans; i += 1024) {
+        const Span s = span(i, rising);
+        if (i < kSpans) kept[i] = s;
+    }
+    for (int g = tid; g <= slots; g += 1024) count[g] = some[g] = 0;
+    rising = __syncthreads_and(rising);
+    auto span_again = [&](int64_t i) {
+        bool ok = true;
+        return i < kSpans ? kept[i] : span(i, ok);
     };
     auto group_of = [&](int r) -> int {
         int64_t lo = 0, hi = lines.lines;  // off[lo] <= r < off[hi], if offsets rise
@@ -218,37 +241,32 @@ __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int
         if (lines.off[lo + 1] <= r) return slots;
         return group_of_line(lo);
     };
-    // a place in its group for each lane's row: lanes of one group together where the wave's rows all have it
-    auto take = [&](bool on, int g) -> int {
+    // a count of its group for each lane's row: lanes of one group together where the wave's rows all have it
+    auto take = [&](int* counts, bool on, int g) -> int {
         const unsigned long long mask = __ballot(on);
         if (mask == 0ull) return 0;
         const int leader = __ffsll((long long)mask) - 1;
         const int g0 = __shfl(g, leader, 64);
         if (__ballot(on && g != g0) == 0ull) {
             int base = 0;
-            if (lane == leader) base = atomicAdd(&count[g0], __popcll(mask));
+            if (lane == leader) base = atomicAdd(&counts[g0], __popcll(mask));
             return __shfl(base, leader, 64) + __popcll(mask & ((1ull << lane) - 1ull));
         }
-        return on ? atomicAdd(&count[g], 1) : 0;
-    };
-    // Line i of lines.lines + 2: its rows and its group.
-    struct Span {
-        int lo, hi, g;
-    };
-    auto span = [&](int64_t i) {
-        if (i < lines.lines) return Span{(int)lines.off[i], (int)lines.off[i + 1], group_of_line(i)};
-        if (i == lines.lines) return Span{0, lines.lines ? (int)lines.off[0] : m, slots};
-        return Span{lines.lines ? (int)lines.off[lines.lines] : m, m, slots};
+        return on ? atomicAdd(&counts[g], 1) : 0;
     };
     if (rising) {
-        for (int64_t i = tid; i < lines.lines + 2; i += 1024) {
-            const Span s = span(i);
-            if (s.hi > s.lo) atomicAdd(&count[s.g], s.hi - s.lo);
+        for (int64_t i = tid; i < spans; i += 1024) {
+            const Span s = span_again(i);
+            if (s.hi > s.lo) {
+                atomicAdd(&count[s.g], s.hi - s.lo);
+                some[s.g] = s.lo;  // any of them
+            }
         }
     } else {
         for (int r0 = 0; r0 < m; r0 += 1024) {
-            const int r = r0 + tid;
-            (void)take(r < m, r < m ? group_of(r) : 0);
+            const int r = r0 + tid, g = r < m ? group_of(r) : 0;
+            (void)take(count, r < m, g);
+            if (r < m) some[g] = r;
         }
     }
     __syncthreads();
@@ -263,58 +281,42 @@ __global__ __launch_bounds__(1024) void plan_kernel(AdaptLines lines, int m, int
                 const int v = __shfl_up(upto, o, 64);
                 if (lane >= o) upto += v;
             }
-            if (g <= slots) first[g] = before + upto - mine;
+            if (g <= slots) start[g] = cursor[g] = (before + upto - mine) * unit;
             before += __shfl(upto, 63, 64);
         }
         if (lane == 0) *plan.units = before;
     }
     __syncthreads();
-    // the units' slots
+    // the units' slots, and the places that the last unit of a group has no row for
     for (int g = tid; g <= slots; g += 1024) {
-        const int n = count[g], units = (n + unit - 1) / unit;
-        for (int u = 0; u < units; ++u) plan.slot[first[g] + u] = g;
-        count[g] = 0;
+        const int n = count[g], first = start[g] / unit;
+        for (int u = 0; u * unit < n; ++u) plan.slot[first + u] = g;
+        for (int x = n; x % unit; ++x) plan.rows[start[g] + x] = some[g];
     }
-    __syncthreads();
     if (rising) {
-        const bool brief = m / max(lines.lines, (int64_t)1) < 16;
-        for (int64_t i = brief ? tid : wave; i < lines.lines + 2; i += brief ? 1024 : 16) {
-            const Span s = span(i);
-            if (s.hi <= s.lo) continue;
-            if (brief && s.hi - s.lo < 1024) {
-                int* to = plan.rows + first[s.g] * unit + atomicAdd(&count[s.g], s.hi - s.lo);
+        // a thread a line where they are short, a wave where they are not
+        const int most = m / max(lines.lines, (int64_t)1) < 16 ? 1024 : 0;
+        if (most)
+            for (int64_t i = tid; i < spans; i += 1024) {
+                const Span s = span_again(i);
+                if (s.hi <= s.lo || s.hi - s.lo >= most) continue;
+                int* to = plan.rows + atomicAdd(&cursor[s.g], s.hi - s.lo);
                 for (int r = s.lo; r < s.hi; ++r) to[r - s.lo] = r;
-            } else if (!brief) {
-                int at = 0;
-                if (lane == 0) at = atomicAdd(&count[s.g], s.hi - s.lo);
-                int* to = plan.rows + first[s.g] * unit + __shfl(at, 0, 64);
-                for (int r = s.lo + lane; r < s.hi; r += 64) to[r - s.lo] = r;
             }
-        }
-        if (brief) {
-            // the few long lines among brief ones, by waves
-            for (int64_t i = wave; i < lines.lines + 2; i += 16) {
-                const Span s = span(i);
-                if (s.hi - s.lo < 1024) continue;
-                int at = 0;
-                if (lane == 0) at = atomicAdd(&count[s.g], s.hi - s.lo);
-                int* to = plan.rows + first[s.g] * unit + __shfl(at, 0, 64);
-                for (int r = s.lo + lane; r < s.hi; r += 64) to[r - s.lo] = r;
-            }
+        for (int64_t i = wave; i < spans; i += 16) {
+            const Span s = span_again(i);
+            if (s.hi <= s.lo || s.hi - s.lo < most) continue;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&cursor[s.g], s.hi - s.lo);
+            int* to = plan.rows + __shfl(at, 0, 64);
+            for (int r = s.lo + lane; r < s.hi; r += 64) to[r - s.lo] = r;
         }
     } else {
         for (int r0 = 0; r0 < m; r0 += 1024) {
             const int r = r0 + tid;
-            const int g = r < m ? group_of(r) : 0;
-            const int at = take(r < m, g);
-            if (r < m) plan.rows[first[g] * unit + at] = r;
+            const int at = take(cursor, r < m, r < m ? group_of(r) : 0);
+            if (r < m) plan.rows[at] = r;
         }
-    }
-    __syncthreads();  // the rows are placed, count is the groups' again
-    for (int g = tid; g <= slots; g += 1024) {
-        const int n = count[g];
-        int* rows = plan.rows + first[g] * unit;
-        for (int x = n; x % unit; ++x) rows[x] = rows[0];
     }
 }
 
@@ -886,7 +888,7 @@ int make_plan(const Adapters& ad, const AdaptLines& lines, int64_t m, int unit, 
                  one ? lines.off : nullptr, one ? lines.slot : nullptr};
     *units = plan_units(m, std::min<int64_t>(std::min<int64_t>(ad.slots, lines.lines) + 1, m), unit);
     if (one) return PPOCR_OK;
-    plan_kernel<<<1, 1024, (size_t)(ad.slots + 1) * 8, st>>>(lines, (int)m, ad.slots, unit, *plan);
+    plan_kernel<<<1, 1024, (size_t)(ad.slots + 1) * 16, st>>>(lines, (int)m, ad.slots, unit, *plan);
     PPOCR_HIP(hipGetLastError());
     return PPOCR_OK;
 }
