@@ -43,7 +43,8 @@ __device__ __forceinline__ uint16_t down(float v, uint16_t) { return __builtin_b
 
 template <typename T>
 struct alignas(16) Wide {
-    T v[16 / sizeof(T)];
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
 };
 
 // The tensor that a chunk belongs to.
@@ -57,49 +58,78 @@ __device__ __forceinline__ int tensor_of(const Table& t, int chunk) {
     return lo;
 }
 
+// A chunk's values in a thread's registers: 16 bytes at a time where the tensor is aligned to that, else value by
+// value.  All loads are issued together, from addresses held inside the chunk; values past its end count as 0.
 template <typename T>
-__device__ __forceinline__ double chunk_squares(const void* in, int64_t at, int n) {
-    constexpr int V = 16 / sizeof(T), R = kChunkBytes / 16 / kThreads;
-    const T* p = (const T*)in + at;
-    double s = 0.0;
-    if (reinterpret_cast<uintptr_t>(in) % 16 == 0 && n == kChunkBytes / (int)sizeof(T)) {
-        Wide<T> w[R];
+struct Chunk {
+    static constexpr int V = Wide<T>::N, R = kChunkBytes / 16 / kThreads;
+    Wide<T> w[R];
+    // the values of piece r that are the chunk's own
+    static __device__ __forceinline__ int place(bool wide, int r, int v) {
+        const int x = r * kThreads + threadIdx.x;
+        return wide ? x * V + v : (r * V + v) * kThreads + (int)threadIdx.x;
+    }
+    __device__ __forceinline__ void load(const T* p, int n, bool wide) {
+        if (wide) {
+            const int last = (n - 1) / V;  // the last piece may reach past the chunk: then value by value
+            const bool whole = n % V == 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r) w[r] = reinterpret_cast<const Wide<T>*>(p)[r * kThreads + threadIdx.x];
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const double x = (double)up(w[r].v[v]);
-                s = fma(x, x, s);
+            for (int r = 0; r < R; ++r) {
+                const int x = min(r * kThreads + (int)threadIdx.x, whole ? last : max(last - 1, 0));
+                if (whole || last > 0) w[r] = reinterpret_cast<const Wide<T>*>(p)[x];
             }
-    } else {
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const double x = (double)up(p[i]);
-            s = fma(x, x, s);
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if (r * kThreads + (int)threadIdx.x == last) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) w[r].v[v] = p[min(last * V + v, n - 1)];
+                    }
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int v = 0; v < V; ++v) w[r].v[v] = p[min(place(false, r, v), n - 1)];
         }
     }
+};
+
+template <typename T>
+__device__ __forceinline__ double chunk_squares(const void* in, int64_t at, int n) {
+    using C = Chunk<T>;
+    const bool wide = reinterpret_cast<uintptr_t>(in) % 16 == 0;
+    C c;
+    c.load((const T*)in + at, n, wide);
+    double s = 0.0;
+#pragma unroll
+    for (int r = 0; r < C::R; ++r)
+#pragma unroll
+        for (int v = 0; v < C::V; ++v) {
+            const double x = C::place(wide, r, v) < n ? (double)up(c.w[r].v[v]) : 0.0;
+            s = fma(x, x, s);
+        }
     return s;
 }
 
 template <typename T>
 __device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t at, int n, float scale) {
-    constexpr int V = 16 / sizeof(T), R = kChunkBytes / 16 / kThreads;
-    const T* p = (const T*)in + at;
+    using C = Chunk<T>;
     T* q = (T*)out + at;
-    if ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) % 16 == 0 &&
-        n == kChunkBytes / (int)sizeof(T)) {
-        Wide<T> w[R];
+    const bool wide = (reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) % 16 == 0;
+    C c;
+    c.load((const T*)in + at, n, wide);
 #pragma unroll
-        for (int r = 0; r < R; ++r) w[r] = reinterpret_cast<const Wide<T>*>(p)[r * kThreads + threadIdx.x];
+    for (int r = 0; r < C::R; ++r) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
+        for (int v = 0; v < C::V; ++v) c.w[r].v[v] = down(up(c.w[r].v[v]) * scale, T());
+        if (wide && C::place(true, r, C::V - 1) < n) {
+            reinterpret_cast<Wide<T>*>(q)[r * kThreads + threadIdx.x] = c.w[r];
+        } else {
 #pragma unroll
-            for (int v = 0; v < V; ++v) w[r].v[v] = down(up(w[r].v[v]) * scale, T());
-            reinterpret_cast<Wide<T>*>(q)[r * kThreads + threadIdx.x] = w[r];
+            for (int v = 0; v < C::V; ++v)
+                if (C::place(wide, r, v) < n) q[C::place(wide, r, v)] = c.w[r].v[v];
         }
-    } else {
-        for (int i = threadIdx.x; i < n; i += kThreads) q[i] = down(up(p[i]) * scale, T());
     }
 }
 
@@ -115,12 +145,20 @@ __device__ __forceinline__ double block_sum(double s, double* red) {
     return s;
 }
 
+// A workgroup takes chunks one behind the other, so that it looks for its tensor once: chunks `first` .. `last`.
+__device__ __forceinline__ void share_of(int chunks, int* first, int* last) {
+    const int each = chunks / (int)gridDim.x, more = chunks % (int)gridDim.x, b = blockIdx.x;
+    *first = b * each + min(b, more);
+    *last = *first + each + (b < more ? 1 : 0);
+}
+
 __global__ __launch_bounds__(kThreads) void squares_kernel(Table t, double* __restrict__ parts) {
     __shared__ double red[kThreads / 64];
-    const int chunks = t.first[t.tensors];
+    int c, last;
+    share_of(t.first[t.tensors], &c, &last);
     double s = 0.0;
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int i = tensor_of(t, c);
+    for (int i = c < last ? tensor_of(t, c) : 0; c < last; ++c) {
+        if (c >= t.first[i + 1]) ++i;
         const int per = kChunkBytes / (t.bf16[i] ? 2 : 4);
         const int64_t at = (int64_t)(c - t.first[i]) * per;
         const int n = (int)min((int64_t)per, t.count[i] - at);
@@ -136,14 +174,17 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Table t, const double* 
                                                          float* __restrict__ norm_out) {
     __shared__ double red[kThreads / 64];
     double s = 0.0;
+#pragma unroll 4
     for (int64_t i = threadIdx.x; i < nparts; i += kThreads) s += parts[i];
     const double norm = sqrt(block_sum(s, red));
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     // gradients whose norm is no finite number stay as they are: the caller sees the norm
     const float scale = norm > (double)most && norm < (double)INFINITY ? (float)((double)most / norm) : 1.0f;
-    const int chunks = t.first[t.tensors];
-    for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
-        const int i = tensor_of(t, c);
+    int first, last;
+    share_of(t.first[t.tensors], &first, &last);
+    int c = last - 1;
+    for (int i = c >= first ? tensor_of(t, c) : 0; c >= first; --c) {
+        if (c < t.first[i]) --i;
         if (scale == 1.0f && t.in[i] == t.out[i]) continue;
         const int per = kChunkBytes / (t.bf16[i] ? 2 : 4);
         const int64_t at = (int64_t)(c - t.first[i]) * per;
