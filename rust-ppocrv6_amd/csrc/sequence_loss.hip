@@ -28,17 +28,40 @@ struct Sums {
     int x, y;
 };
 
-// Sums over the lanes of a team, the same in each lane.  For G > 64 through LDS, every lane of the
-// workgroup (one team) calling it.
+// v plus the value of a lane of the same 16, through the registers' own lane paths.
+template <int CTRL>
+__device__ __forceinline__ double add_lane(double v) {
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)u, CTRL, 0xF, 0xF, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(u >> 32), CTRL, 0xF, 0xF, true);
+    return v + __builtin_bit_cast(double, ((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
+}
+// Sum over a team's lanes of the wave: neighbours, pairs, then the mirror images within 8 and 16 lanes, which hold the
+// other half's sums.
+template <int G>
+__device__ __forceinline__ double lane_sum(double v) {
+    v = add_lane<0xB1>(v);   // lanes 1 0 3 2
+    v = add_lane<0x4E>(v);   // lanes 2 3 0 1
+    v = add_lane<0x141>(v);  // mirrored in 8
+    v = add_lane<0x140>(v);  // mirrored in 16
+    if constexpr (G >= 32) v += __shfl_xor(v, 16, 64);
+    if constexpr (G >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+// Lanes of this lane's team (of its wave, for larger teams) that hold `on`.
+template <int G>
+__device__ __forceinline__ int team_count(bool on) {
+    const unsigned long long mask = __ballot(on);
+    if constexpr (G >= 64) return __popcll(mask);
+    else return __popcll((mask >> (threadIdx.x & 63 & ~(G - 1))) & ((1ull << G) - 1));
+}
+
+// Sums over the lanes of a team, the same in each lane; the counts are those of its waves already.  For G > 64
+// through LDS, every lane of the workgroup (one team) calling it.
 template <int G>
 __device__ __forceinline__ Sums team_sum(Sums v, Sums* red) {
-#pragma unroll
-    for (int o = (G < 64 ? G : 64) / 2; o >= 1; o >>= 1) {
-        v.a += __shfl_xor(v.a, o, 64);
-        v.b += __shfl_xor(v.b, o, 64);
-        v.x += __shfl_xor(v.x, o, 64);
-        v.y += __shfl_xor(v.y, o, 64);
-    }
+    v.a = lane_sum<G>(v.a);
+    v.b = lane_sum<G>(v.b);
     if constexpr (G > 64) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -54,24 +77,26 @@ __device__ __forceinline__ Sums team_sum(Sums v, Sums* red) {
     return v;
 }
 
-__device__ __forceinline__ int64_t clamp_row(int64_t r, int64_t m) { return r < 0 ? 0 : r > m ? m : r; }
+// Steps are numbered in 32 bits (the entry points take up to 2^30): an array's element is its base, the same for the
+// wave, and a 32-bit offset.
+__device__ __forceinline__ unsigned clamp_row(int64_t r, int64_t m) { return (unsigned)(r < 0 ? 0 : r > m ? m : r); }
 
 // The steps that no line covers have no gradient: workgroup `part` of `parts` clears its share.
 __device__ __forceinline__ void clear_uncovered(const LineSteps& s, float* row_grad, int part, int parts) {
-    int64_t first = s.m, last = s.m;
+    unsigned first = (unsigned)s.m, last = first;
     if (s.lines > 0) {
         first = clamp_row(s.off[0], s.m);
         last = max(clamp_row(s.off[s.lines], s.m), first);
     }
-    const int64_t step = (int64_t)parts * blockDim.x;
-    for (int64_t r = (int64_t)part * blockDim.x + threadIdx.x; r < first; r += step) row_grad[r] = 0.0f;
-    for (int64_t r = last + (int64_t)part * blockDim.x + threadIdx.x; r < s.m; r += step) row_grad[r] = 0.0f;
+    const unsigned step = parts * blockDim.x;
+    for (unsigned r = part * blockDim.x + threadIdx.x; r < first; r += step) row_grad[r] = 0.0f;
+    for (unsigned r = last + part * blockDim.x + threadIdx.x; r < (unsigned)s.m; r += step) row_grad[r] = 0.0f;
 }
 
-// e^t - t - 1 to a few units of the last place: near 0 by its series, whose terms up to t^13 / 13! leave
-// less than 2^-26 of the value at |t| = 1, as the difference would lose all of it.
-__device__ __forceinline__ float exp_tail(float t, float em1) {
-    if (__builtin_fabsf(t) >= 1.0f) return em1 - t;
+// e^t - t - 1 (kl) and e^t - 1 (em1) to a few units of the last place.  Below 1 by the series of the first, whose terms up
+// to t^13 / 13! leave less than 2^-26 of the value at |t| = 1, as the difference would lose all of it near 0; the
+// second is the first plus t.
+__device__ __forceinline__ void exp_tail(float t, float& kl, float& em1) {
     float p = 1.0f / 6227020800.0f;
     p = fmaf(p, t, 1.0f / 479001600.0f);
     p = fmaf(p, t, 1.0f / 39916800.0f);
@@ -84,12 +109,18 @@ __device__ __forceinline__ float exp_tail(float t, float em1) {
     p = fmaf(p, t, 1.0f / 24.0f);
     p = fmaf(p, t, 1.0f / 6.0f);
     p = fmaf(p, t, 0.5f);
-    return p * t * t;
+    kl = p * t * t;
+    em1 = kl + t;
+    if (!(__builtin_fabsf(t) < 1.0f)) {
+        const float e = expf(t);
+        em1 = e - 1.0f;
+        kl = em1 - t;
+    }
 }
 
 struct PolicyRow {
     float x, old, ref, adv;
-    bool there;
+    int target;
 };
 
 // Which side of the clipping's border a step lies on is decided on the difference of the logarithms in 64
@@ -110,18 +141,16 @@ __global__ __launch_bounds__(threads_of(G)) void policy_kernel(LineSteps s, Poli
     const int l = threadIdx.x % G;
     const int64_t line = (int64_t)blockIdx.x * TEAMS + threadIdx.x / G;
     if (line >= s.lines) return;  // G > 64: the same for the workgroup
-    const int64_t lo = clamp_row(s.off[line], s.m), hi = max(clamp_row(s.off[line + 1], s.m), lo);
+    const unsigned lo = clamp_row(s.off[line], s.m), hi = max(clamp_row(s.off[line + 1], s.m), lo);
     const float line_adv = a.per_row ? 0.0f : a.adv[line];
 
-    auto fetch = [&](int64_t r) {
-        PolicyRow p{0.0f, 0.0f, 0.0f, line_adv, false};
-        if (r < hi) {
-            p.there = !s.target || s.target[r] >= 0;
-            p.x = s.loss[r];
-            p.old = a.old[r];
-            if constexpr (REF) p.ref = a.ref[r];
-            if (a.per_row) p.adv = a.adv[r];
-        }
+    // loads that nothing stands between: of a step of the line in any case, what they hold is looked at later
+    auto fetch = [&](unsigned r) {
+        const unsigned at = min(r, hi - 1);
+        PolicyRow p{s.loss[at], a.old[at], 0.0f, line_adv, 0};
+        if constexpr (REF) p.ref = a.ref[at];
+        if (a.per_row) p.adv = a.adv[at];
+        if (s.target) p.target = s.target[at];
         return p;
     };
     // the step's gradient; its value, divergence and clipping into v, kl and cut
@@ -134,8 +163,8 @@ __global__ __launch_bounds__(threads_of(G)) void policy_kernel(LineSteps s, Poli
         float slope = cut || p.adv == 0.0f ? 0.0f : ratio * p.adv;
         kl = 0.0f;
         if constexpr (REF) {
-            const float t = p.x - p.ref, em1 = expm1f(t);
-            kl = exp_tail(t, em1);
+            float em1;
+            exp_tail(p.x - p.ref, kl, em1);
             v = fmaf(a.beta, kl, v);
             slope = fmaf(a.beta, em1, slope);
         }
@@ -145,35 +174,35 @@ __global__ __launch_bounds__(threads_of(G)) void policy_kernel(LineSteps s, Poli
     Sums sum{0.0, 0.0, 0, 0};
     float slope[kKeep];
     bool there[kKeep];
-    for (int64_t base = lo; base < hi; base += kKeep * G) {
+    for (unsigned base = lo; base < hi; base += kKeep * G) {
         PolicyRow p[kKeep];
 #pragma unroll
         for (int i = 0; i < kKeep; ++i) p[i] = fetch(base + i * G + l);
 #pragma unroll
         for (int i = 0; i < kKeep; ++i) {
+            there[i] = false;
+            if (base + i * G >= hi) continue;  // the same for the team: places that no lane has a step for
             float v, kl;
             bool cut;
             slope[i] = eval(p[i], v, kl, cut);
-            there[i] = p[i].there;
-            if (there[i]) {
-                sum.a += (double)v;
-                sum.b += (double)kl;
-                sum.x += 1;
-                sum.y += cut ? 1 : 0;
-            }
+            there[i] = base + i * G + l < hi && p[i].target >= 0;
+            sum.a += there[i] ? (double)v : 0.0;
+            if constexpr (REF) sum.b += there[i] ? (double)kl : 0.0;
+            sum.x += team_count<G>(there[i]);
+            sum.y += team_count<G>(there[i] && cut);
         }
     }
     sum = team_sum<G>(sum, red);
     const float count = (float)max(sum.x, 1);
     if (l == 0) {
-        if (a.loss) a.loss[line] = (float)(sum.a / (double)count);
-        if (a.kl) a.kl[line] = (float)(sum.b / (double)count);
+        if (a.loss) a.loss[line] = (float)sum.a / count;
+        if (a.kl) a.kl[line] = (float)sum.b / count;
         if (a.clipped) a.clipped[line] = (float)sum.y / count;
     }
     if (!a.row_grad) return;
     const float g = a.grad ? a.grad[line] : 1.0f;
     const float share = g / count;
-    auto put = [&](int64_t r, bool on, float d) {
+    auto put = [&](unsigned r, bool on, float d) {
         if (r < hi) a.row_grad[r] = on && g != 0.0f ? share * d : 0.0f;
     };
     if (hi - lo <= kKeep * G) {
@@ -181,7 +210,7 @@ __global__ __launch_bounds__(threads_of(G)) void policy_kernel(LineSteps s, Poli
         for (int i = 0; i < kKeep; ++i) put(lo + i * G + l, there[i], slope[i]);
         return;
     }
-    for (int64_t base = lo; base < hi; base += kKeep * G) {
+    for (unsigned base = lo; base < hi; base += kKeep * G) {
         PolicyRow p[kKeep];
 #pragma unroll
         for (int i = 0; i < kKeep; ++i) p[i] = fetch(base + i * G + l);
@@ -189,7 +218,7 @@ __global__ __launch_bounds__(threads_of(G)) void policy_kernel(LineSteps s, Poli
         for (int i = 0; i < kKeep; ++i) {
             float v, kl;
             bool cut;
-            put(base + i * G + l, p[i].there, eval(p[i], v, kl, cut));
+            put(base + i * G + l, p[i].target >= 0, eval(p[i], v, kl, cut));
         }
     }
 }
@@ -208,46 +237,48 @@ __global__ __launch_bounds__(threads_of(G)) void preference_kernel(LineSteps s, 
     const int l = threadIdx.x % G;
     const int64_t pair = (int64_t)blockIdx.x * TEAMS + threadIdx.x / G;
     if (2 * pair >= s.lines) return;  // G > 64: the same for the workgroup
-    const int64_t o0 = clamp_row(s.off[2 * pair], s.m), o1 = clamp_row(s.off[2 * pair + 1], s.m);
-    const int64_t o2 = clamp_row(s.off[2 * pair + 2], s.m);
+    const unsigned o0 = clamp_row(s.off[2 * pair], s.m), o1 = clamp_row(s.off[2 * pair + 1], s.m);
+    const unsigned o2 = clamp_row(s.off[2 * pair + 2], s.m);
     // step t of the pair: the chosen line's steps, then the other's
-    const int64_t la = max(o1 - o0, (int64_t)0), len = la + max(o2 - o1, (int64_t)0);
-    auto row_of = [&](int64_t t) { return t < la ? o0 + t : o1 + (t - la); };
+    const unsigned la = o1 > o0 ? o1 - o0 : 0, len = la + (o2 > o1 ? o2 - o1 : 0);
+    const unsigned from_a = o0, from_b = o1 - la;  // (modulo 2^32)
+    auto row_of = [&](unsigned t) { return (t < la ? from_a : from_b) + t; };
     Sums sum{0.0, 0.0, 0, 0};
     unsigned on = 0;
     int at = 0;
-    for (int64_t base = 0; base < len; base += kKeep * G) {
+    for (unsigned base = 0; base < len; base += kKeep * G) {
         float x[kKeep], ref[kKeep];
-        bool there[kKeep];
+        int target[kKeep];
 #pragma unroll
         for (int i = 0; i < kKeep; ++i) {
-            const int64_t t = base + i * G + l;
-            x[i] = ref[i] = 0.0f;
-            there[i] = false;
-            if (t < len) {
-                const int64_t r = row_of(t);
-                there[i] = !s.target || s.target[r] >= 0;
-                x[i] = s.loss[r];
-                if constexpr (REF) ref[i] = a.ref[r];
-            }
+            const unsigned r = row_of(min(base + i * G + l, len - 1));
+            x[i] = s.loss[r];
+            ref[i] = 0.0f;
+            if constexpr (REF) ref[i] = a.ref[r];
+            target[i] = s.target ? s.target[r] : 0;
         }
 #pragma unroll
         for (int i = 0; i < kKeep; ++i) {
-            const double gain = there[i] ? (double)ref[i] - (double)x[i] : 0.0;
-            if (base + i * G + l < la) {
-                sum.a += gain;
-                sum.x += there[i] ? 1 : 0;
-            } else {
-                sum.b += gain;
-                sum.y += there[i] ? 1 : 0;
-            }
-            if (at < kBits) on |= (there[i] ? 1u : 0u) << at;
+            if (base + i * G >= len) break;  // the same for the team
+            const bool there = base + i * G + l < len && target[i] >= 0;
+            const double gain = there ? (double)ref[i] - (double)x[i] : 0.0;
+            const bool chosen = base + i * G + l < la;
+            sum.a += chosen ? gain : 0.0;
+            sum.b += chosen ? 0.0 : gain;
+            sum.x += team_count<G>(there && chosen);
+            sum.y += team_count<G>(there && !chosen);
+            if (at < kBits) on |= (there ? 1u : 0u) << at;
             ++at;
         }
     }
     sum = team_sum<G>(sum, red);
-    const double wa = a.average ? (double)a.beta / max(sum.x, 1) : (double)a.beta;
-    const double wb = a.average ? (double)a.beta / max(sum.y, 1) : (double)a.beta;
+    double wa = a.beta, wb = wa;
+    if (a.average) {
+        // both weights from one division
+        const double na = max(sum.x, 1), nb = max(sum.y, 1), each = wa / (na * nb);
+        wa = each * nb;
+        wb = each * na;
+    }
     const double ra = wa * sum.a, rb = wb * sum.b, h = ra - rb;
     // s(-|h|) = e / (1 + e) with e = exp(-|h|), the rounding of |h| to 32 bits put back into the exponential
     const double big = __builtin_fabs(h);
@@ -255,7 +286,8 @@ __global__ __launch_bounds__(threads_of(G)) void preference_kernel(LineSteps s, 
     const float left = hf < INFINITY ? (float)(big - (double)hf) : 0.0f;
     const float e = expf(-hf) * (1.0f - left);
     const float small = e / (1.0f + e), large = 1.0f / (1.0f + e);
-    const float soft = log1pf(e);
+    // log(1 + e), what the sum lost put back
+    const float one = 1.0f + e, soft = logf(one) + (e - (one - 1.0f)) / one;
     const float up = h >= 0.0 ? soft : hf + soft, down = h >= 0.0 ? hf + soft : soft;  // -log s(h), -log s(-h)
     const float keep = 1.0f - a.smoothing;
     if (l == 0) {
@@ -270,8 +302,8 @@ __global__ __launch_bounds__(threads_of(G)) void preference_kernel(LineSteps s, 
     const float slope = a.smoothing * (h >= 0.0 ? large : small) - keep * (h >= 0.0 ? small : large);
     const float da = g == 0.0f ? 0.0f : -g * slope * (float)wa, db = g == 0.0f ? 0.0f : g * slope * (float)wb;
     at = 0;
-    for (int64_t t = l; t < len; t += G, ++at) {
-        const int64_t r = row_of(t);
+    for (unsigned t = l; t < len; t += G, ++at) {
+        const unsigned r = row_of(t);
         const bool there = at < kBits ? (on >> at) & 1u : !s.target || s.target[r] >= 0;
         a.row_grad[r] = there ? (t < la ? da : db) : 0.0f;
     }
