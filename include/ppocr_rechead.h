@@ -446,12 +446,14 @@ int ppocr_layernorm_backward_dev(void* d_dy, void* d_x, const float* d_w, const 
 /* ---------------------------------------------------------------- adapting the head
  * No counterpart in the reference, which has one head: many users' versions of it, each a low-rank
  * adapter beside the shared weights, and the rest of what they are trained with.  Types, workspaces, streams and
- * equal bits as for the training entry points above. */
+ * equal bits as for the training entry points above.  No output may overlap an input or another output, but where it
+ * says so. */
 
 /* A head with `slots` (1 to 4096) places for adapters of up to max_rank (1 to 64): a handle on the same
  * weights, which every ppocr_rh_ call takes as it takes `head` (without any adapter), with device
- * memory for the adapters of about 4 n max_rank bytes a slot (max_rank rounded up to 16, 32 or 64).  `head` and the new handle may be destroyed in any order.  Heads that
- * the matrix kernels take (k of 73 to 80 or 113 to 120, an FP32 head's weights below 32768) only. */
+ * memory for the adapters of about 4 n max_rank bytes a slot (max_rank rounded up to 16, 32 or 64).  `head` and the
+ * new handle may be destroyed in any order.  Heads that the matrix kernels take (k of 73 to 80 or 113 to 120, an FP32
+ * head's weights below 32768, an INT8 head's scales 2^-34 at least and within 2^40 of each other) only. */
 int ppocr_ra_create(const ppocr_rh_t* head, int64_t slots, int64_t max_rank, ppocr_rh_t** out);
 void ppocr_ra_destroy(ppocr_rh_t* h); /* ppocr_rh_destroy */
 int ppocr_ra_shape(const ppocr_rh_t* h, int64_t* slots, int64_t* max_rank);
@@ -469,9 +471,11 @@ int ppocr_ra_set_dev(ppocr_rh_t* h, int64_t slot, void* d_down, void* d_up, int6
  * that no line covers.  The `_dev` forms read the lines on the device as ppocr_rh_decode_dev does; a row
  * that lies in several lines (offsets that go backwards) takes the adapter of one of them.
  * Both operands of every product are fp16 halves (three products of 11 bits each, int8 weights exactly), the
- * rows at a power of two that their own largest value sets, summed in fp32: 22 bits of each row's largest
- * products, whatever the rows beside it hold.  A row that holds an infinity or NaN has NaN logits; decoded, it is class 0.
- * There is no mode and no precision guard. */
+ * rows at a power of two that their own largest value sets, summed in fp32: 22 bits of each row's and of the
+ * adapter's largest products, and the same bits whatever the rows beside it hold.  The head's products lose a bit for each
+ * power of two by which an adapter's largest scale |up| sum |down| passes 2^31 (an INT8 head: 2^22 times the largest of its
+ * scales, where they lie within 2^32 of each other).  A row that holds an infinity or NaN has NaN logits; decoded, it is class 0.  There is no mode and no
+ * precision guard. */
 size_t ppocr_ra_workspace_bytes(const ppocr_rh_t* h, int64_t m);
 int ppocr_ra_logits(const ppocr_rh_t* h, const float* a, const int64_t* line_off, int64_t lines, const int32_t* line_slot,
                     float* out);

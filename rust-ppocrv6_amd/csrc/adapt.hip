@@ -11,9 +11,9 @@
 // LDS, and each wave reads its adapter's tile from L2.
 //
 // Arithmetic: fp16 halves of both operands (22 bits), as the head's F16X2 mode, all in one fp32
-// accumulator: up is held divided by the class's scale.  Each row is scaled by the power of two that its
-// largest value sets, so rows of any size keep their bits, whatever the rows beside them hold, and no row
-// has to be computed again.  u = down a is computed by each wave before its first tile, from the rows it
+// accumulator: up is held divided by the class's unit (its scale, or where a head's lie far apart that times a
+// power of two).  Each row is scaled by the power of two that its largest value sets, so rows of any size keep
+// their bits, whatever the rows beside them hold, and no row has to be computed again.  u = down a is computed by each wave before its first tile, from the rows it
 // holds; the products' layout is that of the operand that the next product needs.
 #include <algorithm>
 
@@ -66,20 +66,20 @@ __global__ __launch_bounds__(64) void down_range_kernel(const T* __restrict__ do
 }
 
 // The value that the up records hold before their power of two.
-__device__ __forceinline__ float up_value(float v, float scale, float class_scale) { return v * scale / class_scale; }
+__device__ __forceinline__ float up_value(float v, float scale, float unit) { return v * scale / unit; }
 
-// range[1][t]: the largest |up[.][t]| over its class's scale (maxima of non-negative bits: any order gives the
+// range[1][t]: the largest |up[.][t]| over its class's unit (maxima of non-negative bits: any order gives the
 // same).
 template <typename T>
 __global__ __launch_bounds__(256) void up_range_kernel(const T* __restrict__ up, int rank, float scale,
-                                                       const float* __restrict__ class_scale, int64_t n, unsigned* range) {
+                                                       const float* __restrict__ unit, int64_t n, unsigned* range) {
     __shared__ unsigned top[kAdaptMostRank];
     if (threadIdx.x < kAdaptMostRank) top[threadIdx.x] = 0u;
     __syncthreads();
     const int64_t count = n * rank;
     for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < count; x += (int64_t)gridDim.x * 256) {
         const int64_t j = x / rank;
-        const float v = __builtin_fabsf(up_value(value<T>(up[x]), scale, class_scale[j]));
+        const float v = __builtin_fabsf(up_value(value<T>(up[x]), scale, unit[j]));
         if (v < INFINITY) atomicMax(&top[x - j * rank], __float_as_uint(v));
     }
     __syncthreads();
@@ -129,7 +129,7 @@ __device__ __forceinline__ int rank_of(int s, int h, int e) { return 32 * (s >> 
 // up record of a 32-class tile: [half][step][h][class][8].
 template <typename T>
 __global__ __launch_bounds__(256) void up_record_kernel(const T* __restrict__ up, int rank, float scale,
-                                                        const float* __restrict__ class_scale, int64_t n, int steps,
+                                                        const float* __restrict__ unit, int64_t n, int steps,
                                                         const unsigned* __restrict__ range, uint8_t* rec) {
     __shared__ int exps[kAdaptMostRank];
     if (threadIdx.x < kAdaptMostRank) exps[threadIdx.x] = (int)threadIdx.x < rank ? down_exp(range, threadIdx.x) : 0;
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void up_record_kernel(const T* __restrict__ up
         const int t = rank_of(s, h, e);
         const int64_t j = (int64_t)blockIdx.x * 32 + i;
         float v = 0.0f;
-        if (t < rank && j < n) v = ldexpf(up_value(value<T>(up[j * rank + t]), scale, class_scale[j]), exps[t] - shift);
+        if (t < rank && j < n) v = ldexpf(up_value(value<T>(up[j * rank + t]), scale, unit[j]), exps[t] - shift);
         const unsigned short hi = half_bits(v);
         p[x] = hi;
         p[per + x] = half_bits(v - (float)__builtin_bit_cast(_Float16, hi));
@@ -151,20 +151,20 @@ __global__ __launch_bounds__(256) void up_record_kernel(const T* __restrict__ up
 }
 
 template <typename T>
-int set_slot(const Adapters& ad, int slot, const T* down, const T* up, int rank, float scale, const float* class_scale, int64_t n,
-             int64_t k, hipStream_t st) {
+int set_slot(const Adapters& ad, int slot, const T* down, const T* up, int rank, float scale, int64_t n, int64_t k,
+             hipStream_t st) {
     unsigned* range = ad.range + (size_t)slot * 2 * kAdaptMostRank;
     down_range_kernel<T><<<kAdaptMostRank, 64, 0, st>>>(down, rank, (int)k, range);
     PPOCR_HIP(hipGetLastError());
     if (rank) {
         const unsigned grid = (unsigned)std::min<int64_t>((n * rank + 1023) / 1024, 1024);
-        up_range_kernel<T><<<grid, 256, 0, st>>>(up, rank, scale, class_scale, n, range);
+        up_range_kernel<T><<<grid, 256, 0, st>>>(up, rank, scale, ad.unit, n, range);
         PPOCR_HIP(hipGetLastError());
     }
     down_record_kernel<T><<<16, 256, 0, st>>>(down, rank, (int)k, ad.G, ad.steps, range, ad.down + slot * ad.down_bytes(),
                                               ad.meta + slot);
     PPOCR_HIP(hipGetLastError());
-    up_record_kernel<T><<<(unsigned)ad.tiles, 256, 0, st>>>(up, rank, scale, class_scale, n, ad.steps, range,
+    up_record_kernel<T><<<(unsigned)ad.tiles, 256, 0, st>>>(up, rank, scale, ad.unit, n, ad.steps, range,
                                                             ad.up + slot * ad.up_bytes());
     PPOCR_HIP(hipGetLastError());
     return PPOCR_OK;
@@ -190,7 +190,7 @@ int64_t plan_units(int64_t m, int64_t groups, int unit) { return m / unit + grou
 // Where the offsets rise, whole lines are counted and placed (a wave a line, or a thread a line where they are
 // short; the rows before the first and behind the last line are two lines more); the first kSpans are kept in LDS
 // between the two.  Otherwise each row looks for its line, the last whose offset is not above it, so that each is
-// placed once whatever the offsets hold.  Latency bound: 256 lines of 120 PLANUS us (by rows 95), of which most is three
+// placed once whatever the offsets hold.  Latency bound: 256 lines of 120 9 us (by rows 95), of which most is three
 // memory round trips.
 constexpr int kSpans = 1024;
 struct Span {
@@ -397,12 +397,14 @@ __device__ __forceinline__ void load_rows(const AdaptLaunch& x, int64_t row, int
         }
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     odd |= (bool)__shfl_xor((int)odd, 32, 64);
-    // The row's largest value comes to below 2^kTop, in the head's products 2^-shift of it.  A wave whose rows'
-    // largest values all lie in [0.5, 2^kTop) leaves them as they are: the low halves, whose smallest step is
-    // 2^-24, then still hold 24 bits of a row's largest value, and no logit needs the power undone.
-    o.scaled = shift != 0 || __any(!(top >= 0.5f && top < (float)(1 << kTop)));
+    // The row's largest value comes to below 2^kTop, in the head's products 2^-shift of it.  A row whose largest
+    // value lies in [0.5, 2^kTop) is left as it is, whatever the rows beside it need, so that its bits do not depend on
+    // them: the low halves, whose smallest step is 2^-24, then still hold 24 bits of that value.  Where that goes for
+    // all of a wave's rows, no logit needs the power undone.
+    const bool fits = shift == 0 && top >= 0.5f && top < (float)(1 << kTop);
+    o.scaled = __any(!fits);
     int ex = 0;
-    if (o.scaled && top > 0.0f && !odd) ex = max(min(kTop - 1 - ilogbf(top), 126), shift - 126);
+    if (!fits && top > 0.0f && !odd) ex = max(min(kTop - 1 - ilogbf(top), 126), shift - 126);
     o.inv = ldexpf(1.0f, shift - ex);
     const float to = ldexpf(1.0f, ex), lower = ldexpf(1.0f, -shift);
 #pragma unroll
@@ -893,14 +895,14 @@ int make_plan(const Adapters& ad, const AdaptLines& lines, int64_t m, int unit, 
     return PPOCR_OK;
 }
 
-AdaptLaunch launch_of(const TileGeom& tg, const uint8_t* rec, const Adapters& ad, const float* a, int64_t m, int64_t n, int64_t k,
+AdaptLaunch launch_of(const TileGeom& tg, const Adapters& ad, const float* a, int64_t m, int64_t n, int64_t k,
                       int64_t units, int nsplit, const Plan& plan) {
     AdaptLaunch x{};
     x.a = a;
     x.m = m;
     x.k = (int)k;
     x.vec = k % 4 == 0 && reinterpret_cast<uintptr_t>(a) % 16 == 0 ? 1 : 0;
-    x.rec = rec;
+    x.rec = ad.rec;
     x.tiles = tg.tiles;
     x.n = (int)n;
     x.nsplit = nsplit;
@@ -941,15 +943,15 @@ int launch_adapters_clear(const Adapters& ad, hipStream_t st) {
     return PPOCR_OK;
 }
 
-int launch_adapter_set(const Adapters& ad, int slot, const void* down, const void* up, int rank, float scale, int bf16,
-                       const float* class_scale, int64_t n, int64_t k, hipStream_t st) {
-    return bf16 ? set_slot(ad, slot, (const uint16_t*)down, (const uint16_t*)up, rank, scale, class_scale, n, k, st)
-                : set_slot(ad, slot, (const float*)down, (const float*)up, rank, scale, class_scale, n, k, st);
+int launch_adapter_set(const Adapters& ad, int slot, const void* down, const void* up, int rank, float scale, int bf16, int64_t n,
+                       int64_t k, hipStream_t st) {
+    return bf16 ? set_slot(ad, slot, (const uint16_t*)down, (const uint16_t*)up, rank, scale, n, k, st)
+                : set_slot(ad, slot, (const float*)down, (const float*)up, rank, scale, n, k, st);
 }
 
 size_t adapt_workspace(const Adapters& ad, int64_t m) { return m > 0 ? layout_of(ad, m).total : 0; }
 
-int launch_adapt_decode(int cfg, const TileGeom& tg, const uint8_t* rec, const Adapters& ad, const AdaptLines& lines, const float* a,
+int launch_adapt_decode(int cfg, const TileGeom& tg, const Adapters& ad, const AdaptLines& lines, const float* a,
                         int64_t m, int64_t n, int64_t k, int32_t* idx, float* maxprob, const CtcOut& ctc, uint8_t* ws,
                         hipStream_t st) {
     const AdaptLayout L = layout_of(ad, m);
@@ -957,7 +959,7 @@ int launch_adapt_decode(int cfg, const TileGeom& tg, const uint8_t* rec, const A
     int64_t units;
     if (int e = make_plan(ad, lines, m, 32 * blocks_of(m, ad.steps), L, ws, &plan, &units, st)) return e;
     const int nsplit = chunks_of(ad, m);
-    AdaptLaunch x = launch_of(tg, rec, ad, a, m, n, k, units, nsplit, plan);
+    AdaptLaunch x = launch_of(tg, ad, a, m, n, k, units, nsplit, plan);
     x.part = reinterpret_cast<Partial*>(ws + L.part);
     const unsigned grid = (unsigned)grid_of(x.mblocks, nsplit, true);
     if (int e = by_config(cfg, tg.G, ad.steps, [&]<int C, int G, int NR>() {
@@ -975,7 +977,7 @@ int launch_adapt_decode(int cfg, const TileGeom& tg, const uint8_t* rec, const A
     return launch_merge_ctc(x.part, m, nsplit, ctc, idx, maxprob, nullptr, st);
 }
 
-int launch_adapt_logits(int cfg, const TileGeom& tg, const uint8_t* rec, const Adapters& ad, const AdaptLines& lines, const float* a,
+int launch_adapt_logits(int cfg, const TileGeom& tg, const Adapters& ad, const AdaptLines& lines, const float* a,
                         int64_t m, int64_t n, int64_t k, float* out, uint8_t* ws, hipStream_t st) {
     const AdaptLayout L = layout_of(ad, m);
     Plan plan;
@@ -993,7 +995,7 @@ int launch_adapt_logits(int cfg, const TileGeom& tg, const uint8_t* rec, const A
         const int64_t cost = (likely * ns + 255) / 256 * (8 + (tg.tiles + ns - 1) / ns);
         if (best < 0 || cost < best) nsplit = ns, best = cost;
     }
-    AdaptLaunch x = launch_of(tg, rec, ad, a, m, n, k, units, nsplit, plan);
+    AdaptLaunch x = launch_of(tg, ad, a, m, n, k, units, nsplit, plan);
     x.out = out;
     const unsigned grid = (unsigned)(mblocks * nsplit);
     return by_config(cfg, tg.G, ad.steps, [&]<int C, int G, int NR>() {

@@ -22,6 +22,12 @@ struct Adapters {
     uint8_t* up = nullptr;    // [slots + 1][class tiles][halves][steps][2][32][8]
     AdapterMeta* meta = nullptr;
     unsigned* range = nullptr;  // [slots + 1][2][kAdaptMostRank] sizes that a slot's powers of two come from
+    // The head's fp16 records and the classes' units [n]: up is held divided by them, as the products of the
+    // records are.  The head's own, or where its scales lie far apart others with nearer units.
+    const uint8_t* rec = nullptr;
+    const float* unit = nullptr;
+    uint8_t* own_rec = nullptr;
+    float* own_unit = nullptr;
     size_t down_bytes() const;  // of a slot
     size_t up_bytes() const;
 };
@@ -36,16 +42,15 @@ struct AdaptLines {
 // Sets the zero records of every slot.
 int launch_adapters_clear(const Adapters& ad, hipStream_t st);
 // Records of a slot from its adapter, down [rank][k] and up [n][rank] of fp32 or bf16 (rank 0: none).
-// scale [n]: the head's class scales.
-int launch_adapter_set(const Adapters& ad, int slot, const void* down, const void* up, int rank, float scale, int bf16,
-                       const float* class_scale, int64_t n, int64_t k, hipStream_t st);
+int launch_adapter_set(const Adapters& ad, int slot, const void* down, const void* up, int rank, float scale, int bf16, int64_t n,
+                       int64_t k, hipStream_t st);
 
 size_t adapt_workspace(const Adapters& ad, int64_t m);
-// cfg: CFG_H2 (INT8 head) or CFG_HF3 (FP32 head); rec: the head's fp16 records.
-int launch_adapt_logits(int cfg, const TileGeom& tg, const uint8_t* rec, const Adapters& ad, const AdaptLines& lines, const float* a,
-                        int64_t m, int64_t n, int64_t k, float* out, uint8_t* ws, hipStream_t st);
-int launch_adapt_decode(int cfg, const TileGeom& tg, const uint8_t* rec, const Adapters& ad, const AdaptLines& lines, const float* a,
-                        int64_t m, int64_t n, int64_t k, int32_t* idx, float* maxprob, const CtcOut& ctc, uint8_t* ws,
+// cfg: CFG_H2 (INT8 head) or CFG_HF3 (FP32 head).
+int launch_adapt_logits(int cfg, const TileGeom& tg, const Adapters& ad, const AdaptLines& lines, const float* a, int64_t m,
+                        int64_t n, int64_t k, float* out, uint8_t* ws, hipStream_t st);
+int launch_adapt_decode(int cfg, const TileGeom& tg, const Adapters& ad, const AdaptLines& lines, const float* a, int64_t m,
+                        int64_t n, int64_t k, int32_t* idx, float* maxprob, const CtcOut& ctc, uint8_t* ws,
                         hipStream_t st);
 
 struct MergeArgs {

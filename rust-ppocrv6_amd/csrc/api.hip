@@ -402,6 +402,8 @@ void free_handle(ppocr_rh* h) {
         if (h->adapters.up) (void)hipFree(h->adapters.up);
         if (h->adapters.meta) (void)hipFree(h->adapters.meta);
         if (h->adapters.range) (void)hipFree(h->adapters.range);
+        if (h->adapters.own_rec) (void)hipFree(h->adapters.own_rec);
+        if (h->adapters.own_unit) (void)hipFree(h->adapters.own_unit);
         free_handle(h->base);
         delete h;
         return;
@@ -2063,6 +2065,55 @@ int adapt_cfg(const ppocr_rh* h) { return h->quantized ? CFG_H2 : CFG_HF3; }
 // The workspace of an adapted call behind the first bytes, which are left to the head's calls.
 constexpr size_t kAdaptWs = 256;
 
+// An adapter's values are held in fp16 halves in units of their classes' scales, so the units have to lie close to each
+// other.  Packed weights' scales need not: a class whose weights all but vanish has one down to 2^-34, one of zeros
+// 1.  Classes' units are raised to the largest, by up to 2^24, where the scales are further apart than 2^8: the int8
+// values of 7 bits are then held in fp16 that much lower, exactly.
+constexpr float kLeastAdaptScale = 1.0f / (1LL << 34);
+constexpr int kNearUnits = 8, kMostRaise = 24, kMostSpread = kMostRaise + 16;
+int adapt_units(const ppocr_rh* base, Adapters* ad, size_t* total) try {
+    ad->unit = base->d_scale;
+    ad->rec = base->d_rec_h;
+    if (!base->quantized) return PPOCR_OK;
+    const int64_t n = base->n;
+    std::vector<float> unit((size_t)n);
+    PPOCR_HIP(hipMemcpy(unit.data(), base->d_scale, (size_t)n * 4, hipMemcpyDeviceToHost));
+    int top = -1000, least = 1000;
+    for (int64_t i = 0; i < n; ++i) {
+        if (!(std::fabs(unit[i]) >= kLeastAdaptScale && std::isfinite(unit[i])))
+            return bad_arg(kAdaptOp, "scale of class " + std::to_string(i) + " below 2^-34 or not finite");
+        top = std::max(top, std::ilogb(unit[i]));
+        least = std::min(least, std::ilogb(unit[i]));
+    }
+    if (top - least > kMostSpread) return bad_arg(kAdaptOp, "scales of the classes further apart than 2^" + std::to_string(kMostSpread));
+    if (top - least <= kNearUnits) return PPOCR_OK;
+    const TileGeom& g = base->geom;
+    std::vector<uint8_t> rec((size_t)g.tiles * g.rec_bytes());
+    PPOCR_HIP(hipMemcpy(rec.data(), base->d_rec_h, rec.size(), hipMemcpyDeviceToHost));
+    for (int64_t row = 0; row < n; ++row) {
+        const int raise = std::min(top - std::ilogb(unit[row]), kMostRaise), i = (int)(row % 32);
+        const float up = std::ldexp(1.0f, raise), down = std::ldexp(1.0f, -raise);
+        unit[row] *= up;
+        uint8_t* r = rec.data() + (size_t)(row / 32) * g.rec_bytes();
+        uint16_t* frag = reinterpret_cast<uint16_t*>(r);
+        for (int x = 0; x < g.G; ++x)
+            for (int e = 0; e < 8; ++e) {
+                uint16_t& v = frag[((size_t)x * 32 + i) * 8 + e];
+                v = f16_bits_rne(f16_to_float(v) * down);
+            }
+        float* ep = reinterpret_cast<float*>(r + g.frag_bytes());
+        ep[i] *= up;
+        ep[64 + i] *= up;
+    }
+    if (int e = upload(&ad->own_unit, unit.data(), unit.size(), total)) return e;
+    if (int e = upload(&ad->own_rec, rec.data(), rec.size(), total)) return e;
+    ad->unit = ad->own_unit;
+    ad->rec = ad->own_rec;
+    return PPOCR_OK;
+} catch (const std::bad_alloc&) {
+    return fail(PPOCR_ERR_NO_MEMORY, std::string(kAdaptOp) + ": host allocation failed");
+}
+
 int check_adapter(const ppocr_rh* h, int64_t slot, const void* down, const void* up, int64_t rank, float scale) {
     if (int e = check_adapted(h)) return e;
     if (slot < 0 || slot >= h->adapters.slots)
@@ -2224,6 +2275,7 @@ int ppocr_ra_create(const ppocr_rh_t* head, int64_t slots, int64_t max_rank, ppo
     ad.steps = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : 4;
     ad.G = h->geom.G;
     ad.tiles = h->geom.tiles;
+    if (int e = adapt_units(base, &ad, &h->device_bytes)) return e;
     const size_t sets = (size_t)slots + 1;
     const size_t bytes[4] = {sets * ad.down_bytes(), sets * ad.up_bytes(), sets * sizeof(AdapterMeta),
                              sets * 2 * kAdaptMostRank * sizeof(unsigned)};
@@ -2257,8 +2309,8 @@ int ppocr_ra_set_dev(ppocr_rh_t* h, int64_t slot, void* d_down, void* d_up, int6
     if (int e = check_adapter(h, slot, d_down, d_up, rank, scale)) return e;
     if (int e = check_dtype(dtype, kAdaptOp)) return e;
     DeviceGuard dg(h->device);
-    return launch_adapter_set(h->adapters, (int)slot, d_down, d_up, (int)rank, scale, dtype == PPOCR_DTYPE_BF16, h->d_scale, h->n,
-                              h->k, (hipStream_t)stream);
+    return launch_adapter_set(h->adapters, (int)slot, d_down, d_up, (int)rank, scale, dtype == PPOCR_DTYPE_BF16, h->n, h->k,
+                              (hipStream_t)stream);
 }
 
 int ppocr_ra_set(ppocr_rh_t* h, int64_t slot, const float* down, const float* up, int64_t rank, float scale) {
@@ -2268,8 +2320,8 @@ int ppocr_ra_set(ppocr_rh_t* h, int64_t slot, const float* down, const float* up
     if (int e = hc.begin({(size_t)(rank * h->k) * 4, (size_t)(rank * h->n) * 4}, {}, 0)) return e;
     if (rank > 0)
         if (int e = hc.copy_in({down, up})) return e;
-    if (int e = launch_adapter_set(h->adapters, (int)slot, hc.in<float>(0), hc.in<float>(1), (int)rank, scale, 0, h->d_scale,
-                                   h->n, h->k, hc.stream()))
+    if (int e = launch_adapter_set(h->adapters, (int)slot, hc.in<float>(0), hc.in<float>(1), (int)rank, scale, 0, h->n, h->k,
+                                   hc.stream()))
         return e;
     return hc.copy_out({});
 }
@@ -2288,7 +2340,7 @@ int ppocr_ra_logits_dev(const ppocr_rh_t* h, const float* d_a, int64_t m, const 
     hipStream_t st = (hipStream_t)stream;
     Workspace ws;
     if (int e = train_workspace(&ws, d_workspace, workspace_bytes, ppocr_ra_workspace_bytes(h, m), st, kAdaptOp)) return e;
-    return launch_adapt_logits(adapt_cfg(h), h->geom, h->d_rec_h, h->adapters, AdaptLines{d_line_off, lines, d_line_slot}, d_a,
+    return launch_adapt_logits(adapt_cfg(h), h->geom, h->adapters, AdaptLines{d_line_off, lines, d_line_slot}, d_a,
                                m, h->n, h->k, d_out, ws.p + kAdaptWs, st);
 }
 
@@ -2326,7 +2378,7 @@ int ppocr_ra_decode_dev(const ppocr_rh_t* h, const float* d_a, int64_t m, const 
     if (m == 0) return launch_merge_ctc(nullptr, 0, 1, ctc, nullptr, nullptr, nullptr, st);
     Workspace ws;
     if (int e = train_workspace(&ws, d_workspace, workspace_bytes, ppocr_ra_workspace_bytes(h, m), st, kAdaptOp)) return e;
-    return launch_adapt_decode(adapt_cfg(h), h->geom, h->d_rec_h, h->adapters, AdaptLines{d_line_off, lines, d_line_slot}, d_a,
+    return launch_adapt_decode(adapt_cfg(h), h->geom, h->adapters, AdaptLines{d_line_off, lines, d_line_slot}, d_a,
                                m, h->n, h->k, d_idx, d_maxprob, ctc, ws.p + kAdaptWs, st);
 }
 

@@ -120,6 +120,59 @@ def test_a_rows_bits_do_not_depend_on_its_company(rh):
         assert np.array_equal(alone, whole[off[i]:off[i + 1]]), i
 
 
+@pytest.mark.parametrize("quant", [True, False])
+def test_a_rows_bits_do_not_depend_on_its_neighbours(rh, quant):
+    """Ordinary rows beside rows of any size, of zeros and of infinities, under one slot: the same bits as beside
+    ordinary ones, and in each of several calls."""
+    rng = np.random.default_rng(19)
+    h = ac.Head(rh, rng, 900, 120, quant, 3, 16)
+    lengths = rng.integers(1, 9, 80)
+    off = ac.offsets(lengths)
+    m = int(off[-1])
+    slot = rng.integers(-1, 3, 80).astype(np.int32)
+    a = rows(rng, h, m)
+    a *= (rng.random((m, 120)) * 2.0 ** rng.integers(-12, 1, (m, 120))).astype(np.float32)  # low halves far below the top
+    b = a.copy()
+    at = rng.random(m) < 0.3
+    b[at] *= (2.0 ** rng.integers(-60, 20, at.sum()))[:, None].astype(np.float32)
+    b[np.flatnonzero(at)[::7]] = 0.0
+    b[np.flatnonzero(at)[::9], 5] = np.inf
+    first, second = ac.Call(h, a, off, slot), ac.Call(h, b, off, slot)
+    za, oa = first.logits().get(), {k: v.get() for k, v in first.decode().items()}
+    for _ in range(4):
+        zb, ob = second.logits().get(), {k: v.get() for k, v in second.decode().items()}
+        assert np.array_equal(za[~at], zb[~at])
+        for k in ("idx", "maxprob"):
+            assert np.array_equal(oa[k][~at], ob[k][~at]), k
+        for x, y in ((first.logits().get(), za), (second.logits().get(), zb)):
+            assert np.array_equal(x, y, equal_nan=True)
+
+
+def test_classes_of_tiny_weights(rh):
+    """An INT8 head with classes of weights that all but vanish, down to the least scale that packing gives and to
+    zeros, beside an ordinary adapter: every class keeps its bits, the head's own calls on the handle theirs."""
+    rng = np.random.default_rng(20)
+    n, k = 300, 120
+    for tiny in (1e-4, 1e-6, 5e-9, 1e-9):
+        w = (rng.standard_normal((n, k)) * 0.05).astype(np.float32)
+        w[::7] *= np.float32(tiny / 0.05)
+        qw = rh.QuantizedWeight.from_f32_transposed(w)
+        h = ac.Head(rh, rng, n, k, True, 1, 16)
+        h.base = rh.RecHead(qw=qw, bias=h.bias)
+        h.w = qw.data.astype(np.float64) * qw.scales.astype(np.float64)[:, None]
+        h.head = rh.AdaptedHead(h.base, 1, 16)
+        down = (rng.standard_normal((16, k)) / np.sqrt(k)).astype(np.float32)
+        up = (rng.standard_normal((n, 16)) * 0.05).astype(np.float32)
+        h.set(0, down, up, 1.0)
+        a = rows(rng, h, 70)
+        call = ac.Call(h, a, [0, 70], [0])
+        check_logits(h, a, [0, 70], [0], call.logits().get(), f"weights of {tiny}")
+        check_decode(h, a, np.array([0, 70]), [0], {x: v.get() for x, v in call.decode().items()}, f"weights of {tiny}")
+        none = ac.Call(h, a, [0, 70], [-1]).logits().get()
+        tc.close(none, *h.exact(a, np.full(70, -1)), "no adapter")
+        assert np.array_equal(h.head.logits(a), h.base.logits(a))
+
+
 def test_rows_of_any_size(rh):
     """Rows scaled by powers of two far apart, of zeros, and rows with infinities and NaN beside them: each keeps
     its own bits."""
@@ -337,6 +390,16 @@ def test_refusals(rh):
     assert L.ppocr_ra_create(odd.handle, 1, 1, ctypes.byref(out)) == rh.PPOCR_ERR_INVALID_ARG
     big = rh.RecHead(w_t=np.full((5, 80), 40000.0, np.float32))
     assert L.ppocr_ra_create(big.handle, 1, 1, ctypes.byref(out)) == rh.PPOCR_ERR_INVALID_ARG
+    # INT8 scales that leave an adapter no unit
+    for bad in (0.0, 1e-12, float("inf"), float("nan")):
+        qw = rh.QuantizedWeight.from_f32_transposed(np.ones((5, 80), np.float32))
+        qw.scales[3] = bad
+        assert L.ppocr_ra_create(rh.RecHead(qw=qw).handle, 1, 1, ctypes.byref(out)) == rh.PPOCR_ERR_INVALID_ARG, bad
+        assert "scale of class 3" in rh._lib.last_error()
+    qw = rh.QuantizedWeight.from_f32_transposed(np.ones((5, 80), np.float32))
+    qw.scales[:] = [1.0, 2.0 ** -20, 2.0 ** 20, 1.0, 2.0 ** -21]
+    assert L.ppocr_ra_create(rh.RecHead(qw=qw).handle, 1, 1, ctypes.byref(out)) == rh.PPOCR_ERR_INVALID_ARG and not out.value
+    assert "further apart" in rh._lib.last_error()
     # a head without adapters
     assert L.ppocr_ra_set_dev(h.base.handle, 0, P, P, 1, 1.0, 0, None) == rh.PPOCR_ERR_INVALID_ARG
     assert L.ppocr_ra_workspace_bytes(h.base.handle, 5) == 0
