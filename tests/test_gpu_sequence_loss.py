@@ -68,7 +68,7 @@ class Preference:
 
 
 LENGTHS = [[1], [7, 0, 1, 64, 65], [120] * 29, [257, 255, 256, 3], [1000, 4097, 2], [1] * 500, [0, 0, 5], [20000], [0],
-           [600] * 5, [5000, 9000]]
+           [600] * 5, [5000, 9000], [16384], [30000, 3, 0, 70001, 65, 20000], [2] * 3 + [300000], [33000, 32999]]
 IDS = [f"{len(x)}x{max(x)}" for x in LENGTHS]
 
 
@@ -273,3 +273,43 @@ def test_captured_and_on_two_streams(rh):
         b.check({k: v.get() for k, v in ob.items()}, "replay")
         b.check({k: v.get() for k, v in oc.items()}, "beside it")
     graph.close()
+
+
+def test_few_long_lines(rh):
+    """Lines that several workgroups share: captured beside a call on another stream, in-bounds for any offsets, steps
+    of no line cleared, a NaN kept to its line, and lines whose grad is 0."""
+    from ppocr_rechead.hip import Stream, synchronize
+    from test_gpu_graph_replay import _Graph
+    rng = np.random.default_rng(10)
+    off = np.array([1000, 41000, 41003, 41003, 150000], np.int64)
+    m = 150500
+    loss, old, ref, target = steps(rng, m)
+    adv, grad = rng.standard_normal(4).astype(np.float32), np.array([1, 2, 3, -0.5], np.float32)
+    a = Policy(rh, loss, old, ref, target, adv, off, grad=grad)
+    b = Preference(rh, loss, ref, target, off, 0.01, 0.1, True)
+    st, other = Stream(), Stream()
+    oa, ob = a.outputs(), b.outputs()
+    graph = _Graph(st, lambda: (a.run(oa, st.h), b.run(ob, st.h)))
+    for _ in range(3):
+        for v in (*oa.values(), *ob.values()):
+            v.d.fill_bytes(0xA5)
+        synchronize()
+        oc, od = b.run(b.outputs(), other.h), a.run(a.outputs(), other.h)
+        graph.replay()
+        other.synchronize()
+        for job, o in ((a, oa), (b, ob), (b, oc), (a, od)):
+            job.check({k: v.get() for k, v in o.items()}, "long lines")
+    graph.close()
+    for back in ([140000, 10, 90000, 20, 60000], [1 << 50, -3, 200, 0, 1 << 40]):
+        a, b = Policy(rh, loss, old, ref, target, adv, back), Preference(rh, loss, ref, target, back)
+        for o in (a.run(a.outputs()), b.run(b.outputs())):
+            for v in o.values():
+                v.get()
+    bad, none = loss.copy(), np.array([1, 1, 1, 0], np.float32)
+    bad[100000] = np.nan
+    target[100000] = 3
+    got = {k: v.get() for k, v in (lambda j: j.run(j.outputs()))(Policy(rh, bad, old, ref, target, adv, off, grad=none)).items()}
+    want, tol = ac.policy64(loss, old, ref, target, adv, False, off, 0.2, 0.28, 0.05, none)
+    assert np.isnan(got["loss"][3]) and (got["row_grad"][41003:] == 0).all()
+    tc.close(got["loss"][:3], want["loss"][:3], tol["loss"][:3], "lines beside a NaN")
+    tc.close(got["row_grad"][:41003], want["row_grad"][:41003], tol["row_grad"][:41003], "gradients beside a NaN")
