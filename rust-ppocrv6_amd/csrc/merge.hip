@@ -65,14 +65,6 @@ __device__ __forceinline__ f32x16 multiply(const Op<float>& a, const Op<float>& 
 }
 __device__ __forceinline__ int result_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
-// Values p[0], p[stride] .. of an operand.
-template <typename T>
-__device__ __forceinline__ Op<T> gather(const T* p, int stride) {
-    Op<T> o;
-#pragma unroll
-    for (int y = 0; y < Op<T>::N; ++y) o.v[y] = p[y * stride];
-    return o;
-}
 // Values at, at + 1, .. of the `width` at p, 0 past them.
 template <typename T>
 __device__ __forceinline__ Op<T> gather_to(const T* p, int at, int width) {
@@ -98,7 +90,8 @@ struct alignas(2 * sizeof(T)) Pair {
 // A workgroup takes a block of rows.  Each wave multiplies the block's up rows with 32 columns of down at a
 // time; w0's pieces are on their way meanwhile.  (Workgroups that kept down as operands over several blocks,
 // half as many: 6.1 us instead of 5.3 for rank 16 of 18710 x 120, 19 instead of 12 for rank 64 of 32768 x 256.)
-template <typename T, int RANK, bool VEC>
+// FULL: the rank is RANK, no address to hold back and no value to clear.
+template <typename T, int RANK, bool VEC, bool FULL>
 __global__ __launch_bounds__(kThreads) void merge_kernel(const T* w0, const T* __restrict__ down, const T* __restrict__ up,
                                                          int64_t n, int k, int rank, bool rank_vec, float s, T* w) {
     constexpr int V = Piece<T>::N, S = RANK / Op<T>::STEP;
@@ -128,30 +121,39 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const T* w0, const T* _
             a[x] = gather_to(ur, t, rank);
         }
     }
-    // FULL: every rank of the operands exists (no addresses to hold back, no values to clear)
-    auto columns = [&]<bool FULL>() {
-        for (int c0 = 32 * wave; c0 < k; c0 += 32 * kWaves) {
-            const int c = min(c0 + i, k - 1);
-            f32x16 acc = {};
+    for (int c0 = 32 * wave; c0 < k; c0 += 32 * kWaves) {
+        const int c = min(c0 + i, k - 1);
+        f32x16 acc = {};
+        if constexpr (FULL) {
 #pragma unroll
             for (int x = 0; x < S; ++x) {
                 Op<T> b;
 #pragma unroll
-                for (int y = 0; y < V; ++y) {
-                    const int t = x * Op<T>::STEP + h * V + y;
-                    const T d = down[(FULL ? t : min(t, rank - 1)) * k + c];
-                    b.v[y] = FULL || t < rank ? d : T(0);
-                }
+                for (int y = 0; y < V; ++y) b.v[y] = down[(x * Op<T>::STEP + h * V + y) * k + c];
                 acc = multiply(a[x], b, acc);
             }
-            if (c0 + i < k) {
+        } else {
+            Op<T> b[S];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sum[result_row(r, h) * k + c] = acc[r];
-            }
+            for (int x = 0; x < S; ++x)
+#pragma unroll
+                for (int y = 0; y < V; ++y) b[x].v[y] = down[min(x * Op<T>::STEP + h * V + y, rank - 1) * k + c];
+            // ranks that do not exist, behind the loads: a value that is looked at holds back the loads behind it
+#pragma unroll
+            for (int x = 0; x < S; ++x)
+                if ((x + 1) * Op<T>::STEP > rank) {
+#pragma unroll
+                    for (int y = 0; y < V; ++y)
+                        if (x * Op<T>::STEP + h * V + y >= rank) b[x].v[y] = T(0);
+                }
+#pragma unroll
+            for (int x = 0; x < S; ++x) acc = multiply(a[x], b[x], acc);
         }
-    };
-    if (rank == RANK) columns.template operator()<true>();
-    else columns.template operator()<false>();
+        if (c0 + i < k) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[result_row(r, h) * k + c] = acc[r];
+        }
+    }
     __syncthreads();
     if constexpr (VEC) {
 #pragma unroll
@@ -441,7 +443,9 @@ int merge(const MergeArgs& x, hipStream_t st) {
     const bool vec = aligned16(x.w) && aligned16(x.out);
     const bool rank_vec = aligned16(x.up) && x.rank % V == 0;
     auto go = [&]<int R>() {
-        auto kern = vec ? merge_kernel<T, R, true> : merge_kernel<T, R, false>;
+        const bool full = x.rank == R;
+        auto kern = vec ? (full ? merge_kernel<T, R, true, true> : merge_kernel<T, R, true, false>)
+                        : (full ? merge_kernel<T, R, false, true> : merge_kernel<T, R, false, false>);
         kern<<<grid, kThreads, lds, st>>>((const T*)x.w, (const T*)x.down, (const T*)x.up, x.n, x.k, x.rank, rank_vec, x.scale,
                                           (T*)x.out);
     };
