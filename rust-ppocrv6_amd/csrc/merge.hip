@@ -211,24 +211,25 @@ __device__ __forceinline__ void dup_rows(const T* __restrict__ dw, const T* __re
     float* red = reinterpret_cast<float*>(lds + L.red);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 31, h = lane >> 5;
     const int nt = L.rp / 32;
-    // VEC: where each piece of a block that this thread moves lies in LDS, the same for every block (past the
-    // block's pieces: -1)
-    const int kv = k / V;
-    int at[VEC ? PER : 1];
-    if constexpr (VEC) {
+    // where each piece of a block that this thread moves lies in LDS, the same for every block (past the
+    // block's pieces: -1).  A block of 32 rows is whole pieces whatever k is; where k is not, a piece may reach into
+    // the next row and is spread value by value.
+    constexpr int PIECES = kRows / V;
+    int at[PER], left[VEC ? 1 : PER];
 #pragma unroll
-        for (int x = 0; x < PER; ++x) {
-            const int p = x * kThreads + tid, r = p / kv;
-            at[x] = r < kRows ? r * L.cpitch + (p - r * kv) * V : -1;
-        }
+    for (int x = 0; x < PER; ++x) {
+        const int p = x * kThreads + tid, r = p * V / k, c = p * V - r * k;
+        at[x] = p < PIECES * k ? r * L.cpitch + c : -1;
+        if constexpr (!VEC) left[x] = k - c;  // values of the piece's first row
     }
-    u32x4 next[VEC ? PER : 1];
+    const bool whole = VEC || aligned16(dw);
+    u32x4 next[PER];
     auto fetch = [&](int64_t row0) {
-        if constexpr (VEC) {
-            const int rows = (int)min((int64_t)kRows, n - row0);
+        const int rows = (int)min((int64_t)kRows, n - row0), last = rows * k / V - 1;
+        if (VEC || (whole && last >= 0)) {
             const u32x4* p = reinterpret_cast<const u32x4*>(dw + row0 * k);
 #pragma unroll
-            for (int x = 0; x < PER; ++x) next[x] = p[min(x * kThreads + tid, rows * kv - 1)];
+            for (int x = 0; x < PER; ++x) next[x] = p[min(x * kThreads + tid, last)];
         }
     };
     int64_t row0 = worker * kRows;
@@ -237,7 +238,7 @@ __device__ __forceinline__ void dup_rows(const T* __restrict__ dw, const T* __re
     // columns and ranks past the tensors' stay 0
     for (int x = tid; x < (int)((L.red - L.down) / 16); x += kThreads) reinterpret_cast<u32x4*>(lds)[x] = u32x4{0, 0, 0, 0};
     __syncthreads();
-    if (VEC && aligned16(down)) {
+    if (const int kv = k / V; VEC && aligned16(down)) {
         for (int x = tid; x < rank * kv; x += kThreads) {
             const int t = x / kv;
             *reinterpret_cast<u32x4*>(ldown + t * L.cpitch + (x - t * kv) * V) = reinterpret_cast<const u32x4*>(down)[x];
@@ -255,7 +256,23 @@ __device__ __forceinline__ void dup_rows(const T* __restrict__ dw, const T* __re
             for (int x = 0; x < PER; ++x)
                 if (at[x] >= 0) *reinterpret_cast<u32x4*>(ldw + at[x]) = next[x];
         } else {
-            for (int x = tid; x < kRows * k; x += kThreads) ldw[x / k * L.cpitch + x % k] = x < rows * k ? dw[row0 * k + x] : T(0);
+            // rows that do not exist hold whatever they held: their results are not written
+            const int pieces = whole ? rows * k / V : 0;
+#pragma unroll
+            for (int x = 0; x < PER; ++x)
+                if (x * kThreads + tid < pieces) {
+                    const Piece<T> q = __builtin_bit_cast(Piece<T>, next[x]);
+                    // (of narrow rows a piece may cover several)
+                    int to = at[x], more = left[x];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        ldw[to] = q.v[v];
+                        const bool over = --more == 0;
+                        to += over ? L.cpitch - k + 1 : 1;
+                        more = over ? k : more;
+                    }
+                }
+            for (int x = pieces * V + tid; x < rows * k; x += kThreads) ldw[x / k * L.cpitch + x % k] = dw[row0 * k + x];
         }
         __syncthreads();
         if (row0 + workers * kRows < n) fetch(row0 + workers * kRows);
@@ -282,7 +299,7 @@ __device__ __forceinline__ void dup_rows(const T* __restrict__ dw, const T* __re
 // ones are a piece of the product each.  The waves take the rows in turn and meet in LDS.
 constexpr int kGroupCols = 64;
 constexpr int kAhead = 2;
-template <typename T, int NT, bool VEC>
+template <typename T, int NT, bool VEC, bool PAIRS>
 __device__ __forceinline__ void ddown_rows(const T* __restrict__ dw, const T* __restrict__ up, int k, int rank, int64_t first,
                                            int64_t last, int c0, float* __restrict__ out, float* lds) {
     constexpr int V = Piece<T>::N, STEP = Op<T>::STEP;
@@ -295,7 +312,7 @@ __device__ __forceinline__ void ddown_rows(const T* __restrict__ dw, const T* __
     // together.  Columns and ranks that do not exist meet no others in the products, rows that do not are
     // cleared before their use.
     const int ci = min(c0 + 2 * i, VEC ? k - 2 : k - 1), cj = min(c0 + 2 * i + 1, k - 1);
-    const int ti = NT == 2 ? min(2 * i, VEC ? rank - 2 : rank - 1) : min(i, rank - 1), tj = min(2 * i + 1, rank - 1);
+    const int ti = NT == 2 ? min(2 * i, PAIRS ? rank - 2 : rank - 1) : min(i, rank - 1), tj = min(2 * i + 1, rank - 1);
     auto fetch = [&](Rows& w, int64_t j0) {
         if (j0 >= last) return;  // the same for the wave
         const T* dp = dw + j0 * k;
@@ -307,7 +324,7 @@ __device__ __forceinline__ void ddown_rows(const T* __restrict__ dw, const T* __
             if constexpr (VEC) w.d[y] = *reinterpret_cast<const Pair<T>*>(dp + j * k + ci);
             else w.d[y] = Pair<T>{{dp[j * k + ci], dp[j * k + cj]}};
             if constexpr (NT == 1) w.u[y].v[0] = up_[j * rank + ti];
-            else if constexpr (VEC) w.u[y] = *reinterpret_cast<const Pair<T>*>(up_ + j * rank + ti);
+            else if constexpr (PAIRS) w.u[y] = *reinterpret_cast<const Pair<T>*>(up_ + j * rank + ti);
             else w.u[y] = Pair<T>{{up_[j * rank + ti], up_[j * rank + tj]}};
         }
     };
@@ -387,7 +404,8 @@ __device__ __forceinline__ void ddown_rows(const T* __restrict__ dw, const T* __
 // The first workgroups take ddown, by groups of rows and of 64 columns, the others dup: dw comes from memory
 // once and from the caches the second time.  (One pass that kept both in a workgroup left a sum of ddown per
 // workgroup: rank 64 of 32768 x 256, 512 sums of 64 KB beside 17 MB of dw, took 27 us where this takes 20.)
-template <typename T, int NT, bool VEC>
+// VEC: rows of dw are read in pieces of 16 bytes, PAIRS: those of up in pairs.
+template <typename T, int NT, bool VEC, bool PAIRS>
 __global__ __launch_bounds__(kThreads) void merge_backward_kernel(const T* __restrict__ dw, const T* __restrict__ down,
                                                                   const T* __restrict__ up, int64_t n, int k, int rank, float s,
                                                                   T* dup, float* part, int parts, int64_t rows_each) {
@@ -397,7 +415,7 @@ __global__ __launch_bounds__(kThreads) void merge_backward_kernel(const T* __res
     if (b < groups * parts) {
         const int g = b / groups, c0 = (b - g * groups) * kGroupCols;
         const int64_t first = g * rows_each;
-        ddown_rows<T, NT, VEC>(dw, up, k, rank, first, min(first + rows_each, n), c0, part + (int64_t)g * rank * k,
+        ddown_rows<T, NT, VEC, PAIRS>(dw, up, k, rank, first, min(first + rows_each, n), c0, part + (int64_t)g * rank * k,
                                reinterpret_cast<float*>(lds));
     } else {
         dup_rows<T, VEC>(dw, down, n, k, rank, s, dup, b - groups * parts, (int)gridDim.x - groups * parts, lds);
@@ -469,9 +487,11 @@ int backward(const MergeArgs& x, void* ddown, void* dup, float* part, hipStream_
     // rank 16 of 18710 x 120: 12.8 us with 512, 14.2 with 256)
     const int64_t held = 256 * std::min<int64_t>(3, 160 * 1024 / (int64_t)lds) - (ddown ? groups * parts : 0);
     const unsigned grid = (unsigned)((ddown ? groups * parts : 0) + (dup ? std::min(blocks, std::max<int64_t>(held, 256)) : 0));
-    const bool vec = aligned16(x.dw) && aligned16(x.up) && x.k % V == 0 && x.rank % 2 == 0;
+    const bool vec = aligned16(x.dw) && x.k % V == 0, pairs = aligned16(x.up) && x.rank % 2 == 0;
     auto go = [&]<int NT>() {
-        auto kern = vec ? merge_backward_kernel<T, NT, true> : merge_backward_kernel<T, NT, false>;
+        constexpr bool P = NT == 2;  // (up is read in pairs for two pieces of the product)
+        auto kern = vec ? (P && pairs ? merge_backward_kernel<T, NT, true, P> : merge_backward_kernel<T, NT, true, false>)
+                        : (P && pairs ? merge_backward_kernel<T, NT, false, P> : merge_backward_kernel<T, NT, false, false>);
         kern<<<grid, kThreads, lds, st>>>((const T*)x.dw, (const T*)x.down, (const T*)x.up, x.n, x.k, x.rank, x.scale, (T*)dup,
                                           ddown ? part : nullptr, parts, rows_each);
     };

@@ -51,7 +51,8 @@ class Merge:
 
 
 SHAPES = [(1, 1, 1), (5, 3, 2), (33, 120, 16), (100, 80, 64), (300, 256, 17), (257, 255, 33), (31, 8, 63), (64, 33, 31),
-          (2000, 120, 8), (6906, 80, 32), (18710, 120, 16), (9000, 256, 64)]
+          (2000, 120, 8), (6906, 80, 32), (18710, 120, 16), (9000, 256, 64),
+          (3001, 2, 3), (5003, 1, 64), (777, 13, 35), (40001, 7, 17), (20011, 185, 59)]
 
 
 @pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
