@@ -19,6 +19,7 @@
 // their bits, whatever the rows beside them hold, and no row has to be computed again.  u = down a is computed by each wave before its first tile, from the rows it
 // holds; the products' layout is that of the operand that the next product needs.
 #include <algorithm>
+#include <cmath>
 
 #include "adapt.hpp"
 #include "head_mfma.hpp"
@@ -855,10 +856,13 @@ struct AdaptLayout {
 int blocks_of(int64_t m, int steps) { return steps == 4 && m > 2048 ? 2 : 1; }
 int per_cu_of(int steps) { return steps == 4 ? 1 : 2; }
 // Vocabulary chunks of the statistics pass: the count with the fewest tile times, as the head's (stats_nsplit), of
-// the row blocks that the plan is likely to make, half a unit lost a slot.
+// the row blocks that the plan is likely to make: half a unit lost for each slot and for the rows of none, and as many
+// more as that is uncertain by (a row block too many makes a round of its own: a page under 8 adapters of rank 64
+// 89 us in 16 chunks, 115 in 24, which would fill one round if every slot lost half a unit).
 int chunks_of(const Adapters& ad, int64_t m) {
     const int64_t unit = 32 * blocks_of(m, ad.steps), slots = 32 * (int64_t)per_cu_of(ad.steps), fixed = 8;
-    const int64_t whole = (m + unit - 1) / unit, units = whole + std::min<int64_t>(ad.slots, whole) / 2;
+    const double groups = (double)std::min<int64_t>(ad.slots + 1, (m + unit - 1) / unit);
+    const int64_t units = (int64_t)std::ceil((double)m / (double)unit + groups / 2 + 1.3 * std::sqrt(groups / 12));
     const int64_t mblocks = (units + kWaves - 1) / kWaves;
     int best = 1;
     int64_t best_cost = -1;

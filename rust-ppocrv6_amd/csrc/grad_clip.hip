@@ -5,8 +5,8 @@
 // leaves one partial sum a workgroup, the second has each workgroup add all of them up in the same order
 // (8 KB from L2) and scale its share, so no launch and no workgroup waits in between for a single value.
 // Squares are exact in 64 bits and summed there: neither the squares of small gradients vanish nor those
-// of large ones overflow.  34M bf16 gradients in 56 tensors: 15.1 us for the squares (4.5 TB/s; from the caches where
-// the backward pass left them) and 20.5 for the second kernel (6.6 TB/s, its reads mostly from the caches), 44 us the call;
+// of large ones overflow.  34M bf16 gradients in 56 tensors: 15.8 us for the squares (4.3 TB/s; from the caches where
+// the backward pass left them) and 22.5 for the second kernel (6 TB/s, its reads mostly from the caches), 44 us the call;
 // a single adapter's two tensors 4 us each, which is what two launches take.
 //
 // The tensors' addresses and sizes go to the kernels as arguments, kTable tensors a launch: nothing is

@@ -9,8 +9,8 @@
 // exact products either way, summed in 32 bits.  ddown sums over all n rows: each workgroup keeps the sum
 // over its rows in registers and leaves it to a second kernel, which adds the workgroups' sums in a fixed order.
 //
-// rank 16 of fp32 18710 x 120: forward 5.9 us (3.2 TB/s from and to the caches), backward 9.5 + 3.0.  rank 64 of bf16
-// 32768 x 256: 12.9 us (2.9 TB/s), 16.4 + 2.4.  Latency bounds them, a round trip to memory and one through LDS for each
+// rank 16 of fp32 18710 x 120: forward 6.0 us (3.1 TB/s from and to the caches), backward 9.6 + 3.2.  rank 64 of bf16
+// 32768 x 256: 13.5 us (2.8 TB/s), 17.5 + 4.0.  Latency bounds them, a round trip to memory and one through LDS for each
 // block of rows, with few waves to cover it: the operands of the rank products take the registers.
 #include <algorithm>
 

@@ -11,7 +11,7 @@
 // lines): the sums go through the team in a fixed order, and the gradient, which needs them, is written from what the
 // lanes kept in registers; the steps beyond them are read again.  Sums are held in 64 bits.
 //
-// 4M steps in 32768 lines under a policy loss, 101 MB: 27.4 us, 3.7 TB/s (a copy: 5.1); in 16384 pairs, 68 MB: 19.8 us.
+// 4M steps in 32768 lines under a policy loss, 101 MB: 28 us, 3.6 TB/s (a copy: 5.1); in 16384 pairs, 68 MB: 19.8 us.
 // Vector instructions bound both: some 400 a wave of 64 lanes and 4 steps a lane (the exponentials, the sums in 64 bits,
 // the clipping's border), which is why loads are held back by nothing and sums use the registers' lane paths (34 and
 // 22 us with shuffles and branches around the loads).  Small calls are bound by the launch: a page's 2245 steps 4 us.
