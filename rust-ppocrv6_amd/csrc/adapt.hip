@@ -9,9 +9,8 @@
 // Rows are put in order by slot (plan_kernel) and padded to units of 32, so that a wave's rows have one
 // adapter; the four waves of a workgroup, each with a unit of its own, share the head's weight tiles through
 // LDS, and each wave reads its adapter's tile from L2.  30720 rows of an INT8 head under 64 adapters of rank 32:
-// 368 us in the statistics kernel, 386 GFLOP of halves at 1.05 PFLOP/s, the matrix units busy for 56% of them (the head's
-// own pass: 58%); the clock under that load, not memory, sets the rest.  The plan before it takes 9 us, the join of
-// the chunks behind it 8.
+// 368 us in the statistics kernel, 386 GFLOP of halves at 1.05 PFLOP/s, the matrix units busy for 57% of them at 1.81 GHz
+// (the head's own pass: 58%).  The plan before it takes 9 us, the join of the chunks behind it 8.
 //
 // Arithmetic: fp16 halves of both operands (22 bits), as the head's F16X2 mode, all in one fp32
 // accumulator: up is held divided by the class's unit (its scale, or where a head's lie far apart that times a
