@@ -473,8 +473,8 @@ int ppocr_ra_set_dev(ppocr_rh_t* h, int64_t slot, void* d_down, void* d_up, int6
  * Both operands of every product are fp16 halves (three products of 11 bits each, int8 weights exactly), the
  * rows at a power of two that their own largest value sets, summed in fp32: 22 bits of each row's and of the
  * adapter's largest products, and the same bits whatever the rows beside it hold.  The head's products lose a bit for each
- * power of two by which an adapter's largest scale |up| sum |down| passes 2^31 (an INT8 head: 2^22 times the largest of its
- * scales, where they lie within 2^32 of each other).  A row that holds an infinity or NaN has NaN logits; decoded, it is class 0.  There is no mode and no
+ * power of two by which an adapter's largest scale |up| sum |down| passes 2^22 times an FP32 head's largest weight or an INT8
+ * head's largest scale (where its scales lie within 2^32 of each other).  A row that holds an infinity or NaN has NaN logits; decoded, it is class 0.  There is no mode and no
  * precision guard. */
 size_t ppocr_ra_workspace_bytes(const ppocr_rh_t* h, int64_t m);
 int ppocr_ra_logits(const ppocr_rh_t* h, const float* a, const int64_t* line_off, int64_t lines, const int32_t* line_slot,

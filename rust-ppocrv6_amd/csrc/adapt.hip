@@ -14,7 +14,7 @@
 //
 // Arithmetic: fp16 halves of both operands (22 bits), as the head's F16X2 mode, all in one fp32
 // accumulator: up is held divided by the class's unit (its scale, or where a head's lie far apart that times a
-// power of two).  Each row is scaled by the power of two that its largest value sets, so rows of any size keep
+// power of two; of an FP32 head a power of two above the class's weights).  Each row is scaled by the power of two that its largest value sets, so rows of any size keep
 // their bits, whatever the rows beside them hold, and no row has to be computed again.  u = down a is computed by each wave before its first tile, from the rows it
 // holds; the products' layout is that of the operand that the next product needs.
 #include <algorithm>

@@ -23,7 +23,8 @@ struct Adapters {
     AdapterMeta* meta = nullptr;
     unsigned* range = nullptr;  // [slots + 1][2][kAdaptMostRank] sizes that a slot's powers of two come from
     // The head's fp16 records and the classes' units [n]: up is held divided by them, as the products of the
-    // records are.  The head's own, or where its scales lie far apart others with nearer units.
+    // records are.  An INT8 head's own, or where its scales lie far apart others with nearer units; for an FP32 head
+    // records of each class's weights over a power of two.
     const uint8_t* rec = nullptr;
     const float* unit = nullptr;
     uint8_t* own_rec = nullptr;

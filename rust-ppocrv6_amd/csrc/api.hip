@@ -2071,12 +2071,39 @@ constexpr size_t kAdaptWs = 256;
 // values of 7 bits are then held in fp16 that much lower, exactly.
 constexpr float kLeastAdaptScale = 1.0f / (1LL << 34);
 constexpr int kNearUnits = 8, kMostRaise = 24, kMostSpread = kMostRaise + 16;
+//
+// An FP32 head's own records hold weights to 2^-25, whatever their size.  Here each class has as its unit the power
+// of two above its largest weight (2^kNearUnits below the largest unit at least): 22 bits of it and more.
 int adapt_units(const ppocr_rh* base, Adapters* ad, size_t* total) try {
     ad->unit = base->d_scale;
     ad->rec = base->d_rec_h;
-    if (!base->quantized) return PPOCR_OK;
-    const int64_t n = base->n;
+    const int64_t n = base->n, k = base->k;
     std::vector<float> unit((size_t)n);
+    if (!base->quantized) {
+        std::vector<float> w((size_t)(n * k)), bias((size_t)n);
+        PPOCR_HIP(hipMemcpy(w.data(), base->d_w, w.size() * 4, hipMemcpyDeviceToHost));
+        PPOCR_HIP(hipMemcpy(bias.data(), base->d_bias, bias.size() * 4, hipMemcpyDeviceToHost));
+        constexpr int kLeast = -34;
+        std::vector<int> power((size_t)n, kLeast);
+        int top = kLeast;
+        for (int64_t i = 0; i < n; ++i) {
+            float most = 0.0f;
+            for (int64_t c = 0; c < k; ++c) most = std::max(most, std::fabs(w[(size_t)(i * k + c)]));
+            if (most > 0.0f && std::isfinite(most)) power[i] = std::max(std::ilogb(most) + 1, kLeast);
+            top = std::max(top, power[i]);
+        }
+        for (int64_t i = 0; i < n; ++i) {
+            const int p = std::max(power[i], top - kNearUnits);
+            unit[i] = std::ldexp(1.0f, p);
+            for (int64_t c = 0; c < k; ++c) w[(size_t)(i * k + c)] *= std::ldexp(1.0f, -p);
+        }
+        const std::vector<uint8_t> rec = build_records(base->geom, n, k, nullptr, w.data(), unit.data(), bias.data(), true);
+        if (int e = upload(&ad->own_unit, unit.data(), unit.size(), total)) return e;
+        if (int e = upload(&ad->own_rec, rec.data(), rec.size(), total)) return e;
+        ad->unit = ad->own_unit;
+        ad->rec = ad->own_rec;
+        return PPOCR_OK;
+    }
     PPOCR_HIP(hipMemcpy(unit.data(), base->d_scale, (size_t)n * 4, hipMemcpyDeviceToHost));
     int top = -1000, least = 1000;
     for (int64_t i = 0; i < n; ++i) {

@@ -173,6 +173,34 @@ def test_classes_of_tiny_weights(rh):
         assert np.array_equal(h.head.logits(a), h.base.logits(a))
 
 
+def test_fp32_heads_of_any_size(rh):
+    """FP32 heads whose weights are all small, all large, or far apart from class to class: 22 bits of each class's
+    weights, and of classes 2^-8 of the largest and below the same of that."""
+    rng = np.random.default_rng(21)
+    n, k = 300, 120
+    for size in (2.0 ** -30, 1e-6, 1e-3, 1.0, 3000.0, None):
+        w = (rng.standard_normal((n, k)) * 0.2).astype(np.float32)
+        w *= (10.0 ** rng.uniform(-9, 0, (n, 1))).astype(np.float32) if size is None else np.float32(size)
+        w[5] = 0.0
+        h = ac.Head(rh, rng, n, k, False, 2, 16, ranks=[0, 0])
+        h.base = rh.RecHead(w_t=w, bias=h.bias)
+        h.w = w.astype(np.float64)
+        h.head = rh.AdaptedHead(h.base, 2, 16)
+        most = np.abs(w).max()
+        down = (rng.standard_normal((16, k)) / np.sqrt(k)).astype(np.float32)
+        for slot, up in enumerate((1e-3, 1.0)):
+            h.set(slot, down, (rng.standard_normal((n, 16)) * up * most).astype(np.float32), 1.0)
+        a = (rng.standard_normal((90, k)) * 4).astype(np.float32)
+        off, slot = ac.offsets([30, 30, 30]), [0, 1, -1]
+        z, e = h.exact(a, h.rows_of(90, off, slot))
+        # two halves of values below 2 p, p the power of two above 2^-8 of the largest weight or the class's: 2^-25 of a
+        # unit of p each, of the weights against the rows and of up (its powers of two undone) against u
+        unit = np.maximum(np.maximum(np.abs(w).max(axis=1), 2.0 ** -8 * most), 2.0 ** -35) * 2
+        rough = np.abs(a).max(axis=1, keepdims=True) * unit * 2.0 ** -25
+        e = e + rough * (k + 16)
+        tc.close(ac.Call(h, a, off, slot).logits().get(), z, e, f"weights of {size}")
+
+
 def test_rows_of_any_size(rh):
     """Rows scaled by powers of two far apart, of zeros, and rows with infinities and NaN beside them: each keeps
     its own bits."""
