@@ -11,7 +11,7 @@
 // lines): the sums go through the team in a fixed order, and the gradient, which needs them, is written from what the
 // lanes kept in registers; the steps beyond them are read again.  Sums are held in 64 bits.
 //
-// 4M steps in 32768 lines under a policy loss, 101 MB: 28 us, 3.6 TB/s (a copy: 5.1); in 16384 pairs, 68 MB: 19.8 us.
+// 4M steps in 32768 lines under a policy loss, 101 MB: 27.4 us, 3.7 TB/s (a copy: 5.1); in 16384 pairs, 68 MB: 19.8 us.
 // Vector instructions bound both: some 400 a wave of 64 lanes and 4 steps a lane (the exponentials, the sums in 64 bits,
 // the clipping's border), which is why loads are held back by nothing and sums use the registers' lane paths (34 and
 // 22 us with shuffles and branches around the loads).  Small calls are bound by the launch: a page's 2245 steps 4 us.
@@ -134,9 +134,10 @@ struct Border {
     float top, bottom;    // 1 + high, 1 - low
 };
 
+// The arguments' structures are passed by value: by reference 4M steps take 28.4 us instead of 27.4.
 // Loads that nothing stands between: of a step of the line in any case, what they hold is looked at later.
 template <bool REF>
-__device__ __forceinline__ PolicyRow policy_fetch(const LineSteps& s, const PolicyArgs& a, float line_adv, unsigned r, unsigned hi) {
+__device__ __forceinline__ PolicyRow policy_fetch(LineSteps s, PolicyArgs a, float line_adv, unsigned r, unsigned hi) {
     const unsigned at = min(r, hi - 1);
     PolicyRow p{s.loss[at], a.old[at], 0.0f, line_adv, 0};
     if constexpr (REF) p.ref = a.ref[at];
@@ -146,7 +147,7 @@ __device__ __forceinline__ PolicyRow policy_fetch(const LineSteps& s, const Poli
 }
 // The step's gradient; its value, divergence and clipping into v, kl and cut.
 template <bool REF>
-__device__ __forceinline__ float policy_eval(const PolicyRow& p, const Border& bo, float beta, float& v, float& kl, bool& cut) {
+__device__ __forceinline__ float policy_eval(PolicyRow p, Border bo, float beta, float& v, float& kl, bool& cut) {
     const double far = (double)p.old - (double)p.x;
     cut = p.adv > 0.0f ? far > bo.above : p.adv < 0.0f && far < bo.below;
     const float ratio = expf(p.old - p.x);
@@ -164,7 +165,7 @@ __device__ __forceinline__ float policy_eval(const PolicyRow& p, const Border& b
 }
 // Sums of a team's lanes over steps lo .. hi - 1; the slopes of the last turn, and which of its steps count, stay.
 template <int G, bool REF>
-__device__ __forceinline__ Sums policy_sums(const LineSteps& s, const PolicyArgs& a, const Border& bo, float line_adv, unsigned lo,
+__device__ __forceinline__ Sums policy_sums(LineSteps s, PolicyArgs a, Border bo, float line_adv, unsigned lo,
                                             unsigned hi, int l, float (&slope)[kKeep], bool (&there)[kKeep]) {
     Sums sum{0.0, 0.0, 0, 0};
     for (unsigned base = lo; base < hi; base += kKeep * G) {
@@ -192,7 +193,7 @@ __device__ __forceinline__ void policy_put(const PolicyArgs& a, float g, float s
 }
 // Gradients of steps lo .. hi - 1, each computed again.
 template <int G, bool REF>
-__device__ __forceinline__ void policy_grads(const LineSteps& s, const PolicyArgs& a, const Border& bo, float line_adv, float g,
+__device__ __forceinline__ void policy_grads(LineSteps s, PolicyArgs a, Border bo, float line_adv, float g,
                                              float share, unsigned lo, unsigned hi, int l) {
     for (unsigned base = lo; base < hi; base += kKeep * G) {
         PolicyRow p[kKeep];
@@ -219,7 +220,7 @@ __device__ __forceinline__ float policy_line_outputs(const PolicyArgs& a, int64_
     return *g / count;
 }
 template <int G, bool REF>
-__device__ __forceinline__ void policy_line(const LineSteps& s, const PolicyArgs& a, const Border& bo, int64_t line, unsigned lo,
+__device__ __forceinline__ void policy_line(LineSteps s, PolicyArgs a, Border bo, int64_t line, unsigned lo,
                                             unsigned hi, int l, Sums* red) {
     const float line_adv = a.per_row ? 0.0f : a.adv[line];
     float slope[kKeep], g;
