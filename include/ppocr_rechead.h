@@ -445,37 +445,40 @@ int ppocr_layernorm_backward_dev(void* d_dy, void* d_x, const float* d_w, const 
 
 /* ---------------------------------------------------------------- adapting the head
  * No counterpart in the reference, which has one head: many users' versions of it, each a low-rank
- * adapter beside the shared weights, and the rest of what they are trained with.  Types, workspaces, streams and
- * equal bits as for the training entry points above.  No output may overlap an input or another output, but where it
- * says so. */
+ * adapter beside the shared weights, and the rest of what they are trained with.  Types,
+ * workspaces, streams and equal bits as for the training entry points above.  No output may
+ * overlap an input or another output, but where it says so. */
 
-/* A head with `slots` (1 to 4096) places for adapters of up to max_rank (1 to 64): a handle on the same
- * weights, which every ppocr_rh_ call takes as it takes `head` (without any adapter), with device
- * memory for the adapters of about 4 n max_rank bytes a slot (max_rank rounded up to 16, 32 or 64).  `head` and the
- * new handle may be destroyed in any order.  Heads that the matrix kernels take (k of 73 to 80 or 113 to 120, an FP32
- * head's weights below 32768, an INT8 head's scales 2^-34 at least and within 2^40 of each other) only. */
+/* A head with `slots` (1 to 4096) places for adapters of up to max_rank (1 to 64): a handle on the
+ * same weights, which every ppocr_rh_ call takes as it takes `head` (without any adapter), with device
+ * memory for the adapters of about 4 n max_rank bytes a slot (max_rank rounded up to 16, 32 or 64),
+ * and for an FP32 head's weights once more.  `head` and the new handle may be destroyed in any order.
+ * Heads that the matrix kernels take (k of 73 to 80 or 113 to 120, an FP32 head's weights below 32768,
+ * an INT8 head's scales 2^-34 at least and within 2^40 of each other) only. */
 int ppocr_ra_create(const ppocr_rh_t* head, int64_t slots, int64_t max_rank, ppocr_rh_t** out);
 void ppocr_ra_destroy(ppocr_rh_t* h); /* ppocr_rh_destroy */
 int ppocr_ra_shape(const ppocr_rh_t* h, int64_t* slots, int64_t* max_rank);
-/* Puts an adapter into a slot: with down [rank][k] and up [n][rank], lines that name the slot get scale * up
- * (down a) added to the logits of a row a.  rank 0 empties the slot (down and up may be NULL).  The adapter
- * is laid out in the slot, and the tensors are not kept.  The `_dev` form enqueues on `stream`; calls that read the slot on
- * other streams must be ordered with it by the caller, sets of different slots need not be. */
+/* Puts an adapter into a slot: with down [rank][k] and up [n][rank], lines that name the slot get
+ * scale * up (down a) added to the logits of a row a.  rank 0 empties the slot (down and up may be
+ * NULL).  The adapter is laid out in the slot, and the tensors are not kept.  The `_dev` form enqueues
+ * on `stream`; calls that read the slot on other streams must be ordered with it by the caller, sets
+ * of different slots need not be. */
 int ppocr_ra_set(ppocr_rh_t* h, int64_t slot, const float* down, const float* up, int64_t rank, float scale);
 int ppocr_ra_set_dev(ppocr_rh_t* h, int64_t slot, void* d_down, void* d_up, int64_t rank, float scale, int dtype,
                      void* stream);
 
 /* ppocr_rh_logits and ppocr_rh_decode with an adapter for each line: line i's rows line_off[i] ..
- * line_off[i+1] of a [m][k] run under slot line_slot[i].  A negative slot is none: the head alone; so is,
- * in the `_dev` forms, one of `slots` and above (the host forms refuse it), a slot that holds no adapter, and for logits every row
- * that no line covers.  The `_dev` forms read the lines on the device as ppocr_rh_decode_dev does; a row
- * that lies in several lines (offsets that go backwards) takes the adapter of one of them.
- * Both operands of every product are fp16 halves (three products of 11 bits each, int8 weights exactly), the
- * rows at a power of two that their own largest value sets, summed in fp32: 22 bits of each row's and of the
- * adapter's largest products, and the same bits whatever the rows beside it hold.  The head's products lose a bit for each
- * power of two by which an adapter's largest scale |up| sum |down| passes 2^22 times an FP32 head's largest weight or an INT8
- * head's largest scale (where its scales lie within 2^32 of each other).  A row that holds an infinity or NaN has NaN logits; decoded, it is class 0.  There is no mode and no
- * precision guard. */
+ * line_off[i+1] of a [m][k] run under slot line_slot[i].  A negative slot is none: the head alone; so
+ * is, in the `_dev` forms, one of `slots` and above (the host forms refuse it), a slot that holds no
+ * adapter, and for logits every row that no line covers.  The `_dev` forms read the lines on the
+ * device as ppocr_rh_decode_dev does; a row that lies in several lines (offsets that go backwards)
+ * takes the adapter of one of them. Both operands of every product are fp16 halves (three products of
+ * 11 bits each, int8 weights exactly), the rows at a power of two that their own largest value sets,
+ * summed in fp32: 22 bits of each row's and of the adapter's largest products, and the same bits
+ * whatever the rows beside it hold.  The head's products lose a bit for each power of two by which an
+ * adapter's largest scale |up| sum |down| passes 2^22 times an FP32 head's largest weight or an INT8
+ * head's largest scale (where its scales lie within 2^32 of each other).  A row that holds an infinity
+ * or NaN has NaN logits; decoded, it is class 0.  There is no mode and no precision guard. */
 size_t ppocr_ra_workspace_bytes(const ppocr_rh_t* h, int64_t m);
 int ppocr_ra_logits(const ppocr_rh_t* h, const float* a, const int64_t* line_off, int64_t lines, const int32_t* line_slot,
                     float* out);
@@ -487,15 +490,15 @@ int ppocr_ra_decode_dev(const ppocr_rh_t* h, const float* d_a, int64_t m, const 
                         const int32_t* d_line_slot, int32_t* d_idx, float* d_maxprob, int32_t* d_seq, int64_t* d_seq_len,
                         float* d_score, void* d_workspace, size_t workspace_bytes, void* stream);
 
-/* The weight that an adapter is trained under, out = w_t + scale up down [n][k], for the losses above, whose dw_t
- * is then its gradient; out may be w_t.  rank is 1 to 64, k 1 to 256, n 1 to 2^24; all tensors are of `dtype`, products and sums in
- * fp32 of exact products, rounded once. */
+/* The weight that an adapter is trained under, out = w_t + scale up down [n][k], for the losses above,
+ * whose dw_t is then its gradient; out may be w_t.  rank is 1 to 64, k 1 to 256, n 1 to 2^24; all
+ * tensors are of `dtype`, products and sums in fp32 of exact products, rounded once. */
 int ppocr_ra_merge(const float* w_t, const float* down, const float* up, int64_t n, int64_t k, int64_t rank, float scale,
                    float* out);
 int ppocr_ra_merge_dev(void* d_w_t, void* d_down, void* d_up, int64_t n, int64_t k, int64_t rank, float scale, int dtype,
                        void* d_out, void* stream);
-/* Its gradients for the adapter, from the merged weight's: ddown = scale up^T dw_t [rank][k] and dup = scale dw_t
- * down^T [n][rank].  Each may be NULL (not computed); none may overlap an input. */
+/* Its gradients for the adapter, from the merged weight's: ddown = scale up^T dw_t [rank][k] and dup =
+ * scale dw_t down^T [n][rank].  Each may be NULL (not computed); none may overlap an input. */
 size_t ppocr_ra_merge_workspace_bytes(int64_t n, int64_t k, int64_t rank);
 int ppocr_ra_merge_backward(const float* dw_t, const float* down, const float* up, int64_t n, int64_t k, int64_t rank,
                             float scale, float* ddown, float* dup);
@@ -503,20 +506,23 @@ int ppocr_ra_merge_backward_dev(void* d_dw_t, void* d_down, void* d_up, int64_t 
                                 int dtype, void* d_ddown, void* d_dup, void* d_workspace, size_t workspace_bytes,
                                 void* stream);
 
-/* Losses over lines of steps, from the steps' cross entropies as ppocr_xent_forward writes them (minus the
- * log probability of each step's class).  Line i is steps line_off[i] .. line_off[i+1] of the m; the host form
- * refuses offsets that do not start at 0, go backwards or pass m, the `_dev` form clamps them into [0, m] (a line whose end precedes
- * its start is empty; what offsets that go backwards give is not specified).  A step whose target is negative does not count,
- * whatever the arrays hold for it (target NULL: all count).  row_grad [m] is the gradient by each
- * step's cross entropy, which ppocr_xent_backward takes as its grad; it is written whole, 0 for steps that do
- * not count and steps of no line.  Any output may be NULL, and m and lines up to 2^30.
+/* Losses over lines of steps, from the steps' cross entropies as ppocr_xent_forward writes them (minus
+ * the log probability of each step's class).  Line i is steps line_off[i] .. line_off[i+1] of the m;
+ * the host form refuses offsets that do not start at 0, go backwards or pass m, the `_dev` form clamps
+ * them into [0, m] (a line whose end precedes its start is empty; what offsets that go backwards give
+ * is not specified).  A step whose target is negative does not count, whatever the arrays hold for it
+ * (target NULL: all count).  row_grad [m] is the gradient by each step's cross entropy, which
+ * ppocr_xent_backward takes as its grad; it is written whole, 0 for steps that do not count and steps
+ * of no line.  Any output may be NULL, and m and lines up to 2^30.
  *
- * The clipped policy loss.  With x = loss[r], rho = exp(old_loss[r] - x) and A the advantage (adv [m] if
- * adv_per_row, else [lines]), a step's value is -min(rho A, min(max(rho, 1 - clip_low), 1 + clip_high) A) + beta (e^t - t - 1),
- * t = x - ref_loss[r], the divergence from a reference policy (ref_loss NULL: no such term).  line_loss[i] is the mean of the
- * values of a line's steps that count (0 if none), line_kl the mean divergence, line_clipped the share of steps whose clipped product is the smaller one.
- * Steps exactly at the border are not clipped; the side is decided on old_loss - loss in 64 bits.  grad [lines]: the gradient by line_loss
- * (NULL: 1); a line whose grad is 0 has zeros.  clip_low is 0 to 1, clip_high at least 0, beta finite. */
+ * The clipped policy loss.  With x = loss[r], rho = exp(old_loss[r] - x) and A the advantage (adv [m]
+ * if adv_per_row, else [lines]), a step's value is -min(rho A, min(max(rho, 1 - clip_low), 1 +
+ * clip_high) A) + beta (e^t - t - 1), t = x - ref_loss[r], the divergence from a reference policy
+ * (ref_loss NULL: no such term).  line_loss[i] is the mean of the values of a line's steps that count
+ * (0 if none), line_kl the mean divergence, line_clipped the share of steps whose clipped product is
+ * the smaller one. Steps exactly at the border are not clipped; the side is decided on old_loss - loss
+ * in 64 bits.  grad [lines]: the gradient by line_loss (NULL: 1); a line whose grad is 0 has zeros.
+ * clip_low is 0 to 1, clip_high at least 0, beta finite. */
 int ppocr_policy_loss(const float* loss, const float* old_loss, const float* ref_loss, const int32_t* target,
                       const float* adv, int adv_per_row, const int64_t* line_off, int64_t lines, int64_t m, float clip_low,
                       float clip_high, float beta, const float* grad, float* line_loss, float* line_kl,
@@ -526,10 +532,11 @@ int ppocr_policy_loss_dev(const float* d_loss, const float* d_old_loss, const fl
                           float clip_low, float clip_high, float beta, const float* d_grad, float* d_line_loss,
                           float* d_line_kl, float* d_line_clipped, float* d_row_grad, void* stream);
 /* The loss of a preference for one reading of an image over another: of the 2 pairs lines, line 2p is
- * preferred over line 2p + 1.  A line's reward is beta sum (ref_loss - loss) over its steps that count (average:
- * their mean; ref_loss NULL: 0), h the difference of the pair's rewards, and pair_loss = -(1 - smoothing) log s(h) - smoothing
- * log s(-h) with the logistic s.  reward [2 pairs]; grad [pairs]: the gradient by pair_loss (NULL: 1); a
- * pair whose grad is 0 has zeros.  smoothing is 0 to 1, beta finite. */
+ * preferred over line 2p + 1.  A line's reward is beta sum (ref_loss - loss) over its steps that count
+ * (average: their mean; ref_loss NULL: 0), h the difference of the pair's rewards, and pair_loss = -(1
+ * - smoothing) log s(h) - smoothing log s(-h) with the logistic s.  reward [2 pairs]; grad [pairs]:
+ * the gradient by pair_loss (NULL: 1); a pair whose grad is 0 has zeros.  smoothing is 0 to 1, beta
+ * finite. */
 int ppocr_preference_loss(const float* loss, const float* ref_loss, const int32_t* target, const int64_t* line_off,
                           int64_t pairs, int64_t m, float beta, float smoothing, int average, const float* grad,
                           float* pair_loss, float* reward, float* row_grad);
@@ -538,11 +545,13 @@ int ppocr_preference_loss_dev(const float* d_loss, const float* d_ref_loss, cons
                               int average, const float* d_grad, float* d_pair_loss, float* d_reward,
                               float* d_row_grad, void* stream);
 
-/* The norm of `count` (up to 65536) gradient tensors together, norm = sqrt(sum of all squares), and each of them times
- * min(1, max_norm / norm): tensor i has sizes[i] (up to 2^40) values of type dtypes[i] at grads[i] and is written to out[i],
- * which is grads[i] or overlaps none of them (out NULL: in place).  Two outputs may not overlap.  A norm that is not finite
- * leaves the gradients as they are; max_norm INFINITY only takes the norm.  Squares are summed in 64 bits.  The tables are host arrays in both
- * forms (read before the call returns), the tensors of the `_dev` form and norm (may be NULL) device memory; the host form takes fp32. */
+/* The norm of `count` (up to 65536) gradient tensors together, norm = sqrt(sum of all squares), and
+ * each of them times min(1, max_norm / norm): tensor i has sizes[i] (up to 2^40) values of type
+ * dtypes[i] at grads[i] and is written to out[i], which is grads[i] or overlaps none of them (out
+ * NULL: in place).  Two outputs may not overlap.  A norm that is not finite leaves the gradients as
+ * they are; max_norm INFINITY only takes the norm.  Squares are summed in 64 bits.  The tables are
+ * host arrays in both forms (read before the call returns), the tensors of the `_dev` form and norm
+ * (may be NULL) device memory; the host form takes fp32. */
 size_t ppocr_grad_clip_workspace_bytes(const int64_t* sizes, int64_t count);
 int ppocr_grad_clip(void* const* grads, void* const* out, const int64_t* sizes, int64_t count, float max_norm,
                     float* norm);
