@@ -782,10 +782,12 @@ def _steps(op, loss, others, target, line_off):
     return loss, others, target, line_off
 
 
-def policy_loss(loss, old_loss, adv, line_off, target=None, ref_loss=None, clip_low=0.2, clip_high=0.2, beta=0.0, grad=None):
+def policy_loss(loss, old_loss, adv, line_off, target=None, ref_loss=None, clip_low=0.2, clip_high=0.2, beta=0.0, grad=None,
+                per_step=None):
     """(line_loss, line_kl, line_clipped, row_grad) of the clipped policy loss over lines of steps, from the
     steps' cross entropies now, when they were sampled and under a reference (None: no divergence term).
-    adv: the advantages of the lines, or of the steps.  row_grad is what cross_entropy_backward takes as
+    adv: the advantages of the steps (per_step) or of the lines; None takes it from their number, and refuses
+    as many lines as steps unless each line is one step.  row_grad is what cross_entropy_backward takes as
     grad; grad [lines] is the gradient by line_loss (None: 1)."""
     op = "PolicyLoss"
     loss, (old, ref), target, line_off = _steps(op, loss, (old_loss, ref_loss), target, line_off)
@@ -793,10 +795,16 @@ def policy_loss(loss, old_loss, adv, line_off, target=None, ref_loss=None, clip_
     adv = _f32(adv)
     if adv.shape not in ((lines,), (m,)):
         raise OcrError(op, f"expected advantages of {lines} lines or {m} steps, got shape {list(adv.shape)}")
-    per_row = adv.shape != (lines,)
+    if per_step is None:
+        if m == lines and not (np.diff(line_off) == 1).all():
+            raise OcrError(op, f"{m} advantages for {lines} lines of {m} steps: per_step has to say whose they are")
+        per_step = adv.shape != (lines,)
+    elif adv.shape != ((m,) if per_step else (lines,)):
+        raise OcrError(op, f"expected advantages of {m if per_step else lines} {'steps' if per_step else 'lines'}, "
+                           f"got shape {list(adv.shape)}")
     grad = None if grad is None else _per_row(op, grad, (lines,), np.float32, "grad")
     out = [np.empty(lines, np.float32) for _ in range(3)] + [np.empty(m, np.float32)]
-    _check(_lib.lib().ppocr_policy_loss(_ptr(loss), _ptr(old), _ptr(ref), _ptr(target), _ptr(adv), int(per_row), _ptr(line_off),
+    _check(_lib.lib().ppocr_policy_loss(_ptr(loss), _ptr(old), _ptr(ref), _ptr(target), _ptr(adv), int(bool(per_step)), _ptr(line_off),
                                         lines, m, float(clip_low), float(clip_high), float(beta), _ptr(grad),
                                         *(_ptr(o) for o in out)))
     return tuple(out)
