@@ -158,8 +158,11 @@ __device__ __forceinline__ float policy_eval(PolicyRow p, Border bo, float beta,
     if constexpr (REF) {
         float em1;
         exp_tail(p.x - p.ref, kl, em1);
-        v = fmaf(beta, kl, v);
-        slope = fmaf(beta, em1, slope);
+        // a weight of 0 takes nothing from a divergence beyond every bound either
+        if (beta != 0.0f) {
+            v = fmaf(beta, kl, v);
+            slope = fmaf(beta, em1, slope);
+        }
     }
     return slope;
 }

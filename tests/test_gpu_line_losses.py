@@ -1,0 +1,37 @@
+"""Losses over lines of steps where a term, a sum or a mean leaves the numbers of 32 bits, and where only some of the
+outputs are asked for."""
+import numpy as np
+import pytest
+
+import adapt_common as ac
+import train_common as tc
+from test_gpu_sequence_loss import Policy, Preference
+
+pytestmark = pytest.mark.gpu
+
+# lines in one workgroup each, and lines that several share
+LENGTHS = [[5, 1, 70], [900, 300], [40000, 3000, 20000]]
+
+
+def outputs_of(job, keys=None):
+    o = job.outputs()
+    return {k: v.get() for k, v in job.run({k: o[k] for k in (keys or o)}).items()}
+
+
+@pytest.mark.parametrize("lengths", LENGTHS, ids=["short", "long", "split"])
+def test_divergences_without_a_weight(rh, lengths):
+    """beta 0 and a reference: the divergence is reported, infinite where 32 bits do not hold it, and is no part of the
+    loss and of the gradients."""
+    rng = np.random.default_rng(1)
+    off = ac.offsets(lengths)
+    m = int(off[-1])
+    loss = (rng.random(m) * 3).astype(np.float32)
+    ref = (loss + rng.standard_normal(m) * 0.3).astype(np.float32)
+    loss[::5] += 100
+    ref[::5] = 0.5
+    old = (loss + rng.standard_normal(m) * 0.2).astype(np.float32)
+    job = Policy(rh, loss, old, ref, None, rng.standard_normal(len(lengths)).astype(np.float32), off, beta=0.0)
+    got = outputs_of(job)
+    kl = got.pop("kl")
+    assert (kl[np.add.reduceat(loss > 90, off[:-1]) > 0] == np.inf).all() and not np.isnan(kl).any()
+    job.check(got, "beta 0")
