@@ -519,8 +519,9 @@ int ppocr_ra_merge_backward_dev(void* d_dw_t, void* d_down, void* d_up, int64_t 
  * if adv_per_row, else [lines]), a step's value is -min(rho A, min(max(rho, 1 - clip_low), 1 +
  * clip_high) A) + beta (e^t - t - 1), t = x - ref_loss[r], the divergence from a reference policy
  * (ref_loss NULL: no such term; beta 0: line_kl alone).  line_loss[i] is the mean of the values of a line's steps that count
- * (0 if none), line_kl the mean divergence, line_clipped the share of steps whose clipped product is
- * the smaller one. Steps exactly at the border are not clipped; the side is decided on old_loss - loss
+ * (0 if none), line_kl the mean divergence (each step's value, slope and divergence is a 32-bit
+ * number, infinite above the largest), line_clipped the share of steps whose clipped product is
+ * the smaller one.  Steps exactly at the border are not clipped; the side is decided on old_loss - loss
  * in 64 bits.  grad [lines]: the gradient by line_loss (NULL: 1); a line whose grad is 0 has zeros.
  * clip_low is 0 to 1, clip_high at least 0, beta finite. */
 int ppocr_policy_loss(const float* loss, const float* old_loss, const float* ref_loss, const int32_t* target,

@@ -211,12 +211,17 @@ __device__ __forceinline__ void policy_grads(LineSteps s, PolicyArgs a, Border b
         }
     }
 }
+// The mean of `count` values; their sum may pass the largest 32-bit number where the mean does not.
+__device__ __forceinline__ float mean_of(double sum, float count) {
+    const float s = (float)sum;
+    return __builtin_fabsf(s) < INFINITY ? s / count : (float)(sum / (double)count);
+}
 // A line's outputs, and what its gradients are multiplied with.
 __device__ __forceinline__ float policy_line_outputs(const PolicyArgs& a, int64_t line, const Sums& sum, bool write, float* g) {
     const float count = (float)max(sum.x, 1);
     if (write) {
-        if (a.loss) a.loss[line] = (float)sum.a / count;
-        if (a.kl) a.kl[line] = (float)sum.b / count;
+        if (a.loss) a.loss[line] = mean_of(sum.a, count);
+        if (a.kl) a.kl[line] = mean_of(sum.b, count);
         if (a.clipped) a.clipped[line] = (float)sum.y / count;
     }
     *g = a.grad ? a.grad[line] : 1.0f;

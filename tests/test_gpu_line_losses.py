@@ -35,3 +35,23 @@ def test_divergences_without_a_weight(rh, lengths):
     kl = got.pop("kl")
     assert (kl[np.add.reduceat(loss > 90, off[:-1]) > 0] == np.inf).all() and not np.isnan(kl).any()
     job.check(got, "beta 0")
+
+
+@pytest.mark.parametrize("lengths", LENGTHS, ids=["short", "long", "split"])
+def test_means_of_large_values(rh, lengths):
+    """Values whose sum passes the largest number of 32 bits, and their mean does not."""
+    off = ac.offsets(lengths)
+    m = int(off[-1])
+    loss = np.full(m, 88.0, np.float32)
+    adv = np.array([3e38, -3e38, 1e38], np.float32)[:len(lengths)]
+    job = Policy(rh, loss, loss, np.full(m, 0.5, np.float32), None, adv, off, beta=1.0)  # divergences of e^87.5
+    got = outputs_of(job)
+    assert np.isfinite(got["kl"]).all()
+    # a step's value in the second line, and its slope in the first, is 3e38 + e^87.5 = 4.0e38 itself, above the largest
+    # number, 3.4028e38
+    assert (np.isinf(got["loss"]) == (np.arange(len(lengths)) == 1)).all()
+    want, tol = ac.policy64(loss, loss, np.full(m, 0.5, np.float32), None, adv, False, off, 0.2, 0.28, 1.0)
+    want["loss"][1:2] = np.inf
+    want["row_grad"][:off[1]] = got["row_grad"][:off[1]]
+    for k, v in got.items():
+        tc.close(v, want[k], tol[k], f"means {k}")
