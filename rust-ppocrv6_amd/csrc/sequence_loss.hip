@@ -330,7 +330,8 @@ __device__ __forceinline__ void preference_pair_outputs(const PreferenceArgs& a,
     const float up = h >= 0.0 ? soft : hf + soft, down = h >= 0.0 ? hf + soft : soft;  // -log s(h), -log s(-h)
     const float keep = 1.0f - a.smoothing;
     if (write) {
-        if (a.loss) a.loss[pair] = a.smoothing == 0.0f ? up : fmaf(keep, up, a.smoothing * down);
+        // a weight of 0 takes nothing from a loss beyond every bound
+        if (a.loss) a.loss[pair] = a.smoothing == 0.0f ? up : keep == 0.0f ? down : fmaf(keep, up, a.smoothing * down);
         if (a.reward) {
             a.reward[2 * pair] = (float)ra;
             a.reward[2 * pair + 1] = (float)rb;

@@ -55,3 +55,14 @@ def test_means_of_large_values(rh, lengths):
     want["row_grad"][:off[1]] = got["row_grad"][:off[1]]
     for k, v in got.items():
         tc.close(v, want[k], tol[k], f"means {k}")
+
+
+def test_all_smoothing_under_an_infinite_margin(rh):
+    """smoothing 1 is the other line's loss alone, whatever the margin."""
+    loss = np.array([3e38] * 4 + [0.5, 1.0] + [3e38] * 4, np.float32)
+    off = [0, 4, 5, 6, 10]
+    job = Preference(rh, loss, None, None, off, 1.0, 1.0)
+    got = outputs_of(job, ("loss", "row_grad"))
+    assert got["loss"][0] == 0 and got["loss"][1] == np.inf
+    want, tol = ac.preference64(loss, None, None, off, 1.0, 1.0, False)
+    tc.close(got["row_grad"], want["row_grad"], tol["row_grad"], "row_grad")
