@@ -513,17 +513,21 @@ int ppocr_ra_merge_backward_dev(void* d_dw_t, void* d_down, void* d_up, int64_t 
  * is not specified).  A step whose target is negative does not count, whatever the arrays hold for it
  * (target NULL: all count).  row_grad [m] is the gradient by each step's cross entropy, which
  * ppocr_xent_backward takes as its grad; it is written whole, 0 for steps that do not count and steps
- * of no line.  Any output may be NULL, and m and lines up to 2^30.
+ * of no line.  Any output may be NULL, and m and lines up to 2^30.  Equal bits are those of calls
+ * that ask for row_grad, or that do not: long lines are split over the GPU with it, and a line's
+ * sums (64 bits) are then added in another order.  Split are fewer than 128 lines (or pairs) of
+ * 16384 steps on average and above; without row_grad, and where one line is far longer than the
+ * rest of 128 and more, a line is one workgroup's work (0.7 ns a step).
  *
- * The clipped policy loss.  With x = loss[r], rho = exp(old_loss[r] - x) and A the advantage (adv [m]
- * if adv_per_row, else [lines]), a step's value is -min(rho A, min(max(rho, 1 - clip_low), 1 +
+ * The clipped policy loss.  With x = loss[r], rho = exp(old_loss[r] - x) and A the advantage (adv
+ * [m] if adv_per_row, else [lines]), a step's value is -min(rho A, min(max(rho, 1 - clip_low), 1 +
  * clip_high) A) + beta (e^t - t - 1), t = x - ref_loss[r], the divergence from a reference policy
- * (ref_loss NULL: no such term; beta 0: line_kl alone).  line_loss[i] is the mean of the values of a line's steps that count
- * (0 if none), line_kl the mean divergence (each step's value, slope and divergence is a 32-bit
- * number, infinite above the largest), line_clipped the share of steps whose clipped product is
- * the smaller one.  Steps exactly at the border are not clipped; the side is decided on old_loss - loss
- * in 64 bits.  grad [lines]: the gradient by line_loss (NULL: 1); a line whose grad is 0 has zeros.
- * clip_low is 0 to 1, clip_high at least 0, beta finite. */
+ * (ref_loss NULL: no such term; beta 0: line_kl alone).  line_loss[i] is the mean of the values of a
+ * line's steps that count (0 if none), line_kl the mean divergence (each step's value, slope and
+ * divergence is a 32-bit number, infinite above the largest), line_clipped the share of steps whose
+ * clipped product is the smaller one.  Steps exactly at the border are not clipped; the side is
+ * decided on old_loss - loss in 64 bits.  grad [lines]: the gradient by line_loss (NULL: 1); a line
+ * whose grad is 0 has zeros.  clip_low is 0 to 1, clip_high at least 0, beta finite. */
 int ppocr_policy_loss(const float* loss, const float* old_loss, const float* ref_loss, const int32_t* target,
                       const float* adv, int adv_per_row, const int64_t* line_off, int64_t lines, int64_t m, float clip_low,
                       float clip_high, float beta, const float* grad, float* line_loss, float* line_kl,
