@@ -553,8 +553,10 @@ int ppocr_preference_loss_dev(const float* d_loss, const float* d_ref_loss, cons
 /* The norm of `count` (up to 65536) gradient tensors together, norm = sqrt(sum of all squares), and
  * each of them times min(1, max_norm / norm): tensor i has sizes[i] (up to 2^40) values of type
  * dtypes[i] at grads[i] and is written to out[i], which is grads[i] or overlaps none of them (out
- * NULL: in place).  Two outputs may not overlap.  A norm that is not finite leaves the gradients as
- * they are; max_norm INFINITY only takes the norm.  Squares are summed in 64 bits.  The tables are
+ * NULL: in place).  Two outputs may not overlap.  The norm is held in 64 bits, where squares are
+ * summed too: one above the largest 32-bit number scales the gradients as any other and is written
+ * to norm as infinity.  A NaN or infinity among the gradients leaves them all as they are; max_norm
+ * INFINITY only takes the norm.  The tables are
  * host arrays in both forms (read before the call returns), the tensors of the `_dev` form and norm
  * (may be NULL) device memory; the host form takes fp32. */
 size_t ppocr_grad_clip_workspace_bytes(const int64_t* sizes, int64_t count);

@@ -115,7 +115,7 @@ __device__ __forceinline__ double chunk_squares(const void* in, int64_t at, int 
 }
 
 template <typename T>
-__device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t at, int n, float scale) {
+__device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t at, int n, float power, float scale) {
     using C = Chunk<T>;
     T* q = (T*)out + at;
     const bool wide = (reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) % 16 == 0;
@@ -124,7 +124,7 @@ __device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t a
 #pragma unroll
     for (int r = 0; r < C::R; ++r) {
 #pragma unroll
-        for (int v = 0; v < C::V; ++v) c.w[r].v[v] = down(up(c.w[r].v[v]) * scale, T());
+        for (int v = 0; v < C::V; ++v) c.w[r].v[v] = down(up(c.w[r].v[v]) * power * scale, T());
         if (wide && C::place(true, r, C::V - 1) < n) {
             reinterpret_cast<Wide<T>*>(q)[r * kThreads + threadIdx.x] = c.w[r];
         } else {
@@ -181,7 +181,12 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Table t, const double* 
     const double norm = sqrt(block_sum(s, red));
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     // gradients whose norm is no finite number stay as they are: the caller sees the norm
-    const float scale = norm > (double)most && norm < (double)INFINITY ? (float)((double)most / norm) : 1.0f;
+    const double factor = norm > (double)most && norm < (double)INFINITY ? (double)most / norm : 1.0;
+    // Below the normal numbers 32 bits hold few bits of a factor, or none, while its products with values as large as
+    // such a norm has are ordinary numbers.  The values meet a power of two first then, and what is left of the factor is
+    // 2^-126 and more: the first product is exact wherever the second does not come to 0.
+    const int below = factor < 0x1p-126 ? min(-126 - ilogb(factor), 149) : 0;
+    const float power = (float)ldexp(1.0, -below), scale = (float)ldexp(factor, below);
     int first, last;
     share_of(t.first[t.tensors], &first, &last);
     int c = last - 1;
@@ -191,8 +196,8 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Table t, const double* 
         const int per = kChunkBytes / (t.bf16[i] ? 2 : 4);
         const int64_t at = (int64_t)(c - t.first[i]) * per;
         const int n = (int)min((int64_t)per, t.count[i] - at);
-        if (t.bf16[i]) chunk_scale<uint16_t>(t.in[i], t.out[i], at, n, scale);
-        else chunk_scale<float>(t.in[i], t.out[i], at, n, scale);
+        if (t.bf16[i]) chunk_scale<uint16_t>(t.in[i], t.out[i], at, n, power, scale);
+        else chunk_scale<float>(t.in[i], t.out[i], at, n, power, scale);
     }
 }
 
