@@ -2066,9 +2066,10 @@ int adapt_cfg(const ppocr_rh* h) { return h->quantized ? CFG_H2 : CFG_HF3; }
 constexpr size_t kAdaptWs = 256;
 
 // An adapter's values are held in fp16 halves in units of their classes' scales, so the units have to lie close to each
-// other.  Packed weights' scales need not: a class whose weights all but vanish has one down to 2^-34, one of zeros
-// 1.  Classes' units are raised to the largest, by up to 2^24, where the scales are further apart than 2^8: the int8
-// values of 7 bits are then held in fp16 that much lower, exactly.
+// other.  Packed weights' scales need not: a class whose weights all but vanish has one down to 2^-34.  Classes' units are
+// raised to the largest, by up to 2^24, where the scales are further apart than 2^8: the int8 values of 7 bits are
+// then held in fp16 that much lower, exactly.  A class of zeros has the scale 1 from packing, which says nothing of its
+// adapter's size: the others' units do not follow it, and its own becomes the largest of theirs.
 constexpr float kLeastAdaptScale = 1.0f / (1LL << 34);
 constexpr int kNearUnits = 8, kMostRaise = 24, kMostSpread = kMostRaise + 16;
 //
@@ -2105,32 +2106,42 @@ int adapt_units(const ppocr_rh* base, Adapters* ad, size_t* total) try {
         return PPOCR_OK;
     }
     PPOCR_HIP(hipMemcpy(unit.data(), base->d_scale, (size_t)n * 4, hipMemcpyDeviceToHost));
+    std::vector<int8_t> q((size_t)(n * k));
+    PPOCR_HIP(hipMemcpy(q.data(), base->d_q, q.size(), hipMemcpyDeviceToHost));
+    // a class of zeros has whatever scale; its unit is free, and becomes one near the others'
+    std::vector<bool> zeros((size_t)n);
     int top = -1000, least = 1000;
     for (int64_t i = 0; i < n; ++i) {
         if (!(std::fabs(unit[i]) >= kLeastAdaptScale && std::isfinite(unit[i])))
             return bad_arg(kAdaptOp, "scale of class " + std::to_string(i) + " below 2^-34 or not finite");
+        const int8_t* row = q.data() + i * k;
+        zeros[i] = std::all_of(row, row + k, [](int8_t v) { return v == 0; });
+        if (zeros[i]) continue;
         top = std::max(top, std::ilogb(unit[i]));
         least = std::min(least, std::ilogb(unit[i]));
     }
+    // nothing but zeros: the least unit, which an adapter of any size may pass, there being no products to scale down
+    if (top < least) top = least = std::ilogb(kLeastAdaptScale);
+    bool far = top - least > kNearUnits;
+    for (int64_t i = 0; i < n; ++i) far = far || (zeros[i] && std::abs(std::ilogb(unit[i]) - top) > kNearUnits);
     if (top - least > kMostSpread) return bad_arg(kAdaptOp, "scales of the classes further apart than 2^" + std::to_string(kMostSpread));
-    if (top - least <= kNearUnits) return PPOCR_OK;
+    if (!far) return PPOCR_OK;
     const TileGeom& g = base->geom;
     std::vector<uint8_t> rec((size_t)g.tiles * g.rec_bytes());
     PPOCR_HIP(hipMemcpy(rec.data(), base->d_rec_h, rec.size(), hipMemcpyDeviceToHost));
     for (int64_t row = 0; row < n; ++row) {
-        const int raise = std::min(top - std::ilogb(unit[row]), kMostRaise), i = (int)(row % 32);
-        const float up = std::ldexp(1.0f, raise), down = std::ldexp(1.0f, -raise);
-        unit[row] *= up;
+        const int power = top - std::ilogb(unit[row]), raise = zeros[row] ? power : std::min(power, kMostRaise), i = (int)(row % 32);
+        unit[row] = std::ldexp(unit[row], raise);
         uint8_t* r = rec.data() + (size_t)(row / 32) * g.rec_bytes();
         uint16_t* frag = reinterpret_cast<uint16_t*>(r);
-        for (int x = 0; x < g.G; ++x)
+        for (int x = 0; x < g.G && !zeros[row]; ++x)
             for (int e = 0; e < 8; ++e) {
                 uint16_t& v = frag[((size_t)x * 32 + i) * 8 + e];
-                v = f16_bits_rne(f16_to_float(v) * down);
+                v = f16_bits_rne(std::ldexp(f16_to_float(v), -raise));
             }
         float* ep = reinterpret_cast<float*>(r + g.frag_bytes());
-        ep[i] *= up;
-        ep[64 + i] *= up;
+        ep[i] = std::ldexp(ep[i], raise);
+        ep[64 + i] = std::ldexp(ep[64 + i], raise);
     }
     if (int e = upload(&ad->own_unit, unit.data(), unit.size(), total)) return e;
     if (int e = upload(&ad->own_rec, rec.data(), rec.size(), total)) return e;

@@ -1,0 +1,82 @@
+"""Adapters beside heads whose classes have scales far apart, classes without any weight among them: what is kept of
+each class's products."""
+import numpy as np
+import pytest
+
+import adapt_common as ac
+import train_common as tc
+from train_common import U24
+
+pytestmark = pytest.mark.gpu
+
+N, K, RANK = 96, 120, 4
+
+
+def adapted(rh, rng, w, quant, up):
+    """A head of weights w, and an adapter of the sizes `up` [n, 1] in slot 0."""
+    h = ac.Head(rh, rng, N, K, quant, 1, RANK, ranks=[0])
+    h.bias = np.zeros(N, np.float32)
+    if quant:
+        qw = rh.QuantizedWeight.from_f32_transposed(w)
+        h.base = rh.RecHead(qw=qw, bias=h.bias)
+        h.w = qw.data.astype(np.float64) * qw.scales.astype(np.float64)[:, None]
+    else:
+        h.base = rh.RecHead(w_t=w, bias=h.bias)
+        h.w = w.astype(np.float64)
+    h.head = rh.AdaptedHead(h.base, 1, RANK)
+    sign = lambda shape: np.where(rng.random(shape) < 0.5, -1.0, 1.0)
+    down = (rng.uniform(0.5, 1, (RANK, K)) * sign((RANK, K)) / np.sqrt(K)).astype(np.float32)
+    h.set(0, down, (rng.uniform(0.5, 1, (N, RANK)) * sign((N, RANK)) * up).astype(np.float32), 1.0)
+    return h
+
+
+def check(h, rng, label):
+    """Rows of one value each, so that few roundings hide what the operands lost.  Halves keep 2^-22: of the row, down
+    and u each once, of up once, and the two products of low halves left out: 6 for an adapter's product, one more for the
+    row's value in u; 3 for the head's (relative to the class's largest weight).  Sums of 3 products a rank and of 3 of the
+    head's, u's 3, up's two roundings and some of the epilogue: 3 rank + 12 half steps."""
+    m = 40
+    a = np.zeros((m, K), np.float32)
+    a[np.arange(m), rng.integers(0, K, m)] = (2.0 ** 13 * rng.uniform(1, 2, m)).astype(np.float32)
+    down, up, scale = h.adapters[0]
+    a64 = a.astype(np.float64)
+    z = a64 @ h.w.T + (a64 @ down.T) @ up.T
+    mag = (np.abs(a64) @ np.abs(down).T) @ np.abs(up).T
+    head = np.abs(a64).max(axis=1, keepdims=True) * np.abs(h.w).max(axis=1)
+    e = mag * (7 * 2.0 ** -22 + (3 * RANK + 12) * U24) + head * (3 * 2.0 ** -22 + (3 * RANK + 12) * U24)
+    off, slot = [0, m], [0]
+    tc.close(ac.Call(h, a, off, slot).logits().get(), z, e, label)
+    o = ac.Call(h, a, [0, m // 2, m], [0, 0]).decode()
+    top = z.max(axis=1)
+    assert (z[np.arange(m), o["idx"].get()] >= top - 2 * e.max(axis=1)).all(), label
+
+
+@pytest.mark.parametrize("size", [1e-2, 1e-4, 1e-5, 1e-7, 1e-8])
+@pytest.mark.parametrize("quant", [True, False], ids=["q", "w"])
+def test_classes_of_zeros(rh, quant, size):
+    """Unused classes do not cost the others' adapters any bits, and keep their own."""
+    rng = np.random.default_rng(1)
+    w = (rng.standard_normal((N, K)) * size).astype(np.float32)
+    w[[0, 7, 40, N - 1]] = 0.0
+    h = adapted(rh, rng, w, quant, size)
+    check(h, rng, f"zeros beside weights of {size}")
+    a = (rng.standard_normal((9, K)) * 2).astype(np.float32)
+    assert np.array_equal(h.head.logits(a), h.base.logits(a))
+
+
+def test_nothing_but_zeros(rh):
+    for quant in (True, False):
+        rng = np.random.default_rng(2)
+        check(adapted(rh, rng, np.zeros((N, K), np.float32), quant, 0.05), rng, f"zeros, INT8 {quant}")
+
+
+def test_zeros_of_any_scale(rh):
+    """A head of zeros whose scales lie further apart than any units may."""
+    rng = np.random.default_rng(4)
+    h = adapted(rh, rng, np.zeros((N, K), np.float32), True, 0.05)
+    qw = rh.QuantizedWeight.from_f32_transposed(np.zeros((N, K), np.float32))
+    qw.scales[:] = 2.0 ** rng.integers(-34, 90, N)
+    h.base = rh.RecHead(qw=qw, bias=h.bias)
+    h.head = rh.AdaptedHead(h.base, 1, RANK)
+    h.set(0, *(v.astype(np.float32) for v in h.adapters[0][:2]), 1.0)
+    check(h, rng, "zeros of any scale")
