@@ -471,14 +471,17 @@ int ppocr_ra_set_dev(ppocr_rh_t* h, int64_t slot, void* d_down, void* d_up, int6
  * line_off[i+1] of a [m][k] run under slot line_slot[i].  A negative slot is none: the head alone; so
  * is, in the `_dev` forms, one of `slots` and above (the host forms refuse it), a slot that holds no
  * adapter, and for logits every row that no line covers.  The `_dev` forms read the lines on the
- * device as ppocr_rh_decode_dev does; a row that lies in several lines (offsets that go backwards)
- * takes the adapter of one of them. Both operands of every product are fp16 halves (three products of
- * 11 bits each, int8 weights exactly), the rows at a power of two that their own largest value sets,
- * summed in fp32: 22 bits of each row's and of the adapter's largest products, and the same bits
- * whatever the rows beside it hold.  The head's products lose a bit for each power of two by which an
- * adapter's largest scale |up| sum |down| passes 2^22 times an FP32 head's largest weight or an INT8
- * head's largest scale (where its scales lie within 2^32 of each other).  A row that holds an infinity
- * or NaN has NaN logits; decoded, it is class 0.  There is no mode and no precision guard. */
+ * device as ppocr_rh_decode_dev does; where offsets go backwards a row takes the adapter of one of
+ * the lines that it lies in, or none.  Both operands of every product are fp16 halves (three products
+ * of 11 bits each, int8 weights exactly), the rows at a power of two that their own largest value
+ * sets, summed in fp32: 22 bits of each row's, of each class's and of its adapter's largest products,
+ * and the same bits whatever the rows beside it hold.  Classes whose weights (an INT8 head's scales,
+ * but for classes of zeros) lie more than 2^15 below the largest, of an INT8 head 2^22, lose a bit of
+ * theirs and of an adapter of that size for each further power of two.  The head's products lose one
+ * for each power of two by which an adapter's largest scale |up| sum |down| passes 2^16 times an FP32
+ * head's largest weight or an INT8 head's largest scale (2^29 times the least class's, if that is
+ * more).  A row that holds an infinity or NaN has NaN logits; decoded, it is class 0.  There is no mode
+ * and no precision guard. */
 size_t ppocr_ra_workspace_bytes(const ppocr_rh_t* h, int64_t m);
 int ppocr_ra_logits(const ppocr_rh_t* h, const float* a, const int64_t* line_off, int64_t lines, const int32_t* line_slot,
                     float* out);

@@ -2065,16 +2065,20 @@ int adapt_cfg(const ppocr_rh* h) { return h->quantized ? CFG_H2 : CFG_HF3; }
 // The workspace of an adapted call behind the first bytes, which are left to the head's calls.
 constexpr size_t kAdaptWs = 256;
 
-// An adapter's values are held in fp16 halves in units of their classes' scales, so the units have to lie close to each
-// other.  Packed weights' scales need not: a class whose weights all but vanish has one down to 2^-34.  Classes' units are
-// raised to the largest, by up to 2^24, where the scales are further apart than 2^8: the int8 values of 7 bits are
-// then held in fp16 that much lower, exactly.  A class of zeros has the scale 1 from packing, which says nothing of its
-// adapter's size: the others' units do not follow it, and its own becomes the largest of theirs.
-constexpr float kLeastAdaptScale = 1.0f / (1LL << 34);
-constexpr int kNearUnits = 8, kMostRaise = 24, kMostSpread = kMostRaise + 16;
+// An adapter's values are held in fp16 halves in units of their classes' weights: an INT8 head's scales, an FP32 head's
+// powers of two above each class's largest weight (its own records hold weights to 2^-25, whatever their size).  One power
+// of two for a slot brings the largest below 2^14, the head's products with it, so the units have to lie close to each
+// other: they are raised to 2^-kNearUnits of the largest.  Halves keep 22 bits of 2^-3 and above.  Within kNearUnits
+// nothing is lost then: an adapter of one size in all classes is 2 and more in the class of the largest unit.  Beyond, a
+// class loses what it is raised by; of an INT8 head less 10 bits, its weights being 2^7 units, its adapter's of that
+// size.  (All units brought to the largest one kept 32 - D bits of classes 2^D below it; those of INT8 heads now keep 22
+// up to D = 22.)
 //
-// An FP32 head's own records hold weights to 2^-25, whatever their size.  Here each class has as its unit the power
-// of two above its largest weight (2^kNearUnits below the largest unit at least): 22 bits of it and more.
+// Scales of packed weights go down to 2^-34.  int8 values of 7 bits are exact in fp16 when raised by up to 2^24.  A class of
+// zeros has the scale 1 from packing, which says nothing of its adapter's size: the others' units do not follow it, and
+// its own becomes the largest of theirs.
+constexpr float kLeastAdaptScale = 1.0f / (1LL << 34);
+constexpr int kNearUnits = 12, kMostRaise = 24, kMostSpread = kMostRaise + 16;
 int adapt_units(const ppocr_rh* base, Adapters* ad, size_t* total) try {
     ad->unit = base->d_scale;
     ad->rec = base->d_rec_h;
@@ -2130,7 +2134,8 @@ int adapt_units(const ppocr_rh* base, Adapters* ad, size_t* total) try {
     std::vector<uint8_t> rec((size_t)g.tiles * g.rec_bytes());
     PPOCR_HIP(hipMemcpy(rec.data(), base->d_rec_h, rec.size(), hipMemcpyDeviceToHost));
     for (int64_t row = 0; row < n; ++row) {
-        const int power = top - std::ilogb(unit[row]), raise = zeros[row] ? power : std::min(power, kMostRaise), i = (int)(row % 32);
+        const int power = top - std::ilogb(unit[row]), i = (int)(row % 32);
+        const int raise = zeros[row] ? power : std::clamp(power - kNearUnits, 0, kMostRaise);
         unit[row] = std::ldexp(unit[row], raise);
         uint8_t* r = rec.data() + (size_t)(row / 32) * g.rec_bytes();
         uint16_t* frag = reinterpret_cast<uint16_t*>(r);

@@ -80,3 +80,16 @@ def test_zeros_of_any_scale(rh):
     h.head = rh.AdaptedHead(h.base, 1, RANK)
     h.set(0, *(v.astype(np.float32) for v in h.adapters[0][:2]), 1.0)
     check(h, rng, "zeros of any scale")
+
+
+@pytest.mark.parametrize("common", [False, True], ids=["own", "common"])
+@pytest.mark.parametrize("quant,size", [(True, 1e-3), (True, 1e-5), (True, 1e-6), (True, 1e-7), (False, 1e-3), (False, 1e-5)])
+def test_scales_far_apart(rh, quant, size, common):
+    """One class of weights far above the others', the adapter in proportion to each class's weights or the same in
+    all."""
+    rng = np.random.default_rng(3)
+    w = (rng.standard_normal((N, K)) * size).astype(np.float32)
+    w[11] = (rng.standard_normal(K) * 0.5).astype(np.float32)
+    up = np.full((N, 1), 0.5 if common else size)
+    up[11] = 0.5
+    check(adapted(rh, rng, w, quant, up), rng, f"one class above {size}")
