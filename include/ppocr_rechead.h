@@ -472,7 +472,8 @@ int ppocr_ra_set_dev(ppocr_rh_t* h, int64_t slot, void* d_down, void* d_up, int6
  * is, in the `_dev` forms, one of `slots` and above (the host forms refuse it), a slot that holds no
  * adapter, and for logits every row that no line covers.  The `_dev` forms read the lines on the
  * device as ppocr_rh_decode_dev does; where offsets go backwards a row takes the adapter of one of
- * the lines that it lies in, or none.  Both operands of every product are fp16 halves (three products
+ * the lines that it lies in, or none.  Decoding leaves idx, maxprob and seq of rows of no line as
+ * they were.  Both operands of every product are fp16 halves (three products
  * of 11 bits each, int8 weights exactly), the rows at a power of two that their own largest value
  * sets, summed in fp32: 22 bits of each row's, of each class's and of its adapter's largest products,
  * and the same bits whatever the rows beside it hold.  Classes whose weights (an INT8 head's scales,

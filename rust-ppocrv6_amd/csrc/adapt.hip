@@ -12,11 +12,12 @@
 // 368 us in the statistics kernel, 386 GFLOP of halves at 1.05 PFLOP/s, the matrix units busy for 57% of them at 1.81 GHz
 // (the head's own pass: 58%).  The plan before it takes 9 us, the join of the chunks behind it 8.
 //
-// Arithmetic: fp16 halves of both operands (22 bits), as the head's F16X2 mode, all in one fp32
-// accumulator: up is held divided by the class's unit (its scale, or where a head's lie far apart that times a
-// power of two; of an FP32 head a power of two above the class's weights).  Each row is scaled by the power of two that its largest value sets, so rows of any size keep
-// their bits, whatever the rows beside them hold, and no row has to be computed again.  u = down a is computed by each wave before its first tile, from the rows it
-// holds; the products' layout is that of the operand that the next product needs.
+// Arithmetic: fp16 halves of both operands (22 bits), as the head's F16X2 mode, all in one fp32 accumulator: up is
+// held divided by the class's unit (its scale, or where a head's lie far apart that times a power of two; of an FP32
+// head a power of two above the class's weights).  Each row is scaled by the power of two that its largest value sets,
+// so rows of any size keep their bits, whatever the rows beside them hold, and no row has to be computed again.  u =
+// down a is computed by each wave before its first tile, from the rows it holds; the products' layout is that of the
+// operand that the next product needs.
 #include <algorithm>
 #include <cmath>
 

@@ -11,10 +11,17 @@
 // lines): the sums go through the team in a fixed order, and the gradient, which needs them, is written from what the
 // lanes kept in registers; the steps beyond them are read again.  Sums are held in 64 bits.
 //
-// 4M steps in 32768 lines under a policy loss, 101 MB: 27.4 us, 3.7 TB/s (a copy: 5.1); in 16384 pairs, 68 MB: 19.8 us.
-// Vector instructions bound both: some 400 a wave of 64 lanes and 4 steps a lane (the exponentials, the sums in 64 bits,
-// the clipping's border), which is why loads are held back by nothing and sums use the registers' lane paths (34 and
-// 22 us with shuffles and branches around the loads).  Small calls are bound by the launch: a page's 2245 steps 4 us.
+// 4M steps in 32768 lines under a policy loss, 101 MB: 28.1 us, 3.6 TB/s (a copy: 5.1); in 16384 pairs, 68 MB: 19.5 us.
+// Vector instructions bound the policy loss: some 400 a wave of 64 lanes and 4 steps a lane (the exponentials, the sums in
+// 64 bits, the clipping's border), 21 us of issue, which is why loads are held back by nothing and sums use the
+// registers' lane paths (34 and 22 us with shuffles and branches around the loads).  The preference loss has 12 us of
+// them; the rest is memory's latency, of which a pair of more than 256 steps has two turns.  Small calls are bound by the
+// launch: a page's 2245 steps 4 us.
+//
+// In 32 bits are a step's differences old - x and x - ref and what is taken from them: a difference is off by half a step
+// of itself at most, which is no more than the rounding of the larger cross entropy put into it (both are positive, so
+// the difference is the smaller), and the ratio and the divergence by that.  The logistic and its logarithm are in 32 bits
+// too, with what the rounding of h lost put back.
 #include <algorithm>
 #include <cmath>
 
