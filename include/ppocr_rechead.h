@@ -468,21 +468,21 @@ int ppocr_ra_set_dev(ppocr_rh_t* h, int64_t slot, void* d_down, void* d_up, int6
                      void* stream);
 
 /* ppocr_rh_logits and ppocr_rh_decode with an adapter for each line: line i's rows line_off[i] ..
- * line_off[i+1] of a [m][k] run under slot line_slot[i].  A negative slot is none: the head alone; so
- * is, in the `_dev` forms, one of `slots` and above (the host forms refuse it), a slot that holds no
- * adapter, and for logits every row that no line covers.  The `_dev` forms read the lines on the
+ * line_off[i+1] of a [m][k] run under slot line_slot[i].  A negative slot is none: the head alone;
+ * so is, in the `_dev` forms, one of `slots` and above (the host forms refuse it), a slot that holds
+ * no adapter, and for logits every row that no line covers.  The `_dev` forms read the lines on the
  * device as ppocr_rh_decode_dev does; where offsets go backwards a row takes the adapter of one of
  * the lines that it lies in, or none.  Decoding leaves idx, maxprob and seq of rows of no line as
- * they were.  Both operands of every product are fp16 halves (three products
- * of 11 bits each, int8 weights exactly), the rows at a power of two that their own largest value
- * sets, summed in fp32: 22 bits of each row's, of each class's and of its adapter's largest products,
- * and the same bits whatever the rows beside it hold.  Classes whose weights (an INT8 head's scales,
- * but for classes of zeros) lie more than 2^15 below the largest, of an INT8 head 2^22, lose a bit of
- * theirs and of an adapter of that size for each further power of two.  The head's products lose one
- * for each power of two by which an adapter's largest scale |up| sum |down| passes 2^16 times an FP32
- * head's largest weight or an INT8 head's largest scale (2^29 times the least class's, if that is
- * more).  A row that holds an infinity or NaN has NaN logits; decoded, it is class 0.  There is no mode
- * and no precision guard. */
+ * they were.  Both operands of every product are fp16 halves (three products of 11 bits each, int8
+ * weights exactly), the rows at a power of two that their own largest value sets, summed in fp32: 22
+ * bits of each row's, of each class's and of its adapter's largest products, and the same bits
+ * whatever the rows beside it hold.  Classes whose weights (an INT8 head's scales, but for classes
+ * of zeros) lie more than 2^14 below the largest, of an INT8 head 2^21, lose a bit of an adapter of
+ * that size, and of an FP32 head's weights, for each further power of two.  The head's products lose
+ * one for each power of two by which an adapter's largest scale |up| sum |down| passes 2^16 times an
+ * FP32 head's largest weight or an INT8 head's largest scale (2^29 times the least class's, if that
+ * is more).  A row that holds an infinity or NaN has NaN logits; decoded, it is class 0.  There is
+ * no mode and no precision guard. */
 size_t ppocr_ra_workspace_bytes(const ppocr_rh_t* h, int64_t m);
 int ppocr_ra_logits(const ppocr_rh_t* h, const float* a, const int64_t* line_off, int64_t lines, const int32_t* line_slot,
                     float* out);
@@ -560,9 +560,9 @@ int ppocr_preference_loss_dev(const float* d_loss, const float* d_ref_loss, cons
  * NULL: in place).  Two outputs may not overlap.  The norm is held in 64 bits, where squares are
  * summed too: one above the largest 32-bit number scales the gradients as any other and is written
  * to norm as infinity.  A NaN or infinity among the gradients leaves them all as they are; max_norm
- * INFINITY only takes the norm.  The tables are
- * host arrays in both forms (read before the call returns), the tensors of the `_dev` form and norm
- * (may be NULL) device memory; the host form takes fp32. */
+ * INFINITY only takes the norm.  The tables are host arrays in both forms (read before the call
+ * returns), the tensors of the `_dev` form and norm (may be NULL) device memory; the host form takes
+ * fp32. */
 size_t ppocr_grad_clip_workspace_bytes(const int64_t* sizes, int64_t count);
 int ppocr_grad_clip(void* const* grads, void* const* out, const int64_t* sizes, int64_t count, float max_norm,
                     float* norm);

@@ -2069,10 +2069,10 @@ constexpr size_t kAdaptWs = 256;
 // powers of two above each class's largest weight (its own records hold weights to 2^-25, whatever their size).  One power
 // of two for a slot brings the largest below 2^14, the head's products with it, so the units have to lie close to each
 // other: they are raised to 2^-kNearUnits of the largest.  Halves keep 22 bits of 2^-3 and above.  Within kNearUnits
-// nothing is lost then: an adapter of one size in all classes is 2 and more in the class of the largest unit.  Beyond, a
+// nothing is lost then: an adapter of one size in all classes is 1 and more in the class of the largest unit.  Beyond, a
 // class loses what it is raised by; of an INT8 head less 10 bits, its weights being 2^7 units, its adapter's of that
-// size.  (All units brought to the largest one kept 32 - D bits of classes 2^D below it; those of INT8 heads now keep 22
-// up to D = 22.)
+// size.  (All units brought to the largest one kept 31 - D bits of an INT8 head's class 2^D below it; 22 are now kept up to
+// D = 21.)
 //
 // Scales of packed weights go down to 2^-34.  int8 values of 7 bits are exact in fp16 when raised by up to 2^24.  A class of
 // zeros has the scale 1 from packing, which says nothing of its adapter's size: the others' units do not follow it, and
