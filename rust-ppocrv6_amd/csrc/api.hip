@@ -2127,7 +2127,11 @@ int adapt_units(const ppocr_rh* base, Adapters* ad, size_t* total) try {
     // nothing but zeros: the least unit, which an adapter of any size may pass, there being no products to scale down
     if (top < least) top = least = std::ilogb(kLeastAdaptScale);
     bool far = top - least > kNearUnits;
-    for (int64_t i = 0; i < n; ++i) far = far || (zeros[i] && std::abs(std::ilogb(unit[i]) - top) > kNearUnits);
+    // (an adapter of the size of weights of 2^7 units keeps its 22 bits in a unit up to 2^10 above theirs)
+    for (int64_t i = 0; i < n; ++i) {
+        const int above = std::ilogb(unit[i]) - top;
+        far = far || (zeros[i] && (above > 10 || above < -kNearUnits));
+    }
     if (top - least > kMostSpread) return bad_arg(kAdaptOp, "scales of the classes further apart than 2^" + std::to_string(kMostSpread));
     if (!far) return PPOCR_OK;
     const TileGeom& g = base->geom;

@@ -93,3 +93,22 @@ def test_scales_far_apart(rh, quant, size, common):
     up = np.full((N, 1), 0.5 if common else size)
     up[11] = 0.5
     check(adapted(rh, rng, w, quant, up), rng, f"one class above {size}")
+
+
+@pytest.mark.parametrize("apart", range(8, 15))
+def test_zeros_keep_22_bits(rh, apart):
+    """A class of zeros beside scales of 2^-apart: with a row, a down and a scale of powers of two its logit is the product
+    of the row's value and up, exactly, if 22 bits of up are kept (24 hold the sum of both halves' products)."""
+    rng = np.random.default_rng(5)
+    w = rng.integers(-126, 127, (N, K)) * 2.0 ** -apart
+    w[:, 3] = 127 * 2.0 ** -apart  # the largest value: the scale
+    w[[7, 40]] = 0.0
+    h = adapted(rh, rng, w.astype(np.float32), True, 0.0)
+    down = np.zeros((1, K), np.float32)
+    down[0, 5] = 1.0
+    up = ((2 ** 21 + 2 * rng.integers(0, 2 ** 20, (N, 1)) + 1) * 2.0 ** (6 - apart - 21)).astype(np.float32)  # half the weights' size
+    h.set(0, down, up, 1.0)
+    a = np.zeros((1, K), np.float32)
+    a[0, 5] = 2.0 ** 13
+    z = h.head.logits_lines(a, [0, 1], [0])
+    assert np.array_equal(z[0, [7, 40]], 2.0 ** 13 * up[[7, 40], 0])
