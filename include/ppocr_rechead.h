@@ -452,8 +452,8 @@ int ppocr_layernorm_backward_dev(void* d_dy, void* d_x, const float* d_w, const 
 /* A head with `slots` (1 to 4096) places for adapters of up to max_rank (1 to 64): a handle on the
  * same weights, which every ppocr_rh_ call takes as it takes `head` (without any adapter), with device
  * memory for the adapters of about 4 n max_rank bytes a slot (max_rank rounded up to 16, 32 or 64),
- * and for the weights of an FP32 head, or an INT8 head's whose scales lie apart, once more.  `head` and the new handle may be destroyed in any order.
- * Heads that the matrix kernels take (k of 73 to 80 or 113 to 120, an FP32 head's weights below 32768,
+ * and for the weights of an FP32 head, or an INT8 head's whose scales lie apart, once more.  `head`
+ * and the new handle may be destroyed in any order.  Heads that the matrix kernels take (k of 73 to 80 or 113 to 120, an FP32 head's weights below 32768,
  * an INT8 head's scales 2^-34 at least and, but for classes of zeros, within 2^40 of each other) only. */
 int ppocr_ra_create(const ppocr_rh_t* head, int64_t slots, int64_t max_rank, ppocr_rh_t** out);
 void ppocr_ra_destroy(ppocr_rh_t* h); /* ppocr_rh_destroy */

@@ -112,3 +112,66 @@ def test_zeros_keep_22_bits(rh, apart):
     a[0, 5] = 2.0 ** 13
     z = h.head.logits_lines(a, [0, 1], [0])
     assert np.array_equal(z[0, [7, 40]], 2.0 ** 13 * up[[7, 40], 0])
+
+
+def bits22(rng, n, power):
+    """Odd numbers of 22 bits in [2^power, 2^(power + 1)), of either sign."""
+    v = (2 ** 21 + 2 * rng.integers(0, 2 ** 20, n) + 1) * 2.0 ** (power - 21)
+    return (v * np.where(rng.random(n) < 0.5, -1, 1)).astype(np.float32)
+
+
+@pytest.mark.parametrize("apart", [0, 4, 11, 12, 13, 14, 17, 21])
+def test_22_bits_of_int8_classes_far_apart(rh, apart):
+    """Half of the classes 2^apart below the others, the adapter in proportion: its products are exact, as those of zeros."""
+    rng = np.random.default_rng(6)
+    power = np.where(np.arange(N) % 2 == 0, -8, -8 - apart)
+    w = rng.integers(-126, 127, (N, K)) * 2.0 ** power[:, None]
+    w[:, 3], w[:, 5] = 127 * 2.0 ** power, 0.0
+    h = adapted(rh, rng, w.astype(np.float32), True, 0.0)
+    # a down whose sum all but fills its power of two: half of it where the row is
+    down = np.full((1, K), 0.499 / (K - 1), np.float32)
+    down[0, 5] = 0.5
+    up = (bits22(rng, N, 6) * 2.0 ** power).astype(np.float32)[:, None]
+    h.set(0, down, up, 1.0)
+    a = np.zeros((1, K), np.float32)
+    a[0, 5] = 2.0 ** 13
+    assert np.array_equal(h.head.logits_lines(a, [0, 1], [0])[0], 2.0 ** 12 * up[:, 0])
+
+
+@pytest.mark.parametrize("apart", [0, 4, 8, 9, 11, 12, 13, 14])
+def test_22_bits_of_fp32_classes_far_apart(rh, apart):
+    """The same beside an FP32 head, whose own weights keep their bits as well."""
+    rng = np.random.default_rng(7)
+    power = np.where(np.arange(N) % 2 == 0, -3, -3 - apart)
+    w = (rng.uniform(-1, 1, (N, K)) * 2.0 ** power[:, None]).astype(np.float32)
+    w[:, 3], w[:, 5] = bits22(rng, N, -1) * 2.0 ** power, 0.0
+    h = adapted(rh, rng, w, False, 0.0)
+    down = np.full((1, K), 0.499 / (K - 1), np.float32)
+    down[0, 5] = 0.5
+    up = (bits22(rng, N, -1) * 2.0 ** power).astype(np.float32)[:, None]
+    h.set(0, down, up, 1.0)
+    a = np.zeros((2, K), np.float32)
+    a[0, 5], a[1, 3] = 2.0 ** 13, 2.0 ** 13
+    z = h.head.logits_lines(a, [0, 1, 2], [0, -1])
+    assert np.array_equal(z[0], 2.0 ** 12 * up[:, 0])
+    assert np.array_equal(z[1], 2.0 ** 13 * w[:, 3])
+
+
+@pytest.mark.parametrize("quant", [True, False], ids=["q", "w"])
+@pytest.mark.parametrize("apart,over", [(0, 16), (12, 16), (21, 16), (0, 28), (3, 25)])
+def test_the_heads_bits_beside_large_adapters(rh, quant, apart, over):
+    """An adapter 2^16 times an FP32 head's largest weight or an INT8 head's largest scale (2^28 times the least, where that
+    is more): the head's products keep 22 bits of a row that the adapter does not meet."""
+    rng = np.random.default_rng(8)
+    power = np.where(np.arange(N) % 2 == 0, -8, -8 - apart)
+    w = rng.integers(-126, 127, (N, K)) * 2.0 ** power[:, None]
+    w[:, 3], w[:, 5], w[:, 7] = 127 * 2.0 ** power, 0.0, 64 * 2.0 ** power
+    h = adapted(rh, rng, w.astype(np.float32), quant, 0.0)
+    down = np.zeros((1, K), np.float32)
+    down[0, 5] = 1.0
+    largest = 2.0 ** -8 if quant else 127 * 2.0 ** -8
+    h.set(0, down, np.full((N, 1), largest * 2.0 ** over, np.float32), 1.0)
+    a = np.zeros((3, K), np.float32)
+    a[:, 7] = bits22(rng, 3, 0) * np.array([2.0 ** 14, 2.0 ** -20, 1], np.float32)
+    z = h.head.logits_lines(a, [0, 3], [0])
+    assert np.array_equal(z, (a[:, 7:8].astype(np.float64) * w[:, 7]).astype(np.float32))
